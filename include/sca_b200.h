@@ -373,6 +373,41 @@ SCA_ABI int sca_launch_kv_append_batched(void* layer_k, void* layer_v, const voi
                                          int64_t max_blocks_per_seq, const ScaKvCacheShape* shape,
                                          int64_t elem_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* 8-bit KV cache (no counterpart in the reference).                                             */
+/* A row - one token of one kv head - is D codes of type e4m3 and one scale 2^e, e in [-14, 7]:   */
+/* the smallest e with min(max |x|, 57344) <= 448 * 2^e; code = x * 2^-e to nearest even, at most  */
+/* 448 in size (NaN stays NaN); value = code * 2^e, exact in fp16 and bf16.                       */
+/* codes  [num_blocks, block_size, kv_heads, D], 16-byte aligned, D a multiple of 16 up to 256     */
+/* scales [num_blocks, kv_heads, block_size rounded up to 16], one byte e + 15                     */
+/* ------------------------------------------------------------------------------------------ */
+typedef struct ScaFp8Layer {
+    void* k_codes;
+    void* v_codes;
+    uint8_t* k_scales;
+    uint8_t* v_scales;
+} ScaFp8Layer;
+
+/* sca_launch_kv_append into an 8-bit layer: rows [num_tokens, kv_heads, D] of `dtype_id` (fp32, fp16, bf16) are quantised
+ * as they are written; slots < 0 or beyond the pool are skipped. The slots of a call are distinct. */
+SCA_ABI int sca_launch_kv_append_fp8(const ScaFp8Layer* layer, const void* k_new, const void* v_new,
+                                     const int32_t* slot_mapping, int64_t num_tokens,
+                                     const ScaKvCacheShape* shape, int32_t dtype_id, void* stream);
+/* sca_launch_kv_append_batched into an 8-bit layer. */
+SCA_ABI int sca_launch_kv_append_batched_fp8(const ScaFp8Layer* layer, const void* k_new, const void* v_new,
+                                             const int32_t* page_table, const int32_t* seq_lens,
+                                             int64_t num_seqs, int64_t max_blocks_per_seq,
+                                             const ScaKvCacheShape* shape, int32_t dtype_id, void* stream);
+/* Reads the listed blocks (device memory) back: out [num_blocks, block_size, kv_heads, D] of `dtype_id`, 16-byte aligned;
+ * invalid ids read as zeros. */
+SCA_ABI int sca_launch_kv_gather_fp8(const void* codes, const uint8_t* scales, const int32_t* block_ids,
+                                     int64_t num_blocks, void* out, const ScaKvCacheShape* shape,
+                                     int32_t dtype_id, void* stream);
+/* sca_launch_decode_auto over an 8-bit paged cache: params->k / v are the codes of the pools, the strides of K and V are
+ * those of the pool and are not read; q and out are fp16 or bf16, block_size a multiple of 4. `cluster_ctas` may be null. */
+SCA_ABI int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, const uint8_t* k_scales,
+                                           const uint8_t* v_scales, int32_t* cluster_ctas, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,555 @@
+// Paged decode attention (one query token per head) over the 8-bit KV cache of kv_fp8.cuh.
+//
+// Per (sequence, head): s_j = scale * q . k_j, out = sum_j exp(s_j) v_j / sum_j exp(s_j) over the sequence's tokens, with
+// k_j = 2^e_j codes_j and v_j likewise. The schedule, the merge of the parts and the one-launch form on clusters are those of
+// the 16-bit cache (decode_common.cuh); what differs is the pass over a piece of a sequence:
+//
+//   * bytes: 2 * (D + 1) per token and kv head, read once for all query heads of the kv head. 4 * D FLOPs per byte pair and
+//     query head: at eight heads 16 FLOPs a byte, so the products run on the tensor cores and HBM stays the bound;
+//   * a warp takes 32 tokens at a time - as many bytes as 16 tokens of a 16-bit cache - through its own ring of 16-byte
+//     cp.async copies, no CTA barrier in the loop. The scales come with them in 4-byte copies (4 tokens of a page);
+//   * the tokens are the rows of the products and the query heads their 8 columns, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so
+//     that a group of up to 8 heads wastes nothing (with the heads as rows half of each product would be padding). Codes go
+//     from the ring to fp16 operands in registers: cvt for two codes at a time, exact. The order in which the products walk
+//     along D and the rows of V^T is free, and chosen so that a lane's operands lie side by side in the ring (no ldmatrix, no
+//     transposition of V: a byte permutation pairs two tokens' codes ahead of the cvt);
+//   * the scale of K multiplies the scores in fp32; the scale of V multiplies V's codes in fp16, which is exact too (see
+//     kv_fp8.cuh). Applied to P instead it would cost less, but P in fp16 has no range for it: 2^21 between two rows of V;
+//   * bf16 queries become fp16 by a power of two per head that puts the largest at 2^14: exact but for numbers below 2^-28 of
+//     it; P is rounded to fp16 (2^-11 of numbers up to 1), V and K not at all. Sums and statistics are fp32.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "decode_common.cuh"
+#include "kv_fp8.cuh"
+
+namespace sca_b200 {
+namespace {
+
+constexpr int kTokens = 32;              // of a warp's step
+constexpr int kSpan = kWarps * kTokens;  // of a CTA's step
+
+struct Fp8Scales {
+    const uint8_t* k;
+    const uint8_t* v;
+};
+
+template <int D>
+struct Fp8Geom {
+    static constexpr int kChunks = D / 16;  // 16-byte pieces of a row
+    static constexpr bool kSwizzle = kChunks % 8 == 0;
+    static constexpr int kTileBytes = kTokens * D;
+    static constexpr int kStageBytes = 2 * kTileBytes + 2 * kTokens;  // K, V, scales of K, scales of V
+    static constexpr int kStages = D <= 64 ? 4 : 3;
+    static constexpr int kWarpBytes = kStages * kStageBytes;
+    static constexpr int kSmemBytes = kWarps * kWarpBytes;
+    static constexpr int kWordsK = D / 16;  // words of K (4 codes) a lane holds per row: its quarter of the row
+    static constexpr int kWordsV = D / 32;  // words of V a lane holds per row: its eighth
+    static_assert(D % 32 == 0 && D <= 256, "head_dim");
+    static_assert(kWarpBytes >= 2 * (32 + 16 * D) * 4, "merge staging and the CTA's partial must fit in a warp's ring");
+};
+
+// A phase of 8 lanes reads rows {r, r + 1} of K, 4 adjacent pieces each, or rows {r, r + 2, r + 4, r + 6} of V, 2 adjacent pieces.
+template <int D>
+__device__ __forceinline__ int PieceK(int row, int piece) { return Fp8Geom<D>::kSwizzle ? piece ^ ((row & 1) << 2) : piece; }
+template <int D>
+__device__ __forceinline__ int PieceV(int row, int piece) { return Fp8Geom<D>::kSwizzle ? piece ^ (((row >> 1) & 3) << 1) : piece; }
+
+__device__ __forceinline__ uint2 LdsV2(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t Lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t Lds16(uint32_t addr) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t Lds8(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];\n" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void CpAsync4(uint32_t smem_dst, const void* gmem_src, int src_bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_dst), "l"(gmem_src), "r"(src_bytes) : "memory");
+}
+// The transpose of an 8x8 matrix of 16-bit numbers spread over the warp as an operand is (row lane / 4, columns 2 * (lane % 4)).
+__device__ __forceinline__ uint32_t Transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// First code of word w of a lane's share of a K row (c = lane % 4): 16 codes in a row of 64, then 8 in what is left.
+template <int D>
+__device__ __forceinline__ int CodeK(int w, int c) { return w < 4 * (D / 64) ? (w / 4) * 64 + 16 * c + 4 * (w % 4) : (D / 64) * 64 + 8 * c + 4 * (w % 4); }
+// The same of a V row (g = lane / 4): 16 codes in a row of 128, then an eighth of what is left.
+template <int D>
+__device__ __forceinline__ int CodeV(int w, int g) {
+    return w < 4 * (D / 128) ? (w / 4) * 128 + 16 * g + 4 * (w % 4) : (D / 128) * 128 + (D % 128 / 8) * g + 4 * (w - 4 * (D / 128));
+}
+template <int D>
+__device__ __forceinline__ void LoadK(uint32_t tile, int row, int c, uint32_t (&words)[Fp8Geom<D>::kWordsK]) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const uint4 v = LdsV4(tile + row * D + PieceK<D>(row, 4 * i + c) * 16);
+        words[4 * i] = v.x, words[4 * i + 1] = v.y, words[4 * i + 2] = v.z, words[4 * i + 3] = v.w;
+    }
+    if constexpr (D % 64 != 0) {
+        const uint2 v = LdsV2(tile + row * D + CodeK<D>(4 * (D / 64), c));
+        words[4 * (D / 64)] = v.x, words[4 * (D / 64) + 1] = v.y;
+    }
+}
+template <int D>
+__device__ __forceinline__ void LoadV(uint32_t tile, int row, int g, uint32_t (&words)[Fp8Geom<D>::kWordsV]) {
+    constexpr int kFull = D / 128;
+#pragma unroll
+    for (int i = 0; i < kFull; ++i) {
+        const uint4 v = LdsV4(tile + row * D + PieceV<D>(row, 8 * i + g) * 16);
+        words[4 * i] = v.x, words[4 * i + 1] = v.y, words[4 * i + 2] = v.z, words[4 * i + 3] = v.w;
+    }
+    if constexpr (D % 128 == 64) {
+        const uint2 v = LdsV2(tile + row * D + CodeV<D>(4 * kFull, g));
+        words[4 * kFull] = v.x, words[4 * kFull + 1] = v.y;
+    } else {
+#pragma unroll
+        for (int w = 4 * kFull; w < D / 32; ++w) words[w] = Lds32(tile + row * D + CodeV<D>(w, g));
+    }
+}
+
+// Tokens [j_begin, j_end) of one (sequence, kv head, head chunk): see DecodeSegment in decode.cu. kHi: more than 8 heads.
+template <typename T, int D, bool kHi, bool kToShared>
+__device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp8Scales& scales, unsigned char* smem, const int64_t b,
+                                           const int hk, const int hc, const int64_t j_begin, const int64_t j_end, const int slot) {
+    using G = Fp8Geom<D>;
+    constexpr int kCols = kHi ? 2 : 1;  // head columns of 8
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    const int g = lane >> 2;
+    const int c = lane & 3;
+    const int group = static_cast<int>(p.num_heads / p.num_kv_heads);
+    const int head0 = hk * group + hc * 16;
+    const int nheads = min(16, group - hc * 16);
+
+    const int ntiles = j_end > j_begin ? static_cast<int>((j_end - j_begin + kTokens - 1) / kTokens) : 0;
+    const int my_tiles = ntiles > warp ? (ntiles - warp + kWarps - 1) / kWarps : 0;
+
+    // ---- queries: columns of B, heads 8 * t + g; `unit` turns a product of codes into a score in the log2 domain ----
+    uint32_t qb[kCols][G::kWordsK][2];
+    float unit[kCols][2];  // of heads 8 * t + 2 * c, + 1
+    {
+        const T* q_base = reinterpret_cast<const T*>(p.q) + b * p.q_stride.s_b;
+        const float scale_log2 = p.scale * kLog2e;
+#pragma unroll
+        for (int t = 0; t < kCols; ++t) {
+            const bool mine = 8 * t + g < nheads;
+            const T* q_row = q_base + (head0 + 8 * t + g) * p.q_stride.s_h;
+            float factor = 1.0f, amax = 0.0f;
+#pragma unroll
+            for (int w = 0; w < G::kWordsK; ++w) {
+                const uint2 v = mine ? *reinterpret_cast<const uint2*>(q_row + CodeK<D>(w, c)) : make_uint2(0, 0);
+                qb[t][w][0] = v.x, qb[t][w][1] = v.y;
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(qb[t][w][i] << 16)), fabsf(__uint_as_float(qb[t][w][i] & 0xffff0000u))));
+                    }
+                }
+            }
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // 2^14 over the power of two at or below amax; for numbers below 2^-112 (and rows of zeros) 2^126
+                const int k = max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -112);
+                const float to_half = fp8::PowerOfTwo(14 - k);
+                factor = fp8::PowerOfTwo(k - 14 < -126 ? -126 : k - 14);
+#pragma unroll
+                for (int w = 0; w < G::kWordsK; ++w) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        qb[t][w][i] = Pack2<__half>(__uint_as_float(qb[t][w][i] << 16) * to_half, __uint_as_float(qb[t][w][i] & 0xffff0000u) * to_half);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) unit[t][i] = __shfl_sync(0xffffffffu, factor, (2 * c + i) * 4) * scale_log2;
+        }
+    }
+
+    const unsigned char* k_base = static_cast<const unsigned char*>(p.k) + hk * D;
+    const unsigned char* v_base = static_cast<const unsigned char*>(p.v) + hk * D;
+    const int64_t row_bytes = p.num_kv_heads * D;
+    const int32_t* table_row = p.page_table + b * p.max_blocks_per_seq;
+    const int block_size = static_cast<int>(p.block_size);
+    const int64_t scale_row = fp8::ScaleRow(block_size);
+
+    unsigned char* ring = smem + warp * G::kWarpBytes;
+    const uint32_t ring_addr = SmemAddr(ring);
+
+    // This lane's token of the next tile to be issued, as (page of the sequence, offset in the page), moved on by kSpan tokens
+    // per tile without a division, and the page's table entry, fetched one tile ahead.
+    int64_t page = 0;
+    int offset = 0;
+    int32_t phys_next = -1;
+    const int64_t page_step = kSpan / block_size;
+    const int offset_step = kSpan % block_size;
+    auto fetch_entry = [&](int64_t jt) { phys_next = (jt < j_end && page < p.max_blocks_per_seq) ? table_row[page] : -1; };
+    {
+        const int64_t jt = j_begin + warp * kTokens + lane;
+        page = jt / block_size;
+        offset = static_cast<int>(jt - page * block_size);
+        fetch_entry(jt);
+    }
+
+    // Issues the copies of this warp's `tl`-th tile into `stage`, tile after tile; returns which of the 32 tokens there are.
+    auto issue = [&](int tl, int stage) -> uint32_t {
+        const int64_t jt = j_begin + static_cast<int64_t>(warp + tl * kWarps) * kTokens + lane;
+        const bool there = phys_next >= 0 && phys_next < p.num_kv_blocks;
+        const int prow = there ? phys_next * block_size + offset : -1;  // pools stay below 2^31 rows
+        const uint32_t k_stage = ring_addr + stage * G::kStageBytes;
+        const uint32_t v_stage = k_stage + G::kTileBytes;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        if (c == 0) {
+            // block_size is a multiple of 4, and so is the tile's first token: four tokens share a page and a word of scales
+            const int64_t at = there ? (static_cast<int64_t>(phys_next) * p.num_kv_heads + hk) * scale_row + offset : 0;
+            CpAsync4(v_stage + G::kTileBytes + lane, scales.k + at, there ? 4 : 0);
+            CpAsync4(v_stage + G::kTileBytes + kTokens + lane, scales.v + at, there ? 4 : 0);
+        }
+        page += page_step;
+        offset += offset_step;
+        if (offset >= block_size) {
+            offset -= block_size;
+            ++page;
+        }
+        fetch_entry(jt + kSpan);
+#pragma unroll
+        for (int n = 0; n < G::kChunks; ++n) {
+            const int item = lane + 32 * n;
+            const int row = item / G::kChunks;
+            const int piece = item % G::kChunks;
+            const int pr = __shfl_sync(0xffffffffu, prow, row);
+            const int bytes = pr >= 0 ? 16 : 0;
+            const int64_t at = (pr >= 0 ? pr : 0) * row_bytes + piece * 16;
+            CpAsync16(k_stage + row * D + PieceK<D>(row, piece) * 16, k_base + at, bytes);
+            CpAsync16(v_stage + row * D + PieceV<D>(row, piece) * 16, v_base + at, bytes);
+        }
+        CpAsyncCommit();
+        return mask;
+    };
+
+    // ---- running state of heads 8 * t + 2 * c, + 1; scores live in the log2 domain ----
+    float m_run[kCols][2], l_run[kCols][2];
+    float o[kCols][2 * G::kWordsV][4];  // rows CodeV(w, g) + 2 * half, + 1 of O^T
+#pragma unroll
+    for (int t = 0; t < kCols; ++t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m_run[t][i] = -CUDART_INF_F, l_run[t][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2 * G::kWordsV; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][j][e] = 0.0f;
+        }
+    }
+
+    uint32_t masks[G::kStages - 1];
+#pragma unroll
+    for (int s = 0; s < G::kStages - 1; ++s) {
+        masks[s] = 0;
+        if (s < my_tiles) masks[s] = issue(s, s);
+        else CpAsyncCommit();
+    }
+
+    int stage = 0;
+    for (int tl = 0; tl < my_tiles; ++tl) {
+        CpAsyncWait<G::kStages - 2>();
+        __syncwarp();
+        const uint32_t cur = masks[0];
+#pragma unroll
+        for (int s = 0; s + 1 < G::kStages - 1; ++s) masks[s] = masks[s + 1];
+        {
+            const int nt = tl + G::kStages - 1;
+            int nstage = stage + G::kStages - 1;
+            if (nstage >= G::kStages) nstage -= G::kStages;
+            uint32_t mk = 0;
+            if (nt < my_tiles) mk = issue(nt, nstage);
+            else CpAsyncCommit();
+            masks[G::kStages - 2] = mk;
+        }
+        if (cur != 0) {
+            const uint32_t k_stage = ring_addr + stage * G::kStageBytes;
+            const uint32_t v_stage = k_stage + G::kTileBytes;
+            const uint32_t k_scale = v_stage + G::kTileBytes, v_scale = k_scale + kTokens;
+
+            // S^T: tokens 16 * r + g (elements 0, 1: heads 2c, 2c + 1) and 16 * r + g + 8 (elements 2, 3)
+            float s[2][kCols][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                uint32_t lo[G::kWordsK], hi[G::kWordsK];
+                LoadK<D>(k_stage, 16 * r + g, c, lo);
+                LoadK<D>(k_stage, 16 * r + g + 8, c, hi);
+#pragma unroll
+                for (int t = 0; t < kCols; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[r][t][e] = 0.0f;
+                }
+#pragma unroll
+                for (int w = 0; w < G::kWordsK; ++w) {
+                    const uint32_t a0 = fp8::DecodeLow(lo[w]), a1 = fp8::DecodeLow(hi[w]), a2 = fp8::DecodeHigh(lo[w]), a3 = fp8::DecodeHigh(hi[w]);
+#pragma unroll
+                    for (int t = 0; t < kCols; ++t) MmaM16N8K16<__half>(s[r][t], a0, a1, a2, a3, qb[t][w][0], qb[t][w][1]);
+                }
+            }
+            float k_unit[4];  // tokens g, g + 8, g + 16, g + 24
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k_unit[i] = fp8::ScaleOf(Lds8(k_scale + 8 * i + g));
+
+            uint32_t pb[kCols][4];  // P^T, columns of B: tokens 8 * i + 2 * c, + 1 of head 8 * t + g
+#pragma unroll
+            for (int t = 0; t < kCols; ++t) {
+                float alpha[2];
+                float prob[4][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool there = (cur >> (8 * i + g)) & 1u;
+                        x[i] = there ? s[i / 2][t][2 * (i & 1) + h] * (unit[t][h] * k_unit[i]) : -CUDART_INF_F;
+                    }
+                    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float m_new = fmaxf(m_run[t][h], mx);
+                    const float m_safe = m_new == -CUDART_INF_F ? 0.0f : m_new;
+                    alpha[h] = Exp2(m_run[t][h] - m_safe);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) prob[i][h] = Exp2(x[i] - m_safe);
+                    l_run[t][h] = l_run[t][h] * alpha[h] + ((prob[0][h] + prob[1][h]) + (prob[2][h] + prob[3][h]));
+                    m_run[t][h] = m_new;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pb[t][i] = Transpose8x8(Pack2<__half>(prob[i][0], prob[i][1]));
+                // the maximum of a long sequence hardly moves: O is touched where it does
+                if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                    for (int j = 0; j < 2 * G::kWordsV; ++j) {
+                        o[t][j][0] *= alpha[0], o[t][j][1] *= alpha[1], o[t][j][2] *= alpha[0], o[t][j][3] *= alpha[1];
+                    }
+                }
+            }
+
+            // O^T += V^T P^T
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = 16 * r + 2 * c;
+                uint32_t v0[G::kWordsV], v1[G::kWordsV], v8[G::kWordsV], v9[G::kWordsV];
+                LoadV<D>(v_stage, row, g, v0);
+                LoadV<D>(v_stage, row + 1, g, v1);
+                LoadV<D>(v_stage, row + 8, g, v8);
+                LoadV<D>(v_stage, row + 9, g, v9);
+                uint32_t s01 = Lds16(v_scale + row), s89 = Lds16(v_scale + row + 8);
+                if (cur != 0xffffffffu) {
+                    // the scales come four at a time: those of tokens that do not count are anything, and infinity times 0 is not 0
+                    const uint32_t there = cur >> row;
+                    s01 &= ((there & 1u) ? 0xffu : 0u) | ((there & 2u) ? 0xff00u : 0u);
+                    s89 &= ((there & 0x100u) ? 0xffu : 0u) | ((there & 0x200u) ? 0xff00u : 0u);
+                }
+                const uint32_t unit01 = fp8::ScalePair(s01, s01 >> 8), unit89 = fp8::ScalePair(s89, s89 >> 8);
+#pragma unroll
+                for (int w = 0; w < G::kWordsV; ++w) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        // two codes of each of two tokens, paired by code
+                        const uint32_t p01 = __byte_perm(v0[w], v1[w], half ? 0x7362 : 0x5140);
+                        const uint32_t p89 = __byte_perm(v8[w], v9[w], half ? 0x7362 : 0x5140);
+                        const uint32_t a0 = fp8::MulHalf2(fp8::DecodeLow(p01), unit01), a1 = fp8::MulHalf2(fp8::DecodeHigh(p01), unit01);
+                        const uint32_t a2 = fp8::MulHalf2(fp8::DecodeLow(p89), unit89), a3 = fp8::MulHalf2(fp8::DecodeHigh(p89), unit89);
+#pragma unroll
+                        for (int t = 0; t < kCols; ++t) MmaM16N8K16<__half>(o[t][2 * w + half], a0, a1, a2, a3, pb[t][2 * r], pb[t][2 * r + 1]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (++stage == G::kStages) stage = 0;
+    }
+    CpAsyncWait<0>();
+    __syncwarp();
+
+    // ---- per-warp results -> this warp's (now idle) ring, then the CTA's merge ----
+    float* stage_m = reinterpret_cast<float*>(ring);  // [16]
+    float* stage_l = stage_m + 16;                    // [16]
+    float* stage_o = stage_m + 32;                    // [16][D]
+#pragma unroll
+    for (int t = 0; t < kCols; ++t) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float l = l_run[t][h];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const int head = 8 * t + 2 * c + h;
+            if (g == 0) stage_m[head] = m_run[t][h], stage_l[head] = l;
+#pragma unroll
+            for (int w = 0; w < G::kWordsV; ++w) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    *reinterpret_cast<float2*>(stage_o + head * D + CodeV<D>(w, g) + 2 * half) = make_float2(o[t][2 * w + half][h], o[t][2 * w + half][2 + h]);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    MergeWarps<D, G::kWarpBytes, kToShared>(p, smem, b, head0, nheads, slot);
+}
+
+template <typename T, int D, bool kHi>
+__global__ void __launch_bounds__(kThreads)
+decode_fp8_partial_kernel(const ScaDecodeFwdParams p, const Fp8Scales scales, const int head_chunks) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    WalkSchedule<true, kSpan>(p, head_chunks, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end, int slot) {
+        Fp8Segment<T, D, kHi, false>(p, scales, smem, b, hk, hc, j_begin, j_end, slot);
+    });
+}
+
+template <typename T, int D, bool kHi>
+__global__ void __launch_bounds__(kThreads)
+decode_fp8_cluster_kernel(const ScaDecodeFwdParams p, const Fp8Scales scales, const int head_chunks, const int cluster) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    ClusterDecode<T, D, true, kSpan>(p, head_chunks, cluster, smem, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end) {
+        Fp8Segment<T, D, kHi, true>(p, scales, smem, b, hk, hc, j_begin, j_end, 0);
+    });
+}
+
+template <typename T, int D, bool kHi>
+int64_t ResidentCtas() {
+    static PerDevice per_sm;  // per instantiation
+    const int n = per_sm.Get([] {
+        int ctas = 0;
+        const void* fn = reinterpret_cast<const void*>(&decode_fp8_partial_kernel<T, D, kHi>);
+        if (EnsureDynamicSmem(fn, Fp8Geom<D>::kSmemBytes, "decode_fp8_partial_kernel") != SCA_OK ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, decode_fp8_partial_kernel<T, D, kHi>, kThreads, Fp8Geom<D>::kSmemBytes) != cudaSuccess ||
+            ctas < 1) {
+            cudaGetLastError();
+            return -1;
+        }
+        return ctas;
+    });
+    return static_cast<int64_t>(SmCount()) * std::max(1, n);
+}
+
+template <typename T, int D, bool kHi>
+int64_t ResidentClusters(int cluster) {
+    static PerDevice resident[kMaxCluster + 1];  // per instantiation
+    return std::max(0, resident[cluster].Get([cluster] {
+        cudaLaunchAttribute attr{};
+        cudaLaunchConfig_t cfg = ClusterConfig(static_cast<unsigned>(cluster), cluster, Fp8Geom<D>::kSmemBytes, nullptr, &attr);
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, decode_fp8_cluster_kernel<T, D, kHi>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return -1;
+        }
+        return n;
+    }));
+}
+
+// Whether the one-launch kernel is the faster one: the rule of the 16-bit cache (ClusterIsFaster in decode.cu), whose steps have
+// half the tokens and as many bytes.
+bool OneLaunchIsFaster(int64_t units, int64_t steps, int cluster, int64_t resident, bool ragged) {
+    const double busy = static_cast<double>(units * cluster) / resident;
+    const double share = static_cast<double>((steps + cluster - 1) / cluster);
+    const double waves = static_cast<double>(units * steps) / resident;
+    return 4.8 + share * (0.55 + 1.1 * busy) < 11.5 + 1.55 * std::max(1.0, waves * (ragged ? 0.55 : 1.0));
+}
+
+template <typename T, int D, bool kHi>
+int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chunks, cudaStream_t stream, int* cluster_ctas) {
+    using G = Fp8Geom<D>;
+    const int64_t columns = p.num_kv_heads * head_chunks, units = p.batch * columns;
+    const int64_t steps = std::max<int64_t>(1, (std::min(p.seq_kv, p.max_blocks_per_seq * p.block_size) + kSpan - 1) / kSpan);
+    const int64_t resident = ResidentCtas<T, D, kHi>();
+    if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(&decode_fp8_cluster_kernel<T, D, kHi>), G::kSmemBytes, "decode_fp8_cluster_kernel")) return rc;
+    // as many CTAs per cluster as let all clusters run at the same time
+    int cluster = kMaxCluster;
+    while (cluster >= 2 && units > ResidentClusters<T, D, kHi>(cluster)) cluster /= 2;
+    if (cluster < 2 || !OneLaunchIsFaster(units, steps, cluster, resident, p.seq_lens != nullptr)) cluster = 0;
+    *cluster_ctas = cluster;
+    if (cluster > 0) {
+        LaunchDependent(decode_fp8_cluster_kernel<T, D, kHi>, units * cluster, kThreads, G::kSmemBytes, stream, cluster, p, scales, head_chunks, cluster);
+        return CheckLaunch("decode_fp8_cluster_kernel", stream);
+    }
+    if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(&decode_fp8_partial_kernel<T, D, kHi>), G::kSmemBytes, "decode_fp8_partial_kernel")) return rc;
+    // one wave: CTAs per column as many as stay resident, never more than the column has steps (or sequences, with one slot)
+    const int64_t useful = p.num_splits == 1 ? p.batch : p.batch * steps;
+    const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(resident / columns, useful)) : resident;
+    LaunchDependent(decode_fp8_partial_kernel<T, D, kHi>, blocks, kThreads, G::kSmemBytes, stream, 1, p, scales, head_chunks);
+    if (int rc = CheckLaunch("decode_fp8_partial_kernel", stream)) return rc;
+    return LaunchMergeOut(p, stream);
+}
+
+template <typename T, int D>
+int LaunchFp8ForDim(const ScaDecodeFwdParams& p, const Fp8Scales& scales, cudaStream_t stream, int* cluster) {
+    const int group = static_cast<int>(p.num_heads / p.num_kv_heads);
+    const int head_chunks = (group + 15) / 16;
+    return group > 8 ? LaunchFp8<T, D, true>(p, scales, head_chunks, stream, cluster) : LaunchFp8<T, D, false>(p, scales, head_chunks, stream, cluster);
+}
+
+template <typename T>
+int LaunchFp8Typed(const ScaDecodeFwdParams& p, const Fp8Scales& scales, cudaStream_t stream, int* cluster) {
+    switch (p.head_dim) {
+        case 32: return LaunchFp8ForDim<T, 32>(p, scales, stream, cluster);
+        case 64: return LaunchFp8ForDim<T, 64>(p, scales, stream, cluster);
+        case 96: return LaunchFp8ForDim<T, 96>(p, scales, stream, cluster);
+        case 128: return LaunchFp8ForDim<T, 128>(p, scales, stream, cluster);
+        case 160: return LaunchFp8ForDim<T, 160>(p, scales, stream, cluster);
+        case 192: return LaunchFp8ForDim<T, 192>(p, scales, stream, cluster);
+        case 256: return LaunchFp8ForDim<T, 256>(p, scales, stream, cluster);
+        default: break;
+    }
+    return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): head_dim=" + std::to_string(p.head_dim) + " is not instantiated");
+}
+
+}  // namespace
+}  // namespace sca_b200
+
+using namespace sca_b200;
+
+extern "C" int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, const uint8_t* k_scales, const uint8_t* v_scales,
+                                              int32_t* cluster_ctas, void* stream) {
+    ClearError();
+    if (params == nullptr) return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): null parameter block");
+    const ScaDecodeFwdParams& p = *params;
+    if (p.q == nullptr || p.k == nullptr || p.v == nullptr || p.out == nullptr || p.partial_m == nullptr || p.partial_l == nullptr ||
+        p.partial_o == nullptr || p.page_table == nullptr || k_scales == nullptr || v_scales == nullptr) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): null pointer");
+    }
+    if (p.dtype != SCA_DTYPE_F16 && p.dtype != SCA_DTYPE_BF16) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): queries are fp16 or bf16 (dtype id " + std::to_string(p.dtype) + ")");
+    }
+    if (p.num_splits < 1 || p.batch < 1 || p.num_heads < 1 || p.num_kv_heads < 1 || p.num_heads % p.num_kv_heads != 0) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): invalid geometry batch=" + std::to_string(p.batch) + " heads=" +
+                                              std::to_string(p.num_heads) + " kv_heads=" + std::to_string(p.num_kv_heads));
+    }
+    if (p.block_size <= 0 || p.block_size % 4 != 0 || p.max_blocks_per_seq <= 0 || p.num_kv_blocks <= 0 || p.num_kv_blocks * p.block_size > 0x7fffffffLL) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): block_size=" + std::to_string(p.block_size) +
+                                              " (a multiple of 4), and a pool and a table that are not empty nor beyond 2^31 tokens");
+    }
+    if (!Aligned16(p.q) || !Aligned16(p.k) || !Aligned16(p.v) || p.q_stride.s_b % 8 != 0 || p.q_stride.s_h % 8 != 0 ||
+        (reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales)) % 4 != 0) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): q and codes must be 16-byte aligned, scales 4-byte aligned, "
+                                          "strides of q multiples of 8 elements");
+    }
+    const Fp8Scales scales{k_scales, v_scales};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int cluster = 0;
+    const int rc = p.dtype == SCA_DTYPE_F16 ? LaunchFp8Typed<__half>(p, scales, s, &cluster) : LaunchFp8Typed<__nv_bfloat16>(p, scales, s, &cluster);
+    if (cluster_ctas != nullptr) *cluster_ctas = cluster;
+    return rc;
+}

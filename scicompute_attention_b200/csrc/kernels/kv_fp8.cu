@@ -1,0 +1,295 @@
+// The 8-bit KV cache (kv_fp8.cuh): rows are quantised as they are written, blocks are read back as 16- or 32-bit numbers.
+//
+// Both kernels move every byte once: a row of D numbers of w bytes is read, D + 1 bytes are written, or the other way round.
+#include <algorithm>
+#include <string>
+
+#include "common.cuh"
+#include "kv_fp8.cuh"
+
+namespace sca_b200 {
+namespace {
+
+constexpr int kFp8Threads = 256;
+
+// Eight consecutive numbers of a row.
+template <typename T>
+__device__ __forceinline__ void Load8(const T* src, bool aligned, float (&x)[8]) {
+    if (aligned) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            const T* t = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = ToFloat(t[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = ToFloat(src[i]);
+    }
+}
+
+// Where rows go: `slots` (one per token), or the page table at position seq_lens[token] - 1 (one token per sequence).
+struct AppendTarget {
+    uint8_t *k_codes, *v_codes, *k_scales, *v_scales;
+    const int32_t* slots;
+    const int32_t* page_table;
+    const int32_t* seq_lens;
+    int64_t max_blocks_per_seq;
+    int64_t num_blocks;
+    int block_size, heads, head_dim;
+    bool aligned;  // the new rows start on 16-byte boundaries
+};
+
+// Slot of a token, -1 where it is not stored.
+template <bool kBatched>
+__device__ __forceinline__ int64_t SlotOf(const AppendTarget& a, int64_t token) {
+    if constexpr (!kBatched) {
+        const int32_t slot = a.slots[token];
+        return slot >= 0 && slot < a.num_blocks * a.block_size ? slot : -1;
+    } else {
+        const int pos = a.seq_lens[token] - 1;
+        if (pos < 0) return -1;
+        const int logical = pos / a.block_size;
+        if (logical >= a.max_blocks_per_seq) return -1;
+        const int32_t phys = a.page_table[token * a.max_blocks_per_seq + logical];
+        if (phys < 0 || phys >= a.num_blocks) return -1;
+        return static_cast<int64_t>(phys) * a.block_size + (pos - logical * a.block_size);
+    }
+}
+
+// kLanes lanes of a warp (the smallest power of two that covers D / 8) take a row of K and the same row of V: 8 numbers each,
+// the largest by shuffles, 8 codes each. I: type of a row's number.
+template <typename T, int kLanes, bool kBatched, typename I>
+__global__ void __launch_bounds__(kFp8Threads)
+kv_append_fp8_kernel(const T* k_new, const T* v_new, const I rows, const AppendTarget a) {
+    BeginAfterPredecessor();
+    constexpr int kRows = kFp8Threads / kLanes;  // of a CTA
+    const int piece = threadIdx.x % kLanes;
+    const bool in_row = piece * 8 < a.head_dim;
+    for (I base = static_cast<I>(blockIdx.x) * kRows; base < rows; base += static_cast<I>(gridDim.x) * kRows) {
+        const I row = base + threadIdx.x / kLanes;
+        const bool mine = row < rows && in_row;
+        float x[2][8];
+        if (mine) {
+            Load8(k_new + static_cast<int64_t>(row) * a.head_dim + piece * 8, a.aligned, x[0]);
+            Load8(v_new + static_cast<int64_t>(row) * a.head_dim + piece * 8, a.aligned, x[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[0][i] = x[1][i] = 0.0f;
+        }
+        const I token = row / a.heads;
+        const int head = static_cast<int>(row - token * a.heads);
+        const int64_t slot = row < rows ? SlotOf<kBatched>(a, token) : -1;
+        float amax[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float m = 0.0f;  // fmaxf passes over NaN
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[s][i]));
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            amax[s] = fminf(m, fp8::kLargest);
+        }
+        if (!mine || slot < 0) continue;
+        const int64_t block = slot / a.block_size;
+        const int offset = static_cast<int>(slot - block * a.block_size);
+        const int64_t code_at = (slot * a.heads + head) * a.head_dim + piece * 8;
+        const int64_t scale_at = (block * a.heads + head) * fp8::ScaleRow(a.block_size) + offset;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int e = fp8::ExponentFor(amax[s]);
+            const float inv = fp8::PowerOfTwo(-e);
+            uint2 codes;
+            codes.x = fp8::Encode2(x[s][0] * inv, x[s][1] * inv) | fp8::Encode2(x[s][2] * inv, x[s][3] * inv) << 16;
+            codes.y = fp8::Encode2(x[s][4] * inv, x[s][5] * inv) | fp8::Encode2(x[s][6] * inv, x[s][7] * inv) << 16;
+            *reinterpret_cast<uint2*>((s == 0 ? a.k_codes : a.v_codes) + code_at) = codes;
+            if (piece == 0) (s == 0 ? a.k_scales : a.v_scales)[scale_at] = static_cast<uint8_t>(e + 15);
+        }
+    }
+}
+
+// 16 codes per thread and turn.
+template <typename T, typename I>
+__global__ void __launch_bounds__(kFp8Threads)
+kv_gather_fp8_kernel(const uint8_t* codes, const uint8_t* scales, const int32_t* ids, const I total, T* out, const int64_t num_blocks,
+                     const int block_size, const int heads, const int head_dim) {
+    BeginAfterPredecessor();
+    const int pieces = head_dim / 16;
+    const I block_pieces = static_cast<I>(block_size) * heads * pieces;
+    for (I idx = static_cast<I>(blockIdx.x) * kFp8Threads + threadIdx.x; idx < total; idx += static_cast<I>(gridDim.x) * kFp8Threads) {
+        const I i = idx / block_pieces;
+        const int within = static_cast<int>(idx - i * block_pieces);
+        const int32_t phys = ids[i];
+        uint4 c = make_uint4(0, 0, 0, 0);
+        uint32_t byte = 15;
+        if (phys >= 0 && phys < num_blocks) {
+            const int row = within / pieces;
+            const int token = row / heads, head = row - token * heads;
+            c = reinterpret_cast<const uint4*>(codes)[static_cast<int64_t>(phys) * block_pieces + within];
+            byte = scales[(static_cast<int64_t>(phys) * heads + head) * fp8::ScaleRow(block_size) + token];
+        }
+        const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+        uint32_t h[8];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) h[2 * w] = fp8::DecodeLow(words[w]), h[2 * w + 1] = fp8::DecodeHigh(words[w]);
+        T* dst = out + static_cast<int64_t>(idx) * 16;
+        if constexpr (sizeof(T) == 4) {
+            const float s = fp8::ScaleOf(byte);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float2 lo = fp8::UnpackHalf2(h[2 * w]), hi = fp8::UnpackHalf2(h[2 * w + 1]);
+                reinterpret_cast<float4*>(dst)[w] = make_float4(lo.x * s, lo.y * s, hi.x * s, hi.y * s);
+            }
+        } else {
+            const uint32_t pair = fp8::ScalePair(byte, byte);
+            const float s = fp8::ScaleOf(byte);
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                if constexpr (std::is_same<T, __half>::value) {
+                    h[w] = fp8::MulHalf2(h[w], pair);
+                } else {
+                    const float2 f = fp8::UnpackHalf2(h[w]);
+                    h[w] = Pack2<T>(f.x * s, f.y * s);
+                }
+            }
+            reinterpret_cast<uint4*>(dst)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            reinterpret_cast<uint4*>(dst)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+    }
+}
+
+// A grid that covers the work once, at most a few waves of the machine: the loops are grid-stride.
+int64_t Fp8Grid(int64_t ctas) { return std::max<int64_t>(1, std::min(ctas, static_cast<int64_t>(SmCount()) * 32)); }
+
+int CheckFp8Shape(const ScaKvCacheShape* shape, const char* what) {
+    if (shape == nullptr) return Fail(SCA_INVALID_ARGUMENT, std::string(what) + ": null shape");
+    if (shape->num_blocks <= 0 || shape->block_size <= 0 || shape->num_kv_heads <= 0) {
+        return Fail(SCA_INVALID_ARGUMENT, std::string(what) + ": non-positive geometry");
+    }
+    if (shape->head_dim <= 0 || shape->head_dim > 256 || shape->head_dim % 16 != 0) {
+        return Fail(SCA_INVALID_ARGUMENT, std::string(what) + ": head_dim=" + std::to_string(shape->head_dim) +
+                                              " (rows of an 8-bit cache are multiples of 16 up to 256)");
+    }
+    if (shape->num_blocks * shape->block_size > 0x7fffffffLL || shape->block_size * shape->num_kv_heads > 0x3fffffLL) {
+        return Fail(SCA_INVALID_ARGUMENT, std::string(what) + ": slots beyond 32 bits");
+    }
+    return SCA_OK;
+}
+
+template <typename T, bool kBatched, typename I>
+void LaunchAppend(const void* k_new, const void* v_new, I rows, const AppendTarget& a, cudaStream_t stream) {
+    auto go = [&](auto lanes) {
+        constexpr int kLanes = decltype(lanes)::value;
+        constexpr int kRows = kFp8Threads / kLanes;
+        LaunchDependent(kv_append_fp8_kernel<T, kLanes, kBatched, I>, Fp8Grid((static_cast<int64_t>(rows) + kRows - 1) / kRows), kFp8Threads, 0,
+                        stream, 1, static_cast<const T*>(k_new), static_cast<const T*>(v_new), rows, a);
+    };
+    const int pieces = a.head_dim / 8;
+    if (pieces <= 4) go(std::integral_constant<int, 4>{});
+    else if (pieces <= 8) go(std::integral_constant<int, 8>{});
+    else if (pieces <= 16) go(std::integral_constant<int, 16>{});
+    else go(std::integral_constant<int, 32>{});
+}
+
+template <bool kBatched>
+int AppendRows(const ScaFp8Layer& l, const void* k_new, const void* v_new, int64_t tokens, const ScaKvCacheShape& shape, AppendTarget a,
+               int32_t dtype_id, cudaStream_t stream, const char* what) {
+    a.k_codes = static_cast<uint8_t*>(l.k_codes);
+    a.v_codes = static_cast<uint8_t*>(l.v_codes);
+    a.k_scales = static_cast<uint8_t*>(l.k_scales);
+    a.v_scales = static_cast<uint8_t*>(l.v_scales);
+    a.num_blocks = shape.num_blocks;
+    a.block_size = static_cast<int>(shape.block_size);
+    a.heads = static_cast<int>(shape.num_kv_heads);
+    a.head_dim = static_cast<int>(shape.head_dim);
+    a.aligned = Aligned16(k_new) && Aligned16(v_new);
+    if (!Aligned16(a.k_codes) || !Aligned16(a.v_codes)) return Fail(SCA_INVALID_ARGUMENT, std::string(what) + ": the codes must be 16-byte aligned");
+    const int64_t rows = tokens * shape.num_kv_heads;
+    auto typed = [&](auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        // what the loop may step past `rows` fits the narrow counter too
+        if (rows < (1ll << 31)) LaunchAppend<T, kBatched, uint32_t>(k_new, v_new, static_cast<uint32_t>(rows), a, stream);
+        else LaunchAppend<T, kBatched, int64_t>(k_new, v_new, rows, a, stream);
+    };
+    switch (dtype_id) {
+        case SCA_DTYPE_F32: typed(static_cast<float*>(nullptr)); break;
+        case SCA_DTYPE_F16: typed(static_cast<__half*>(nullptr)); break;
+        case SCA_DTYPE_BF16: typed(static_cast<__nv_bfloat16*>(nullptr)); break;
+        default: return Fail(SCA_INVALID_ARGUMENT, std::string(what) + ": unsupported dtype id");
+    }
+    return CheckLaunch("kv_append_fp8_kernel", stream);
+}
+
+bool AnyNull(const ScaFp8Layer* l) {
+    return l == nullptr || l->k_codes == nullptr || l->v_codes == nullptr || l->k_scales == nullptr || l->v_scales == nullptr;
+}
+
+}  // namespace
+}  // namespace sca_b200
+
+using namespace sca_b200;
+
+extern "C" int sca_launch_kv_append_fp8(const ScaFp8Layer* layer, const void* k_new, const void* v_new, const int32_t* slot_mapping,
+                                        int64_t num_tokens, const ScaKvCacheShape* shape, int32_t dtype_id, void* stream) {
+    ClearError();
+    if (AnyNull(layer) || k_new == nullptr || v_new == nullptr || slot_mapping == nullptr) {
+        return Fail(SCA_INVALID_ARGUMENT, "kv append (fp8): null pointer");
+    }
+    if (num_tokens <= 0) return Fail(SCA_INVALID_ARGUMENT, "kv append (fp8): num_tokens <= 0");
+    if (int rc = CheckFp8Shape(shape, "kv append (fp8)")) return rc;
+    AppendTarget a{};
+    a.slots = slot_mapping;
+    return AppendRows<false>(*layer, k_new, v_new, num_tokens, *shape, a, dtype_id, static_cast<cudaStream_t>(stream), "kv append (fp8)");
+}
+
+extern "C" int sca_launch_kv_append_batched_fp8(const ScaFp8Layer* layer, const void* k_new, const void* v_new, const int32_t* page_table,
+                                                const int32_t* seq_lens, int64_t num_seqs, int64_t max_blocks_per_seq,
+                                                const ScaKvCacheShape* shape, int32_t dtype_id, void* stream) {
+    ClearError();
+    if (AnyNull(layer) || k_new == nullptr || v_new == nullptr || page_table == nullptr || seq_lens == nullptr) {
+        return Fail(SCA_INVALID_ARGUMENT, "kv append (batched, fp8): null pointer");
+    }
+    if (num_seqs <= 0 || max_blocks_per_seq <= 0) {
+        return Fail(SCA_INVALID_ARGUMENT, "kv append (batched, fp8): num_seqs/max_blocks_per_seq <= 0");
+    }
+    if (int rc = CheckFp8Shape(shape, "kv append (batched, fp8)")) return rc;
+    AppendTarget a{};
+    a.page_table = page_table;
+    a.seq_lens = seq_lens;
+    a.max_blocks_per_seq = max_blocks_per_seq;
+    return AppendRows<true>(*layer, k_new, v_new, num_seqs, *shape, a, dtype_id, static_cast<cudaStream_t>(stream), "kv append (batched, fp8)");
+}
+
+extern "C" int sca_launch_kv_gather_fp8(const void* codes, const uint8_t* scales, const int32_t* block_ids, int64_t num_blocks, void* out,
+                                        const ScaKvCacheShape* shape, int32_t dtype_id, void* stream) {
+    ClearError();
+    if (codes == nullptr || scales == nullptr || block_ids == nullptr || out == nullptr) {
+        return Fail(SCA_INVALID_ARGUMENT, "kv gather (fp8): null pointer");
+    }
+    if (num_blocks <= 0) return SCA_OK;
+    if (int rc = CheckFp8Shape(shape, "kv gather (fp8)")) return rc;
+    if (!Aligned16(codes) || !Aligned16(out)) return Fail(SCA_INVALID_ARGUMENT, "kv gather (fp8): codes and output must be 16-byte aligned");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t total = num_blocks * shape->block_size * shape->num_kv_heads * (shape->head_dim / 16);
+    const int64_t grid = Fp8Grid((total + kFp8Threads - 1) / kFp8Threads);
+    auto typed = [&](auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        auto go = [&](auto count) {
+            LaunchDependent(kv_gather_fp8_kernel<T, decltype(count)>, grid, kFp8Threads, 0, s, 1, static_cast<const uint8_t*>(codes), scales,
+                            block_ids, count, static_cast<T*>(out), shape->num_blocks, static_cast<int>(shape->block_size),
+                            static_cast<int>(shape->num_kv_heads), static_cast<int>(shape->head_dim));
+        };
+        if (total < (1ll << 31)) go(static_cast<uint32_t>(total));
+        else go(total);
+    };
+    switch (dtype_id) {
+        case SCA_DTYPE_F32: typed(static_cast<float*>(nullptr)); break;
+        case SCA_DTYPE_F16: typed(static_cast<__half*>(nullptr)); break;
+        case SCA_DTYPE_BF16: typed(static_cast<__nv_bfloat16*>(nullptr)); break;
+        default: return Fail(SCA_INVALID_ARGUMENT, "kv gather (fp8): unsupported dtype id");
+    }
+    return CheckLaunch("kv_gather_fp8_kernel", s);
+}

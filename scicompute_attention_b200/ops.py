@@ -18,6 +18,7 @@ import math
 import struct
 import threading
 import warnings
+from typing import NamedTuple
 
 import torch
 
@@ -186,6 +187,7 @@ def acquire_scratch_fp32(elements: int, device: torch.device, kind: int = 1, *, 
 
 
 DECODE_STEP_TOKENS = 64  # tokens one CTA of the decode kernel consumes per step (4 warps x 16)
+FP8_STEP_TOKENS = 128    # the same over an 8-bit cache (4 warps x 32)
 
 
 def slots_for_schedule(column_steps: int, longest_steps: int, columns: int, sms: int) -> int:
@@ -210,13 +212,14 @@ def splits_for(seq_kv: int, batch: int, num_kv_heads: int, group: int, sms: int)
     return slots_for_schedule(max(1, batch) * steps, steps, num_kv_heads * ((group + 15) // 16), sms)
 
 
-def paged_splits_for(typical_len: int, num_seqs: int, num_kv_heads: int, group: int, sms: int, longest_len: int = 0) -> int:
+def paged_splits_for(typical_len: int, num_seqs: int, num_kv_heads: int, group: int, sms: int, longest_len: int = 0,
+                     step_tokens: int = DECODE_STEP_TOKENS) -> int:
     """Slot count for a ragged batch of mean length `typical_len`; the longest sequence is taken as twice the mean
     unless `longest_len` says otherwise."""
     if typical_len <= 0:
         return 1
-    steps = -(-typical_len // DECODE_STEP_TOKENS)
-    longest = -(-longest_len // DECODE_STEP_TOKENS) if longest_len > 0 else 2 * steps
+    steps = -(-typical_len // step_tokens)
+    longest = -(-longest_len // step_tokens) if longest_len > 0 else 2 * steps
     return slots_for_schedule(max(1, num_seqs) * steps, longest, num_kv_heads * ((group + 15) // 16), sms)
 
 
@@ -679,3 +682,182 @@ def kv_gather(layer, block_ids, *, stream=None) -> torch.Tensor:
                                      out.data_ptr(), C.byref(shape), layer.element_size(),
                                      _stream_ptr(stream)))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit KV cache
+# ------------------------------------------------------------------------------------------------
+class Fp8Pool(NamedTuple):
+    """K or V of one layer in 8 bits. A row - one token of one kv head - is D codes of type e4m3 and one scale 2^e with e in [-14, 7], the
+    smallest one with min(max |x|, 57344) <= 448 * 2^e; value = code * 2^e, exact in fp16 and bf16. Numbers beyond +-57344 (bf16, fp32)
+    are kept as +-57344, NaN stays NaN.
+
+    codes   float8_e4m3fn (or uint8) [num_blocks, block_size, H_kv, D], D a multiple of 16 up to 256
+    scales  uint8 [num_blocks, H_kv, block_size rounded up to 16]: e + 15
+
+    The operators take any pair of such tensors. Blocks are freed by kv_reset on the codes: a code of 0 is 0 under every scale."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def fp8_scale_row(block_size: int) -> int:
+    """Bytes of scales per block and kv head."""
+    return -(-block_size // 16) * 16
+
+
+def fp8_pool(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, *, device="cuda") -> Fp8Pool:
+    """An empty pool: every value 0."""
+    return Fp8Pool(torch.zeros((num_blocks, block_size, num_kv_heads, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                   torch.full((num_blocks, num_kv_heads, fp8_scale_row(block_size)), 15, dtype=torch.uint8, device=device))
+
+
+def _require_one_device(first: torch.Tensor, *others: torch.Tensor) -> None:
+    for t in others:
+        if t.device != first.device:
+            raise _lib.ScaError(4, f"tensors on {first.device} and {t.device}: a call's tensors are on one device")
+
+
+def _require_fp8_pool(pool) -> None:
+    codes, scales = pool
+    _require_cuda(codes, scales)
+    if codes.dim() != 4 or codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or not codes.is_contiguous():
+        raise _lib.ScaError(4, f"codes must be contiguous float8_e4m3fn [num_blocks, block_size, H_kv, D]; got {codes.dtype}{list(codes.shape)}")
+    nblk, bs, hkv, _ = codes.shape
+    if scales.dtype != torch.uint8 or tuple(scales.shape) != (nblk, hkv, fp8_scale_row(bs)) or not scales.is_contiguous():
+        raise _lib.ScaError(4, f"scales must be contiguous uint8 {[nblk, hkv, fp8_scale_row(bs)]}; got {scales.dtype}{list(scales.shape)}")
+
+
+def _require_fp8_pools(layer_k, layer_v) -> None:
+    _require_fp8_pool(layer_k)
+    _require_fp8_pool(layer_v)
+    if layer_k[0].shape != layer_v[0].shape:
+        raise _lib.ScaError(4, "pool geometry mismatch")
+
+
+def _require_fp8_rows(codes, rows: int, k_new, v_new) -> None:
+    _require_cuda(k_new, v_new)
+    if k_new.dtype != v_new.dtype:
+        raise _lib.ScaError(4, "k_new/v_new shape or dtype mismatch")
+    width = codes.shape[2] * codes.shape[3]
+    for t in (k_new, v_new):
+        if not t.is_contiguous() or t.dim() < 1 or t.shape[0] < rows or t.numel() != t.shape[0] * width:
+            raise _lib.ScaError(4, f"new K / V must be contiguous [{rows}, {codes.shape[2]}, {codes.shape[3]}]; got {t.dtype}{list(t.shape)}")
+
+
+def _fp8_layer(layer_k, layer_v):
+    return _lib.Fp8Layer(layer_k[0].data_ptr(), layer_v[0].data_ptr(), layer_k[1].data_ptr(), layer_v[1].data_ptr())
+
+
+def _elsewhere(t: torch.Tensor, stream) -> bool:
+    """Whether a launch without a stream of its own has to make the tensors' device the current one."""
+    return stream is None and t.device.index != torch.cuda.current_device()
+
+
+def kv_append_fp8(layer_k, layer_v, k_new, v_new, slot_mapping, *, stream=None) -> None:
+    """kv_append into an 8-bit layer (two Fp8Pool): k_new/v_new [num_tokens, H_kv, D] of float32, float16 or bfloat16 are quantised as they
+    are written; slot_mapping int32 [num_tokens] on the device, slots < 0 or beyond the pool are skipped. The slots of a call are distinct:
+    one that is named twice is left with pieces of both rows."""
+    _require_fp8_pools(layer_k, layer_v)
+    _require_fp8_rows(layer_k[0], k_new.shape[0], k_new, v_new)
+    _require_ints("slot_mapping", slot_mapping, k_new.shape[0])
+    _require_one_device(k_new, v_new, slot_mapping, *layer_k, *layer_v)
+    if k_new.shape[0] == 0:
+        return
+    if _elsewhere(k_new, stream):
+        with torch.cuda.device(k_new.device):
+            return kv_append_fp8(layer_k, layer_v, k_new, v_new, slot_mapping)
+    shape = _kv_shape(layer_k[0])
+    check(lib().sca_launch_kv_append_fp8(C.byref(_fp8_layer(layer_k, layer_v)), k_new.data_ptr(), v_new.data_ptr(), slot_mapping.data_ptr(),
+                                         k_new.shape[0], C.byref(shape), dtype_id(k_new.dtype), _stream_ptr(stream)))
+
+
+def kv_append_batched_fp8(layer_k, layer_v, k_new, v_new, page_table, seq_lens, *, stream=None) -> None:
+    """kv_append_batched into an 8-bit layer: one new token per sequence, at position seq_lens[s] - 1 of its pages."""
+    _require_fp8_pools(layer_k, layer_v)
+    _require_fp8_rows(layer_k[0], k_new.shape[0], k_new, v_new)
+    _require_cuda(page_table)
+    _require_table(page_table, k_new.shape[0])
+    _require_ints("seq_lens", seq_lens, k_new.shape[0])
+    _require_one_device(k_new, v_new, page_table, seq_lens, *layer_k, *layer_v)
+    if k_new.shape[0] == 0:
+        return
+    if _elsewhere(k_new, stream):
+        with torch.cuda.device(k_new.device):
+            return kv_append_batched_fp8(layer_k, layer_v, k_new, v_new, page_table, seq_lens)
+    shape = _kv_shape(layer_k[0])
+    check(lib().sca_launch_kv_append_batched_fp8(C.byref(_fp8_layer(layer_k, layer_v)), k_new.data_ptr(), v_new.data_ptr(), page_table.data_ptr(),
+                                                 seq_lens.data_ptr(), k_new.shape[0], page_table.shape[1], C.byref(shape),
+                                                 dtype_id(k_new.dtype), _stream_ptr(stream)))
+
+
+def kv_gather_fp8(layer, block_ids, dtype, *, stream=None) -> torch.Tensor:
+    """Reads blocks of an 8-bit pool back: [len(block_ids), block_size, H_kv, D] of `dtype` (float32, float16 or bfloat16). Ids outside the
+    pool read as zeros."""
+    _require_fp8_pool(layer)
+    _require_ints("block_ids", block_ids, 0)
+    codes, scales = layer
+    _require_one_device(codes, scales, block_ids)
+    kind = dtype_id(dtype)
+    if _elsewhere(codes, stream):
+        with torch.cuda.device(codes.device):
+            return kv_gather_fp8(layer, block_ids, dtype)
+    shape = _kv_shape(codes)
+    out = _empty((block_ids.numel(),) + tuple(codes.shape[1:]), dtype, codes.device, stream)
+    if out.numel() > 0:
+        check(lib().sca_launch_kv_gather_fp8(codes.data_ptr(), scales.data_ptr(), block_ids.data_ptr(), block_ids.numel(), out.data_ptr(),
+                                             C.byref(shape), kind, _stream_ptr(stream)))
+    return out
+
+
+def paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, *, block_size: int, scale=None, typical_len: int = 0, longest_len: int = 0,
+                        stream=None, return_stats: bool = False):
+    """paged_attention over an 8-bit cache: q [num_seqs, H_q, 1, D] of float16 or bfloat16, pools as Fp8Pool with a block_size that is a
+    multiple of 4; table, lengths and hints as there. The new tokens' K / V are in the cache (kv_append_batched_fp8)."""
+    _require_cuda(q, page_table, seq_lens)
+    _require_fp8_pools(k_pool, v_pool)
+    if q.dim() != 4:
+        raise _lib.ScaError(4, f"paged_attention expects q=[num_seqs, H_q, seq_q, D]; got ndims={q.dim()}")
+    s, hq, sq, d = q.shape
+    if sq != 1:
+        raise _lib.ScaError(5, f"paged attention implements the decode form only (seq_q=1); got seq_q={sq}")
+    codes = k_pool[0]
+    nblk, bs, hkv, dk = codes.shape
+    if bs != block_size or dk != d:
+        raise _lib.ScaError(4, "pool geometry mismatch")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise _lib.ScaError(4, f"attention over an 8-bit cache takes float16 or bfloat16 queries; got {q.dtype}")
+    if hkv < 1 or hq % hkv != 0:
+        raise _lib.ScaError(4, f"num_heads={hq} % num_kv_heads={hkv} != 0")
+    _require_packed("q", q)
+    _require_table(page_table, s)
+    if seq_lens is not None:
+        _require_ints("seq_lens", seq_lens, s)
+    _require_one_device(q, page_table, *k_pool, *v_pool, *(() if seq_lens is None else (seq_lens,)))
+    if _elsewhere(q, stream):
+        with torch.cuda.device(q.device):
+            return paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, block_size=block_size, scale=scale, typical_len=typical_len,
+                                       longest_len=longest_len, return_stats=return_stats)
+    max_blocks, upper = page_table.shape[1], nblk * bs
+    device, handle = q.device, _stream_ptr(stream)
+    splits = paged_splits_for(typical_len if typical_len > 0 else min(upper, max_blocks * bs), s, hkv, hq // hkv, sm_count(device), longest_len,
+                              FP8_STEP_TOKENS)
+    base = s * hq * splits
+    ws = acquire_scratch_fp32(base * (2 + d), device, stream=stream, handle=handle)
+    out = _empty((s, hq, 1, d), q.dtype, device, stream)
+    p = DecodeFwdParams()
+    p.q, p.k, p.v, p.out = q.data_ptr(), codes.data_ptr(), v_pool[0].data_ptr(), out.data_ptr()
+    scratch = ws.data_ptr()
+    p.partial_m, p.partial_l, p.partial_o = scratch, scratch + 4 * base, scratch + 8 * base
+    p.batch, p.num_heads, p.num_kv_heads, p.seq_kv, p.head_dim, p.num_splits = s, hq, hkv, upper, d, splits
+    p.q_stride = DecodeStrides(hq * d, d, d)
+    p.o_stride = DecodeStrides(hq * d, d, d)
+    p.scale = effective_scale(scale, d)
+    p.dtype = dtype_id(q.dtype)
+    p.seq_lens = seq_lens.data_ptr() if seq_lens is not None else None
+    p.page_table = page_table.data_ptr()
+    p.block_size, p.max_blocks_per_seq, p.num_kv_blocks = bs, max_blocks, nblk
+    cluster = C.c_int32(0)
+    check(lib().sca_launch_paged_attention_fp8(C.byref(p), k_pool[1].data_ptr(), v_pool[1].data_ptr(), C.byref(cluster), handle))
+    if not return_stats:
+        return out
+    return out, {"num_splits": cluster.value or splits, "cluster": cluster.value, "workspace_bytes": base * (2 + d) * 4}
