@@ -407,6 +407,10 @@ SCA_ABI int sca_launch_kv_gather_fp8(const void* codes, const uint8_t* scales, c
  * those of the pool and are not read; q and out are fp16 or bf16, block_size a multiple of 4. `cluster_ctas` may be null. */
 SCA_ABI int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, const uint8_t* k_scales,
                                            const uint8_t* v_scales, int32_t* cluster_ctas, void* stream);
+/* sca_launch_flash_paged over an 8-bit paged cache: params->k_pool / v_pool are the codes, scales 16-byte aligned, q and out are fp16 or
+ * bf16. What lies behind a sequence's last token counts for nothing, whatever it is. */
+SCA_ABI int sca_launch_flash_paged_fp8(const ScaFlashPagedParams* params, const uint8_t* k_scales,
+                                       const uint8_t* v_scales, void* stream);
 
 #ifdef __cplusplus
 }

@@ -27,6 +27,7 @@ EXPORTED_SYMBOLS = [
     "sca_peer_buffer_destroy", "sca_peer_exchange_status", "sca_peer_exchange_clear", "sca_launch_seqsplit_exchange",
     "sca_flash_varlen_workspace_bytes", "sca_launch_flash_varlen", "sca_launch_flash_paged",
     "sca_launch_kv_append_fp8", "sca_launch_kv_append_batched_fp8", "sca_launch_kv_gather_fp8", "sca_launch_paged_attention_fp8",
+    "sca_launch_flash_paged_fp8",
     "sca_mgpu_unique_id", "sca_mgpu_init", "sca_mgpu_allgather_triples", "sca_mgpu_abort", "sca_mgpu_destroy",
 ]
 
@@ -172,6 +173,7 @@ def lib() -> C.CDLL:
                                                                                             C.c_int32, C.c_void_p]
     l.sca_launch_kv_gather_fp8.argtypes = [C.c_void_p] * 3 + [C.c_int64, C.c_void_p, C.POINTER(KvCacheShape), C.c_int32, C.c_void_p]
     l.sca_launch_paged_attention_fp8.argtypes = [C.POINTER(DecodeFwdParams), C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.c_void_p]
+    l.sca_launch_flash_paged_fp8.argtypes = [C.POINTER(FlashPagedParams), C.c_void_p, C.c_void_p, C.c_void_p]
     l.sca_mgpu_unique_id.argtypes = [C.c_char_p]
     l.sca_mgpu_init.argtypes = [C.c_char_p, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]
     l.sca_mgpu_allgather_triples.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32]

@@ -1,0 +1,40 @@
+// Chunks of new tokens over a paged cache of 8 bits: the prefill kernels whose converters rewrite codes of K and V as fp16 (kKv8 in
+// flash_kernel.cuh).
+#include "flash_kernel.cuh"
+
+namespace sca_b200 {
+namespace flash {
+namespace {
+
+template <typename T, int DP, int QT, int BN, bool kSplit>
+int Launch(int64_t ctas, int cluster, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
+           const FlashKernelParams& p) {
+    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, true, true, kSplit, true>;
+    constexpr int kSmem = FlashGeom<DP, QT, BN, true>::kSmemBytes;
+    if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kSmem, "flash_fwd_sm100_kernel")) return rc;
+    LaunchDependent(kernel, ctas, FlashThreads<T, DP, QT, true>(), kSmem, stream, cluster, map_q, map_k, map_v, p);
+    return SCA_OK;
+}
+
+}  // namespace
+
+template <typename T, int DP, int QT, int BN>
+int LaunchKv8(int64_t items, unsigned grid, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
+              const FlashKernelParams& p) {
+    if (p.cluster > 1) return Launch<T, DP, QT, BN, true>(items * p.cluster, p.cluster, stream, map_q, map_k, map_v, p);
+    return Launch<T, DP, QT, BN, false>(grid, 1, stream, map_q, map_k, map_v, p);
+}
+
+#define SCA_KV8(T, DP, QT)                                                                                                          \
+    template int LaunchKv8<T, DP, QT, 128>(int64_t, unsigned, cudaStream_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, \
+                                           const FlashKernelParams&);
+SCA_KV8(__half, 64, 2)
+SCA_KV8(__half, 128, 2)
+SCA_KV8(__half, 256, 1)
+SCA_KV8(__nv_bfloat16, 64, 2)
+SCA_KV8(__nv_bfloat16, 128, 2)
+SCA_KV8(__nv_bfloat16, 256, 1)
+#undef SCA_KV8
+
+}  // namespace flash
+}  // namespace sca_b200

@@ -58,6 +58,25 @@ int MakeMap(CUtensorMap* map, const void* base, int dtype_id, int64_t d, int64_t
     return SCA_OK;
 }
 
+// The codes of a layer of an 8-bit cache, [rows = num_blocks * block_size][kv_heads][D]: box = `width` codes of one page of one kv head,
+// rows of `width` bytes one behind the other (no swizzle), what lies beyond D or the pool reads as zero.
+int MakeCodesMap(CUtensorMap* map, const void* base, int64_t d, int64_t rows, int64_t heads, int box_rows, int width, const char* what) {
+    EncodeTiledFn encode = GetEncodeTiled();
+    if (encode == nullptr) return Fail(SCA_CUDA_ERROR, "flash attention: cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads), 1};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(heads * d), static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows * heads * d)};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(width), static_cast<cuuint32_t>(box_rows), 1, 1};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) {
+        return Fail(SCA_INVALID_ARGUMENT, std::string("flash attention: tensor map for ") + what + " rejected (CUresult " +
+                                              std::to_string(static_cast<int>(rc)) + "); codes must be 16-byte aligned");
+    }
+    return SCA_OK;
+}
+
 // One host-visible word per device that a kernel sets when one of its bounded waits expires (1 + the warp that
 // gave up). The words live in one pinned, mapped, portable allocation; sca_flash_status reads and clears them.
 
@@ -211,6 +230,7 @@ int UploadVarlenWork(const VarlenWork& vw, int tokens_per_entry, int block_n, bo
 struct PagedWork {
     const int32_t* page_table;
     int64_t num_blocks, block_size, max_blocks_per_seq;
+    const uint8_t *k_scales, *v_scales;  // an 8-bit pool (kv_fp8.cuh); null: f.dtype_id
 };
 
 int CheckFlash(cudaStream_t stream) {
@@ -271,7 +291,12 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
     }
     if (int rc = MakeMap(&map_q, f.q, f.dtype_id, f.head_dim, f.num_heads, f.seq_q, f.batch, f.q_sh, f.q_ss, f.q_sb, 1 << pack_shift,
                          "q", kBlockM >> pack_shift)) return rc;
-    if (paged != nullptr) {
+    if (paged != nullptr && paged->k_scales != nullptr) {
+        const int64_t rows = paged->num_blocks * paged->block_size;
+        const int page = static_cast<int>(paged->block_size);
+        if (int rc = MakeCodesMap(&map_k, f.k, f.head_dim, rows, f.num_kv_heads, page, DP / G::kParts, "k codes")) return rc;
+        if (int rc = MakeCodesMap(&map_v, f.v, f.head_dim, rows, f.num_kv_heads, page, DP, "v codes")) return rc;
+    } else if (paged != nullptr) {
         // the pool as [rows = blocks * block_size, H_kv, D]; one box = one page of one kv head and column block
         const int64_t rows = paged->num_blocks * paged->block_size;
         const int64_t row_elems = f.num_kv_heads * f.head_dim;
@@ -330,6 +355,13 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
         p.block_size = static_cast<int>(paged->block_size);
         p.block_shift = 0;
         while ((1 << p.block_shift) < p.block_size) ++p.block_shift;
+        if (paged->k_scales != nullptr) {
+            p.k_scales = paged->k_scales;
+            p.v_scales = paged->v_scales;
+            p.scale_row = static_cast<int>(fp8::ScaleRow(paged->block_size));
+            if (int rc = LaunchKv8<T, DP, QT, BN>(ctas, grid, stream, map_q, map_k, map_v, p)) return rc;
+            return CheckFlash(stream);
+        }
         if (p.cluster > 1) {
             if (int rc = LaunchSplit<T, DP, QT, BN, true, true>(ctas, stream, map_q, map_k, map_v, p)) return rc;
             return CheckFlash(stream);
@@ -487,8 +519,10 @@ extern "C" int sca_launch_flash_varlen(const ScaFlashVarlenParams* params, void*
     return Fail(SCA_CUDA_ERROR, std::string("flash varlen: on the host: ") + e.what());
 }
 
-extern "C" int sca_launch_flash_paged(const ScaFlashPagedParams* params, void* stream) try {
-    ClearError();
+namespace {
+
+// Chunks over a paged cache; `k_scales` null: of f.dtype_id, else of 8 bits.
+int LaunchPaged(const ScaFlashPagedParams* params, const uint8_t* k_scales, const uint8_t* v_scales, void* stream) {
     if (params == nullptr || params->cu_seqlens_q == nullptr || params->seq_lens_kv == nullptr) {
         return Fail(SCA_INVALID_ARGUMENT, "flash paged: null parameter block or host lengths");
     }
@@ -543,7 +577,7 @@ extern "C" int sca_launch_flash_paged(const ScaFlashPagedParams* params, void* s
     if (int rc = ValidateFlash(&f)) return rc;
     VarlenWork vw{x.cu_seqlens_q, cu_kv.data(), x.num_seqs, x.workspace, x.workspace_bytes};
     if (int rc = CheckSequences(vw, f.causal != 0)) return rc;
-    PagedWork pw{x.page_table, x.num_blocks, x.block_size, x.max_blocks_per_seq};
+    PagedWork pw{x.page_table, x.num_blocks, x.block_size, x.max_blocks_per_seq, k_scales, v_scales};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (f.dtype_id) {
         case SCA_DTYPE_F16: return LaunchFlashTyped<__half>(f, s, &vw, &pw);
@@ -551,6 +585,22 @@ extern "C" int sca_launch_flash_paged(const ScaFlashPagedParams* params, void* s
         default: break;
     }
     return Fail(SCA_INVALID_ARGUMENT, "flash paged: unsupported dtype id");
+}
+
+}  // namespace
+
+extern "C" int sca_launch_flash_paged(const ScaFlashPagedParams* params, void* stream) try {
+    ClearError();
+    return LaunchPaged(params, nullptr, nullptr, stream);
 } catch (const std::exception& e) {  // host memory for the work list
     return Fail(SCA_CUDA_ERROR, std::string("flash paged: on the host: ") + e.what());
+}
+
+extern "C" int sca_launch_flash_paged_fp8(const ScaFlashPagedParams* params, const uint8_t* k_scales, const uint8_t* v_scales, void* stream) try {
+    ClearError();
+    if (k_scales == nullptr || v_scales == nullptr) return Fail(SCA_INVALID_ARGUMENT, "flash paged (fp8): null scales");
+    if (!Aligned16(k_scales) || !Aligned16(v_scales)) return Fail(SCA_INVALID_ARGUMENT, "flash paged (fp8): scales must be 16-byte aligned");
+    return LaunchPaged(params, k_scales, v_scales, stream);
+} catch (const std::exception& e) {  // host memory for the work list
+    return Fail(SCA_CUDA_ERROR, std::string("flash paged (fp8): on the host: ") + e.what());
 }

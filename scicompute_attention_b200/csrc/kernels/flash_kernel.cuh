@@ -38,6 +38,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "kv_fp8.cuh"
 #include "kv_ring.cuh"
 #include "sm100.cuh"
 
@@ -69,7 +70,8 @@ constexpr int kMaxSplit = 8;               // CTAs that share an item at most (t
 
 // DP: padded head dim (64 / 128 / 256); QT: query tiles per CTA; BN: keys per KV tile.
 // 64 and 128 run two query tiles; 256 needs 256 TMEM columns for O, so it runs one.
-template <int DP, int QT, int BN>
+// kKv8: K and V come from an 8-bit cache (kv_fp8.cuh).
+template <int DP, int QT, int BN, bool kKv8 = false>
 struct FlashGeom {
     static constexpr int kKBlocks = DP / 64;               // 64-element (128-byte) column blocks per row
     static constexpr int kQBlockBytes = kBlockM * 128;      // one column block of a query tile
@@ -81,9 +83,14 @@ struct FlashGeom {
     static constexpr int kVKeys = BN / kParts;              // keys of V in a slot
     static constexpr int kVBlockBytes = kVKeys * 128;       // one column block of V in a slot
     static constexpr int kSlotBytes = BN * DP * 2 / kParts;
-    static constexpr int kSlots = RingOf(DP).slots;
+    static constexpr int kSlots = kKv8 ? RawRingOf(DP).slots : RingOf(DP).slots;
+    // kKv8: a raw slot holds the codes of a load, key by key, and their scales: BN bytes, twice as many with pages of 8 keys
+    static constexpr int kRawSlots = kKv8 ? RawRingOf(DP).raw_slots : 0;
+    static constexpr int kRawCodes = kSlotBytes / 2;
+    static constexpr int kRawBytes = kRawCodes + 2 * BN;
+    static constexpr int kRingBytes = kSlots * kSlotBytes + kRawSlots * kRawBytes;
     static constexpr int kBarrierBytes = 512;
-    static constexpr int kSmemBytes = 1024 + QT * kQTileBytes + kSlots * kSlotBytes + kBarrierBytes;
+    static constexpr int kSmemBytes = 1024 + QT * kQTileBytes + kRingBytes + kBarrierBytes;
     static constexpr int kSCol = 0;                         // S_t at kSCol + t * BN
     static constexpr int kOCol = 256;                       // O_t at kOCol + t * DP
     // P_t has columns of its own wherever O leaves room for them: S_t(j+1) then goes out as soon as S_t(j) is in registers
@@ -125,6 +132,8 @@ struct FlashKernelParams {
     int max_blocks_per_seq, num_kv_blocks;
     int block_size, block_shift;  // block_size = 1 << block_shift
     int cluster;  // kSplit kernels: CTAs that share an item
+    const uint8_t *k_scales, *v_scales;  // kKv8 kernels: [num_kv_blocks][kv_heads][scale_row]
+    int scale_row;
 };
 
 // 16 elements of an output row: one 32-byte store where every row starts on a 32-byte boundary, else two of 16 bytes. A
@@ -155,16 +164,79 @@ __device__ __forceinline__ int TilesFor(int m0, int tokens, int seq_q, int seq_k
 
 // Warps that rewrite V as fp16. At D=256 a step has twice the bytes and its slots are the scarce thing: two warps 173 us,
 // three 172, four 146 (B=1, S=3000, lasting load). One warp is too few at D=128 (four prompts of 4096: 632 against 595).
-template <typename T, int DP>
+template <typename T, int DP, bool kKv8 = false>
 constexpr int ConverterWarps() {
-    return PvFormat<T>::kConvertV ? RingOf(DP).converters : 0;
+    return kKv8 || PvFormat<T>::kConvertV ? RingOf(DP).converters : 0;
 }
 // Warps of a CTA: 0 TMA and tensor-memory owner, 1 MMA, 2 and 3 V converters (idle for fp16), then four per query tile for
 // the softmax, then what converters are left.
 constexpr int kFirstSoftmax = 4;
-template <typename T, int DP, int QT>
+template <typename T, int DP, int QT, bool kKv8 = false>
 constexpr int FlashThreads() {
-    return 32 * (kFirstSoftmax + 4 * QT + (ConverterWarps<T, DP>() > 2 ? ConverterWarps<T, DP>() - 2 : 0));
+    return 32 * (kFirstSoftmax + 4 * QT + (ConverterWarps<T, DP, kKv8>() > 2 ? ConverterWarps<T, DP, kKv8>() - 2 : 0));
+}
+
+// kKv8, one converter warp: `kRows` rows of `kWidth` codes, a row behind the other at `codes`, become fp16 numbers in the layout of the
+// ring: column blocks of 64 numbers, `block_bytes` apart, rows of 128 bytes, 128-byte swizzle. Lane l holds the scale of row l in
+// scale[0] and of row 32 + l in scale[1] (pairs of fp16; 0: the row counts for nothing, whatever its codes). `row0`: the first row's
+// place in the tile, a multiple of 8. 8 codes per lane and turn: reads of 8 bytes and writes of 16 both touch every bank once.
+template <int kRows, int kWidth>
+__device__ __forceinline__ void ConvertRows(uint32_t codes, uint32_t slot, int row0, uint32_t block_bytes, const uint32_t (&scale)[2], int lane) {
+    constexpr int kPieces = kWidth / 8;              // of a row
+    constexpr int kRowsPerTurn = 32 / kPieces;
+    static_assert(kPieces == 8 || kPieces == 16 || kPieces == 32, "a turn covers whole rows");
+    static_assert(kRows <= 64, "two scales per lane");
+    const int piece = lane % kPieces, sub = lane / kPieces;
+    const uint32_t src = codes + row0 * kWidth + lane * 8;
+    const uint32_t dst = slot + (piece / 8) * block_bytes + (row0 + sub) * 128;
+    const bool whole = __all_sync(0xffffffffu, scale[0] != 0u && (kRows <= 32 || scale[1] != 0u));
+    auto turns = [&](auto all) {
+#pragma unroll
+        for (int i = 0; i < kRows / kRowsPerTurn; ++i) {
+            const int row = i * kRowsPerTurn;  // + sub
+            uint2 c;
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(src + row * kWidth));
+            const uint32_t unit = __shfl_sync(0xffffffffu, scale[row / 32], (row & 31) + sub);
+            if (!decltype(all)::value && unit == 0u) c = make_uint2(0u, 0u);
+            const uint32_t v0 = fp8::MulHalf2(fp8::DecodeLow(c.x), unit), v1 = fp8::MulHalf2(fp8::DecodeHigh(c.x), unit);
+            const uint32_t v2 = fp8::MulHalf2(fp8::DecodeLow(c.y), unit), v3 = fp8::MulHalf2(fp8::DecodeHigh(c.y), unit);
+            const uint32_t at = dst + (((piece % 8) ^ ((row & 7) | (kRowsPerTurn > 1 ? sub : 0))) << 4) + row * 128;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
+        }
+    };
+    if (whole) turns(std::true_type{});
+    else turns(std::false_type{});
+}
+
+// kKv8, bf16 queries: the row of a query tile that this thread looks after becomes fp16 numbers, times the power of two that puts the
+// row's largest number at 2^14: exact but for numbers below 2^-28 of it. Returns the power of two that undoes it.
+template <int DP>
+__device__ __forceinline__ float HalveQueryRow(uint32_t tile, int row) {
+    constexpr int kBlocks = DP / 64;
+    const uint32_t base = tile + row * 128;
+    const uint32_t turn = static_cast<uint32_t>(row & 7);
+    auto at = [&](int i) { return base + (i / 8) * (kBlockM * 128) + (((i % 8) ^ turn) << 4); };
+    uint32_t most = 0;  // two bf16 numbers without their signs compare as whole numbers do
+#pragma unroll
+    for (int i = 0; i < 8 * kBlocks; ++i) {
+        const uint4 v = LdsV4(at(i));
+        const uint32_t m01 = __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), m23 = __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu);
+        most = __vmaxu2(most, __vmaxu2(m01, m23));
+    }
+    const int k = max(static_cast<int>(max(most >> 16, most & 0xffffu) >> 7) - 127, -112);  // numbers below 2^-112 and zeros: 2^126
+    const float to_half = fp8::PowerOfTwo(14 - k);
+#pragma unroll
+    for (int i = 0; i < 8 * kBlocks; ++i) {
+        const uint4 v = LdsV4(at(i));
+        uint32_t h[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = UnpackBf16(h[e]);
+            h[e] = Pack2<__half>(f.x * to_half, f.y * to_half);
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(i)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+    }
+    return fp8::PowerOfTwo(max(k - 14, -126));
 }
 
 // kVarlen: the work list comes from the (sequence, query block) table of a packed ragged batch; otherwise it is
@@ -172,18 +244,21 @@ constexpr int FlashThreads() {
 // kPaged (only with kVarlen): K and V of a sequence are scattered over the pages of a KV pool.
 // kSplit: the CTAs of a cluster share one item of one query tile. Each takes a part of its KV tiles, and the parts are merged
 // through distributed shared memory at the end (SplitCluster says when).
-template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kSplit = false>
-__global__ void __launch_bounds__(FlashThreads<T, DP, QT>(), 1)
+// kKv8 (only with kPaged): the pages hold codes, which the converters rewrite as fp16; the products of the scores run in fp16 too, for bf16
+// queries after HalveQueryRow.
+template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kSplit = false, bool kKv8 = false>
+__global__ void __launch_bounds__(FlashThreads<T, DP, QT, kKv8>(), 1)
 flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p) {
-    using G = FlashGeom<DP, QT, BN>;
+    using G = FlashGeom<DP, QT, BN, kKv8>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem_base = (SmemAddr(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (smem_base - SmemAddr(smem_raw));
 
     const uint32_t q_smem = smem_base;
     const uint32_t ring_smem = smem_base + QT * G::kQTileBytes;
-    const uint32_t bar_base = ring_smem + G::kSlots * G::kSlotBytes;
+    const uint32_t raw_smem = ring_smem + G::kSlots * G::kSlotBytes;
+    const uint32_t bar_base = ring_smem + G::kRingBytes;
     auto bar = [&](int i) { return bar_base + 8u * i; };
     // Barriers. A wait names a phase by its parity, so it is sound where the role knows that the phase before is over and
     // that the one after cannot be. For all but o_done the role waits for every phase in turn, and the next one takes an
@@ -202,14 +277,19 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     constexpr int kPLast = kOFree + kTiles;         // [kTiles]
     constexpr int kVReady = kPLast + kTiles;        // [kSlots] bf16: V tile rewritten as fp16 in place
     constexpr int kSRead = kVReady + G::kSlots;     // [kTiles] kOwnP: scores in registers
-    constexpr int kNumBars = kSRead + kTiles;
+    constexpr int kRawFull = kSRead + kTiles;       // [kRawSlots] kKv8: codes and scales have landed
+    constexpr int kRawEmpty = kRawFull + G::kRawSlots;  // [kRawSlots] kKv8: the converters have read them
+    constexpr int kQHalf = kRawEmpty + G::kRawSlots;    // [kTiles] kKv8, bf16: the query tile is fp16
+    constexpr bool kHalveQ = kKv8 && std::is_same<T, __nv_bfloat16>::value;
+    constexpr int kNumBars = kQHalf + (kHalveQ ? kTiles : 0);
     auto full_bar = [&](bool is_v, uint32_t slot) { return bar(kKvFull + RingFullBarrier(is_v, static_cast<int>(slot), G::kSlots)); };
     using PT = typename PvFormat<T>::type;
-    constexpr bool kCvtInKernel = PvFormat<T>::kConvertV;
-    constexpr int kConverters = ConverterWarps<T, DP>();
+    constexpr bool kCvtInKernel = kKv8 || PvFormat<T>::kConvertV;
+    constexpr int kConverters = ConverterWarps<T, DP, kKv8>();
     // P is handed over in two pieces: the first kPEarly keys let P V start while the rest is still in the softmax
     constexpr int kPEarly = DP == 256 ? 64 : 96;
     static_assert(!kPaged || kVarlen, "paged K/V runs on the packed work list");
+    static_assert(!kKv8 || kPaged, "the 8-bit cache is paged");
     static_assert(kNumBars * 8 + 16 <= G::kBarrierBytes, "barrier area too small");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_base - smem_base) + kNumBars * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -315,6 +395,13 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             MbarInit<1>(bar(kKvEmpty + i));
             if constexpr (kCvtInKernel) MbarInit<32 * kConverters>(bar(kVReady + i));
         }
+        if constexpr (kKv8) {
+            for (int i = 0; i < G::kRawSlots; ++i) {
+                MbarInit<1>(bar(kRawFull + i));
+                MbarInit<kConverters>(bar(kRawEmpty + i));
+            }
+            for (int i = 0; kHalveQ && i < kTiles; ++i) MbarInit<4>(bar(kQHalf + i));
+        }
         *abort_flag = 0;
         FenceBarrierInit();
     }
@@ -332,7 +419,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     bool failed = false;
     // kSplit: a row of a CTA's part is {O[DP], m, l}, padded so that neighbouring rows lie on different banks
     constexpr int kPartLd = DP + 4;
-    static_assert(!kSplit || kBlockM * kPartLd * 4 <= G::kSlots * G::kSlotBytes, "a part has to fit the ring");
+    static_assert(!kSplit || kBlockM * kPartLd * 4 <= G::kRingBytes, "a part has to fit the ring");
 
     if (warp == 0 && kPaged) {
         // ================================ TMA producer, paged K/V ===================================
@@ -400,6 +487,38 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 const bool mapped = phys >= 0 && phys < p.num_kv_blocks;
                 const uint32_t valid = __ballot_sync(0xffffffffu, mapped);
+                if constexpr (kKv8) {
+                    const uint32_t raw = kv_loads % (kKv8 ? G::kRawSlots : 1);
+                    const int part8 = it % kParts;
+                    const int first_page = is_v ? part8 * pages_per_v : 0, pages = is_v ? pages_per_v : pages_per_tile;
+                    const uint32_t width = is_v ? DP : DP / kParts;  // codes of a key in this load
+                    const uint32_t wanted = (pages >= 32 ? 0xffffffffu : (1u << pages) - 1u) << first_page;
+                    const uint32_t full = bar(kRawFull + raw);
+                    if (lane == 0) {
+                        ok = MbarWait(bar(kRawEmpty + raw), ((kv_loads / (kKv8 ? G::kRawSlots : 1)) & 1u) ^ 1u, abort_flag);
+                        if (ok) {
+                            if (!is_v) valid_ring[(tiles_before + tile) % kValidRing] = valid;
+                            MbarExpectTx(full, G::kRawCodes + __popc(valid & wanted) * p.scale_row);
+                        }
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                    if (!ok) break;
+                    uint32_t dst = raw_smem + raw * G::kRawBytes;
+                    uint32_t scale_dst = dst + G::kRawCodes;
+                    const uint8_t* scales = is_v ? p.v_scales : p.k_scales;
+                    for (int pg = first_page; pg < first_page + pages; ++pg) {
+                        const int32_t id = __shfl_sync(0xffffffffu, phys, pg);
+                        const bool there = (valid >> pg) & 1u;
+                        if (ElectOne()) {
+                            TmaLoad4D(dst, is_v ? &map_v : &map_k, full, is_v ? 0 : part8 * static_cast<int>(width),
+                                      there ? (id << p.block_shift) : (p.num_kv_blocks << p.block_shift), w.h_kv, 0);
+                            if (there) BulkLoad(scale_dst, scales + (static_cast<int64_t>(id) * p.kv_heads + w.h_kv) * p.scale_row, p.scale_row, full);
+                        }
+                        dst += width << p.block_shift;
+                        scale_dst += p.scale_row;
+                    }
+                    continue;
+                }
                 const uint32_t slot = kv_loads % G::kSlots;
                 const uint32_t phase = (kv_loads / G::kSlots) & 1u;
                 if (lane == 0) {
@@ -490,7 +609,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else if (warp == 1) {
         // ================================ MMA issuer ================================================
         if (ElectOne()) {
-            constexpr uint32_t fmt = std::is_same<T, __half>::value ? kFmtF16 : kFmtBf16;
+            constexpr uint32_t fmt = kKv8 || std::is_same<T, __half>::value ? kFmtF16 : kFmtBf16;
             constexpr uint32_t idesc_s = MakeInstrDesc(fmt, fmt, 0, 0, kBlockM, BN);  // Q K^T: both K-major
             // P V: V is MN-major; both operands in the P V format (fp16 also for bf16 inputs, see PvFormat)
             constexpr uint32_t fmt_pv = PvFormat<T>::kConvertV ? kFmtF16 : fmt;
@@ -540,7 +659,11 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             uint32_t kv_base = 0;           // ring position of this item's K_0
             RingPhases k_phases, v_phases;  // of the K barriers and of v_ready (no converter: the V barriers)
             bool ok = true;
-            auto k_landed = [&](uint32_t slot) { return MbarWait(full_bar(false, slot), k_phases.Take(slot), abort_flag); };
+            auto q_landed = [&](int t, uint32_t parity) { return MbarWait(bar((kHalveQ ? kQHalf : kQFull) + t), parity, abort_flag); };
+            auto k_landed = [&](uint32_t slot) {
+                if constexpr (kKv8) return MbarWait(bar(kVReady + slot), v_phases.Take(slot), abort_flag);  // K and V in turn, one barrier
+                return MbarWait(full_bar(false, slot), k_phases.Take(slot), abort_flag);
+            };
             auto v_ready = [&](uint32_t slot) {
                 return MbarWait(kCvtInKernel ? bar(kVReady + slot) : full_bar(true, slot), v_phases.Take(slot), abort_flag);
             };
@@ -578,7 +701,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
                     for (int t = 0; t < QT; ++t) {
                         if (!ok) break;
-                        if (w.ntiles[t] > 0) ok = MbarWait(bar(kQFull + t), q_uses[t] & 1u, abort_flag);
+                        if (w.ntiles[t] > 0) ok = q_landed(t, q_uses[t] & 1u);
                         ok = ok && score_step(t, k, w.ntiles[t] > 0, t == 0, w.ntiles[t] == 1);
                     }
                     for (int j = 0; j < n && ok; ++j) {
@@ -621,7 +744,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const Item w = decode_item(idx);
                 auto slot_of = [&](int it) { return (kv_base + it) % G::kSlots; };
                 for (int t = 0; t < QT && ok; ++t) {
-                    if (w.ntiles[t] > 0) ok = MbarWait(bar(kQFull + t), q_uses[t] & 1u, abort_flag);
+                    if (w.ntiles[t] > 0) ok = q_landed(t, q_uses[t] & 1u);
                 }
                 if (ok && w.n_max > 0) {
                     ok = k_landed(slot_of(0));
@@ -671,10 +794,12 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             failed = !ok;
         }
     } else if (converter >= 0 && converter < kConverters) {
-        // ================================ V converter (bf16) ========================================
+        // ================================ V converter (bf16), K and V converter (kKv8) ==============
         // Walks the ring in the producer's order; every V tile is rewritten in place from bf16 to fp16 once its
-        // bytes have landed, then handed to the MMA thread through v_ready. K tiles are not touched.
+        // bytes have landed, then handed to the MMA thread through v_ready. K tiles are not touched. kKv8: the codes
+        // of K and V go from their raw slot into a slot of the ring.
         uint32_t kv_loads = 0;
+        uint32_t tiles_before = 0;  // kKv8: index into valid_ring
         RingPhases v_phases;
         bool ok = true;
         for (int r = 0; r < rounds && ok; ++r) {
@@ -682,8 +807,43 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (idx < 0) continue;
             const Item w = decode_item(idx);
             for (int it = 0; it < 2 * w.n_max * kParts && ok; ++it, ++kv_loads) {
-                if (!RingOrder(it / kParts, w.n_max, kOwnP).is_v) continue;
+                const RingLoad load = RingOrder(it / kParts, w.n_max, kOwnP);
+                if (!kKv8 && !load.is_v) continue;
                 const uint32_t slot = kv_loads % G::kSlots;
+                if constexpr (kKv8) {
+                    const uint32_t raw = kv_loads % (kKv8 ? G::kRawSlots : 1);
+                    ok = __all_sync(0xffffffffu, MbarWait(bar(kRawFull + raw), (kv_loads / (kKv8 ? G::kRawSlots : 1)) & 1u, abort_flag) &&
+                                                     MbarWait(bar(kKvEmpty + slot), ((kv_loads / G::kSlots) & 1u) ^ 1u, abort_flag));
+                    if (!ok) break;
+                    const uint32_t codes = raw_smem + raw * G::kRawBytes, target = ring_smem + slot * G::kSlotBytes;
+                    const uint32_t pages = valid_ring[(tiles_before + load.tile) % kValidRing];
+                    const int key0 = ((kSplit ? w.first_tile : 0) + load.tile) * BN;
+                    const int part = it % kParts;
+                    auto convert = [&](auto rows_of_load, auto width, int tile_row0, uint32_t block_bytes) {
+                        constexpr int kRows = decltype(rows_of_load)::value / kConverters;  // of this warp
+                        const int row0 = converter * kRows;
+                        uint32_t scale[2] = {0u, 0u};
+#pragma unroll
+                        for (int i = 0; i < (kRows + 31) / 32; ++i) {
+                            const int row = row0 + 32 * i + (lane & (kRows < 32 ? kRows - 1 : 31)), tile_row = tile_row0 + row;
+                            const bool there = ((pages >> (tile_row >> p.block_shift)) & 1u) && key0 + tile_row < w.seq_kv;
+                            uint32_t byte;
+                            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(codes + G::kRawCodes + (row >> p.block_shift) * p.scale_row + (row & (p.block_size - 1))));
+                            scale[i] = there ? fp8::ScalePair(byte, byte) : 0u;
+                        }
+                        ConvertRows<kRows, decltype(width)::value>(codes, target, row0, block_bytes, scale, lane);
+                    };
+                    if (load.is_v) {
+                        convert(std::integral_constant<int, G::kVKeys>{}, std::integral_constant<int, DP>{}, part * G::kVKeys, G::kVBlockBytes);
+                    } else {
+                        convert(std::integral_constant<int, BN>{}, std::integral_constant<int, DP / kParts>{}, 0, G::kKBlockBytes);
+                    }
+                    FenceProxyAsync();  // generic-proxy writes -> visible to the tensor core's reads
+                    MbarArrive(bar(kVReady + slot));
+                    __syncwarp();
+                    if (lane == 0) MbarArrive(bar(kRawEmpty + raw));
+                    continue;
+                }
                 ok = __all_sync(0xffffffffu, MbarWait(full_bar(true, slot), v_phases.Take(slot), abort_flag));
                 if (!ok) break;
                 uint4* tile = reinterpret_cast<uint4*>(smem + (ring_smem - smem_base) + slot * G::kSlotBytes);
@@ -702,6 +862,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 FenceProxyAsync();  // generic-proxy writes -> visible to the tensor core's reads
                 MbarArrive(bar(kVReady + slot));
             }
+            tiles_before += static_cast<uint32_t>(w.n_max);
         }
         failed = !ok;
     } else if (warp >= kFirstSoftmax && warp < kEndSoftmax) {
@@ -714,6 +875,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const uint32_t p_addr = tmem_base + lane_bits + G::kPCol + t * G::kPStride;
         const uint32_t o_addr = tmem_base + lane_bits + G::kOCol + t * DP;
         uint32_t steps = 0;  // KV tiles this group has processed (phase of s_full / p_full / o_done)
+        uint32_t items = 0;  // kHalveQ: query tiles it has rewritten (phase of q_full)
         uint32_t tiles_before = 0;  // paged K/V: KV tiles of the items this CTA has finished (index into valid_ring)
         float* part_row = reinterpret_cast<float*>(smem + (ring_smem - smem_base)) + row_in_tile * kPartLd;  // kSplit
         const uint32_t all_pages = kPaged ? ((BN >> p.block_shift) >= 32 ? 0xffffffffu : (1u << (BN >> p.block_shift)) - 1u) : 0u;
@@ -736,6 +898,17 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             const int row = m_t + (row_in_tile >> p.pack_shift);                 // token of the sequence
             const int head = w.h + (row_in_tile & ((1 << p.pack_shift) - 1));
+            float scale_log2 = p.scale_log2;
+            if constexpr (kHalveQ) {
+                ok = __all_sync(0xffffffffu, MbarWait(bar(kQFull + t), items & 1u, abort_flag));
+                if (!ok) break;
+                ++items;
+                // not 0, which would make NaN of the -inf of masked columns: scores of tiny rows under a tiny scale are 0 either way
+                scale_log2 = fmaxf(scale_log2 * HalveQueryRow<DP>(q_smem + t * G::kQTileBytes, row_in_tile), fp8::PowerOfTwo(-126));
+                FenceProxyAsync();
+                __syncwarp();
+                if (lane == 0) MbarArrive(bar(kQHalf + t));
+            }
             float m_ref = -CUDART_INF_F;  // reference point of the exponentials (log2 domain)
             float l_sum = 0.0f;
 
@@ -801,7 +974,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                             mx4[e] = Max3(mx4[e], __uint_as_float(sc[i / 32][i % 32 + e]), __uint_as_float(sc[i / 32][i % 32 + 4 + e]));
                         }
                     }
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;  // scale > 0
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;  // scale > 0
                     const bool move = mx > m_ref + kRescaleThreshold;  // false for a fully masked row (-inf)
                     if (__any_sync(0xffffffffu, move)) {
                         const float alpha = move ? Exp2(m_ref - mx) : 1.0f;  // m_ref = -inf -> 0
@@ -829,7 +1002,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // the products half of the time, gains 2 % (528 against 535 us at B=4, S=4096); D=64, where they mostly
                 // run side by side, loses 10 % (359 against 322 us at B=3, S=2900).
                 constexpr bool kBehind = DP != 64;
-                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+                const float2 scale2 = make_float2(scale_log2, scale_log2);
                 float2 sum[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] = make_float2(0.0f, 0.0f);
@@ -990,7 +1163,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         __syncthreads();
 #pragma unroll 4
-        for (int item = threadIdx.x; item < rows * (DP / 4); item += FlashThreads<T, DP, QT>()) {
+        for (int item = threadIdx.x; item < rows * (DP / 4); item += FlashThreads<T, DP, QT, kKv8>()) {
             const int i = item / (DP / 4), d = item % (DP / 4) * 4;
             int token, head;
             if (!out_row(row0 + i, &token, &head) || d >= p.head_dim) continue;
@@ -1014,6 +1187,10 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged>
 int LaunchSplit(int64_t items, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
                 const FlashKernelParams& p);
+// The kernels over an 8-bit cache are compiled in flash_fp8.cu; p.cluster > 1: the CTAs of a cluster share an item.
+template <typename T, int DP, int QT, int BN>
+int LaunchKv8(int64_t items, unsigned grid, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
+              const FlashKernelParams& p);
 // Clusters of `cluster` CTAs that run at the same time (0 when the device cannot say).
 template <typename T, int DP, int QT, int BN>
 int ResidentClusters(int cluster);

@@ -24,6 +24,17 @@ constexpr RingShape RingOf(int padded_dim) {
     return padded_dim == 64 ? RingShape{8, true, 1, 2} : padded_dim == 128 ? RingShape{5, false, 1, 2} : RingShape{5, true, 2, 4};
 }
 
+// The ring where K and V come from an 8-bit cache: codes land in raw slots of half the size, the converters rewrite each load as fp16
+// into a slot of the ring, K like V. Raw slots and slots are taken in the order of the loads, each with a full and an empty barrier:
+// the loads fill raw slots and the converters slots, so that every barrier has one kind of producer and whoever waits sees each phase.
+struct RawRingShape {
+    int slots;
+    int raw_slots;
+};
+constexpr RawRingShape RawRingOf(int padded_dim) {
+    return padded_dim == 64 ? RawRingShape{6, 6} : RawRingShape{3, 4};
+}
+
 struct RingLoad {
     bool is_v;
     int tile;

@@ -103,6 +103,13 @@ __device__ __forceinline__ void TmaLoad4D(uint32_t smem_dst, const CUtensorMap* 
         : "memory");
 }
 
+// `bytes` of global memory to shared memory of this CTA, counted on `bar`; both addresses and the size are multiples of 16.
+__device__ __forceinline__ void BulkLoad(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 // ---- tensor memory -----------------------------------------------------------------------------------
 __device__ __forceinline__ void TmemAlloc(uint32_t smem_result, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_result), "r"(columns)

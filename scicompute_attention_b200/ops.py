@@ -861,3 +861,44 @@ def paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, *, block_size: 
     if not return_stats:
         return out
     return out, {"num_splits": cluster.value or splits, "cluster": cluster.value, "workspace_bytes": base * (2 + d) * 4}
+
+
+def flash_attention_paged_fp8(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_kv, *, causal=True, scale=None, stream=None):
+    """flash_attention_paged over an 8-bit cache: q packed [T_q, H_q, D] of float16 or bfloat16, pools as Fp8Pool; the rest as there. The
+    new tokens' K / V are in the cache (kv_append_fp8)."""
+    import numpy as np
+    _require_cuda(q, page_table)
+    _require_fp8_pools(k_pool, v_pool)
+    codes = k_pool[0]
+    if q.dim() != 3 or not q.is_contiguous():
+        raise _lib.ScaError(4, "paged prefill expects packed q [T, H, D]")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise _lib.ScaError(4, f"attention over an 8-bit cache takes float16 or bfloat16 queries; got {q.dtype}")
+    cu_q = np.ascontiguousarray(cu_seqlens_q, dtype=np.int32)
+    lens = np.ascontiguousarray(seq_lens_kv, dtype=np.int32)
+    if lens.ndim != 1 or cu_q.ndim != 1 or cu_q.shape[0] != lens.shape[0] + 1:
+        raise _lib.ScaError(4, "cu_seqlens_q needs num_seqs + 1 entries, seq_lens_kv and the page table num_seqs")
+    n = lens.shape[0]
+    _require_table(page_table, n)
+    tq, hq, d = q.shape
+    nblk, bs, hkv, dk = codes.shape
+    if dk != d:
+        raise _lib.ScaError(4, "pool head_dim differs from q")
+    _require_one_device(q, page_table, *k_pool, *v_pool)
+    if _elsewhere(q, stream):
+        with torch.cuda.device(q.device):
+            return flash_attention_paged_fp8(q, k_pool, v_pool, page_table, cu_q, lens, causal=causal, scale=scale)
+    out = _empty(q.shape, q.dtype, q.device, stream)
+    ws_bytes = lib().sca_flash_varlen_workspace_bytes(n, tq)
+    ws = _empty(max(int(ws_bytes), 16), torch.uint8, q.device, stream)
+    p = _lib.FlashPagedParams()
+    p.q, p.out, p.k_pool, p.v_pool, p.page_table = q.data_ptr(), out.data_ptr(), codes.data_ptr(), v_pool[0].data_ptr(), page_table.data_ptr()
+    p.total_q, p.num_heads, p.num_kv_heads, p.head_dim, p.num_seqs = tq, hq, hkv, d, n
+    p.num_blocks, p.block_size, p.max_blocks_per_seq = nblk, bs, page_table.shape[1]
+    p.cu_seqlens_q, p.seq_lens_kv = cu_q.ctypes.data, lens.ctypes.data
+    p.scale = effective_scale(scale, d)
+    p.causal = 1 if causal else 0
+    p.dtype_id = dtype_id(q.dtype)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+    check(lib().sca_launch_flash_paged_fp8(C.byref(p), k_pool[1].data_ptr(), v_pool[1].data_ptr(), _stream_ptr(stream)))
+    return out
