@@ -12,7 +12,9 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -25,6 +27,7 @@ namespace {
 
 constexpr int64_t kMaxSplits = 64;         // as MAX_SPLITS, DECODE_STEP_TOKENS in ops.py
 constexpr int64_t kDecodeStepTokens = 64;
+constexpr int64_t kFp8StepTokens = 128;    // as FP8_STEP_TOKENS
 
 PyObject* g_scratch = nullptr;          // ops._scratch: threading.local with the dict `pool`
 PyObject* g_acquire_scratch = nullptr;  // ops.acquire_scratch_fp32
@@ -214,10 +217,11 @@ int64_t SlotsForSchedule(int64_t column_steps, int64_t longest_steps, int64_t co
     const int64_t per_cta = std::max<int64_t>(1, (column_steps + sharers - 1) / sharers);
     return std::max<int64_t>(2, std::min((longest_steps + per_cta - 1) / per_cta + 1, kMaxSplits));
 }
-int64_t Steps(int64_t tokens) { return (tokens + kDecodeStepTokens - 1) / kDecodeStepTokens; }
+int64_t Steps(int64_t tokens, int64_t step = kDecodeStepTokens) { return (tokens + step - 1) / step; }
 
-// The rest of a decode call whose inputs and strides are in `p`: scratch, output, launch.
-PyObject* FinishDecode(ScaDecodeFwdParams& p, const at::Tensor& q, PyObject* q_obj) {
+// The rest of a decode call whose inputs and strides are in `p`: scratch, output, launch(p, stream).
+template <typename L>
+PyObject* FinishDecode(ScaDecodeFwdParams& p, const at::Tensor& q, PyObject* q_obj, const L& launch) {
     void* stream = CurrentStream();
     const int64_t base = p.batch * p.num_heads * p.num_splits, d = p.head_dim;
     PyObject* device = PyObject_GetAttrString(q_obj, "device");
@@ -234,8 +238,11 @@ PyObject* FinishDecode(ScaDecodeFwdParams& p, const at::Tensor& q, PyObject* q_o
     at::Tensor out = Empty({p.batch, p.num_heads, 1, d}, q, q.scalar_type());
     p.out = out.data_ptr();
     p.partial_m = scratch, p.partial_l = scratch + base, p.partial_o = scratch + 2 * base;
-    if (const int rc = Launch([&] { return sca_launch_decode_auto(&p, nullptr, stream); })) return NotLaunched(rc);
+    if (const int rc = Launch([&] { return launch(&p, stream); })) return NotLaunched(rc);
     return THPVariable_Wrap(std::move(out));
+}
+PyObject* FinishDecode(ScaDecodeFwdParams& p, const at::Tensor& q, PyObject* q_obj) {
+    return FinishDecode(p, q, q_obj, [](const ScaDecodeFwdParams* params, void* stream) { return sca_launch_decode_auto(params, nullptr, stream); });
 }
 
 // decode(q, k, v, scale, layout, seq_lens)
@@ -454,6 +461,159 @@ PyObject* Gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- 8-bit KV cache --------------------------------------------------------------------------------------------------------
+// K or V of a layer, as _require_fp8_pool in ops.py.
+bool Fp8Pool(const at::Tensor* codes, const at::Tensor* scales, ScaKvCacheShape* s) {
+    if (codes == nullptr || scales == nullptr || (codes->scalar_type() != at::kFloat8_e4m3fn && codes->scalar_type() != at::kByte) ||
+        !PoolShape(*codes, s)) {
+        return false;
+    }
+    return scales->scalar_type() == at::kByte && scales->dim() == 3 && scales->is_contiguous() && scales->size(0) == s->num_blocks &&
+           scales->size(1) == s->num_kv_heads && scales->size(2) == (s->block_size + 15) / 16 * 16;
+}
+// The pools of a layer, handed over as codes and scales of K, codes and scales of V.
+struct Fp8Layer {
+    const at::Tensor *k, *ks, *v, *vs;
+    ScaKvCacheShape shape{};
+    ScaFp8Layer layer{};
+    bool Take(PyObject* const* a) {
+        k = Plain(a[0]), ks = Plain(a[1]), v = Plain(a[2]), vs = Plain(a[3]);
+        ScaKvCacheShape other;
+        if (!Fp8Pool(k, ks, &shape) || !Fp8Pool(v, vs, &other) || k->sizes() != v->sizes()) return false;
+        layer = ScaFp8Layer{k->data_ptr(), v->data_ptr(), static_cast<uint8_t*>(ks->data_ptr()), static_cast<uint8_t*>(vs->data_ptr())};
+        return Here(*k) && Here(*ks) && Here(*v) && Here(*vs);
+    }
+    // On the current device.
+    static bool Here(const at::Tensor& t) { return t.device().index() == c10::cuda::current_device(); }
+};
+bool Fp8Rows(const at::Tensor& k, const at::Tensor& v, const Fp8Layer& l) {
+    const int64_t width = l.shape.num_kv_heads * l.shape.head_dim;
+    if (k.dim() < 1 || v.dim() < 1 || k.scalar_type() != v.scalar_type() || !k.is_contiguous() || !v.is_contiguous()) return false;
+    const int64_t rows = k.size(0);
+    return rows > 0 && v.size(0) >= rows && k.numel() == rows * width && v.numel() == v.size(0) * width && Fp8Layer::Here(k) && Fp8Layer::Here(v);
+}
+
+// append_fp8(k_codes, k_scales, v_codes, v_scales, k_new, v_new, slots)
+PyObject* AppendFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        Fp8Layer l;
+        int32_t dtype;
+        if (n != 7 || !l.Take(a)) return NotTaken();
+        const at::Tensor *kn = Plain(a[4]), *vn = Plain(a[5]), *slots = Plain(a[6]);
+        if (!kn || !vn || !slots || !Fp8Rows(*kn, *vn, l) || !DtypeId(*kn, &dtype) || !Ints(*slots, kn->size(0)) || !Fp8Layer::Here(*slots)) return NotTaken();
+        void* stream = CurrentStream();
+        const int rc = Launch([&] {
+            return sca_launch_kv_append_fp8(&l.layer, kn->data_ptr(), vn->data_ptr(), static_cast<const int32_t*>(slots->data_ptr()), kn->size(0),
+                                            &l.shape, dtype, stream);
+        });
+        return rc == SCA_OK ? Done() : NotLaunched(rc);
+    });
+}
+
+// append_batched_fp8(k_codes, k_scales, v_codes, v_scales, k_new, v_new, page_table, seq_lens)
+PyObject* AppendBatchedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        Fp8Layer l;
+        int32_t dtype;
+        if (n != 8 || !l.Take(a)) return NotTaken();
+        const at::Tensor *kn = Plain(a[4]), *vn = Plain(a[5]), *table = Plain(a[6]), *lens = Plain(a[7]);
+        if (!kn || !vn || !table || !lens || !Fp8Rows(*kn, *vn, l) || !DtypeId(*kn, &dtype) || !Table(*table, kn->size(0)) ||
+            !Ints(*lens, kn->size(0)) || !Fp8Layer::Here(*table) || !Fp8Layer::Here(*lens)) {
+            return NotTaken();
+        }
+        void* stream = CurrentStream();
+        const int rc = Launch([&] {
+            return sca_launch_kv_append_batched_fp8(&l.layer, kn->data_ptr(), vn->data_ptr(), static_cast<const int32_t*>(table->data_ptr()),
+                                                    static_cast<const int32_t*>(lens->data_ptr()), kn->size(0), table->size(1), &l.shape, dtype, stream);
+        });
+        return rc == SCA_OK ? Done() : NotLaunched(rc);
+    });
+}
+
+// gather_fp8(codes, scales, block_ids, dtype)
+PyObject* GatherFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        if (n != 4 || !THPDtype_Check(a[3])) return NotTaken();
+        const at::Tensor *codes = Plain(a[0]), *scales = Plain(a[1]), *ids = Plain(a[2]);
+        ScaKvCacheShape shape;
+        const at::ScalarType type = reinterpret_cast<THPDtype*>(a[3])->scalar_type;
+        const int32_t dtype = type == at::kFloat ? SCA_DTYPE_F32 : type == at::kHalf ? SCA_DTYPE_F16 : type == at::kBFloat16 ? SCA_DTYPE_BF16 : -1;
+        if (!Fp8Pool(codes, scales, &shape) || !ids || !Ints(*ids, 1) || dtype < 0 || !Fp8Layer::Here(*codes) || !Fp8Layer::Here(*scales) ||
+            !Fp8Layer::Here(*ids)) {
+            return NotTaken();
+        }
+        at::Tensor out = Empty({ids->numel(), shape.block_size, shape.num_kv_heads, shape.head_dim}, *codes, type);
+        void* stream = CurrentStream();
+        const int rc = Launch([&] {
+            return sca_launch_kv_gather_fp8(codes->data_ptr(), static_cast<const uint8_t*>(scales->data_ptr()),
+                                            static_cast<const int32_t*>(ids->data_ptr()), ids->numel(), out.data_ptr(), &shape, dtype, stream);
+        });
+        return rc == SCA_OK ? THPVariable_Wrap(std::move(out)) : NotLaunched(rc);
+    });
+}
+
+// paged_fp8(k_codes, k_scales, v_codes, v_scales, q, page_table, seq_lens, block_size, scale, typical_len, longest_len)
+PyObject* PagedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        Fp8Layer l;
+        int64_t block_size, typical, longest;
+        ScaDecodeFwdParams p{};
+        if (n != 11 || !l.Take(a) || !Int(a[7], &block_size) || !Int(a[9], &typical) || !Int(a[10], &longest)) return NotTaken();
+        const at::Tensor *q = Plain(a[4]), *table = Plain(a[5]), *lens = nullptr;
+        if (a[6] != Py_None && (lens = Plain(a[6])) == nullptr) return NotTaken();
+        if (!q || !table || q->dim() != 4 || q->size(2) != 1 || q->size(3) != l.shape.head_dim || block_size != l.shape.block_size ||
+            !q->is_contiguous() || !DtypeId(*q, &p.dtype) || p.dtype == SCA_DTYPE_F32 || !Table(*table, q->size(0)) ||
+            (lens != nullptr && (!Ints(*lens, q->size(0)) || !Fp8Layer::Here(*lens))) || !Fp8Layer::Here(*q) || !Fp8Layer::Here(*table)) {
+            return NotTaken();
+        }
+        p.batch = q->size(0), p.num_heads = q->size(1), p.head_dim = l.shape.head_dim, p.num_kv_heads = l.shape.num_kv_heads;
+        const int64_t d = p.head_dim;
+        if (p.num_kv_heads < 1 || p.num_heads % p.num_kv_heads != 0 || !Scale(a[8], d, &p.scale)) return NotTaken();
+        p.seq_kv = l.shape.num_blocks * block_size;
+        const int64_t mean = typical > 0 ? typical : std::min(p.seq_kv, table->size(1) * block_size), steps = Steps(mean, kFp8StepTokens);
+        const int64_t most = longest > 0 ? Steps(longest, kFp8StepTokens) : 2 * steps, group = p.num_heads / p.num_kv_heads;
+        const int64_t sms = at::cuda::getDeviceProperties(q->device().index())->multiProcessorCount;
+        p.num_splits = mean <= 0 ? 1 : SlotsForSchedule(std::max<int64_t>(1, p.batch) * steps, most, p.num_kv_heads * ((group + 15) / 16), sms);
+        p.q = q->data_ptr(), p.k = l.layer.k_codes, p.v = l.layer.v_codes;
+        p.q_stride = ScaDecodeStrides{p.num_heads * d, d, d};
+        p.o_stride = p.q_stride;
+        p.seq_lens = lens != nullptr ? static_cast<const int32_t*>(lens->data_ptr()) : nullptr;
+        p.page_table = static_cast<const int32_t*>(table->data_ptr());
+        p.block_size = block_size, p.max_blocks_per_seq = table->size(1), p.num_kv_blocks = l.shape.num_blocks;
+        return FinishDecode(p, *q, a[4], [&](const ScaDecodeFwdParams* params, void* stream) {
+            return sca_launch_paged_attention_fp8(params, l.layer.k_scales, l.layer.v_scales, nullptr, stream);
+        });
+    });
+}
+
+// chunk_fp8(k_codes, k_scales, v_codes, v_scales, q, page_table, cu_q, seq_lens, causal, scale)
+PyObject* ChunkFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        Fp8Layer l;
+        HostInts cu_q, lens;
+        bool causal;
+        ScaFlashPagedParams p{};
+        if (n != 10 || !l.Take(a) || !cu_q.Take(a[6]) || !lens.Take(a[7]) || !Flag(a[8], &causal)) return NotTaken();
+        const at::Tensor *q = Plain(a[4]), *table = Plain(a[5]);
+        if (!q || !table || q->dim() != 3 || q->size(2) != l.shape.head_dim || !q->is_contiguous() || !DtypeId(*q, &p.dtype_id) ||
+            p.dtype_id == SCA_DTYPE_F32 || !Table(*table, lens.size()) || cu_q.size() != lens.size() + 1 || !Scale(a[9], q->size(2), &p.scale) ||
+            !Fp8Layer::Here(*q) || !Fp8Layer::Here(*table)) {
+            return NotTaken();
+        }
+        p.total_q = q->size(0), p.num_heads = q->size(1), p.head_dim = q->size(2), p.num_seqs = lens.size();
+        p.num_blocks = l.shape.num_blocks, p.block_size = l.shape.block_size, p.num_kv_heads = l.shape.num_kv_heads;
+        p.max_blocks_per_seq = table->size(1);
+        at::Tensor out = Empty(q->sizes(), *q, q->scalar_type()), ws = VarlenWorkspace(p.num_seqs, p.total_q, *q);
+        p.q = q->data_ptr(), p.out = out.data_ptr(), p.k_pool = l.layer.k_codes, p.v_pool = l.layer.v_codes;
+        p.page_table = static_cast<const int32_t*>(table->data_ptr());
+        p.cu_seqlens_q = cu_q.data(), p.seq_lens_kv = lens.data(), p.causal = causal;
+        p.workspace = ws.data_ptr(), p.workspace_bytes = ws.numel();
+        void* stream = CurrentStream();
+        if (const int rc = Launch([&] { return sca_launch_flash_paged_fp8(&p, l.layer.k_scales, l.layer.v_scales, stream); })) return NotLaunched(rc);
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 // init(scratch_local, acquire_scratch, check)
 PyObject* Init(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 3) {
@@ -482,6 +642,8 @@ PyObject* Slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef g_methods[] = {SCA_METHOD("init", Init), SCA_METHOD("flash", Flash), SCA_METHOD("decode", Decode), SCA_METHOD("paged", Paged),
                            SCA_METHOD("varlen", Varlen), SCA_METHOD("chunk", Chunk), SCA_METHOD("append", Append),
                            SCA_METHOD("append_batched", AppendBatched), SCA_METHOD("reset", Reset), SCA_METHOD("gather", Gather),
+                           SCA_METHOD("append_fp8", AppendFp8), SCA_METHOD("append_batched_fp8", AppendBatchedFp8),
+                           SCA_METHOD("gather_fp8", GatherFp8), SCA_METHOD("paged_fp8", PagedFp8), SCA_METHOD("chunk_fp8", ChunkFp8),
                            SCA_METHOD("slots", Slots), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Plain operator calls without the Python in between.", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -757,6 +757,8 @@ def kv_append_fp8(layer_k, layer_v, k_new, v_new, slot_mapping, *, stream=None) 
     """kv_append into an 8-bit layer (two Fp8Pool): k_new/v_new [num_tokens, H_kv, D] of float32, float16 or bfloat16 are quantised as they
     are written; slot_mapping int32 [num_tokens] on the device, slots < 0 or beyond the pool are skipped. The slots of a call are distinct:
     one that is named twice is left with pieces of both rows."""
+    if stream is None and _native().append_fp8(*layer_k, *layer_v, k_new, v_new, slot_mapping):
+        return
     _require_fp8_pools(layer_k, layer_v)
     _require_fp8_rows(layer_k[0], k_new.shape[0], k_new, v_new)
     _require_ints("slot_mapping", slot_mapping, k_new.shape[0])
@@ -773,6 +775,8 @@ def kv_append_fp8(layer_k, layer_v, k_new, v_new, slot_mapping, *, stream=None) 
 
 def kv_append_batched_fp8(layer_k, layer_v, k_new, v_new, page_table, seq_lens, *, stream=None) -> None:
     """kv_append_batched into an 8-bit layer: one new token per sequence, at position seq_lens[s] - 1 of its pages."""
+    if stream is None and _native().append_batched_fp8(*layer_k, *layer_v, k_new, v_new, page_table, seq_lens):
+        return
     _require_fp8_pools(layer_k, layer_v)
     _require_fp8_rows(layer_k[0], k_new.shape[0], k_new, v_new)
     _require_cuda(page_table)
@@ -793,6 +797,10 @@ def kv_append_batched_fp8(layer_k, layer_v, k_new, v_new, page_table, seq_lens, 
 def kv_gather_fp8(layer, block_ids, dtype, *, stream=None) -> torch.Tensor:
     """Reads blocks of an 8-bit pool back: [len(block_ids), block_size, H_kv, D] of `dtype` (float32, float16 or bfloat16). Ids outside the
     pool read as zeros."""
+    if stream is None:
+        out = _native().gather_fp8(*layer, block_ids, dtype)
+        if out is not None:
+            return out
     _require_fp8_pool(layer)
     _require_ints("block_ids", block_ids, 0)
     codes, scales = layer
@@ -813,6 +821,10 @@ def paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, *, block_size: 
                         stream=None, return_stats: bool = False):
     """paged_attention over an 8-bit cache: q [num_seqs, H_q, 1, D] of float16 or bfloat16, pools as Fp8Pool with a block_size that is a
     multiple of 4; table, lengths and hints as there. The new tokens' K / V are in the cache (kv_append_batched_fp8)."""
+    if stream is None and not return_stats:
+        out = _native().paged_fp8(*k_pool, *v_pool, q, page_table, seq_lens, block_size, scale, typical_len, longest_len)
+        if out is not None:
+            return out
     _require_cuda(q, page_table, seq_lens)
     _require_fp8_pools(k_pool, v_pool)
     if q.dim() != 4:
@@ -866,6 +878,10 @@ def paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, *, block_size: 
 def flash_attention_paged_fp8(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_kv, *, causal=True, scale=None, stream=None):
     """flash_attention_paged over an 8-bit cache: q packed [T_q, H_q, D] of float16 or bfloat16, pools as Fp8Pool; the rest as there. The
     new tokens' K / V are in the cache (kv_append_fp8)."""
+    if stream is None:
+        out = _native().chunk_fp8(*k_pool, *v_pool, q, page_table, cu_seqlens_q, seq_lens_kv, causal, scale)
+        if out is not None:
+            return out
     import numpy as np
     _require_cuda(q, page_table)
     _require_fp8_pools(k_pool, v_pool)
