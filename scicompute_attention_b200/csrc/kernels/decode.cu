@@ -48,7 +48,7 @@ struct DecodeGeom {
     static constexpr int kKRounds = D / 32;         // 16-byte K loads per lane and token tile half
     static constexpr int kVRounds = (D + 63) / 64;  // groups of eight n8 output tiles
     static_assert(D % 32 == 0, "head_dim must be a multiple of 32");
-    static_assert(kWarpBytes >= 2 * (32 + 16 * D) * 4, "merge staging and the CTA's partial must fit in a warp's ring");
+    static_assert(kWarpBytes >= MergeBytes<D>(), "merge staging and the CTA's partial must fit in a warp's ring");
 };
 
 __device__ __forceinline__ float2 Unpack2Bf16(uint32_t v) {
@@ -71,7 +71,7 @@ constexpr int kSpan = kWarps * kTile;
 
 // One segment = tokens [j_begin, j_end) of one (sequence, kv head, head chunk): streams K/V once, keeps the running
 // softmax state of up to 16 query heads, and leaves one (m, l, O) partial per head: in `slot` of the partial arrays, or
-// (kToShared) in this CTA's shared memory at CtaPartial<D>(smem): m[16] in the log2 domain, l[16], O[16][D].
+// (kToShared) in this CTA's shared memory (see MergeWarps): m[16] in the log2 domain, l[16], O[16][D].
 template <typename T, int D, bool kPaged, bool kHi, bool kToShared = false>
 __device__ __forceinline__ void DecodeSegment(const ScaDecodeFwdParams& p, unsigned char* smem, const int64_t b,
                                               const int hk, const int hc, const int64_t j_begin, const int64_t j_end,

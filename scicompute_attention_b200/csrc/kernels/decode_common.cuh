@@ -32,12 +32,16 @@ __device__ __forceinline__ int64_t StepsFor(int64_t len) {
     return t > 0 ? t : 1;
 }
 
+// Bytes of a warp's ring that the end of a segment takes: {m[16], l[16], O[16][D]} of the warp, {m[16], l[16]} of the CTA.
+template <int D>
+constexpr int MergeBytes() { return (64 + 16 * D) * 4; }
 template <int D>
 __device__ __forceinline__ float* CtaPartial(unsigned char* smem) {
     return reinterpret_cast<float*>(smem) + 32 + 16 * D;  // behind warp 0's staging area, inside its ring
 }
 // The end of a segment: the warps' results, each in its ring as {m[16], l[16], O[16][D]}, become the CTA's: in `slot` of the
-// partial arrays, or (kToShared) at CtaPartial<D>(smem).
+// partial arrays, or (kToShared) m and l at CtaPartial<D>(smem) and O in the place of warp 0's, each number written by the thread
+// that alone has read it.
 template <int D, int kWarpBytes, bool kToShared>
 __device__ __forceinline__ void MergeWarps(const ScaDecodeFwdParams& p, unsigned char* smem, const int64_t b, const int head0,
                                            const int nheads, const int slot) {
@@ -60,8 +64,8 @@ __device__ __forceinline__ void MergeWarps(const ScaDecodeFwdParams& p, unsigned
             l_all += wm[16 + row] * wgt;
         }
         if (kToShared) {
+            reinterpret_cast<float*>(smem)[32 + row * D + d] = acc;
             float* partial = CtaPartial<D>(smem);
-            partial[32 + row * D + d] = acc;
             if (d == 0) {
                 partial[row] = m_all;
                 partial[16 + row] = l_all;
@@ -263,7 +267,7 @@ __device__ __forceinline__ void ClusterDecode(const ScaDecodeFwdParams& p, const
     const int group = static_cast<int>(p.num_heads / p.num_kv_heads);
     const int head0 = hk * group + hc * 16;
     const int total = min(16, group - hc * 16) * D;
-    const uint32_t partial = SmemAddr(CtaPartial<D>(smem));
+    const uint32_t partial = SmemAddr(CtaPartial<D>(smem)), partial_o = SmemAddr(smem) + 32 * 4;
     T* out = reinterpret_cast<T*>(p.out) + b * p.o_stride.s_b;
     for (int item = rank * kThreads + threadIdx.x; item < total; item += cluster * kThreads) {
         const int row = item / D, d = item % D;
@@ -278,7 +282,7 @@ __device__ __forceinline__ void ClusterDecode(const ScaDecodeFwdParams& p, const
             if (m[r] == -CUDART_INF_F) continue;
             const float weight = Exp2(m[r] - m_all);
             l_all += LoadFromRank(partial + 4 * (16 + row), r) * weight;
-            acc += LoadFromRank(partial + 4 * (32 + row * D + d), r) * weight;
+            acc += LoadFromRank(partial_o + 4 * (row * D + d), r) * weight;
         }
         const float inv = l_all > 0.0f ? 1.0f / l_all : 0.0f;
         out[(head0 + row) * p.o_stride.s_h + d] = FromFloat<T>(acc * inv);

@@ -6,7 +6,7 @@
 //
 //   * bytes: 2 * (D + 1) per token and kv head, read once for all query heads of the kv head. 4 * D FLOPs per byte pair and
 //     query head: at eight heads 16 FLOPs a byte, so the products run on the tensor cores and HBM stays the bound;
-//   * a warp takes 32 tokens at a time - as many bytes as 16 tokens of a 16-bit cache - through its own ring of 16-byte
+//   * a warp takes 32 tokens at a time (16 above D=128) - as many bytes as 16 tokens of a 16-bit cache - through its own ring of 16-byte
 //     cp.async copies, no CTA barrier in the loop. The scales come with them in 4-byte copies (4 tokens of a page);
 //   * the tokens are the rows of the products and the query heads their 8 columns, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so
 //     that a group of up to 8 heads wastes nothing (with the heads as rows half of each product would be padding). Codes go
@@ -27,54 +27,43 @@
 namespace sca_b200 {
 namespace {
 
-constexpr int kTokens = 32;              // of a warp's step
-constexpr int kSpan = kWarps * kTokens;  // of a CTA's step
+constexpr int kSpan = 128;  // tokens of a CTA's unit of the schedule
 
 struct Fp8Scales {
     const uint8_t* k;
     const uint8_t* v;
 };
 
-template <int D>
+// kHi: more than 8 heads.
+template <int D, bool kHi>
 struct Fp8Geom {
+    static constexpr int kTokens = D > 128 ? 16 : 32;  // of a warp's step
+    // CTAs that stay on an SM: what the registers of O and Q leave room for (FP8 slots in ops.py counts on it)
+    static constexpr int kCtas = D <= 64 ? 4 : kHi && D > 96 ? 2 : 3;
+
     static constexpr int kChunks = D / 16;  // 16-byte pieces of a row
-    static constexpr bool kSwizzle = kChunks % 8 == 0;
     static constexpr int kTileBytes = kTokens * D;
     static constexpr int kStageBytes = 2 * kTileBytes + 2 * kTokens;  // K, V, scales of K, scales of V
-    static constexpr int kStages = D <= 64 ? 4 : 3;
-    static constexpr int kWarpBytes = kStages * kStageBytes;
+    static constexpr int kStages = D <= 64 || kCtas == 2 ? 3 : 2;
+    static constexpr int kWarpBytes = std::max(kStages * kStageBytes, MergeBytes<D>());  // a warp's ring, and then its results
     static constexpr int kSmemBytes = kWarps * kWarpBytes;
     static constexpr int kWordsK = D / 16;  // words of K (4 codes) a lane holds per row: its quarter of the row
     static constexpr int kWordsV = D / 32;  // words of V a lane holds per row: its eighth
     static_assert(D % 32 == 0 && D <= 256, "head_dim");
-    static_assert(kWarpBytes >= 2 * (32 + 16 * D) * 4, "merge staging and the CTA's partial must fit in a warp's ring");
+    static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "shared memory of an SM");
 };
 
 // A phase of 8 lanes reads rows {r, r + 1} of K, 4 adjacent pieces each, or rows {r, r + 2, r + 4, r + 6} of V, 2 adjacent pieces.
 template <int D>
-__device__ __forceinline__ int PieceK(int row, int piece) { return Fp8Geom<D>::kSwizzle ? piece ^ ((row & 1) << 2) : piece; }
+__device__ __forceinline__ int PieceK(int row, int piece) { return D % 128 == 0 ? piece ^ ((row & 1) << 2) : piece; }
 template <int D>
-__device__ __forceinline__ int PieceV(int row, int piece) { return Fp8Geom<D>::kSwizzle ? piece ^ (((row >> 1) & 3) << 1) : piece; }
+__device__ __forceinline__ int PieceV(int row, int piece) { return D % 128 == 0 ? piece ^ (((row >> 1) & 3) << 1) : piece; }
 
-__device__ __forceinline__ uint2 LdsV2(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint32_t Lds32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint32_t Lds16(uint32_t addr) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint32_t Lds8(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u8 %0, [%1];\n" : "=r"(v) : "r"(addr));
-    return v;
+// The products as functions of their operands: not volatile, so that those of independent rows may overlap.
+__device__ __forceinline__ void Mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void CpAsync4(uint32_t smem_dst, const void* gmem_src, int src_bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_dst), "l"(gmem_src), "r"(src_bytes) : "memory");
@@ -82,7 +71,7 @@ __device__ __forceinline__ void CpAsync4(uint32_t smem_dst, const void* gmem_src
 // The transpose of an 8x8 matrix of 16-bit numbers spread over the warp as an operand is (row lane / 4, columns 2 * (lane % 4)).
 __device__ __forceinline__ uint32_t Transpose8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 
@@ -95,40 +84,88 @@ __device__ __forceinline__ int CodeV(int w, int g) {
     return w < 4 * (D / 128) ? (w / 4) * 128 + 16 * g + 4 * (w % 4) : (D / 128) * 128 + (D % 128 / 8) * g + 4 * (w - 4 * (D / 128));
 }
 template <int D>
-__device__ __forceinline__ void LoadK(uint32_t tile, int row, int c, uint32_t (&words)[Fp8Geom<D>::kWordsK]) {
+__device__ __forceinline__ void LoadK(const unsigned char* tile, int row, int c, uint32_t (&words)[D / 16]) {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
-        const uint4 v = LdsV4(tile + row * D + PieceK<D>(row, 4 * i + c) * 16);
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + row * D + PieceK<D>(row, 4 * i + c) * 16);
         words[4 * i] = v.x, words[4 * i + 1] = v.y, words[4 * i + 2] = v.z, words[4 * i + 3] = v.w;
     }
     if constexpr (D % 64 != 0) {
-        const uint2 v = LdsV2(tile + row * D + CodeK<D>(4 * (D / 64), c));
+        const uint2 v = *reinterpret_cast<const uint2*>(tile + row * D + CodeK<D>(4 * (D / 64), c));
         words[4 * (D / 64)] = v.x, words[4 * (D / 64) + 1] = v.y;
     }
 }
 template <int D>
-__device__ __forceinline__ void LoadV(uint32_t tile, int row, int g, uint32_t (&words)[Fp8Geom<D>::kWordsV]) {
+__device__ __forceinline__ void LoadV(const unsigned char* tile, int row, int g, uint32_t (&words)[D / 32]) {
     constexpr int kFull = D / 128;
 #pragma unroll
     for (int i = 0; i < kFull; ++i) {
-        const uint4 v = LdsV4(tile + row * D + PieceV<D>(row, 8 * i + g) * 16);
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + row * D + PieceV<D>(row, 8 * i + g) * 16);
         words[4 * i] = v.x, words[4 * i + 1] = v.y, words[4 * i + 2] = v.z, words[4 * i + 3] = v.w;
     }
     if constexpr (D % 128 == 64) {
-        const uint2 v = LdsV2(tile + row * D + CodeV<D>(4 * kFull, g));
+        const uint2 v = *reinterpret_cast<const uint2*>(tile + row * D + CodeV<D>(4 * kFull, g));
         words[4 * kFull] = v.x, words[4 * kFull + 1] = v.y;
     } else {
 #pragma unroll
-        for (int w = 4 * kFull; w < D / 32; ++w) words[w] = Lds32(tile + row * D + CodeV<D>(w, g));
+        for (int w = 4 * kFull; w < D / 32; ++w) words[w] = *reinterpret_cast<const uint32_t*>(tile + row * D + CodeV<D>(w, g));
     }
+}
+
+// The end of a segment: MergeWarps of decode_common.cuh with the weights of the warps computed once per row and O four numbers at a
+// time (at D=256 it took 6200 clocks of a segment the other way).
+template <int D, int kWarpBytes, bool kToShared>
+__device__ __forceinline__ void MergeFp8Warps(const ScaDecodeFwdParams& p, unsigned char* smem, const int64_t b, const int head0,
+                                              const int nheads, const int slot) {
+    __shared__ float weights[16][kWarps];
+    __syncthreads();
+    if (threadIdx.x < nheads) {
+        const int row = threadIdx.x;
+        float m[kWarps], m_all = -CUDART_INF_F, l_all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            m[w] = reinterpret_cast<const float*>(smem + w * kWarpBytes)[row];
+            m_all = fmaxf(m_all, m[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float weight = m[w] == -CUDART_INF_F ? 0.0f : Exp2(m[w] - m_all);
+            weights[row][w] = weight;
+            l_all += reinterpret_cast<const float*>(smem + w * kWarpBytes)[16 + row] * weight;
+        }
+        if (kToShared) {
+            float* partial = CtaPartial<D>(smem);
+            partial[row] = m_all;
+            partial[16 + row] = l_all;
+        } else {
+            const int64_t flat = (b * p.num_heads + head0 + row) * p.num_splits + slot;
+            p.partial_m[flat] = m_all * kLn2;  // in natural units, as the 16-bit cache's
+            p.partial_l[flat] = l_all;
+        }
+    }
+    __syncthreads();
+    for (int item = threadIdx.x; item < nheads * (D / 4); item += kThreads) {
+        const int row = item / (D / 4), d = item % (D / 4) * 4;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float weight = weights[row][w];
+            const float4 x = *reinterpret_cast<const float4*>(smem + w * kWarpBytes + (32 + row * D + d) * 4);  // zeros where a warp had no key
+            acc.x = fmaf(x.x, weight, acc.x), acc.y = fmaf(x.y, weight, acc.y), acc.z = fmaf(x.z, weight, acc.z), acc.w = fmaf(x.w, weight, acc.w);
+        }
+        if (kToShared) *reinterpret_cast<float4*>(smem + (32 + row * D + d) * 4) = acc;
+        else *reinterpret_cast<float4*>(p.partial_o + ((b * p.num_heads + head0 + row) * p.num_splits + slot) * D + d) = acc;
+    }
+    __syncthreads();  // the rings double as merge staging: nobody refills them before everyone has read
 }
 
 // Tokens [j_begin, j_end) of one (sequence, kv head, head chunk): see DecodeSegment in decode.cu. kHi: more than 8 heads.
 template <typename T, int D, bool kHi, bool kToShared>
 __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp8Scales& scales, unsigned char* smem, const int64_t b,
                                            const int hk, const int hc, const int64_t j_begin, const int64_t j_end, const int slot) {
-    using G = Fp8Geom<D>;
-    constexpr int kCols = kHi ? 2 : 1;  // head columns of 8
+    using G = Fp8Geom<D, kHi>;
+    constexpr int kTokens = G::kTokens, kRows = kTokens / 16;  // rows of products, 16 tokens each
+    constexpr int kCols = kHi ? 2 : 1;                          // head columns of 8
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
     const int g = lane >> 2;
@@ -139,6 +176,95 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
 
     const int ntiles = j_end > j_begin ? static_cast<int>((j_end - j_begin + kTokens - 1) / kTokens) : 0;
     const int my_tiles = ntiles > warp ? (ntiles - warp + kWarps - 1) / kWarps : 0;
+
+    const unsigned char* k_base = static_cast<const unsigned char*>(p.k) + hk * D;
+    const unsigned char* v_base = static_cast<const unsigned char*>(p.v) + hk * D;
+    const uint32_t row_pieces = static_cast<uint32_t>(p.num_kv_heads * G::kChunks);
+    const int32_t* table_row = p.page_table + b * p.max_blocks_per_seq;
+    const int block_size = static_cast<int>(p.block_size);
+    const int64_t scale_row = fp8::ScaleRow(block_size);
+
+    unsigned char* ring = smem + warp * G::kWarpBytes;
+    const uint32_t ring_addr = SmemAddr(ring);
+
+    // This lane's token of the next tile to be issued, as (page of the sequence, offset in the page), moved on by the tokens of
+    // the CTA's warps per tile without a division, and the page's table entry, fetched one tile ahead.
+    const int token = lane % kTokens;
+    constexpr int kStep = kWarps * kTokens;
+    int page = 0, offset = 0;
+    int32_t phys_next = -1;
+    const int page_step = kStep / block_size, offset_step = kStep % block_size;
+    auto fetch_entry = [&](int64_t jt) { phys_next = (jt < j_end && page < p.max_blocks_per_seq) ? table_row[page] : -1; };
+    {
+        const int64_t jt = j_begin + warp * kTokens + token;
+        page = static_cast<int>(jt / block_size);
+        offset = static_cast<int>(jt - static_cast<int64_t>(page) * block_size);
+        fetch_entry(jt);
+    }
+
+    // Issues the copies of this warp's `tl`-th tile into `stage`, tile after tile; returns which of its tokens there are.
+    auto issue = [&](int tl, int stage) -> uint32_t {
+        const int64_t jt = j_begin + static_cast<int64_t>(warp + tl * kWarps) * kTokens + token;
+        const bool there = phys_next >= 0 && phys_next < p.num_kv_blocks;
+        // place of the row in 16-byte pieces; pools stay below 2^32 of them
+        const uint32_t at = there ? static_cast<uint32_t>(phys_next * block_size + offset) * row_pieces : 0u;
+        const uint32_t k_stage = ring_addr + stage * G::kStageBytes;
+        const uint32_t v_stage = k_stage + G::kTileBytes;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        if (c == 0 && lane < kTokens) {
+            // block_size is a multiple of 4, and so is the tile's first token: four tokens share a page and a word of scales
+            const int64_t scales_at = there ? (static_cast<int64_t>(phys_next) * p.num_kv_heads + hk) * scale_row + offset : 0;
+            CpAsync4(v_stage + G::kTileBytes + lane, scales.k + scales_at, there ? 4 : 0);
+            CpAsync4(v_stage + G::kTileBytes + kTokens + lane, scales.v + scales_at, there ? 4 : 0);
+        }
+        page += page_step;
+        offset += offset_step;
+        if (offset >= block_size) {
+            offset -= block_size;
+            ++page;
+        }
+        fetch_entry(jt + kStep);
+        auto copy = [&](auto whole) {
+#pragma unroll
+            for (int n = 0; n < kTokens * G::kChunks / 32; ++n) {
+                const int item = lane + 32 * n;
+                const int row = item / G::kChunks;
+                const int piece = item % G::kChunks;
+                const uint64_t from = static_cast<uint64_t>(__shfl_sync(0xffffffffu, at, row)) * 16u;
+                const uint32_t k_dst = k_stage + row * D + PieceK<D>(row, piece) * 16, v_dst = v_stage + row * D + PieceV<D>(row, piece) * 16;
+                const int bytes = decltype(whole)::value || ((mask >> row) & 1u) ? 16 : 0;
+                CpAsync16(k_dst, k_base + piece * 16 + from, bytes);
+                CpAsync16(v_dst, v_base + piece * 16 + from, bytes);
+            }
+        };
+        if (mask == 0xffffffffu) copy(std::true_type{});
+        else copy(std::false_type{});
+        CpAsyncCommit();
+        return mask;
+    };
+
+    // ---- running state of heads 8 * t + 2 * c, + 1; m_run in units of `unit`, which is positive ----
+    float m_run[kCols][2], l_run[kCols][2];
+    float o[kCols][2 * G::kWordsV][4];  // rows CodeV(w, g) + 2 * half, + 1 of O^T
+#pragma unroll
+    for (int t = 0; t < kCols; ++t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m_run[t][i] = -CUDART_INF_F, l_run[t][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2 * G::kWordsV; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][j][e] = 0.0f;
+        }
+    }
+
+    constexpr uint32_t kAllTokens = 0xffffffffu;  // 16 tokens to a tile: lanes 16 to 31 look at the same ones
+    uint32_t masks[G::kStages - 1];
+#pragma unroll
+    for (int s = 0; s < G::kStages - 1; ++s) {
+        masks[s] = 0;
+        if (s < my_tiles) masks[s] = issue(s, s);
+        else CpAsyncCommit();
+    }
 
     // ---- queries: columns of B, heads 8 * t + g; `unit` turns a product of codes into a score in the log2 domain ----
     uint32_t qb[kCols][G::kWordsK][2];
@@ -178,91 +304,11 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) unit[t][i] = __shfl_sync(0xffffffffu, factor, (2 * c + i) * 4) * scale_log2;
+            for (int i = 0; i < 2; ++i) {
+                // not 0, which would make NaN of a masked token's -inf: scores of tiny rows under a tiny scale are 0 either way
+                unit[t][i] = fmaxf(__shfl_sync(0xffffffffu, factor, (2 * c + i) * 4) * scale_log2, fp8::PowerOfTwo(-126));
+            }
         }
-    }
-
-    const unsigned char* k_base = static_cast<const unsigned char*>(p.k) + hk * D;
-    const unsigned char* v_base = static_cast<const unsigned char*>(p.v) + hk * D;
-    const int64_t row_bytes = p.num_kv_heads * D;
-    const int32_t* table_row = p.page_table + b * p.max_blocks_per_seq;
-    const int block_size = static_cast<int>(p.block_size);
-    const int64_t scale_row = fp8::ScaleRow(block_size);
-
-    unsigned char* ring = smem + warp * G::kWarpBytes;
-    const uint32_t ring_addr = SmemAddr(ring);
-
-    // This lane's token of the next tile to be issued, as (page of the sequence, offset in the page), moved on by kSpan tokens
-    // per tile without a division, and the page's table entry, fetched one tile ahead.
-    int64_t page = 0;
-    int offset = 0;
-    int32_t phys_next = -1;
-    const int64_t page_step = kSpan / block_size;
-    const int offset_step = kSpan % block_size;
-    auto fetch_entry = [&](int64_t jt) { phys_next = (jt < j_end && page < p.max_blocks_per_seq) ? table_row[page] : -1; };
-    {
-        const int64_t jt = j_begin + warp * kTokens + lane;
-        page = jt / block_size;
-        offset = static_cast<int>(jt - page * block_size);
-        fetch_entry(jt);
-    }
-
-    // Issues the copies of this warp's `tl`-th tile into `stage`, tile after tile; returns which of the 32 tokens there are.
-    auto issue = [&](int tl, int stage) -> uint32_t {
-        const int64_t jt = j_begin + static_cast<int64_t>(warp + tl * kWarps) * kTokens + lane;
-        const bool there = phys_next >= 0 && phys_next < p.num_kv_blocks;
-        const int prow = there ? phys_next * block_size + offset : -1;  // pools stay below 2^31 rows
-        const uint32_t k_stage = ring_addr + stage * G::kStageBytes;
-        const uint32_t v_stage = k_stage + G::kTileBytes;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there);
-        if (c == 0) {
-            // block_size is a multiple of 4, and so is the tile's first token: four tokens share a page and a word of scales
-            const int64_t at = there ? (static_cast<int64_t>(phys_next) * p.num_kv_heads + hk) * scale_row + offset : 0;
-            CpAsync4(v_stage + G::kTileBytes + lane, scales.k + at, there ? 4 : 0);
-            CpAsync4(v_stage + G::kTileBytes + kTokens + lane, scales.v + at, there ? 4 : 0);
-        }
-        page += page_step;
-        offset += offset_step;
-        if (offset >= block_size) {
-            offset -= block_size;
-            ++page;
-        }
-        fetch_entry(jt + kSpan);
-#pragma unroll
-        for (int n = 0; n < G::kChunks; ++n) {
-            const int item = lane + 32 * n;
-            const int row = item / G::kChunks;
-            const int piece = item % G::kChunks;
-            const int pr = __shfl_sync(0xffffffffu, prow, row);
-            const int bytes = pr >= 0 ? 16 : 0;
-            const int64_t at = (pr >= 0 ? pr : 0) * row_bytes + piece * 16;
-            CpAsync16(k_stage + row * D + PieceK<D>(row, piece) * 16, k_base + at, bytes);
-            CpAsync16(v_stage + row * D + PieceV<D>(row, piece) * 16, v_base + at, bytes);
-        }
-        CpAsyncCommit();
-        return mask;
-    };
-
-    // ---- running state of heads 8 * t + 2 * c, + 1; scores live in the log2 domain ----
-    float m_run[kCols][2], l_run[kCols][2];
-    float o[kCols][2 * G::kWordsV][4];  // rows CodeV(w, g) + 2 * half, + 1 of O^T
-#pragma unroll
-    for (int t = 0; t < kCols; ++t) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) m_run[t][i] = -CUDART_INF_F, l_run[t][i] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 2 * G::kWordsV; ++j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[t][j][e] = 0.0f;
-        }
-    }
-
-    uint32_t masks[G::kStages - 1];
-#pragma unroll
-    for (int s = 0; s < G::kStages - 1; ++s) {
-        masks[s] = 0;
-        if (s < my_tiles) masks[s] = issue(s, s);
-        else CpAsyncCommit();
     }
 
     int stage = 0;
@@ -282,14 +328,13 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
             masks[G::kStages - 2] = mk;
         }
         if (cur != 0) {
-            const uint32_t k_stage = ring_addr + stage * G::kStageBytes;
-            const uint32_t v_stage = k_stage + G::kTileBytes;
-            const uint32_t k_scale = v_stage + G::kTileBytes, v_scale = k_scale + kTokens;
+            const unsigned char *k_stage = ring + stage * G::kStageBytes, *v_stage = k_stage + G::kTileBytes;
+            const unsigned char *k_scale = v_stage + G::kTileBytes, *v_scale = k_scale + kTokens;
 
             // S^T: tokens 16 * r + g (elements 0, 1: heads 2c, 2c + 1) and 16 * r + g + 8 (elements 2, 3)
-            float s[2][kCols][4];
+            float s[kRows][kCols][4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < kRows; ++r) {
                 uint32_t lo[G::kWordsK], hi[G::kWordsK];
                 LoadK<D>(k_stage, 16 * r + g, c, lo);
                 LoadK<D>(k_stage, 16 * r + g + 8, c, hi);
@@ -302,40 +347,53 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
                 for (int w = 0; w < G::kWordsK; ++w) {
                     const uint32_t a0 = fp8::DecodeLow(lo[w]), a1 = fp8::DecodeLow(hi[w]), a2 = fp8::DecodeHigh(lo[w]), a3 = fp8::DecodeHigh(hi[w]);
 #pragma unroll
-                    for (int t = 0; t < kCols; ++t) MmaM16N8K16<__half>(s[r][t], a0, a1, a2, a3, qb[t][w][0], qb[t][w][1]);
+                    for (int t = 0; t < kCols; ++t) Mma(s[r][t], a0, a1, a2, a3, qb[t][w][0], qb[t][w][1]);
                 }
             }
-            float k_unit[4];  // tokens g, g + 8, g + 16, g + 24
 #pragma unroll
-            for (int i = 0; i < 4; ++i) k_unit[i] = fp8::ScaleOf(Lds8(k_scale + 8 * i + g));
+            for (int i = 0; i < 2 * kRows; ++i) {  // tokens 8 * i + g
+                const float k_unit = fp8::ScaleOf(k_scale[8 * i + g]);
+#pragma unroll
+                for (int t = 0; t < kCols; ++t) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) s[i / 2][t][2 * (i & 1) + h] *= k_unit;
+                }
+            }
+            if (cur != kAllTokens) {
+#pragma unroll
+                for (int i = 0; i < 2 * kRows; ++i) {
+                    if ((cur >> (8 * i + g)) & 1u) continue;
+#pragma unroll
+                    for (int t = 0; t < kCols; ++t) s[i / 2][t][2 * (i & 1)] = s[i / 2][t][2 * (i & 1) + 1] = -CUDART_INF_F;
+                }
+            }
 
-            uint32_t pb[kCols][4];  // P^T, columns of B: tokens 8 * i + 2 * c, + 1 of head 8 * t + g
+            uint32_t pb[kCols][2 * kRows];  // P^T, columns of B: tokens 8 * i + 2 * c, + 1 of head 8 * t + g
 #pragma unroll
             for (int t = 0; t < kCols; ++t) {
                 float alpha[2];
-                float prob[4][2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool there = (cur >> (8 * i + g)) & 1u;
-                        x[i] = there ? s[i / 2][t][2 * (i & 1) + h] * (unit[t][h] * k_unit[i]) : -CUDART_INF_F;
-                    }
-                    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    float mx = fmaxf(s[0][t][h], s[0][t][2 + h]);
+                    if constexpr (kRows == 2) mx = Max3(mx, s[kRows - 1][t][h], s[kRows - 1][t][2 + h]);
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     const float m_new = fmaxf(m_run[t][h], mx);
-                    const float m_safe = m_new == -CUDART_INF_F ? 0.0f : m_new;
-                    alpha[h] = Exp2(m_run[t][h] - m_safe);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) prob[i][h] = Exp2(x[i] - m_safe);
-                    l_run[t][h] = l_run[t][h] * alpha[h] + ((prob[0][h] + prob[1][h]) + (prob[2][h] + prob[3][h]));
+                    const float shift = m_new == -CUDART_INF_F ? 0.0f : -m_new * unit[t][h];
+                    alpha[h] = Exp2(fmaf(m_run[t][h], unit[t][h], shift));
                     m_run[t][h] = m_new;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2 * kRows; ++i) {
+                        float& x = s[i / 2][t][2 * (i & 1) + h];
+                        x = Exp2(fmaf(x, unit[t][h], shift));
+                        sum += x;
+                    }
+                    l_run[t][h] = fmaf(l_run[t][h], alpha[h], sum);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pb[t][i] = Transpose8x8(Pack2<__half>(prob[i][0], prob[i][1]));
+                for (int i = 0; i < 2 * kRows; ++i) pb[t][i] = Transpose8x8(Pack2<__half>(s[i / 2][t][2 * (i & 1)], s[i / 2][t][2 * (i & 1) + 1]));
                 // the maximum of a long sequence hardly moves: O is touched where it does
                 if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
 #pragma unroll
@@ -347,15 +405,15 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
 
             // O^T += V^T P^T
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < kRows; ++r) {
                 const int row = 16 * r + 2 * c;
                 uint32_t v0[G::kWordsV], v1[G::kWordsV], v8[G::kWordsV], v9[G::kWordsV];
                 LoadV<D>(v_stage, row, g, v0);
                 LoadV<D>(v_stage, row + 1, g, v1);
                 LoadV<D>(v_stage, row + 8, g, v8);
                 LoadV<D>(v_stage, row + 9, g, v9);
-                uint32_t s01 = Lds16(v_scale + row), s89 = Lds16(v_scale + row + 8);
-                if (cur != 0xffffffffu) {
+                uint32_t s01 = *reinterpret_cast<const uint16_t*>(v_scale + row), s89 = *reinterpret_cast<const uint16_t*>(v_scale + row + 8);
+                if (cur != kAllTokens) {
                     // the scales come four at a time: those of tokens that do not count are anything, and infinity times 0 is not 0
                     const uint32_t there = cur >> row;
                     s01 &= ((there & 1u) ? 0xffu : 0u) | ((there & 2u) ? 0xff00u : 0u);
@@ -372,7 +430,7 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
                         const uint32_t a0 = fp8::MulHalf2(fp8::DecodeLow(p01), unit01), a1 = fp8::MulHalf2(fp8::DecodeHigh(p01), unit01);
                         const uint32_t a2 = fp8::MulHalf2(fp8::DecodeLow(p89), unit89), a3 = fp8::MulHalf2(fp8::DecodeHigh(p89), unit89);
 #pragma unroll
-                        for (int t = 0; t < kCols; ++t) MmaM16N8K16<__half>(o[t][2 * w + half], a0, a1, a2, a3, pb[t][2 * r], pb[t][2 * r + 1]);
+                        for (int t = 0; t < kCols; ++t) Mma(o[t][2 * w + half], a0, a1, a2, a3, pb[t][2 * r], pb[t][2 * r + 1]);
                     }
                 }
             }
@@ -396,7 +454,7 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
             const int head = 8 * t + 2 * c + h;
-            if (g == 0) stage_m[head] = m_run[t][h], stage_l[head] = l;
+            if (g == 0) stage_m[head] = m_run[t][h] == -CUDART_INF_F ? -CUDART_INF_F : m_run[t][h] * unit[t][h], stage_l[head] = l;
 #pragma unroll
             for (int w = 0; w < G::kWordsV; ++w) {
 #pragma unroll
@@ -406,26 +464,194 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
             }
         }
     }
+    MergeFp8Warps<D, G::kWarpBytes, kToShared>(p, smem, b, head0, nheads, slot);
+}
+
+// The schedule of decode_common.cuh (WalkSchedule: what it does and why) for lists of less than 2^31 steps: the lengths are read once,
+// and nothing is divided in 64 bits. With both it took 3500 clocks until a CTA knew its share; a CTA's K/V is 30000 to 60000.
+template <typename Segment>
+__device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, const int head_chunks, const Segment& segment) {
+    __shared__ int s_part[kWarps][2];
+    __shared__ int s_found[2];
+    WaitForPredecessor();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int columns = static_cast<int>(p.num_kv_heads) * head_chunks, grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+    // grids smaller than the number of columns let every CTA walk several columns, each as its only CTA
+    const int sharers = grid >= columns ? grid / columns : 1;
+    const int share = grid >= columns ? cta / columns : 0;
+    const int first_column = grid >= columns ? cta % columns : cta;
+    const int column_stride = grid >= columns ? columns : grid;
+    if (share >= sharers) return;  // a grid that is no multiple of the column count
+
+    const int batch = static_cast<int>(p.batch), splits = static_cast<int>(p.num_splits);
+    const int cap = static_cast<int>(p.max_blocks_per_seq * p.block_size < 0x7fffff00LL ? p.max_blocks_per_seq * p.block_size : 0x7fffff00LL);
+    auto length = [&](int i) { return max(0, min(p.seq_lens != nullptr ? p.seq_lens[i] : cap, cap)); };
+    auto steps_of = [](int len) { return max(1, static_cast<int>((static_cast<uint32_t>(len) + kSpan - 1) / kSpan)); };
+    // sequences [mine, end_mine) are this thread's
+    const int each = (batch + kThreads - 1) / kThreads;
+    const int mine = min(batch, static_cast<int>(threadIdx.x) * each), end_mine = min(batch, mine + each);
+    int sum = 0, longest = 0;
+    for (int i = mine; i < end_mine; ++i) {
+        const int t = steps_of(length(i));
+        sum += t;
+        longest = max(longest, t);
+    }
+    int up = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += x;
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 31) s_part[warp][0] = up, s_part[warp][1] = longest;
     __syncthreads();
-    MergeWarps<D, G::kWarpBytes, kToShared>(p, smem, b, head0, nheads, slot);
+    int total = 0, first = up - sum;  // steps of the list, and those ahead of this thread's sequences
+    longest = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) first += s_part[w][0];
+        total += s_part[w][0];
+        longest = max(longest, s_part[w][1]);
+    }
+    // at least so many that no sequence falls into more than `splits` pieces; with one slot a column goes to its first CTA
+    const int per_cta = max((total + sharers - 1) / sharers, splits > 1 ? (longest + splits - 2) / (splits - 1) : total);
+    if (static_cast<int64_t>(share) * per_cta >= total) return;
+    const int begin = share * per_cta, end = min(total, begin + per_cta);
+    if (first <= begin && begin < first + sum) {
+        int i = mine, before = first;
+        while (true) {
+            const int t = steps_of(length(i));
+            if (begin < before + t) break;
+            before += t;
+            ++i;
+        }
+        s_found[0] = i;
+        s_found[1] = before;
+    }
+    __syncthreads();
+    const int b_first = s_found[0], before_first = s_found[1];
+    // the merge kernel that follows on the stream may be set up while this grid streams K/V
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+    for (int column = first_column; column < columns; column += column_stride) {
+        const int hk = column / head_chunks, hc = column % head_chunks;
+        int b = b_first, before = before_first, len = length(b), steps = steps_of(len);
+        for (int pos = begin; pos < end;) {
+            const int t0 = pos - before, t1 = min(t0 + (end - pos), steps);
+            const int slot = share - before / per_cta;
+            if (t0 == 0) MarkUnusedSlots(p, b, hk, hc, (before + steps - 1) / per_cta - before / per_cta + 1);
+            const int64_t j_end = min(static_cast<int64_t>(t1) * kSpan, static_cast<int64_t>(len));
+            segment(b, hk, hc, static_cast<int64_t>(t0) * kSpan, j_end, slot);
+            pos += t1 - t0;
+            if (t1 == steps && pos < end) {
+                before += steps;
+                ++b;
+                len = length(b);
+                steps = steps_of(len);
+            }
+        }
+    }
 }
 
 template <typename T, int D, bool kHi>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, Fp8Geom<D, kHi>::kCtas)
 decode_fp8_partial_kernel(const ScaDecodeFwdParams p, const Fp8Scales scales, const int head_chunks) {
     extern __shared__ __align__(128) unsigned char smem[];
-    WalkSchedule<true, kSpan>(p, head_chunks, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end, int slot) {
+    WalkFp8Schedule(p, head_chunks, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end, int slot) {
         Fp8Segment<T, D, kHi, false>(p, scales, smem, b, hk, hc, j_begin, j_end, slot);
     });
 }
 
 template <typename T, int D, bool kHi>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, Fp8Geom<D, kHi>::kCtas)
 decode_fp8_cluster_kernel(const ScaDecodeFwdParams p, const Fp8Scales scales, const int head_chunks, const int cluster) {
     extern __shared__ __align__(128) unsigned char smem[];
     ClusterDecode<T, D, true, kSpan>(p, head_chunks, cluster, smem, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end) {
         Fp8Segment<T, D, kHi, true>(p, scales, smem, b, hk, hc, j_begin, j_end, 0);
     });
+}
+
+// Merges the parts of a row: out = sum_s w_s O_s / sum_s w_s l_s with w_s = exp(m_s - max m). kWarps_ warps to a row, which take parts in
+// turn, a lane 4 numbers of O at a time. Bound by latency: what a row takes is a chain of three loads from L2 (m, l and O), whose
+// parts are all under way at once; one thread per number of O that goes through the parts one by one takes 17 us for the 54 parts of
+// one sequence of 100 thousand tokens.
+template <typename T, int D, int kRowWarps>
+__global__ void __launch_bounds__(256)
+decode_fp8_merge_kernel(const ScaDecodeFwdParams p) {
+    constexpr int kLanes = D >= 128 ? 32 : D / 4;                       // that hold a row of O
+    constexpr int kAtOnce = 32 % kLanes == 0 ? 32 / kLanes : 1;         // parts a warp takes in one turn
+    constexpr int kVecs = (D + 127) / 128;                              // pieces of 4 numbers per lane
+    __shared__ float4 others[kRowWarps > 1 ? 8 : 1][kVecs][kRowWarps > 1 ? 32 : 1];
+    BeginAfterPredecessor();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / kRowWarps) + warp / kRowWarps;
+    const int parts = static_cast<int>(p.num_splits);
+    const bool there = row < p.batch * p.num_heads;
+    const float *m = p.partial_m + row * parts, *l = p.partial_l + row * parts;
+    float m_all = -CUDART_INF_F, l_all = 0.0f;
+    for (int i = lane; i < parts && there; i += 32) m_all = fmaxf(m_all, m[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
+    for (int i = lane; i < parts && there; i += 32) {
+        // a part without a key holds nothing but its m
+        if (m[i] != -CUDART_INF_F) l_all = fmaf(l[i], Exp2((m[i] - m_all) * kLog2e), l_all);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, o);
+    float4 acc[kVecs];
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int sub = kAtOnce > 1 ? lane / kLanes : 0, piece = kAtOnce > 1 ? lane % kLanes : lane;
+#pragma unroll 4
+    for (int s = (warp % kRowWarps) * kAtOnce + sub; s < parts && there; s += kRowWarps * kAtOnce) {
+        const float m_part = m[s];
+        const float w = m_part == -CUDART_INF_F ? 0.0f : Exp2((m_part - m_all) * kLog2e);
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int d = v * 128 + piece * 4;
+            if (D % 128 != 0 && d >= D) continue;
+            float4 x = *reinterpret_cast<const float4*>(p.partial_o + (row * parts + s) * D + d);
+            if (m_part == -CUDART_INF_F) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // not written
+            acc[v].x = fmaf(x.x, w, acc[v].x), acc[v].y = fmaf(x.y, w, acc[v].y), acc[v].z = fmaf(x.z, w, acc[v].z), acc[v].w = fmaf(x.w, w, acc[v].w);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+#pragma unroll
+        for (int o = kLanes; kAtOnce > 1 && o < 32; o <<= 1) {
+            acc[v].x += __shfl_xor_sync(0xffffffffu, acc[v].x, o), acc[v].y += __shfl_xor_sync(0xffffffffu, acc[v].y, o);
+            acc[v].z += __shfl_xor_sync(0xffffffffu, acc[v].z, o), acc[v].w += __shfl_xor_sync(0xffffffffu, acc[v].w, o);
+        }
+        if constexpr (kRowWarps > 1) others[warp][v][lane] = acc[v];
+    }
+    if constexpr (kRowWarps > 1) {
+        __syncthreads();
+        if (warp % kRowWarps != 0) return;
+#pragma unroll
+        for (int i = 1; i < kRowWarps; ++i) {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) {
+                const float4 x = others[warp + i][v][lane];
+                acc[v].x += x.x, acc[v].y += x.y, acc[v].z += x.z, acc[v].w += x.w;
+            }
+        }
+    }
+    if (!there || sub != 0) return;
+    const float inv = l_all > 0.0f ? 1.0f / l_all : 0.0f;
+    T* out = reinterpret_cast<T*>(p.out) + row / p.num_heads * p.o_stride.s_b + row % p.num_heads * p.o_stride.s_h;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+        const int d = v * 128 + piece * 4;
+        if (d < D) *reinterpret_cast<uint2*>(out + d) = make_uint2(Pack2<T>(acc[v].x * inv, acc[v].y * inv), Pack2<T>(acc[v].z * inv, acc[v].w * inv));
+    }
+}
+
+template <typename T, int D>
+int LaunchFp8Merge(const ScaDecodeFwdParams& p, cudaStream_t stream) {
+    const int64_t rows = p.batch * p.num_heads;
+    if (p.num_splits <= 8) LaunchDependent(decode_fp8_merge_kernel<T, D, 1>, (rows + 7) / 8, 256, 0, stream, 1, p);
+    else LaunchDependent(decode_fp8_merge_kernel<T, D, 8>, rows, 256, 0, stream, 1, p);
+    return CheckLaunch("decode_fp8_merge_kernel", stream);
 }
 
 template <typename T, int D, bool kHi>
@@ -434,8 +660,8 @@ int64_t ResidentCtas() {
     const int n = per_sm.Get([] {
         int ctas = 0;
         const void* fn = reinterpret_cast<const void*>(&decode_fp8_partial_kernel<T, D, kHi>);
-        if (EnsureDynamicSmem(fn, Fp8Geom<D>::kSmemBytes, "decode_fp8_partial_kernel") != SCA_OK ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, decode_fp8_partial_kernel<T, D, kHi>, kThreads, Fp8Geom<D>::kSmemBytes) != cudaSuccess ||
+        if (EnsureDynamicSmem(fn, Fp8Geom<D, kHi>::kSmemBytes, "decode_fp8_partial_kernel") != SCA_OK ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, decode_fp8_partial_kernel<T, D, kHi>, kThreads, Fp8Geom<D, kHi>::kSmemBytes) != cudaSuccess ||
             ctas < 1) {
             cudaGetLastError();
             return -1;
@@ -450,7 +676,7 @@ int64_t ResidentClusters(int cluster) {
     static PerDevice resident[kMaxCluster + 1];  // per instantiation
     return std::max(0, resident[cluster].Get([cluster] {
         cudaLaunchAttribute attr{};
-        cudaLaunchConfig_t cfg = ClusterConfig(static_cast<unsigned>(cluster), cluster, Fp8Geom<D>::kSmemBytes, nullptr, &attr);
+        cudaLaunchConfig_t cfg = ClusterConfig(static_cast<unsigned>(cluster), cluster, Fp8Geom<D, kHi>::kSmemBytes, nullptr, &attr);
         int n = 0;
         if (cudaOccupancyMaxActiveClusters(&n, decode_fp8_cluster_kernel<T, D, kHi>, &cfg) != cudaSuccess) {
             cudaGetLastError();
@@ -471,7 +697,7 @@ bool OneLaunchIsFaster(int64_t units, int64_t steps, int cluster, int64_t reside
 
 template <typename T, int D, bool kHi>
 int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chunks, cudaStream_t stream, int* cluster_ctas) {
-    using G = Fp8Geom<D>;
+    using G = Fp8Geom<D, kHi>;
     const int64_t columns = p.num_kv_heads * head_chunks, units = p.batch * columns;
     const int64_t steps = std::max<int64_t>(1, (std::min(p.seq_kv, p.max_blocks_per_seq * p.block_size) + kSpan - 1) / kSpan);
     const int64_t resident = ResidentCtas<T, D, kHi>();
@@ -491,7 +717,7 @@ int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chu
     const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(resident / columns, useful)) : resident;
     LaunchDependent(decode_fp8_partial_kernel<T, D, kHi>, blocks, kThreads, G::kSmemBytes, stream, 1, p, scales, head_chunks);
     if (int rc = CheckLaunch("decode_fp8_partial_kernel", stream)) return rc;
-    return LaunchMergeOut(p, stream);
+    return LaunchFp8Merge<T, D>(p, stream);
 }
 
 template <typename T, int D>
@@ -537,9 +763,21 @@ extern "C" int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, 
         return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): invalid geometry batch=" + std::to_string(p.batch) + " heads=" +
                                               std::to_string(p.num_heads) + " kv_heads=" + std::to_string(p.num_kv_heads));
     }
+    if (p.num_kv_blocks > 0 && p.block_size > 0 && p.num_kv_heads * p.head_dim / 16 > 0xffffffffLL / std::max<int64_t>(1, p.num_kv_blocks * p.block_size)) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): a pool of more than 64 GiB");
+    }
     if (p.block_size <= 0 || p.block_size % 4 != 0 || p.max_blocks_per_seq <= 0 || p.num_kv_blocks <= 0 || p.num_kv_blocks * p.block_size > 0x7fffffffLL) {
         return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): block_size=" + std::to_string(p.block_size) +
                                               " (a multiple of 4), and a pool and a table that are not empty nor beyond 2^31 tokens");
+    }
+    if (p.num_splits > 0x10000 || p.batch * ((p.max_blocks_per_seq * p.block_size + kSpan - 1) / kSpan) > 0x7fff0000LL || p.batch > 0x7fffff) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): num_splits=" + std::to_string(p.num_splits) + ", batch=" + std::to_string(p.batch) +
+                                              ": more work than the schedule counts");
+    }
+    if ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.partial_o) | static_cast<uintptr_t>(p.o_stride.s_b * 2) |
+         static_cast<uintptr_t>(p.o_stride.s_h * 2)) % 8 != 0 || !Aligned16(p.partial_o)) {
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): out must be 8-byte aligned with strides that are multiples of 4 elements, "
+                                          "partial_o 16-byte aligned");
     }
     if (!Aligned16(p.q) || !Aligned16(p.k) || !Aligned16(p.v) || p.q_stride.s_b % 8 != 0 || p.q_stride.s_h % 8 != 0 ||
         (reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales)) % 4 != 0) {

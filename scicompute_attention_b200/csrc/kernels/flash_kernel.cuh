@@ -190,18 +190,30 @@ __device__ __forceinline__ void ConvertRows(uint32_t codes, uint32_t slot, int r
     const uint32_t src = codes + row0 * kWidth + lane * 8;
     const uint32_t dst = slot + (piece / 8) * block_bytes + (row0 + sub) * 128;
     const bool whole = __all_sync(0xffffffffu, scale[0] != 0u && (kRows <= 32 || scale[1] != 0u));
+    constexpr int kTurns = kRows / kRowsPerTurn, kBatch = kTurns < 8 ? kTurns : 8;  // reads under way at once
     auto turns = [&](auto all) {
 #pragma unroll
-        for (int i = 0; i < kRows / kRowsPerTurn; ++i) {
-            const int row = i * kRowsPerTurn;  // + sub
-            uint2 c;
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(src + row * kWidth));
-            const uint32_t unit = __shfl_sync(0xffffffffu, scale[row / 32], (row & 31) + sub);
-            if (!decltype(all)::value && unit == 0u) c = make_uint2(0u, 0u);
-            const uint32_t v0 = fp8::MulHalf2(fp8::DecodeLow(c.x), unit), v1 = fp8::MulHalf2(fp8::DecodeHigh(c.x), unit);
-            const uint32_t v2 = fp8::MulHalf2(fp8::DecodeLow(c.y), unit), v3 = fp8::MulHalf2(fp8::DecodeHigh(c.y), unit);
-            const uint32_t at = dst + (((piece % 8) ^ ((row & 7) | (kRowsPerTurn > 1 ? sub : 0))) << 4) + row * 128;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
+        for (int first = 0; first < kTurns; first += kBatch) {
+            uint2 c[kBatch];
+            uint32_t unit[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c[i].x), "=r"(c[i].y) : "r"(src + (first + i) * kRowsPerTurn * kWidth));
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int row = (first + i) * kRowsPerTurn;  // + sub
+                unit[i] = __shfl_sync(0xffffffffu, scale[row / 32], (row & 31) + sub);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int row = (first + i) * kRowsPerTurn;
+                if (!decltype(all)::value && unit[i] == 0u) c[i] = make_uint2(0u, 0u);
+                const uint32_t v0 = fp8::MulHalf2(fp8::DecodeLow(c[i].x), unit[i]), v1 = fp8::MulHalf2(fp8::DecodeHigh(c[i].x), unit[i]);
+                const uint32_t v2 = fp8::MulHalf2(fp8::DecodeLow(c[i].y), unit[i]), v3 = fp8::MulHalf2(fp8::DecodeHigh(c[i].y), unit[i]);
+                const uint32_t at = dst + (((piece % 8) ^ ((row & 7) | (kRowsPerTurn > 1 ? sub : 0))) << 4) + row * 128;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
+            }
         }
     };
     if (whole) turns(std::true_type{});
@@ -225,16 +237,21 @@ __device__ __forceinline__ float HalveQueryRow(uint32_t tile, int row) {
     }
     const int k = max(static_cast<int>(max(most >> 16, most & 0xffffu) >> 7) - 127, -112);  // numbers below 2^-112 and zeros: 2^126
     const float to_half = fp8::PowerOfTwo(14 - k);
+#pragma unroll 1
+    for (int b = 0; b < kBlocks; ++b) {
+        uint4 v[8];
 #pragma unroll
-    for (int i = 0; i < 8 * kBlocks; ++i) {
-        const uint4 v = LdsV4(at(i));
-        uint32_t h[4] = {v.x, v.y, v.z, v.w};
+        for (int i = 0; i < 8; ++i) v[i] = LdsV4(at(8 * b + i));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = UnpackBf16(h[e]);
-            h[e] = Pack2<__half>(f.x * to_half, f.y * to_half);
+        for (int i = 0; i < 8; ++i) {
+            uint32_t h[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = UnpackBf16(h[e]);
+                h[e] = Pack2<__half>(f.x * to_half, f.y * to_half);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(8 * b + i)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
         }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(i)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
     }
     return fp8::PowerOfTwo(max(k - 14, -126));
 }

@@ -27,7 +27,8 @@ namespace {
 
 constexpr int64_t kMaxSplits = 64;         // as MAX_SPLITS, DECODE_STEP_TOKENS in ops.py
 constexpr int64_t kDecodeStepTokens = 64;
-constexpr int64_t kFp8StepTokens = 128;    // as FP8_STEP_TOKENS
+constexpr int64_t kFp8StepTokens = 128;    // as FP8_STEP_TOKENS, FP8_MAX_SPLITS
+constexpr int64_t kFp8MaxSplits = 512;
 
 PyObject* g_scratch = nullptr;          // ops._scratch: threading.local with the dict `pool`
 PyObject* g_acquire_scratch = nullptr;  // ops.acquire_scratch_fp32
@@ -211,11 +212,11 @@ PyObject* Flash(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // Partial slots per row, as slots_for_schedule in ops.py.
-int64_t SlotsForSchedule(int64_t column_steps, int64_t longest_steps, int64_t columns, int64_t sms) {
+int64_t SlotsForSchedule(int64_t column_steps, int64_t longest_steps, int64_t columns, int64_t sms, int64_t ctas_per_sm = 2, int64_t most = kMaxSplits) {
     if (column_steps <= 0 || longest_steps <= 1) return 1;
-    const int64_t sharers = std::max<int64_t>(1, 2 * sms / std::max<int64_t>(1, columns));
+    const int64_t sharers = std::max<int64_t>(1, ctas_per_sm * sms / std::max<int64_t>(1, columns));
     const int64_t per_cta = std::max<int64_t>(1, (column_steps + sharers - 1) / sharers);
-    return std::max<int64_t>(2, std::min((longest_steps + per_cta - 1) / per_cta + 1, kMaxSplits));
+    return std::max<int64_t>(2, std::min((longest_steps + per_cta - 1) / per_cta + 1, most));
 }
 int64_t Steps(int64_t tokens, int64_t step = kDecodeStepTokens) { return (tokens + step - 1) / step; }
 
@@ -224,11 +225,12 @@ template <typename L>
 PyObject* FinishDecode(ScaDecodeFwdParams& p, const at::Tensor& q, PyObject* q_obj, const L& launch) {
     void* stream = CurrentStream();
     const int64_t base = p.batch * p.num_heads * p.num_splits, d = p.head_dim;
+    const int64_t o_at = (2 * base + 3) / 4 * 4;  // the O of a part starts on 16 bytes
     PyObject* device = PyObject_GetAttrString(q_obj, "device");
     if (device == nullptr) throw std::runtime_error("device");
     float* scratch = nullptr;
     try {
-        scratch = Scratch(base * (2 + d), q, stream, device);
+        scratch = Scratch(o_at + base * d, q, stream, device);
     } catch (...) {
         Py_DECREF(device);
         throw;
@@ -237,7 +239,7 @@ PyObject* FinishDecode(ScaDecodeFwdParams& p, const at::Tensor& q, PyObject* q_o
     if (scratch == nullptr) return NotTaken();
     at::Tensor out = Empty({p.batch, p.num_heads, 1, d}, q, q.scalar_type());
     p.out = out.data_ptr();
-    p.partial_m = scratch, p.partial_l = scratch + base, p.partial_o = scratch + 2 * base;
+    p.partial_m = scratch, p.partial_l = scratch + base, p.partial_o = scratch + o_at;
     if (const int rc = Launch([&] { return launch(&p, stream); })) return NotLaunched(rc);
     return THPVariable_Wrap(std::move(out));
 }
@@ -573,7 +575,8 @@ PyObject* PagedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t mean = typical > 0 ? typical : std::min(p.seq_kv, table->size(1) * block_size), steps = Steps(mean, kFp8StepTokens);
         const int64_t most = longest > 0 ? Steps(longest, kFp8StepTokens) : 2 * steps, group = p.num_heads / p.num_kv_heads;
         const int64_t sms = at::cuda::getDeviceProperties(q->device().index())->multiProcessorCount;
-        p.num_splits = mean <= 0 ? 1 : SlotsForSchedule(std::max<int64_t>(1, p.batch) * steps, most, p.num_kv_heads * ((group + 15) / 16), sms);
+        const int64_t ctas = d <= 64 ? 4 : group > 8 && d > 96 ? 2 : 3;  // as fp8_ctas_per_sm
+        p.num_splits = mean <= 0 ? 1 : SlotsForSchedule(std::max<int64_t>(1, p.batch) * steps, most, p.num_kv_heads * ((group + 15) / 16), sms, ctas, kFp8MaxSplits);
         p.q = q->data_ptr(), p.k = l.layer.k_codes, p.v = l.layer.v_codes;
         p.q_stride = ScaDecodeStrides{p.num_heads * d, d, d};
         p.o_stride = p.q_stride;

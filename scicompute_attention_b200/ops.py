@@ -187,21 +187,22 @@ def acquire_scratch_fp32(elements: int, device: torch.device, kind: int = 1, *, 
 
 
 DECODE_STEP_TOKENS = 64  # tokens one CTA of the decode kernel consumes per step (4 warps x 16)
-FP8_STEP_TOKENS = 128    # the same over an 8-bit cache (4 warps x 32)
+FP8_STEP_TOKENS = 128    # the unit of the schedule over an 8-bit cache
+FP8_MAX_SPLITS = 512     # upper bound of its slot count: one sequence on every CTA of the machine
 
 
-def slots_for_schedule(column_steps: int, longest_steps: int, columns: int, sms: int) -> int:
-    """Partial slots per row for the decode kernel's schedule: one wave of resident CTAs (2 per SM), the same number
+def slots_for_schedule(column_steps: int, longest_steps: int, columns: int, sms: int, ctas_per_sm: int = 2, most: int = MAX_SPLITS) -> int:
+    """Partial slots per row for the decode kernel's schedule: one wave of resident CTAs (2 per SM unless said), the same number
     for every (kv head, head chunk) column; the CTAs of a column split its list of 64-token steps (sequence after
     sequence) into equal contiguous shares, and a sequence cut by share boundaries yields one partial per piece.
     Needed: the pieces of the longest sequence, plus one for a share that starts in its middle. (The reference's rule,
     one CTA per fixed split, is ceil(seq_kv / 512) capped at 16: src/backends/decode/decode_config.hpp:24-31.)"""
     if column_steps <= 0 or longest_steps <= 1:
         return 1
-    resident = 2 * (sms if sms > 0 else 148)
+    resident = ctas_per_sm * (sms if sms > 0 else 148)
     sharers = max(1, resident // max(1, columns))
     per_cta = max(1, -(-column_steps // sharers))
-    return max(2, min(-(-longest_steps // per_cta) + 1, MAX_SPLITS))
+    return max(2, min(-(-longest_steps // per_cta) + 1, most))
 
 
 def splits_for(seq_kv: int, batch: int, num_kv_heads: int, group: int, sms: int) -> int:
@@ -213,14 +214,14 @@ def splits_for(seq_kv: int, batch: int, num_kv_heads: int, group: int, sms: int)
 
 
 def paged_splits_for(typical_len: int, num_seqs: int, num_kv_heads: int, group: int, sms: int, longest_len: int = 0,
-                     step_tokens: int = DECODE_STEP_TOKENS) -> int:
+                     step_tokens: int = DECODE_STEP_TOKENS, ctas_per_sm: int = 2, most: int = MAX_SPLITS) -> int:
     """Slot count for a ragged batch of mean length `typical_len`; the longest sequence is taken as twice the mean
     unless `longest_len` says otherwise."""
     if typical_len <= 0:
         return 1
     steps = -(-typical_len // step_tokens)
     longest = -(-longest_len // step_tokens) if longest_len > 0 else 2 * steps
-    return slots_for_schedule(max(1, num_seqs) * steps, longest, num_kv_heads * ((group + 15) // 16), sms)
+    return slots_for_schedule(max(1, num_seqs) * steps, longest, num_kv_heads * ((group + 15) // 16), sms, ctas_per_sm, most)
 
 
 def _strides(layout: str, seq: int, heads: int, d: int) -> tuple[int, int, int]:
@@ -711,6 +712,11 @@ def fp8_pool(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
                    torch.full((num_blocks, num_kv_heads, fp8_scale_row(block_size)), 15, dtype=torch.uint8, device=device))
 
 
+def fp8_ctas_per_sm(head_dim: int, group: int) -> int:
+    """CTAs of the 8-bit decode kernel that stay on an SM."""
+    return 4 if head_dim <= 64 else 2 if group > 8 and head_dim > 96 else 3
+
+
 def _require_one_device(first: torch.Tensor, *others: torch.Tensor) -> None:
     for t in others:
         if t.device != first.device:
@@ -852,14 +858,15 @@ def paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, *, block_size: 
     max_blocks, upper = page_table.shape[1], nblk * bs
     device, handle = q.device, _stream_ptr(stream)
     splits = paged_splits_for(typical_len if typical_len > 0 else min(upper, max_blocks * bs), s, hkv, hq // hkv, sm_count(device), longest_len,
-                              FP8_STEP_TOKENS)
+                              FP8_STEP_TOKENS, fp8_ctas_per_sm(d, hq // hkv), FP8_MAX_SPLITS)
     base = s * hq * splits
-    ws = acquire_scratch_fp32(base * (2 + d), device, stream=stream, handle=handle)
+    o_at = -(-2 * base // 4) * 4  # the O of a part starts on 16 bytes
+    ws = acquire_scratch_fp32(o_at + base * d, device, stream=stream, handle=handle)
     out = _empty((s, hq, 1, d), q.dtype, device, stream)
     p = DecodeFwdParams()
     p.q, p.k, p.v, p.out = q.data_ptr(), codes.data_ptr(), v_pool[0].data_ptr(), out.data_ptr()
     scratch = ws.data_ptr()
-    p.partial_m, p.partial_l, p.partial_o = scratch, scratch + 4 * base, scratch + 8 * base
+    p.partial_m, p.partial_l, p.partial_o = scratch, scratch + 4 * base, scratch + 4 * o_at
     p.batch, p.num_heads, p.num_kv_heads, p.seq_kv, p.head_dim, p.num_splits = s, hq, hkv, upper, d, splits
     p.q_stride = DecodeStrides(hq * d, d, d)
     p.o_stride = DecodeStrides(hq * d, d, d)
