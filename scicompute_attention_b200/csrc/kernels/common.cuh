@@ -137,6 +137,9 @@ __device__ __forceinline__ void CpAsync16(uint32_t smem_dst, const void* gmem_sr
                  "r"(src_bytes)
                  : "memory");
 }
+__device__ __forceinline__ void CpAsync4(uint32_t smem_dst, const void* gmem_src, int src_bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_dst), "l"(gmem_src), "r"(src_bytes) : "memory");
+}
 __device__ __forceinline__ void CpAsyncCommit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void CpAsyncWait() {

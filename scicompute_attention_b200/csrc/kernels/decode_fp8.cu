@@ -65,9 +65,6 @@ __device__ __forceinline__ void Mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void CpAsync4(uint32_t smem_dst, const void* gmem_src, int src_bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_dst), "l"(gmem_src), "r"(src_bytes) : "memory");
-}
 // The transpose of an 8x8 matrix of 16-bit numbers spread over the warp as an operand is (row lane / 4, columns 2 * (lane % 4)).
 __device__ __forceinline__ uint32_t Transpose8x8(uint32_t v) {
     uint32_t r;

@@ -58,8 +58,8 @@ int MakeMap(CUtensorMap* map, const void* base, int dtype_id, int64_t d, int64_t
     return SCA_OK;
 }
 
-// The codes of a layer of an 8-bit cache, [rows = num_blocks * block_size][kv_heads][D]: box = `width` codes of one page of one kv head,
-// rows of `width` bytes one behind the other (no swizzle), what lies beyond D or the pool reads as zero.
+// The codes of a layer of an 8-bit cache, [rows = num_blocks * block_size][kv_heads][D]: box = `width` codes (64 or 128) of one page of one
+// kv head, keys of `width` bytes one behind the other, swizzled over that width; what lies beyond D or the pool reads as zero.
 int MakeCodesMap(CUtensorMap* map, const void* base, int64_t d, int64_t rows, int64_t heads, int box_rows, int width, const char* what) {
     EncodeTiledFn encode = GetEncodeTiled();
     if (encode == nullptr) return Fail(SCA_CUDA_ERROR, "flash attention: cuTensorMapEncodeTiled is unavailable");
@@ -68,7 +68,8 @@ int MakeCodesMap(CUtensorMap* map, const void* base, int64_t d, int64_t rows, in
     const cuuint32_t box[4] = {static_cast<cuuint32_t>(width), static_cast<cuuint32_t>(box_rows), 1, 1};
     const cuuint32_t elem[4] = {1, 1, 1, 1};
     const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) {
         return Fail(SCA_INVALID_ARGUMENT, std::string("flash attention: tensor map for ") + what + " rejected (CUresult " +
@@ -294,8 +295,8 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
     if (paged != nullptr && paged->k_scales != nullptr) {
         const int64_t rows = paged->num_blocks * paged->block_size;
         const int page = static_cast<int>(paged->block_size);
-        if (int rc = MakeCodesMap(&map_k, f.k, f.head_dim, rows, f.num_kv_heads, page, DP / G::kParts, "k codes")) return rc;
-        if (int rc = MakeCodesMap(&map_v, f.v, f.head_dim, rows, f.num_kv_heads, page, DP, "v codes")) return rc;
+        if (int rc = MakeCodesMap(&map_k, f.k, f.head_dim, rows, f.num_kv_heads, page, FlashGeom<DP, QT, BN, true>::kBoxWidth, "k codes")) return rc;
+        if (int rc = MakeCodesMap(&map_v, f.v, f.head_dim, rows, f.num_kv_heads, page, FlashGeom<DP, QT, BN, true>::kBoxWidth, "v codes")) return rc;
     } else if (paged != nullptr) {
         // the pool as [rows = blocks * block_size, H_kv, D]; one box = one page of one kv head and column block
         const int64_t rows = paged->num_blocks * paged->block_size;

@@ -84,12 +84,13 @@ struct FlashGeom {
     static constexpr int kVBlockBytes = kVKeys * 128;       // one column block of V in a slot
     static constexpr int kSlotBytes = BN * DP * 2 / kParts;
     static constexpr int kSlots = kKv8 ? RawRingOf(DP).slots : RingOf(DP).slots;
-    // kKv8: a raw slot holds the codes of a load, key by key, and their scales: BN bytes, twice as many with pages of 8 keys
+    // kKv8: a raw slot holds the codes of a load, key by key, and a scale for each of its keys
     static constexpr int kRawSlots = kKv8 ? RawRingOf(DP).raw_slots : 0;
     static constexpr int kRawCodes = kSlotBytes / 2;
-    static constexpr int kRawBytes = kRawCodes + 2 * BN;
+    static constexpr int kRawBytes = kRawCodes + BN;        // the scales of all raw slots lie behind the codes of all
+    static constexpr int kBoxWidth = DP < 128 ? DP : 128;   // codes of a key in a box: V of D=256 has two side by side
     static constexpr int kRingBytes = kSlots * kSlotBytes + kRawSlots * kRawBytes;
-    static constexpr int kBarrierBytes = 512;
+    static constexpr int kBarrierBytes = kKv8 ? 1024 : 512;  // kKv8: the last 256 of them are the producers' page rows
     static constexpr int kSmemBytes = 1024 + QT * kQTileBytes + kRingBytes + kBarrierBytes;
     static constexpr int kSCol = 0;                         // S_t at kSCol + t * BN
     static constexpr int kOCol = 256;                       // O_t at kOCol + t * DP
@@ -166,58 +167,61 @@ __device__ __forceinline__ int TilesFor(int m0, int tokens, int seq_q, int seq_k
 // three 172, four 146 (B=1, S=3000, lasting load). One warp is too few at D=128 (four prompts of 4096: 632 against 595).
 template <typename T, int DP, bool kKv8 = false>
 constexpr int ConverterWarps() {
-    return kKv8 || PvFormat<T>::kConvertV ? RingOf(DP).converters : 0;
+    return kKv8 ? RawRingOf(DP).converters : PvFormat<T>::kConvertV ? RingOf(DP).converters : 0;
 }
 // Warps of a CTA: 0 TMA and tensor-memory owner, 1 MMA, 2 and 3 V converters (idle for fp16), then four per query tile for
 // the softmax, then what converters are left.
 constexpr int kFirstSoftmax = 4;
+// kKv8 with two query tiles: the converters are a warpgroup of their own behind the softmax (warp 2 issues loads, warp 3 idles) and hand
+// registers to it: 16 warps are launched with 128 a thread, the softmax wants 168. One query tile: a warp more, which issues loads.
+template <int QT, bool kKv8>
+constexpr bool ConvertersApart() {
+    return kKv8 && QT == 2;
+}
 template <typename T, int DP, int QT, bool kKv8 = false>
 constexpr int FlashThreads() {
-    return 32 * (kFirstSoftmax + 4 * QT + (ConverterWarps<T, DP, kKv8>() > 2 ? ConverterWarps<T, DP, kKv8>() - 2 : 0));
+    return ConvertersApart<QT, kKv8>() ? 512 : 32 * (kFirstSoftmax + 4 * QT + (ConverterWarps<T, DP, kKv8>() > 2 ? ConverterWarps<T, DP, kKv8>() - 2 : 0) + (kKv8 ? 1 : 0));
 }
 
-// kKv8, one converter warp: `kRows` rows of `kWidth` codes, a row behind the other at `codes`, become fp16 numbers in the layout of the
-// ring: column blocks of 64 numbers, `block_bytes` apart, rows of 128 bytes, 128-byte swizzle. Lane l holds the scale of row l in
-// scale[0] and of row 32 + l in scale[1] (pairs of fp16; 0: the row counts for nothing, whatever its codes). `row0`: the first row's
-// place in the tile, a multiple of 8. 8 codes per lane and turn: reads of 8 bytes and writes of 16 both touch every bank once.
-template <int kRows, int kWidth>
-__device__ __forceinline__ void ConvertRows(uint32_t codes, uint32_t slot, int row0, uint32_t block_bytes, const uint32_t (&scale)[2], int lane) {
-    constexpr int kPieces = kWidth / 8;              // of a row
-    constexpr int kRowsPerTurn = 32 / kPieces;
-    static_assert(kPieces == 8 || kPieces == 16 || kPieces == 32, "a turn covers whole rows");
-    static_assert(kRows <= 64, "two scales per lane");
-    const int piece = lane % kPieces, sub = lane / kPieces;
-    const uint32_t src = codes + row0 * kWidth + lane * 8;
-    const uint32_t dst = slot + (piece / 8) * block_bytes + (row0 + sub) * 128;
-    const bool whole = __all_sync(0xffffffffu, scale[0] != 0u && (kRows <= 32 || scale[1] != 0u));
-    constexpr int kTurns = kRows / kRowsPerTurn, kBatch = kTurns < 8 ? kTurns : 8;  // reads under way at once
-    auto turns = [&](auto all) {
+// kKv8, one converter warp: each lane turns `kWidth` codes of a key (64 or 128, the width of a raw box) into fp16 numbers in the layout of
+// the ring: column blocks of 64 numbers, `block_bytes` apart, keys of 128 bytes, 128-byte swizzle. `codes`: where the lane's key lies in
+// its box, which the load has swizzled over its width; `to`: its place in the slot's first column block; `row`: the key's place in the
+// tile. `unit`: its scale as a pair of fp16 numbers, 0: the key counts for nothing, whatever its codes. A lane to a key needs no
+// scales of others, and the swizzles spread the 16-byte reads and writes of 8 lanes over all banks. Few reads under way at once are
+// better than many: what is limited is the queue to the shared memory, which the softmax and the tensor core's operands share (D=256,
+// 20 chunks: two groups of four in flight 885 us, one 848).
+template <int kWidth>
+__device__ __forceinline__ void ConvertKey(uint32_t codes, uint32_t to, int row, uint32_t block_bytes, uint32_t unit) {
+    constexpr int kPieces = kWidth / 16;  // of 16 codes
+    static_assert(kWidth == 64 || kWidth == 128, "width of a raw box");
+    const uint32_t read = codes + ((kWidth == 128 ? row & 7 : (row >> 1) & 3) << 4);  // + 0, then ^ (piece << 4): the low bits of `codes` are 0
+    const uint32_t write = to + ((row & 7) << 4);
 #pragma unroll
-        for (int first = 0; first < kTurns; first += kBatch) {
-            uint2 c[kBatch];
-            uint32_t unit[kBatch];
+    for (int first = 0; first < kPieces; first += 2) {
+        uint4 c[2];
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c[i].x), "=r"(c[i].y) : "r"(src + (first + i) * kRowsPerTurn * kWidth));
-            }
+        for (int i = 0; i < 2; ++i) {
+            c[i] = LdsV4(read ^ ((first + i) << 4));
+            if (unit == 0u) c[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int row = (first + i) * kRowsPerTurn;  // + sub
-                unit[i] = __shfl_sync(0xffffffffu, scale[row / 32], (row & 31) + sub);
-            }
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t words[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int row = (first + i) * kRowsPerTurn;
-                if (!decltype(all)::value && unit[i] == 0u) c[i] = make_uint2(0u, 0u);
-                const uint32_t v0 = fp8::MulHalf2(fp8::DecodeLow(c[i].x), unit[i]), v1 = fp8::MulHalf2(fp8::DecodeHigh(c[i].x), unit[i]);
-                const uint32_t v2 = fp8::MulHalf2(fp8::DecodeLow(c[i].y), unit[i]), v3 = fp8::MulHalf2(fp8::DecodeHigh(c[i].y), unit[i]);
-                const uint32_t at = dst + (((piece % 8) ^ ((row & 7) | (kRowsPerTurn > 1 ? sub : 0))) << 4) + row * 128;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory");
+            for (int half = 0; half < 2; ++half) {
+                const int piece = 2 * (first + i) + half;  // of 8 numbers
+                uint32_t v[4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    v[2 * e] = fp8::MulHalf2(fp8::DecodeLow(words[2 * half + e]), unit);
+                    v[2 * e + 1] = fp8::MulHalf2(fp8::DecodeHigh(words[2 * half + e]), unit);
+                }
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((write ^ ((piece % 8) << 4)) + (piece / 8) * block_bytes), "r"(v[0]),
+                             "r"(v[1]), "r"(v[2]), "r"(v[3])
+                             : "memory");
             }
         }
-    };
-    if (whole) turns(std::true_type{});
-    else turns(std::false_type{});
+    }
 }
 
 // kKv8, bf16 queries: the row of a query tile that this thread looks after becomes fp16 numbers, times the power of two that puts the
@@ -314,14 +318,16 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // it loads the K tile and read by the softmax groups; indexed by the CTA's running KV-tile count
     constexpr int kValidRing = 16;
     volatile uint32_t* valid_ring = reinterpret_cast<volatile uint32_t*>(tmem_slot + 2);
-    static_assert(kNumBars * 8 + 8 + kValidRing * 4 <= G::kBarrierBytes, "barrier area too small");
+    static_assert(kNumBars * 8 + 8 + kValidRing * 4 <= G::kBarrierBytes - (kKv8 ? 256 : 0), "barrier area too small");
 
     constexpr bool kOwnP = G::kOwnP;
     constexpr int kParts = G::kParts;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     constexpr int kEndSoftmax = kFirstSoftmax + 4 * QT;
-    const int converter = warp < kFirstSoftmax ? warp - 2 : warp >= kEndSoftmax ? warp - kEndSoftmax + 2 : -1;
+    constexpr bool kApart = ConvertersApart<QT, kKv8>();
+    constexpr int kProducer1 = kApart ? 2 : kEndSoftmax + 2;  // kKv8: the second warp that issues loads
+    const int converter = kApart ? (warp >= kEndSoftmax ? warp - kEndSoftmax : -1) : warp < kFirstSoftmax ? warp - 2 : warp >= kEndSoftmax ? warp - kEndSoftmax + 2 : -1;
 
     // ---- Packed heads: P = 1 << pack_shift query heads of one kv head share a query tile (row r = token m0 + r / P, head
     // h + r % P). They read the same K/V tiles, so the rows of a short or ragged chunk fill up with other heads instead
@@ -410,11 +416,11 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         for (int i = 0; i < 2 * G::kSlots; ++i) MbarInit<1>(bar(kKvFull + i));
         for (int i = 0; i < G::kSlots; ++i) {
             MbarInit<1>(bar(kKvEmpty + i));
-            if constexpr (kCvtInKernel) MbarInit<32 * kConverters>(bar(kVReady + i));
+            if constexpr (kCvtInKernel) MbarInit<kKv8 ? kConverters : 32 * kConverters>(bar(kVReady + i));
         }
         if constexpr (kKv8) {
             for (int i = 0; i < G::kRawSlots; ++i) {
-                MbarInit<1>(bar(kRawFull + i));
+                MbarInit<1 + 32>(bar(kRawFull + i));  // the codes, and each lane's copy of scales
                 MbarInit<kConverters>(bar(kRawEmpty + i));
             }
             for (int i = 0; kHalveQ && i < kTiles; ++i) MbarInit<4>(bar(kQHalf + i));
@@ -432,13 +438,115 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     TcFenceAfter();
     const uint32_t tmem_base = *tmem_slot;
     BeginAfterPredecessor();
+    // kApart: 128 * (kIssueRegs + 2 * kSoftmaxRegs + kConvertRegs) registers of the 512 * 128 that the CTA was launched with
+    constexpr int kIssueRegs = 96, kSoftmaxRegs = 168, kConvertRegs = 72;
+    static_assert(kIssueRegs + 2 * kSoftmaxRegs + kConvertRegs <= 512, "more registers than the CTA has");
+    if (kApart && warp < kFirstSoftmax) KeepRegisters<kIssueRegs>();
 
     bool failed = false;
     // kSplit: a row of a CTA's part is {O[DP], m, l}, padded so that neighbouring rows lie on different banks
     constexpr int kPartLd = DP + 4;
     static_assert(!kSplit || kBlockM * kPartLd * 4 <= G::kRingBytes, "a part has to fit the ring");
 
-    if (warp == 0 && kPaged) {
+    if (kKv8 && (warp == 0 || warp == kProducer1)) {
+        // ================================ TMA producers, 8-bit cache =================================
+        // Two warps take the loads in turn (raw slots are even in number: a slot belongs to one of them): one that issues all of
+        // them - at 16 tokens to a page 8 boxes of a page each - is what the converters wait for. The lanes fetch the page
+        // ids of a warp's next load ahead and copy its scales, four keys each; one lane issues the boxes, whose rows it finds in shared memory.
+        // A page that is unmapped is loaded from beyond the pool, i.e. zero-filled, and masked through valid_ring.
+        static_assert(!kKv8 || G::kRawSlots % 2 == 0, "each producer fills slots of its own");
+        const int producer = warp == 0 ? 0 : 1;
+        if (lane == 0) {
+            if (producer == 0) PrefetchTensorMap(&map_q);
+            PrefetchTensorMap(&map_k);
+            PrefetchTensorMap(&map_v);
+        }
+        constexpr int kRaw = kKv8 ? G::kRawSlots : 1;
+        int* page_rows = reinterpret_cast<int*>(smem + (bar_base - smem_base) + G::kBarrierBytes - 256) + 32 * producer;
+        uint32_t q_uses[kTiles] = {};
+        uint32_t kv_base = 0;       // loads of the items before
+        uint32_t tiles_before = 0;  // KV tiles of them
+        const int pages_per_tile = BN >> p.block_shift, pages_per_v = G::kVKeys >> p.block_shift;
+        bool ok = true;
+        for (int r = 0; r < rounds && ok; ++r) {
+            const int idx = item_of_round(r);
+            if (idx < 0) continue;
+            const Item w = decode_item(idx);
+            if (producer == 0 && lane == 0) {
+                for (int t = 0; t < QT && ok; ++t) {
+                    if (w.ntiles[t] == 0) continue;
+                    if (q_uses[t] > 0) ok = MbarWait(bar(kQEmpty + t), (q_uses[t] - 1) & 1u, abort_flag);
+                    if (!ok) break;
+                    MbarExpectTx(bar(kQFull + t), G::kQTileBytes);
+                    for (int kb = 0; kb < G::kKBlocks; ++kb) {
+                        TmaLoad4D(q_smem + t * G::kQTileBytes + kb * G::kQBlockBytes, &map_q, bar(kQFull + t), kb * 64,
+                                  w.h, w.q_tok0 + w.m0[t], w.b);
+                    }
+                    ++q_uses[t];
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            const int32_t* row = p.page_table + static_cast<int64_t>(w.seq) * p.max_blocks_per_seq;
+            const int loads = 2 * w.n_max * kParts;
+            auto page_ids = [&](int it) {  // of the tile of load `it`, one per lane
+                if (it >= loads) return -1;
+                const int logical = ((kSplit ? w.first_tile : 0) + RingOrder(it / kParts, w.n_max, kOwnP).tile) * pages_per_tile + lane;
+                const bool in = lane < pages_per_tile && logical < p.max_blocks_per_seq && (static_cast<int64_t>(logical) << p.block_shift) < w.seq_kv;
+                return in ? row[logical] : -1;
+            };
+            int it = (kv_base ^ producer) & 1;
+            int32_t phys, phys_next = page_ids(it);
+            for (; it < loads && ok; it += 2) {
+                phys = phys_next;
+                phys_next = page_ids(it + 2);
+                const RingLoad load = RingOrder(it / kParts, w.n_max, kOwnP);
+                const bool there = phys >= 0 && phys < p.num_kv_blocks;
+                const uint32_t valid = __ballot_sync(0xffffffffu, there);
+                const uint32_t raw = (kv_base + it) % kRaw;
+                const uint32_t full = bar(kRawFull + raw);
+                if (lane == 0) {
+                    ok = MbarWait(bar(kRawEmpty + raw), (((kv_base + it) / kRaw) & 1u) ^ 1u, abort_flag);
+                    if (ok) {
+                        if (!load.is_v) valid_ring[(tiles_before + load.tile) % kValidRing] = valid;
+                        MbarExpectTx(full, G::kRawCodes);
+                    }
+                }
+                page_rows[lane] = there ? phys << p.block_shift : p.num_kv_blocks << p.block_shift;
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                if (!ok) break;
+                const uint32_t dst = raw_smem + raw * G::kRawCodes;
+                const int part = it % kParts;
+                const int first_page = load.is_v ? part * pages_per_v : 0, pages = load.is_v ? pages_per_v : pages_per_tile;
+                __syncwarp();
+                if (ElectOne()) {
+                    auto boxes = [&](const CUtensorMap* map, int column, uint32_t to) {
+#pragma unroll 2
+                        for (int pg = first_page; pg < first_page + pages; ++pg, to += G::kBoxWidth << p.block_shift) TmaLoad4D(to, map, full, column, page_rows[pg], w.h_kv, 0);
+                    };
+                    if (load.is_v) {
+#pragma unroll
+                        for (int box = 0; box < DP / G::kBoxWidth; ++box) boxes(&map_v, box * G::kBoxWidth, dst + box * G::kVKeys * G::kBoxWidth);
+                    } else {
+                        boxes(&map_k, part * G::kBoxWidth, dst);
+                    }
+                }
+                __syncwarp();
+                {
+                    // the scales of four keys of one page per lane; they count as landed when the lane's copies have
+                    const int key = 4 * lane, page = (first_page + (key >> p.block_shift)) & 31;
+                    const int32_t id = __shfl_sync(0xffffffffu, phys, page);
+                    const bool mapped = (valid >> page) & 1u;
+                    const uint8_t* from = (load.is_v ? p.v_scales : p.k_scales) +
+                                          (mapped ? (static_cast<int64_t>(id) * p.kv_heads + w.h_kv) * p.scale_row + (key & (p.block_size - 1)) : 0);
+                    if (key < (pages << p.block_shift)) CpAsync4(raw_smem + G::kRawSlots * G::kRawCodes + raw * BN + key, from, mapped ? 4 : 0);
+                    CpAsyncArrive(full);
+                }
+            }
+            kv_base += static_cast<uint32_t>(loads);
+            tiles_before += static_cast<uint32_t>(w.n_max);
+        }
+        failed = !ok;
+    } else if (warp == 0 && kPaged) {
         // ================================ TMA producer, paged K/V ===================================
         // The whole warp walks the work list: the lanes fetch the page ids of a tile together (one coalesced read
         // of the table row), lane 0 waits for the ring slot and one lane issues a box load per page and column block. The
@@ -504,38 +612,6 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 const bool mapped = phys >= 0 && phys < p.num_kv_blocks;
                 const uint32_t valid = __ballot_sync(0xffffffffu, mapped);
-                if constexpr (kKv8) {
-                    const uint32_t raw = kv_loads % (kKv8 ? G::kRawSlots : 1);
-                    const int part8 = it % kParts;
-                    const int first_page = is_v ? part8 * pages_per_v : 0, pages = is_v ? pages_per_v : pages_per_tile;
-                    const uint32_t width = is_v ? DP : DP / kParts;  // codes of a key in this load
-                    const uint32_t wanted = (pages >= 32 ? 0xffffffffu : (1u << pages) - 1u) << first_page;
-                    const uint32_t full = bar(kRawFull + raw);
-                    if (lane == 0) {
-                        ok = MbarWait(bar(kRawEmpty + raw), ((kv_loads / (kKv8 ? G::kRawSlots : 1)) & 1u) ^ 1u, abort_flag);
-                        if (ok) {
-                            if (!is_v) valid_ring[(tiles_before + tile) % kValidRing] = valid;
-                            MbarExpectTx(full, G::kRawCodes + __popc(valid & wanted) * p.scale_row);
-                        }
-                    }
-                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                    if (!ok) break;
-                    uint32_t dst = raw_smem + raw * G::kRawBytes;
-                    uint32_t scale_dst = dst + G::kRawCodes;
-                    const uint8_t* scales = is_v ? p.v_scales : p.k_scales;
-                    for (int pg = first_page; pg < first_page + pages; ++pg) {
-                        const int32_t id = __shfl_sync(0xffffffffu, phys, pg);
-                        const bool there = (valid >> pg) & 1u;
-                        if (ElectOne()) {
-                            TmaLoad4D(dst, is_v ? &map_v : &map_k, full, is_v ? 0 : part8 * static_cast<int>(width),
-                                      there ? (id << p.block_shift) : (p.num_kv_blocks << p.block_shift), w.h_kv, 0);
-                            if (there) BulkLoad(scale_dst, scales + (static_cast<int64_t>(id) * p.kv_heads + w.h_kv) * p.scale_row, p.scale_row, full);
-                        }
-                        dst += width << p.block_shift;
-                        scale_dst += p.scale_row;
-                    }
-                    continue;
-                }
                 const uint32_t slot = kv_loads % G::kSlots;
                 const uint32_t phase = (kv_loads / G::kSlots) & 1u;
                 if (lane == 0) {
@@ -780,8 +856,11 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     const int it_v = 2 * j + 1;
                     const int it_k = 2 * j + 2;
                     ok = v_ready(slot_of(it_v));
-                    if (ok && j + 1 < w.n_max) ok = k_landed(slot_of(it_k));
+                    // kKv8: K is behind V in the ring of the converters, and P V need not wait for it
+                    bool k_there = kKv8 || j + 1 >= w.n_max;
+                    if (ok && !k_there) ok = k_landed(slot_of(it_k));
                     if (!ok) break;
+                    k_there = !kKv8 || j + 1 >= w.n_max;
                     for (int t = 0; t < QT; ++t) {
                         if (j >= w.ntiles[t]) continue;
                         ok = MbarWait(bar(kPFull + t), steps[t] & 1u, abort_flag);
@@ -793,6 +872,12 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                         if (!ok) break;
                         MmaCommit(bar(kODone + t));
                         ++steps[t];
+                        if (!k_there) {
+                            ok = k_landed(slot_of(it_k));
+                            if (!ok) break;
+                            TcFenceAfter();
+                            k_there = true;
+                        }
                         if (j + 1 < w.ntiles[t]) {
                             issue_s(t, slot_of(it_k), 0);
                             MmaCommit(bar(kSFull + t));
@@ -815,6 +900,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         // Walks the ring in the producer's order; every V tile is rewritten in place from bf16 to fp16 once its
         // bytes have landed, then handed to the MMA thread through v_ready. K tiles are not touched. kKv8: the codes
         // of K and V go from their raw slot into a slot of the ring.
+        if constexpr (kApart) KeepRegisters<kConvertRegs>();
         uint32_t kv_loads = 0;
         uint32_t tiles_before = 0;  // kKv8: index into valid_ring
         RingPhases v_phases;
@@ -832,33 +918,28 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     ok = __all_sync(0xffffffffu, MbarWait(bar(kRawFull + raw), (kv_loads / (kKv8 ? G::kRawSlots : 1)) & 1u, abort_flag) &&
                                                      MbarWait(bar(kKvEmpty + slot), ((kv_loads / G::kSlots) & 1u) ^ 1u, abort_flag));
                     if (!ok) break;
-                    const uint32_t codes = raw_smem + raw * G::kRawBytes, target = ring_smem + slot * G::kSlotBytes;
+                    const uint32_t codes = raw_smem + raw * G::kRawCodes, target = ring_smem + slot * G::kSlotBytes;
                     const uint32_t pages = valid_ring[(tiles_before + load.tile) % kValidRing];
                     const int key0 = ((kSplit ? w.first_tile : 0) + load.tile) * BN;
-                    const int part = it % kParts;
-                    auto convert = [&](auto rows_of_load, auto width, int tile_row0, uint32_t block_bytes) {
-                        constexpr int kRows = decltype(rows_of_load)::value / kConverters;  // of this warp
-                        const int row0 = converter * kRows;
-                        uint32_t scale[2] = {0u, 0u};
-#pragma unroll
-                        for (int i = 0; i < (kRows + 31) / 32; ++i) {
-                            const int row = row0 + 32 * i + (lane & (kRows < 32 ? kRows - 1 : 31)), tile_row = tile_row0 + row;
-                            const bool there = ((pages >> (tile_row >> p.block_shift)) & 1u) && key0 + tile_row < w.seq_kv;
-                            uint32_t byte;
-                            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(codes + G::kRawCodes + (row >> p.block_shift) * p.scale_row + (row & (p.block_size - 1))));
-                            scale[i] = there ? fp8::ScalePair(byte, byte) : 0u;
-                        }
-                        ConvertRows<kRows, decltype(width)::value>(codes, target, row0, block_bytes, scale, lane);
+                    auto convert = [&](auto keys_of_load, int tile_row0, uint32_t block_bytes) {
+                        constexpr int kKeys = decltype(keys_of_load)::value / kConverters;  // of this warp; 16: two boxes side by side
+                        static_assert(kKeys == 32 || (kKeys == 16 && DP == 256), "a lane to a key of a box");
+                        const int row = converter * kKeys + lane % kKeys, box = lane / kKeys, tile_row = tile_row0 + row;
+                        const bool there = ((pages >> (tile_row >> p.block_shift)) & 1u) && key0 + tile_row < w.seq_kv;
+                        uint32_t byte;
+                        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(raw_smem + G::kRawSlots * G::kRawCodes + raw * BN + row));
+                        ConvertKey<G::kBoxWidth>(codes + (box * decltype(keys_of_load)::value + row) * G::kBoxWidth,
+                                                 target + box * (G::kBoxWidth / 64) * block_bytes + row * 128, row, block_bytes,
+                                                 there ? fp8::ScalePair(byte, byte) : 0u);
                     };
-                    if (load.is_v) {
-                        convert(std::integral_constant<int, G::kVKeys>{}, std::integral_constant<int, DP>{}, part * G::kVKeys, G::kVBlockBytes);
-                    } else {
-                        convert(std::integral_constant<int, BN>{}, std::integral_constant<int, DP / kParts>{}, 0, G::kKBlockBytes);
-                    }
+                    if (load.is_v) convert(std::integral_constant<int, G::kVKeys>{}, it % kParts * G::kVKeys, G::kVBlockBytes);
+                    else convert(std::integral_constant<int, BN>{}, 0, G::kKBlockBytes);
                     FenceProxyAsync();  // generic-proxy writes -> visible to the tensor core's reads
-                    MbarArrive(bar(kVReady + slot));
                     __syncwarp();
-                    if (lane == 0) MbarArrive(bar(kRawEmpty + raw));
+                    if (lane == 0) {
+                        MbarArrive(bar(kVReady + slot));
+                        MbarArrive(bar(kRawEmpty + raw));
+                    }
                     continue;
                 }
                 ok = __all_sync(0xffffffffu, MbarWait(full_bar(true, slot), v_phases.Take(slot), abort_flag));
@@ -884,6 +965,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         failed = !ok;
     } else if (warp >= kFirstSoftmax && warp < kEndSoftmax) {
         // ================================ softmax groups ============================================
+        if constexpr (kApart) TakeRegisters<kSoftmaxRegs>();
         const int t = (warp - kFirstSoftmax) >> 2;
         const int quad = warp & 3;
         const int row_in_tile = quad * 32 + lane;

@@ -30,9 +30,10 @@ constexpr RingShape RingOf(int padded_dim) {
 struct RawRingShape {
     int slots;
     int raw_slots;
+    int converters;
 };
 constexpr RawRingShape RawRingOf(int padded_dim) {
-    return padded_dim == 64 ? RawRingShape{6, 6} : RawRingShape{3, 4};
+    return padded_dim == 64 ? RawRingShape{6, 6, 4} : RawRingShape{3, 4, 4};
 }
 
 struct RingLoad {

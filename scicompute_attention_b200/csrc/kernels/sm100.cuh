@@ -103,11 +103,9 @@ __device__ __forceinline__ void TmaLoad4D(uint32_t smem_dst, const CUtensorMap* 
         : "memory");
 }
 
-// `bytes` of global memory to shared memory of this CTA, counted on `bar`; both addresses and the size are multiples of 16.
-__device__ __forceinline__ void BulkLoad(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
+// Arrives on `bar` (one of the arrivals it was set up for) once the cp.async copies that this thread has issued so far have landed.
+__device__ __forceinline__ void CpAsyncArrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- tensor memory -----------------------------------------------------------------------------------
@@ -169,6 +167,17 @@ __device__ __forceinline__ bool ElectOne() {
         "}\n"
         : "=r"(leader));
     return leader != 0;
+}
+
+// A warpgroup gives back all but kCount registers a thread, or takes up to kCount of what others have given back. What all of them
+// hold in the end must not exceed what the CTA was launched with: a taker waits for its share.
+template <int kCount>
+__device__ __forceinline__ void KeepRegisters() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCount));
+}
+template <int kCount>
+__device__ __forceinline__ void TakeRegisters() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCount));
 }
 
 // ---- tcgen05.mma (dense f16/bf16 inputs, f32 accumulate, one CTA) -----------------------------------
