@@ -12,24 +12,43 @@ namespace {
 
 constexpr int kFp8Threads = 256;
 
-// Eight consecutive numbers of a row.
+constexpr int kPiece = 16;  // numbers a lane takes
+
+// kPiece consecutive numbers of a row as they come, by 32-byte loads where `aligned` says that rows start on a 32-byte boundary.
 template <typename T>
-__device__ __forceinline__ void Load8(const T* src, bool aligned, float (&x)[8]) {
-    if (aligned) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+struct Piece {
+    static constexpr int kWords = kPiece * sizeof(T) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void Load(const T* src, bool aligned) {
+        if (aligned) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 8) {
+                asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                             : "l"(reinterpret_cast<const uint32_t*>(src) + i)
+                             : "memory");
+            }
         } else {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            const T* t = reinterpret_cast<const T*>(&v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = ToFloat(t[i]);
+            for (int i = 0; i < kPiece; ++i) reinterpret_cast<T*>(w)[i] = src[i];
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = ToFloat(src[i]);
     }
-}
+    __device__ __forceinline__ float operator[](int i) const { return ToFloat(reinterpret_cast<const T*>(w)[i]); }
+    // The largest number; NaN is passed over.
+    __device__ __forceinline__ float Largest() const {
+        float m = 0.0f;  // fmaxf passes over NaN
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) m = fmaxf(m, fabsf((*this)[i]));
+        return m;
+    }
+    // 16 bits: the same as its bits without the sign, which compare as whole numbers do - with a NaN above all numbers.
+    __device__ __forceinline__ uint32_t LargestBits() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        return max(m >> 16, m & 0xffffu);
+    }
+};
 
 // Where rows go: `slots` (one per token), or the page table at position seq_lens[token] - 1 (one token per sequence).
 struct AppendTarget {
@@ -40,82 +59,106 @@ struct AppendTarget {
     int64_t max_blocks_per_seq;
     int64_t num_blocks;
     int block_size, heads, head_dim;
-    bool aligned;  // the new rows start on 16-byte boundaries
+    bool aligned;  // the new rows start on 32-byte boundaries
 };
 
-// Slot of a token, -1 where it is not stored.
+// Slot of a token, -1 where it is not stored. Pools have less than 2^31 slots.
 template <bool kBatched>
-__device__ __forceinline__ int64_t SlotOf(const AppendTarget& a, int64_t token) {
+__device__ __forceinline__ int SlotOf(const AppendTarget& a, int64_t token) {
     if constexpr (!kBatched) {
-        const int32_t slot = a.slots[token];
-        return slot >= 0 && slot < a.num_blocks * a.block_size ? slot : -1;
+        const int slot = a.slots[token];
+        return slot < a.num_blocks * a.block_size ? slot : -1;
     } else {
         const int pos = a.seq_lens[token] - 1;
         if (pos < 0) return -1;
         const int logical = pos / a.block_size;
         if (logical >= a.max_blocks_per_seq) return -1;
-        const int32_t phys = a.page_table[token * a.max_blocks_per_seq + logical];
+        const int phys = a.page_table[token * a.max_blocks_per_seq + logical];
         if (phys < 0 || phys >= a.num_blocks) return -1;
-        return static_cast<int64_t>(phys) * a.block_size + (pos - logical * a.block_size);
+        return phys * a.block_size + (pos - logical * a.block_size);
     }
 }
 
-// kLanes lanes of a warp (the smallest power of two that covers D / 8) take a row of K and the same row of V: 8 numbers each,
-// the largest by shuffles, 8 codes each. I: type of a row's number.
+// kLanes lanes of a warp (the smallest power of two that covers D / 16) take a row of K and the same row of V: 16 numbers each, the
+// largest by shuffles, 16 codes each. I: type of a row's number. Bound by HBM, and by how much of it is under way: each lane has 64 bytes
+// of K and V on their way (128 of fp32) before it looks at the first.
 template <typename T, int kLanes, bool kBatched, typename I>
 __global__ void __launch_bounds__(kFp8Threads)
 kv_append_fp8_kernel(const T* k_new, const T* v_new, const I rows, const AppendTarget a) {
     BeginAfterPredecessor();
     constexpr int kRows = kFp8Threads / kLanes;  // of a CTA
     const int piece = threadIdx.x % kLanes;
-    const bool in_row = piece * 8 < a.head_dim;
+    const bool in_row = piece * kPiece < a.head_dim;
     for (I base = static_cast<I>(blockIdx.x) * kRows; base < rows; base += static_cast<I>(gridDim.x) * kRows) {
         const I row = base + threadIdx.x / kLanes;
         const bool mine = row < rows && in_row;
-        float x[2][8];
+        Piece<T> x[2];
         if (mine) {
-            Load8(k_new + static_cast<int64_t>(row) * a.head_dim + piece * 8, a.aligned, x[0]);
-            Load8(v_new + static_cast<int64_t>(row) * a.head_dim + piece * 8, a.aligned, x[1]);
+            x[0].Load(k_new + static_cast<int64_t>(row) * a.head_dim + piece * kPiece, a.aligned);
+            x[1].Load(v_new + static_cast<int64_t>(row) * a.head_dim + piece * kPiece, a.aligned);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[0][i] = x[1][i] = 0.0f;
+            for (int i = 0; i < Piece<T>::kWords; ++i) x[0].w[i] = x[1].w[i] = 0;
         }
         const I token = row / a.heads;
         const int head = static_cast<int>(row - token * a.heads);
-        const int64_t slot = row < rows ? SlotOf<kBatched>(a, token) : -1;
+        const int slot = row < rows ? SlotOf<kBatched>(a, token) : -1;
         float amax[2];
+        bool by_value = sizeof(T) == 4;
+        if constexpr (sizeof(T) == 2) {
+            uint32_t most = x[0].LargestBits() << 16 | x[1].LargestBits();  // K and V in one
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            float m = 0.0f;  // fmaxf passes over NaN
+            for (int o = 1; o < kLanes; o <<= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+            amax[0] = fminf(ToFloat(*(reinterpret_cast<const T*>(&most) + 1)), fp8::kLargest);
+            amax[1] = fminf(ToFloat(*reinterpret_cast<const T*>(&most)), fp8::kLargest);
+            constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+            by_value = __any_sync(0xffffffffu, (most >> 16) > kInf || (most & 0xffffu) > kInf);
+        }
+        if (by_value) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[s][i]));
+            for (int s = 0; s < 2; ++s) {
+                float m = x[s].Largest();
 #pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            amax[s] = fminf(m, fp8::kLargest);
+                for (int o = 1; o < kLanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                amax[s] = fminf(m, fp8::kLargest);
+            }
         }
         if (!mine || slot < 0) continue;
-        const int64_t block = slot / a.block_size;
-        const int offset = static_cast<int>(slot - block * a.block_size);
-        const int64_t code_at = (slot * a.heads + head) * a.head_dim + piece * 8;
-        const int64_t scale_at = (block * a.heads + head) * fp8::ScaleRow(a.block_size) + offset;
+        const int block = slot / a.block_size, offset = slot - block * a.block_size;
+        const int64_t code_at = (static_cast<int64_t>(slot) * a.heads + head) * a.head_dim + piece * kPiece;
+        const int64_t scale_at = (static_cast<int64_t>(block) * a.heads + head) * fp8::ScaleRow(a.block_size) + offset;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int e = fp8::ExponentFor(amax[s]);
             const float inv = fp8::PowerOfTwo(-e);
-            uint2 codes;
-            codes.x = fp8::Encode2(x[s][0] * inv, x[s][1] * inv) | fp8::Encode2(x[s][2] * inv, x[s][3] * inv) << 16;
-            codes.y = fp8::Encode2(x[s][4] * inv, x[s][5] * inv) | fp8::Encode2(x[s][6] * inv, x[s][7] * inv) << 16;
-            *reinterpret_cast<uint2*>((s == 0 ? a.k_codes : a.v_codes) + code_at) = codes;
+            uint32_t words[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                words[w] = fp8::Encode2(x[s][4 * w] * inv, x[s][4 * w + 1] * inv) | fp8::Encode2(x[s][4 * w + 2] * inv, x[s][4 * w + 3] * inv) << 16;
+            }
+            *reinterpret_cast<uint4*>((s == 0 ? a.k_codes : a.v_codes) + code_at) = make_uint4(words[0], words[1], words[2], words[3]);
             if (piece == 0) (s == 0 ? a.k_scales : a.v_scales)[scale_at] = static_cast<uint8_t>(e + 15);
         }
     }
 }
 
-// 16 codes per thread and turn.
+// 32 bytes, in one store where `wide` says that they start on a 32-byte boundary.
+__device__ __forceinline__ void Store32(void* dst, const uint32_t (&v)[8], bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                     "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                     : "memory");
+    } else {
+        static_cast<uint4*>(dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        static_cast<uint4*>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+// 16 codes per thread and turn: a thread's numbers are 32 or 64 bytes, whole sectors of their own.
 template <typename T, typename I>
 __global__ void __launch_bounds__(kFp8Threads)
 kv_gather_fp8_kernel(const uint8_t* codes, const uint8_t* scales, const int32_t* ids, const I total, T* out, const int64_t num_blocks,
-                     const int block_size, const int heads, const int head_dim) {
+                     const int block_size, const int heads, const int head_dim, const bool wide) {
     BeginAfterPredecessor();
     const int pieces = head_dim / 16;
     const I block_pieces = static_cast<I>(block_size) * heads * pieces;
@@ -139,9 +182,14 @@ kv_gather_fp8_kernel(const uint8_t* codes, const uint8_t* scales, const int32_t*
         if constexpr (sizeof(T) == 4) {
             const float s = fp8::ScaleOf(byte);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float2 lo = fp8::UnpackHalf2(h[2 * w]), hi = fp8::UnpackHalf2(h[2 * w + 1]);
-                reinterpret_cast<float4*>(dst)[w] = make_float4(lo.x * s, lo.y * s, hi.x * s, hi.y * s);
+            for (int half = 0; half < 2; ++half) {
+                uint32_t f[8];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float2 x = fp8::UnpackHalf2(h[4 * half + w]);
+                    f[2 * w] = __float_as_uint(x.x * s), f[2 * w + 1] = __float_as_uint(x.y * s);
+                }
+                Store32(dst + 8 * half, f, wide);
             }
         } else {
             const uint32_t pair = fp8::ScalePair(byte, byte);
@@ -155,8 +203,7 @@ kv_gather_fp8_kernel(const uint8_t* codes, const uint8_t* scales, const int32_t*
                     h[w] = Pack2<T>(f.x * s, f.y * s);
                 }
             }
-            reinterpret_cast<uint4*>(dst)[0] = make_uint4(h[0], h[1], h[2], h[3]);
-            reinterpret_cast<uint4*>(dst)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+            Store32(dst, h, wide);
         }
     }
 }
@@ -187,11 +234,11 @@ void LaunchAppend(const void* k_new, const void* v_new, I rows, const AppendTarg
         LaunchDependent(kv_append_fp8_kernel<T, kLanes, kBatched, I>, Fp8Grid((static_cast<int64_t>(rows) + kRows - 1) / kRows), kFp8Threads, 0,
                         stream, 1, static_cast<const T*>(k_new), static_cast<const T*>(v_new), rows, a);
     };
-    const int pieces = a.head_dim / 8;
-    if (pieces <= 4) go(std::integral_constant<int, 4>{});
+    const int pieces = a.head_dim / kPiece;
+    if (pieces <= 2) go(std::integral_constant<int, 2>{});
+    else if (pieces <= 4) go(std::integral_constant<int, 4>{});
     else if (pieces <= 8) go(std::integral_constant<int, 8>{});
-    else if (pieces <= 16) go(std::integral_constant<int, 16>{});
-    else go(std::integral_constant<int, 32>{});
+    else go(std::integral_constant<int, 16>{});
 }
 
 template <bool kBatched>
@@ -205,7 +252,7 @@ int AppendRows(const ScaFp8Layer& l, const void* k_new, const void* v_new, int64
     a.block_size = static_cast<int>(shape.block_size);
     a.heads = static_cast<int>(shape.num_kv_heads);
     a.head_dim = static_cast<int>(shape.head_dim);
-    a.aligned = Aligned16(k_new) && Aligned16(v_new);
+    a.aligned = ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 31u) == 0;
     if (!Aligned16(a.k_codes) || !Aligned16(a.v_codes)) return Fail(SCA_INVALID_ARGUMENT, std::string(what) + ": the codes must be 16-byte aligned");
     const int64_t rows = tokens * shape.num_kv_heads;
     auto typed = [&](auto* type) {
@@ -280,7 +327,8 @@ extern "C" int sca_launch_kv_gather_fp8(const void* codes, const uint8_t* scales
         auto go = [&](auto count) {
             LaunchDependent(kv_gather_fp8_kernel<T, decltype(count)>, grid, kFp8Threads, 0, s, 1, static_cast<const uint8_t*>(codes), scales,
                             block_ids, count, static_cast<T*>(out), shape->num_blocks, static_cast<int>(shape->block_size),
-                            static_cast<int>(shape->num_kv_heads), static_cast<int>(shape->head_dim));
+                            static_cast<int>(shape->num_kv_heads), static_cast<int>(shape->head_dim),
+                            (reinterpret_cast<uintptr_t>(out) & 31u) == 0);
         };
         if (total < (1ll << 31)) go(static_cast<uint32_t>(total));
         else go(total);
