@@ -18,6 +18,7 @@
 //   * bf16 queries become fp16 by a power of two per head that puts the largest at 2^14: exact but for numbers below 2^-28 of
 //     it; P is rounded to fp16 (2^-11 of numbers up to 1), V and K not at all. Sums and statistics are fp32.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -482,7 +483,8 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
 
     const int batch = static_cast<int>(p.batch), splits = static_cast<int>(p.num_splits);
     const int cap = static_cast<int>(p.max_blocks_per_seq * p.block_size < 0x7fffff00LL ? p.max_blocks_per_seq * p.block_size : 0x7fffff00LL);
-    auto length = [&](int i) { return max(0, min(p.seq_lens != nullptr ? p.seq_lens[i] : cap, cap)); };
+    const int all = static_cast<int>(min(p.seq_kv, static_cast<int64_t>(cap)));  // without lengths
+    auto length = [&](int i) { return max(0, min(p.seq_lens != nullptr ? p.seq_lens[i] : all, cap)); };
     auto steps_of = [](int len) { return max(1, static_cast<int>((static_cast<uint32_t>(len) + kSpan - 1) / kSpan)); };
     // sequences [mine, end_mine) are this thread's
     const int each = (batch + kThreads - 1) / kThreads;
@@ -510,8 +512,10 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
         total += s_part[w][0];
         longest = max(longest, s_part[w][1]);
     }
-    // at least so many that no sequence falls into more than `splits` pieces; with one slot a column goes to its first CTA
-    const int per_cta = max((total + sharers - 1) / sharers, splits > 1 ? (longest + splits - 2) / (splits - 1) : total);
+    // at least so many that no sequence falls into more than `splits` pieces; with one slot a column goes to its first CTA, unless no sequence
+    // can be cut
+    const int least = splits > 1 ? (longest + splits - 2) / (splits - 1) : longest == 1 ? 1 : total;
+    const int per_cta = max((total + sharers - 1) / sharers, least);
     if (static_cast<int64_t>(share) * per_cta >= total) return;
     const int begin = share * per_cta, end = min(total, begin + per_cta);
     if (first <= begin && begin < first + sum) {
@@ -683,13 +687,18 @@ int64_t ResidentClusters(int cluster) {
     }));
 }
 
-// Whether the one-launch kernel is the faster one: the rule of the 16-bit cache (ClusterIsFaster in decode.cu), whose steps have
-// half the tokens and as many bytes.
-bool OneLaunchIsFaster(int64_t units, int64_t steps, int cluster, int64_t resident, bool ragged) {
+// Whether the one-launch kernel is the faster one for `units` (sequence, kv head, head chunk) columns of `steps` steps of kSpan tokens (the
+// longest) on clusters of `cluster` CTAs. Both times in us, fitted to 350 graph-timed calls on a B200 (D=64 to 256, 1 to 40 sequences of 60 to
+// 30 thousand tokens): a step of a CTA costs more the wider the head, the more heads share it and the more CTAs share the memory; the schedule
+// works on what a ragged batch holds, a cluster waits for the longest sequence. One launch / schedule: D=128, 32 / 8 heads, B=1, S=800
+// 5.9 / 9.9, S=12000 17.1 / 13.8, B=8, S=2000 12.9 / 16.9; D=256, 16 / 2, B=1, S=5000 16.6 / 11.8; D=64, 32 / 2, B=4, S=12000 17.7 / 14.4.
+// The choices take 1 % longer than the faster of the two on average, 29 % at most (40 sequences of 60 tokens, 32 / 2 heads: 11.1 / 8.6).
+bool OneLaunchIsFaster(int64_t units, int64_t steps, int cluster, int64_t resident, int head_dim, bool hi) {
     const double busy = static_cast<double>(units * cluster) / resident;
     const double share = static_cast<double>((steps + cluster - 1) / cluster);
     const double waves = static_cast<double>(units * steps) / resident;
-    return 4.8 + share * (0.55 + 1.1 * busy) < 11.5 + 1.55 * std::max(1.0, waves * (ragged ? 0.55 : 1.0));
+    const double one_launch = 4.5 + share * (0.3 + 0.006 * head_dim + (hi ? 0.35 : 0.0) + 0.009 * head_dim * busy);
+    return one_launch < 8.0 + 0.008 * head_dim + (hi ? 1.0 : 0.0) + 2.1 * std::sqrt(head_dim / 128.0) * (hi ? 1.3 : 1.0) * std::max(1.0, 0.8 * waves);
 }
 
 template <typename T, int D, bool kHi>
@@ -702,7 +711,7 @@ int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chu
     // as many CTAs per cluster as let all clusters run at the same time
     int cluster = kMaxCluster;
     while (cluster >= 2 && units > ResidentClusters<T, D, kHi>(cluster)) cluster /= 2;
-    if (cluster < 2 || !OneLaunchIsFaster(units, steps, cluster, resident, p.seq_lens != nullptr)) cluster = 0;
+    if (cluster < 2 || !OneLaunchIsFaster(units, steps, cluster, resident, D, kHi)) cluster = 0;
     *cluster_ctas = cluster;
     if (cluster > 0) {
         LaunchDependent(decode_fp8_cluster_kernel<T, D, kHi>, units * cluster, kThreads, G::kSmemBytes, stream, cluster, p, scales, head_chunks, cluster);
@@ -710,7 +719,7 @@ int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chu
     }
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(&decode_fp8_partial_kernel<T, D, kHi>), G::kSmemBytes, "decode_fp8_partial_kernel")) return rc;
     // one wave: CTAs per column as many as stay resident, never more than the column has steps (or sequences, with one slot)
-    const int64_t useful = p.num_splits == 1 ? p.batch : p.batch * steps;
+    const int64_t useful = p.batch * steps;
     const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(resident / columns, useful)) : resident;
     LaunchDependent(decode_fp8_partial_kernel<T, D, kHi>, blocks, kThreads, G::kSmemBytes, stream, 1, p, scales, head_chunks);
     if (int rc = CheckLaunch("decode_fp8_partial_kernel", stream)) return rc;

@@ -571,8 +571,9 @@ PyObject* PagedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.batch = q->size(0), p.num_heads = q->size(1), p.head_dim = l.shape.head_dim, p.num_kv_heads = l.shape.num_kv_heads;
         const int64_t d = p.head_dim;
         if (p.num_kv_heads < 1 || p.num_heads % p.num_kv_heads != 0 || !Scale(a[8], d, &p.scale)) return NotTaken();
-        p.seq_kv = l.shape.num_blocks * block_size;
-        const int64_t mean = typical > 0 ? typical : std::min(p.seq_kv, table->size(1) * block_size), steps = Steps(mean, kFp8StepTokens);
+        const int64_t upper = l.shape.num_blocks * block_size;
+        p.seq_kv = longest > 0 && lens != nullptr ? std::min(upper, longest) : upper;
+        const int64_t mean = typical > 0 ? typical : std::min(upper, table->size(1) * block_size), steps = Steps(mean, kFp8StepTokens);
         const int64_t most = longest > 0 ? Steps(longest, kFp8StepTokens) : 2 * steps, group = p.num_heads / p.num_kv_heads;
         const int64_t sms = at::cuda::getDeviceProperties(q->device().index())->multiProcessorCount;
         const int64_t ctas = d <= 64 ? 4 : group > 8 && d > 96 ? 2 : 3;  // as fp8_ctas_per_sm

@@ -867,7 +867,7 @@ def paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, *, block_size: 
     p.q, p.k, p.v, p.out = q.data_ptr(), codes.data_ptr(), v_pool[0].data_ptr(), out.data_ptr()
     scratch = ws.data_ptr()
     p.partial_m, p.partial_l, p.partial_o = scratch, scratch + 4 * base, scratch + 4 * o_at
-    p.batch, p.num_heads, p.num_kv_heads, p.seq_kv, p.head_dim, p.num_splits = s, hq, hkv, upper, d, splits
+    p.batch, p.num_heads, p.num_kv_heads, p.seq_kv, p.head_dim, p.num_splits = s, hq, hkv, min(upper, longest_len) if longest_len > 0 and seq_lens is not None else upper, d, splits
     p.q_stride = DecodeStrides(hq * d, d, d)
     p.o_stride = DecodeStrides(hq * d, d, d)
     p.scale = effective_scale(scale, d)

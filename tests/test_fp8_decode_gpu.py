@@ -74,8 +74,9 @@ def test_ragged_batch(kind, hq, hkv, d, bs):
     check(out, q, k, v, table, lens, bs, ops.effective_scale(None, d), kind)
 
 
-@pytest.mark.parametrize("lens,clusters", [([5], True), ([1000], True), ([40000, 3], False), ([700] * 300, False)])
-def test_both_ways_of_launching(lens, clusters):
+@pytest.mark.parametrize("hints", [True, False])
+@pytest.mark.parametrize("lens,clusters", [([5], True), ([1000], True), ([40000, 3], False), ([700] * 300, False), ([60] * 300, False), ([1, 127] * 200, False)])
+def test_both_ways_of_launching(lens, clusters, hints):
     from scicompute_attention_b200 import ops
     rng = np.random.default_rng(len(lens))
     bs, hq, hkv, d = 16, 8, 2, 128
@@ -84,7 +85,7 @@ def test_both_ways_of_launching(lens, clusters):
     table = make_table(rng, lens, bs, nblk, -(-max(lens) // bs))
     q = torch.from_numpy(rng.standard_normal((len(lens), hq, 1, d))).to(torch.float16).cuda()
     out, stats = ops.paged_attention_fp8(q, to_device(k), to_device(v), torch.from_numpy(table).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
-                                         block_size=bs, typical_len=sum(lens) // len(lens), longest_len=max(lens), return_stats=True)
+                                         block_size=bs, return_stats=True, **(dict(typical_len=sum(lens) // len(lens), longest_len=max(lens)) if hints else {}))
     assert (stats["cluster"] > 0) == clusters
     few = range(0, len(lens), max(1, len(lens) // 4))
     check(out[list(few)], q[list(few)], k, v, table[list(few)], [lens[i] for i in few], bs, ops.effective_scale(None, d), "fp16")
@@ -146,6 +147,20 @@ def test_without_lengths_the_whole_table_is_read():
     q = torch.from_numpy(rng.standard_normal((2, 4, 1, 64))).to(torch.bfloat16).cuda()
     out = ops.paged_attention_fp8(q, to_device(k), to_device(v), torch.from_numpy(table).cuda(), None, block_size=16)
     check(out, q, k, v, table, [96, 96], 16, ops.effective_scale(None, 64), "bf16")
+
+
+@pytest.mark.parametrize("hints", [dict(typical_len=1), dict(typical_len=5000, longest_len=1), dict(longest_len=100000), dict(typical_len=3, longest_len=3)])
+def test_wrong_hints_cost_time_only(hints):
+    from scicompute_attention_b200 import ops
+    rng = np.random.default_rng(14)
+    lens = [3, 900, 40, 2000] * 30
+    nblk = sum(-(-n // 16) for n in lens)
+    k, v = make_pool(rng, nblk, 16, 2, 64), make_pool(rng, nblk, 16, 2, 64)
+    table = make_table(rng, lens, 16, nblk, -(-max(lens) // 16))
+    q = torch.from_numpy(rng.standard_normal((len(lens), 4, 1, 64))).to(torch.float16).cuda()
+    out = ops.paged_attention_fp8(q, to_device(k), to_device(v), torch.from_numpy(table).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), block_size=16, **hints)
+    check(out[:8], q[:8], k, v, table[:8], lens[:8], 16, ops.effective_scale(None, 64), "fp16")
+    check(out[-4:], q[-4:], k, v, table[-4:], lens[-4:], 16, ops.effective_scale(None, 64), "fp16")
 
 
 def test_nan_of_a_token_that_counts_is_seen():
