@@ -742,6 +742,7 @@ def _require_fp8_pools(layer_k, layer_v) -> None:
 
 def _require_fp8_rows(codes, rows: int, k_new, v_new) -> None:
     _require_cuda(k_new, v_new)
+    dtype_id(k_new.dtype)  # one that can be quantised
     if k_new.dtype != v_new.dtype:
         raise _lib.ScaError(4, "k_new/v_new shape or dtype mismatch")
     width = codes.shape[2] * codes.shape[3]
