@@ -452,7 +452,9 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
             const int head = 8 * t + 2 * c + h;
-            if (g == 0) stage_m[head] = m_run[t][h] == -CUDART_INF_F ? -CUDART_INF_F : m_run[t][h] * unit[t][h], stage_l[head] = l;
+            // a maximum passes over NaN: where every score is NaN, so is l, and the merges must not take it for a part without a key
+            const float m = m_run[t][h] != -CUDART_INF_F ? m_run[t][h] * unit[t][h] : l == l ? -CUDART_INF_F : 0.0f;
+            if (g == 0) stage_m[head] = m, stage_l[head] = l;
 #pragma unroll
             for (int w = 0; w < G::kWordsV; ++w) {
 #pragma unroll

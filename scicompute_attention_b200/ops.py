@@ -781,7 +781,7 @@ def kv_append_fp8(layer_k, layer_v, k_new, v_new, slot_mapping, *, stream=None) 
 
 
 def kv_append_batched_fp8(layer_k, layer_v, k_new, v_new, page_table, seq_lens, *, stream=None) -> None:
-    """kv_append_batched into an 8-bit layer: one new token per sequence, at position seq_lens[s] - 1 of its pages."""
+    """kv_append_batched into an 8-bit layer: one new token per sequence, at position seq_lens[s] - 1 of its pages; no two at the same place."""
     if stream is None and _native().append_batched_fp8(*layer_k, *layer_v, k_new, v_new, page_table, seq_lens):
         return
     _require_fp8_pools(layer_k, layer_v)

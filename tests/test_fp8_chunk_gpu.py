@@ -136,3 +136,16 @@ def test_the_same_call_gives_the_same_bits():
     first = run(q, k, v, table, cu, lens)
     for _ in range(30):
         assert torch.equal(run(q, k, v, table, cu, lens), first)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lens,new", [([3001], [37]), ([3001, 500] * 8, [300, 500] * 8)])
+def test_a_query_of_nan_gives_nan(kind, lens, new):
+    rng = np.random.default_rng(22)
+    q, k, v, table, cu, lens = case(rng, lens, new, 16, 8, 2, 128, kind)
+    want = run(q, k, v, table, cu, lens)
+    q[20, 3] = float("nan")
+    got = run(q, k, v, table, cu, lens)
+    assert got[20, 3].isnan().all()
+    got[20, 3] = want[20, 3]
+    assert torch.equal(got, want)

@@ -173,3 +173,23 @@ def test_nan_of_a_token_that_counts_is_seen():
     table, lens = torch.arange(4, dtype=torch.int32, device="cuda")[None], torch.tensor([20], dtype=torch.int32, device="cuda")
     out = ops.paged_attention_fp8(x[:1].view(1, 1, 1, 64), k, v, table, lens, block_size=16)
     assert out.isnan().view(-1).nonzero().view(-1).tolist() == [5]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lens,cluster", [([300, 40], True), ([40000, 40], False)])
+def test_a_query_of_nan_gives_nan(kind, lens, cluster):
+    """Every score of the row is NaN, and so is what comes out, in parts or in one piece; the others keep their numbers."""
+    from scicompute_attention_b200 import ops
+    rng = np.random.default_rng(21)
+    nblk = sum(-(-n // 16) for n in lens)
+    k, v = to_device(make_pool(rng, nblk, 16, 2, 128)), to_device(make_pool(rng, nblk, 16, 2, 128))
+    table = torch.from_numpy(make_table(rng, lens, 16, nblk, -(-max(lens) // 16))).cuda()
+    q = torch.from_numpy(rng.standard_normal((2, 8, 1, 128))).to(TYPES[kind]).cuda()
+    run = lambda: ops.paged_attention_fp8(q, k, v, table, torch.tensor(lens, dtype=torch.int32).cuda(), block_size=16, return_stats=True)
+    want, stats = run()
+    assert (stats["cluster"] > 0) == cluster
+    q[0, 3] = float("nan")
+    got, _ = run()
+    assert got[0, 3].isnan().all()
+    got[0, 3] = want[0, 3]
+    assert torch.equal(got, want)
