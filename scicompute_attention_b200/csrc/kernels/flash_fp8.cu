@@ -8,11 +8,11 @@ namespace {
 
 template <typename T, int DP, int QT, int BN, bool kSplit>
 int Launch(int64_t ctas, int cluster, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
-           const FlashKernelParams& p) {
-    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, true, true, kSplit, true>;
+           const FlashKernelParams& p, const WorkImage& image) {
+    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, true, true, true, kSplit>;
     constexpr int kSmem = FlashGeom<DP, QT, BN, true>::kSmemBytes;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kSmem, "flash_fwd_sm100_kernel")) return rc;
-    LaunchDependent(kernel, ctas, FlashThreads<T, DP, QT, true>(), kSmem, stream, cluster, map_q, map_k, map_v, p);
+    LaunchDependent(kernel, ctas, FlashThreads<T, DP, QT, true>(), kSmem, stream, cluster, map_q, map_k, map_v, p, image);
     return SCA_OK;
 }
 
@@ -20,14 +20,14 @@ int Launch(int64_t ctas, int cluster, cudaStream_t stream, const CUtensorMap& ma
 
 template <typename T, int DP, int QT, int BN>
 int LaunchKv8(int64_t items, unsigned grid, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
-              const FlashKernelParams& p) {
-    if (p.cluster > 1) return Launch<T, DP, QT, BN, true>(items * p.cluster, p.cluster, stream, map_q, map_k, map_v, p);
-    return Launch<T, DP, QT, BN, false>(grid, 1, stream, map_q, map_k, map_v, p);
+              const FlashKernelParams& p, const WorkImage& image) {
+    if (p.cluster > 1) return Launch<T, DP, QT, BN, true>(items * p.cluster, p.cluster, stream, map_q, map_k, map_v, p, image);
+    return Launch<T, DP, QT, BN, false>(grid, 1, stream, map_q, map_k, map_v, p, image);
 }
 
 #define SCA_KV8(T, DP, QT)                                                                                                          \
     template int LaunchKv8<T, DP, QT, 128>(int64_t, unsigned, cudaStream_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, \
-                                           const FlashKernelParams&);
+                                           const FlashKernelParams&, const WorkImage&);
 SCA_KV8(__half, 64, 2)
 SCA_KV8(__half, 128, 2)
 SCA_KV8(__half, 256, 1)

@@ -1,6 +1,7 @@
 // Host side of the prefill: tensor maps, work lists of ragged batches, the choice of the launch. The kernel is in
 // flash_kernel.cuh.
 #include <algorithm>
+#include <cstring>
 #include <mutex>
 #include <type_traits>
 #include <vector>
@@ -189,9 +190,10 @@ int CheckSequences(const VarlenWork& vw, bool causal) {
 }
 
 // Builds {first q token, first kv token, S_q, S_kv} per sequence and the (sequence, query block) list, heaviest
-// block first, and copies both into the workspace (stream-ordered; the host vector may die on return).
+// block first, and copies both into the workspace (stream-ordered; the host vector may die on return), or into `small` where that is given
+// and they fit it; the lists are null then.
 int UploadVarlenWork(const VarlenWork& vw, int tokens_per_entry, int block_n, bool causal, cudaStream_t stream,
-                     const int4** seqs_out, const int2** entries_out, int* num_entries_out) {
+                     const int4** seqs_out, const int2** entries_out, int* num_entries_out, WorkImage* small = nullptr) {
     const size_t seq_bytes = static_cast<size_t>(vw.num_seqs) * sizeof(int4);
     struct Weighted {
         int2 entry;
@@ -219,11 +221,18 @@ int UploadVarlenWork(const VarlenWork& vw, int tokens_per_entry, int block_n, bo
     image.resize((bytes + sizeof(int4) - 1) / sizeof(int4));
     int2* entries = reinterpret_cast<int2*>(reinterpret_cast<unsigned char*>(image.data()) + seq_bytes);
     for (size_t i = 0; i < list.size(); ++i) entries[i] = list[i].entry;
+    *num_entries_out = static_cast<int>(list.size());
+    if (small != nullptr && bytes <= sizeof(small->bytes)) {
+        std::memcpy(small->bytes, image.data(), bytes);
+        small->entries_at = static_cast<int>(seq_bytes);
+        *seqs_out = nullptr;
+        *entries_out = nullptr;
+        return SCA_OK;
+    }
     unsigned char* base = static_cast<unsigned char*>(vw.workspace);
     if (int rc = SendToDevice(base, image.data(), bytes, stream, "cudaMemcpyAsync(varlen work list)")) return rc;
     *seqs_out = reinterpret_cast<const int4*>(base);
     *entries_out = reinterpret_cast<const int2*>(base + seq_bytes);
-    *num_entries_out = static_cast<int>(list.size());
     return SCA_OK;
 }
 
@@ -336,10 +345,12 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
     const int item_tokens = (tiles_per_item * kBlockM) >> pack_shift;
     p.m_blocks = static_cast<int>((f.seq_q + item_tokens - 1) / item_tokens);
     int64_t most_keys = f.seq_kv;  // of a sequence
+    WorkImage small;               // the work list, where p.seqs is null
     if (varlen != nullptr) {
         most_keys = 0;
         for (int64_t i = 0; i < varlen->num_seqs; ++i) most_keys = std::max<int64_t>(most_keys, static_cast<int64_t>(varlen->cu_kv[i + 1]) - varlen->cu_kv[i]);
-        if (int rc = UploadVarlenWork(*varlen, item_tokens, BN, f.causal != 0, stream, &p.seqs, &p.entries, &p.num_entries)) return rc;
+        if (int rc = UploadVarlenWork(*varlen, item_tokens, BN, f.causal != 0, stream, &p.seqs, &p.entries, &p.num_entries,
+                                      paged != nullptr && paged->k_scales != nullptr ? &small : nullptr)) return rc;
     }
     const int64_t ctas = (varlen != nullptr ? static_cast<int64_t>(p.num_entries) : static_cast<int64_t>(p.m_blocks) * p.batch) *
                          (p.heads >> pack_shift);
@@ -360,7 +371,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
             p.k_scales = paged->k_scales;
             p.v_scales = paged->v_scales;
             p.scale_row = static_cast<int>(fp8::ScaleRow(paged->block_size));
-            if (int rc = LaunchKv8<T, DP, QT, BN>(ctas, grid, stream, map_q, map_k, map_v, p)) return rc;
+            if (int rc = LaunchKv8<T, DP, QT, BN>(ctas, grid, stream, map_q, map_k, map_v, p, small)) return rc;
             return CheckFlash(stream);
         }
         if (p.cluster > 1) {
@@ -369,7 +380,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
         }
         const void* fn = reinterpret_cast<const void*>(&flash_fwd_sm100_kernel<T, DP, QT, BN, true, true>);
         if (int rc = EnsureDynamicSmem(fn, G::kSmemBytes, "flash_fwd_sm100_kernel")) return rc;
-        LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, true, true>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p);
+        LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, true, true>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p, NoWorkImage{});
     } else if (varlen != nullptr) {
         if (p.cluster > 1) {
             if (int rc = LaunchSplit<T, DP, QT, BN, true, false>(ctas, stream, map_q, map_k, map_v, p)) return rc;
@@ -377,7 +388,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
         }
         const void* fn = reinterpret_cast<const void*>(&flash_fwd_sm100_kernel<T, DP, QT, BN, true>);
         if (int rc = EnsureDynamicSmem(fn, G::kSmemBytes, "flash_fwd_sm100_kernel")) return rc;
-        LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, true>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p);
+        LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, true>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p, NoWorkImage{});
     } else {
         if (p.cluster > 1) {
             if (int rc = LaunchSplit<T, DP, QT, BN, false, false>(ctas, stream, map_q, map_k, map_v, p)) return rc;
@@ -385,7 +396,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
         }
         const void* fn = reinterpret_cast<const void*>(&flash_fwd_sm100_kernel<T, DP, QT, BN, false>);
         if (int rc = EnsureDynamicSmem(fn, G::kSmemBytes, "flash_fwd_sm100_kernel")) return rc;
-        LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, false>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p);
+        LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, false>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p, NoWorkImage{});
     }
     return CheckFlash(stream);
 }

@@ -464,6 +464,13 @@ PyObject* Gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- 8-bit KV cache --------------------------------------------------------------------------------------------------------
+// Null on top of a library without them; the other operators are served all the same.
+#pragma weak sca_launch_kv_append_fp8
+#pragma weak sca_launch_kv_append_batched_fp8
+#pragma weak sca_launch_kv_gather_fp8
+#pragma weak sca_launch_paged_attention_fp8
+#pragma weak sca_launch_flash_paged_fp8
+
 // K or V of a layer, as _require_fp8_pool in ops.py.
 bool Fp8Pool(const at::Tensor* codes, const at::Tensor* scales, ScaKvCacheShape* s) {
     if (codes == nullptr || scales == nullptr || (codes->scalar_type() != at::kFloat8_e4m3fn && codes->scalar_type() != at::kByte) ||
@@ -500,7 +507,7 @@ PyObject* AppendFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return Guarded([&]() -> PyObject* {
         Fp8Layer l;
         int32_t dtype;
-        if (n != 7 || !l.Take(a)) return NotTaken();
+        if (sca_launch_kv_append_fp8 == nullptr || n != 7 || !l.Take(a)) return NotTaken();
         const at::Tensor *kn = Plain(a[4]), *vn = Plain(a[5]), *slots = Plain(a[6]);
         if (!kn || !vn || !slots || !Fp8Rows(*kn, *vn, l) || !DtypeId(*kn, &dtype) || !Ints(*slots, kn->size(0)) || !Fp8Layer::Here(*slots)) return NotTaken();
         void* stream = CurrentStream();
@@ -517,7 +524,7 @@ PyObject* AppendBatchedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return Guarded([&]() -> PyObject* {
         Fp8Layer l;
         int32_t dtype;
-        if (n != 8 || !l.Take(a)) return NotTaken();
+        if (sca_launch_kv_append_batched_fp8 == nullptr || n != 8 || !l.Take(a)) return NotTaken();
         const at::Tensor *kn = Plain(a[4]), *vn = Plain(a[5]), *table = Plain(a[6]), *lens = Plain(a[7]);
         if (!kn || !vn || !table || !lens || !Fp8Rows(*kn, *vn, l) || !DtypeId(*kn, &dtype) || !Table(*table, kn->size(0)) ||
             !Ints(*lens, kn->size(0)) || !Fp8Layer::Here(*table) || !Fp8Layer::Here(*lens)) {
@@ -535,7 +542,7 @@ PyObject* AppendBatchedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // gather_fp8(codes, scales, block_ids, dtype)
 PyObject* GatherFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return Guarded([&]() -> PyObject* {
-        if (n != 4 || !THPDtype_Check(a[3])) return NotTaken();
+        if (sca_launch_kv_gather_fp8 == nullptr || n != 4 || !THPDtype_Check(a[3])) return NotTaken();
         const at::Tensor *codes = Plain(a[0]), *scales = Plain(a[1]), *ids = Plain(a[2]);
         ScaKvCacheShape shape;
         const at::ScalarType type = reinterpret_cast<THPDtype*>(a[3])->scalar_type;
@@ -560,7 +567,7 @@ PyObject* PagedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Fp8Layer l;
         int64_t block_size, typical, longest;
         ScaDecodeFwdParams p{};
-        if (n != 11 || !l.Take(a) || !Int(a[7], &block_size) || !Int(a[9], &typical) || !Int(a[10], &longest)) return NotTaken();
+        if (sca_launch_paged_attention_fp8 == nullptr || n != 11 || !l.Take(a) || !Int(a[7], &block_size) || !Int(a[9], &typical) || !Int(a[10], &longest)) return NotTaken();
         const at::Tensor *q = Plain(a[4]), *table = Plain(a[5]), *lens = nullptr;
         if (a[6] != Py_None && (lens = Plain(a[6])) == nullptr) return NotTaken();
         if (!q || !table || q->dim() != 4 || q->size(2) != 1 || q->size(3) != l.shape.head_dim || block_size != l.shape.block_size ||
@@ -597,7 +604,7 @@ PyObject* ChunkFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         HostInts cu_q, lens;
         bool causal;
         ScaFlashPagedParams p{};
-        if (n != 10 || !l.Take(a) || !cu_q.Take(a[6]) || !lens.Take(a[7]) || !Flag(a[8], &causal)) return NotTaken();
+        if (sca_launch_flash_paged_fp8 == nullptr || n != 10 || !l.Take(a) || !cu_q.Take(a[6]) || !lens.Take(a[7]) || !Flag(a[8], &causal)) return NotTaken();
         const at::Tensor *q = Plain(a[4]), *table = Plain(a[5]);
         if (!q || !table || q->dim() != 3 || q->size(2) != l.shape.head_dim || !q->is_contiguous() || !DtypeId(*q, &p.dtype_id) ||
             p.dtype_id == SCA_DTYPE_F32 || !Table(*table, lens.size()) || cu_q.size() != lens.size() + 1 || !Scale(a[9], q->size(2), &p.scale) ||

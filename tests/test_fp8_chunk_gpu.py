@@ -149,3 +149,13 @@ def test_a_query_of_nan_gives_nan(kind, lens, new):
     assert got[20, 3].isnan().all()
     got[20, 3] = want[20, 3]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("seqs", [85, 86, 200])
+def test_work_lists_of_any_length(seqs):
+    """Lists of up to 2 KB (85 sequences of one entry) go with the launch, longer ones ahead of it."""
+    from scicompute_attention_b200 import ops
+    rng = np.random.default_rng(23)
+    new = [1 + i % 7 for i in range(seqs)]
+    q, k, v, table, cu, lens = case(rng, [n + 11 * (i % 5) for i, n in enumerate(new)], new, 16, 4, 2, 64, "fp16")
+    check(run(q, k, v, table, cu, lens), q, k, v, table, cu, lens, 16, True, ops.effective_scale(None, 64), "fp16")
