@@ -82,13 +82,13 @@ __device__ __forceinline__ void MergeWarps(const ScaDecodeFwdParams& p, unsigned
     __syncthreads();  // the rings double as merge staging: nobody refills them before everyone has read
 }
 
-// Marks slots [first, num_splits) of every head of one (sequence, kv head, head chunk) as empty (m = -inf; the merge
+// Marks slots [first, end) of every head of one (sequence, kv head, head chunk) as empty (m = -inf; the merge
 // skips such entries without reading l or O).
-__device__ __forceinline__ void MarkUnusedSlots(const ScaDecodeFwdParams& p, int64_t b, int hk, int hc, int first) {
+__device__ __forceinline__ void MarkUnusedSlots(const ScaDecodeFwdParams& p, int64_t b, int hk, int hc, int first, int end) {
     const int group = static_cast<int>(p.num_heads / p.num_kv_heads);
     const int head0 = hk * group + hc * 16;
     const int nheads = min(16, group - hc * 16);
-    const int unused = static_cast<int>(p.num_splits) - first;
+    const int unused = end - first;
     for (int item = threadIdx.x; item < nheads * unused; item += kThreads) {
         const int row = item / unused;
         const int slot = first + item % unused;
@@ -229,7 +229,7 @@ __device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const 
             const int slot = static_cast<int>(share - before / per_cta);
             if (t0 == 0) {
                 const int used = static_cast<int>((before + steps - 1) / per_cta - before / per_cta) + 1;
-                MarkUnusedSlots(p, b, hk, hc, used);
+                MarkUnusedSlots(p, b, hk, hc, used, static_cast<int>(p.num_splits));
             }
             const int64_t j_end = t1 * kSpan < len ? t1 * kSpan : len;
             segment(b, hk, hc, t0 * kSpan, j_end, slot);

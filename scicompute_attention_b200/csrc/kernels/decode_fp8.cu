@@ -28,8 +28,6 @@
 namespace sca_b200 {
 namespace {
 
-constexpr int kSpan = 128;  // tokens of a CTA's unit of the schedule
-
 struct Fp8Scales {
     const uint8_t* k;
     const uint8_t* v;
@@ -39,6 +37,7 @@ struct Fp8Scales {
 template <int D, bool kHi>
 struct Fp8Geom {
     static constexpr int kTokens = D > 128 ? 16 : 32;  // of a warp's step
+    static constexpr int kSpan = kWarps * kTokens;     // of the CTA's: the unit of the schedule (ops.py counts on it)
     // CTAs that stay on an SM: what the registers of O and Q leave room for (FP8 slots in ops.py counts on it)
     static constexpr int kCtas = D <= 64 ? 4 : kHi && D > 96 ? 2 : 3;
 
@@ -185,43 +184,53 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
     unsigned char* ring = smem + warp * G::kWarpBytes;
     const uint32_t ring_addr = SmemAddr(ring);
 
-    // This lane's token of the next tile to be issued, as (page of the sequence, offset in the page), moved on by the tokens of
-    // the CTA's warps per tile without a division, and the page's table entry, fetched one tile ahead.
+    // This lane's token of the tile whose table entry is fetched next, as (page of the sequence, offset in the page), moved on by the tokens
+    // of the CTA's warps per tile without a division, and the entries of the next kAhead tiles: the first loads of a segment wait for
+    // one entry, not for one after the other.
     const int token = lane % kTokens;
-    constexpr int kStep = kWarps * kTokens;
-    int page = 0, offset = 0;
-    int32_t phys_next = -1;
+    constexpr int kStep = kWarps * kTokens, kAhead = G::kStages - 1;
     const int page_step = kStep / block_size, offset_step = kStep % block_size;
-    auto fetch_entry = [&](int64_t jt) { phys_next = (jt < j_end && page < p.max_blocks_per_seq) ? table_row[page] : -1; };
-    {
-        const int64_t jt = j_begin + warp * kTokens + token;
-        page = static_cast<int>(jt / block_size);
-        offset = static_cast<int>(jt - static_cast<int64_t>(page) * block_size);
-        fetch_entry(jt);
-    }
-
-    // Issues the copies of this warp's `tl`-th tile into `stage`, tile after tile; returns which of its tokens there are.
-    auto issue = [&](int tl, int stage) -> uint32_t {
-        const int64_t jt = j_begin + static_cast<int64_t>(warp + tl * kWarps) * kTokens + token;
-        const bool there = phys_next >= 0 && phys_next < p.num_kv_blocks;
-        // place of the row in 16-byte pieces; pools stay below 2^32 of them
-        const uint32_t at = there ? static_cast<uint32_t>(phys_next * block_size + offset) * row_pieces : 0u;
-        const uint32_t k_stage = ring_addr + stage * G::kStageBytes;
-        const uint32_t v_stage = k_stage + G::kTileBytes;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there);
-        if (c == 0 && lane < kTokens) {
-            // block_size is a multiple of 4, and so is the tile's first token: four tokens share a page and a word of scales
-            const int64_t scales_at = there ? (static_cast<int64_t>(phys_next) * p.num_kv_heads + hk) * scale_row + offset : 0;
-            CpAsync4(v_stage + G::kTileBytes + lane, scales.k + scales_at, there ? 4 : 0);
-            CpAsync4(v_stage + G::kTileBytes + kTokens + lane, scales.v + scales_at, there ? 4 : 0);
-        }
+    const uint32_t first_token = static_cast<uint32_t>(j_begin) + warp * kTokens + token;  // lengths are below 2^31
+    int page = static_cast<int>(first_token / block_size), offset = static_cast<int>(first_token) - page * block_size;
+    int32_t entries[kAhead];
+    auto fetch_entry = [&](int tl) -> int32_t {
+        const bool in = first_token + static_cast<uint32_t>(tl) * kStep < static_cast<uint32_t>(j_end) && page < p.max_blocks_per_seq;
+        const int32_t entry = in ? table_row[page] : -1;
         page += page_step;
         offset += offset_step;
         if (offset >= block_size) {
             offset -= block_size;
             ++page;
         }
-        fetch_entry(jt + kStep);
+        return entry;
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) entries[i] = fetch_entry(i);
+
+    // Issues the copies of this warp's `tl`-th tile into `stage`, tile after tile; returns which of its tokens there are.
+    auto issue = [&](int tl, int stage) -> uint32_t {
+        const int32_t phys = entries[0];
+        const bool there = phys >= 0 && phys < p.num_kv_blocks;
+        int at_offset = offset;  // in its page: `offset` is kAhead tiles ahead
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            at_offset -= offset_step;
+            if (at_offset < 0) at_offset += block_size;
+        }
+        // place of the row in 16-byte pieces; pools stay below 2^32 of them
+        const uint32_t at = there ? static_cast<uint32_t>(phys * block_size + at_offset) * row_pieces : 0u;
+        const uint32_t k_stage = ring_addr + stage * G::kStageBytes;
+        const uint32_t v_stage = k_stage + G::kTileBytes;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        if (c == 0 && lane < kTokens) {
+            // block_size is a multiple of 4, and so is the tile's first token: four tokens share a page and a word of scales
+            const int64_t scales_at = there ? (static_cast<int64_t>(phys) * p.num_kv_heads + hk) * scale_row + at_offset : 0;
+            CpAsync4(v_stage + G::kTileBytes + lane, scales.k + scales_at, there ? 4 : 0);
+            CpAsync4(v_stage + G::kTileBytes + kTokens + lane, scales.v + scales_at, there ? 4 : 0);
+        }
+#pragma unroll
+        for (int i = 0; i + 1 < kAhead; ++i) entries[i] = entries[i + 1];
+        entries[kAhead - 1] = fetch_entry(tl + kAhead);
         auto copy = [&](auto whole) {
 #pragma unroll
             for (int n = 0; n < kTokens * G::kChunks / 32; ++n) {
@@ -467,13 +476,21 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
     MergeFp8Warps<D, G::kWarpBytes, kToShared>(p, smem, b, head0, nheads, slot);
 }
 
-// The schedule of decode_common.cuh (WalkSchedule: what it does and why) for lists of less than 2^31 steps: the lengths are read once,
-// and nothing is divided in 64 bits. With both it took 3500 clocks until a CTA knew its share; a CTA's K/V is 30000 to 60000.
-template <typename Segment>
+// What the border between two sequences of a CTA - the end of one segment, the first loads of the next - counts for in its share, in steps.
+// Without it the CTAs with a border end 7 us after the others (96 sequences of 200 to 6000 tokens, 32 / 2 heads, D=64 34.3 / 30.5 us; 64 of
+// 300 to 3000, 32 / 8 heads 34.4 / 32.6). One step or three 31.5.
+constexpr int kBorder = 2;
+// CTAs of a wave that are left out. The merge kernel of the call before may still hold a place on some SM, and the CTA that finds none runs
+// when all the others have: the 96 sequences 37 us with none left out, 34.3 with 2, 31.4 with 4; D=256, 40 of 100 to 5000 34.5, 31.2, 31.0.
+constexpr int kLeftOut = 4;
+
+// The schedule of decode_common.cuh (WalkSchedule: what it does and why) for lists of less than 2^31 steps, with borders that count, shares
+// that differ by a step at most, lengths that are read once, and nothing divided in 64 bits. With the last two it took 3500 clocks until a
+// CTA knew its share; a CTA's K/V is 30000 to 60000.
+template <int kSpan, typename Segment>
 __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, const int head_chunks, const Segment& segment) {
     __shared__ int s_part[kWarps][2];
     __shared__ int s_found[2];
-    WaitForPredecessor();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int columns = static_cast<int>(p.num_kv_heads) * head_chunks, grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
     // grids smaller than the number of columns let every CTA walk several columns, each as its only CTA
@@ -482,6 +499,7 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
     const int first_column = grid >= columns ? cta % columns : cta;
     const int column_stride = grid >= columns ? columns : grid;
     if (share >= sharers) return;  // a grid that is no multiple of the column count
+    WaitForPredecessor();
 
     const int batch = static_cast<int>(p.batch), splits = static_cast<int>(p.num_splits);
     const int cap = static_cast<int>(p.max_blocks_per_seq * p.block_size < 0x7fffff00LL ? p.max_blocks_per_seq * p.block_size : 0x7fffff00LL);
@@ -497,6 +515,8 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
         sum += t;
         longest = max(longest, t);
     }
+    const int border = __syncthreads_or(longest > 1) ? kBorder : 0;
+    sum += (end_mine - mine) * border;
     int up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -514,16 +534,22 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
         total += s_part[w][0];
         longest = max(longest, s_part[w][1]);
     }
+    longest += border;
     // at least so many that no sequence falls into more than `splits` pieces; with one slot a column goes to its first CTA, unless no sequence
     // can be cut
     const int least = splits > 1 ? (longest + splits - 2) / (splits - 1) : longest == 1 ? 1 : total;
-    const int per_cta = max((total + sharers - 1) / sharers, least);
-    if (static_cast<int64_t>(share) * per_cta >= total) return;
-    const int begin = share * per_cta, end = min(total, begin + per_cta);
+    // `sharing` CTAs take `each_share` steps, the first `more` of them one more
+    const int sharing = max(1, min(sharers, total / least)), each_share = total / sharing, more = total - sharing * each_share;
+    if (share >= sharing) return;
+    const int begin = share * each_share + min(share, more), end = begin + each_share + (share < more ? 1 : 0);
+    auto sharer_of = [&](int step) {
+        const int left = step - more * (each_share + 1);
+        return left < 0 ? step / (each_share + 1) : more + left / each_share;
+    };
     if (first <= begin && begin < first + sum) {
         int i = mine, before = first;
         while (true) {
-            const int t = steps_of(length(i));
+            const int t = steps_of(length(i)) + border;
             if (begin < before + t) break;
             before += t;
             ++i;
@@ -538,19 +564,20 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
 
     for (int column = first_column; column < columns; column += column_stride) {
         const int hk = column / head_chunks, hc = column % head_chunks;
-        int b = b_first, before = before_first, len = length(b), steps = steps_of(len);
+        int b = b_first, before = before_first, len = length(b), steps = steps_of(len) + border;
         for (int pos = begin; pos < end;) {
             const int t0 = pos - before, t1 = min(t0 + (end - pos), steps);
-            const int slot = share - before / per_cta;
-            if (t0 == 0) MarkUnusedSlots(p, b, hk, hc, (before + steps - 1) / per_cta - before / per_cta + 1);
-            const int64_t j_end = min(static_cast<int64_t>(t1) * kSpan, static_cast<int64_t>(len));
-            segment(b, hk, hc, static_cast<int64_t>(t0) * kSpan, j_end, slot);
+            const int slot = t0 == 0 ? 0 : share - sharer_of(before);
+            if (t0 == 0) MarkUnusedSlots(p, b, hk, hc, sharer_of(before + steps - 1) - share + 1, splits);
+            const int64_t j_end = min(static_cast<int64_t>(t1 - border) * kSpan, static_cast<int64_t>(len));
+            if (t1 <= border) MarkUnusedSlots(p, b, hk, hc, slot, slot + 1);
+            else segment(b, hk, hc, static_cast<int64_t>(max(t0 - border, 0)) * kSpan, j_end, slot);
             pos += t1 - t0;
             if (t1 == steps && pos < end) {
                 before += steps;
                 ++b;
                 len = length(b);
-                steps = steps_of(len);
+                steps = steps_of(len) + border;
             }
         }
     }
@@ -560,7 +587,7 @@ template <typename T, int D, bool kHi>
 __global__ void __launch_bounds__(kThreads, Fp8Geom<D, kHi>::kCtas)
 decode_fp8_partial_kernel(const ScaDecodeFwdParams p, const Fp8Scales scales, const int head_chunks) {
     extern __shared__ __align__(128) unsigned char smem[];
-    WalkFp8Schedule(p, head_chunks, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end, int slot) {
+    WalkFp8Schedule<Fp8Geom<D, kHi>::kSpan>(p, head_chunks, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end, int slot) {
         Fp8Segment<T, D, kHi, false>(p, scales, smem, b, hk, hc, j_begin, j_end, slot);
     });
 }
@@ -569,7 +596,7 @@ template <typename T, int D, bool kHi>
 __global__ void __launch_bounds__(kThreads, Fp8Geom<D, kHi>::kCtas)
 decode_fp8_cluster_kernel(const ScaDecodeFwdParams p, const Fp8Scales scales, const int head_chunks, const int cluster) {
     extern __shared__ __align__(128) unsigned char smem[];
-    ClusterDecode<T, D, true, kSpan>(p, head_chunks, cluster, smem, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end) {
+    ClusterDecode<T, D, true, Fp8Geom<D, kHi>::kSpan>(p, head_chunks, cluster, smem, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end) {
         Fp8Segment<T, D, kHi, true>(p, scales, smem, b, hk, hc, j_begin, j_end, 0);
     });
 }
@@ -652,7 +679,7 @@ decode_fp8_merge_kernel(const ScaDecodeFwdParams p) {
 template <typename T, int D>
 int LaunchFp8Merge(const ScaDecodeFwdParams& p, cudaStream_t stream) {
     const int64_t rows = p.batch * p.num_heads;
-    if (p.num_splits <= 8) LaunchDependent(decode_fp8_merge_kernel<T, D, 1>, (rows + 7) / 8, 256, 0, stream, 1, p);
+    if (p.num_splits <= 8 || rows > 8 * SmCount()) LaunchDependent(decode_fp8_merge_kernel<T, D, 1>, (rows + 7) / 8, 256, 0, stream, 1, p);
     else LaunchDependent(decode_fp8_merge_kernel<T, D, 8>, rows, 256, 0, stream, 1, p);
     return CheckLaunch("decode_fp8_merge_kernel", stream);
 }
@@ -689,7 +716,7 @@ int64_t ResidentClusters(int cluster) {
     }));
 }
 
-// Whether the one-launch kernel is the faster one for `units` (sequence, kv head, head chunk) columns of `steps` steps of kSpan tokens (the
+// Whether the one-launch kernel is the faster one for `units` (sequence, kv head, head chunk) columns of `steps` times 128 tokens (the
 // longest) on clusters of `cluster` CTAs. Both times in us, fitted to 350 graph-timed calls on a B200 (D=64 to 256, 1 to 40 sequences of 60 to
 // 30 thousand tokens): a step of a CTA costs more the wider the head, the more heads share it and the more CTAs share the memory; the schedule
 // works on what a ragged batch holds, a cluster waits for the longest sequence. One launch / schedule: D=128, 32 / 8 heads, B=1, S=800
@@ -707,22 +734,23 @@ template <typename T, int D, bool kHi>
 int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chunks, cudaStream_t stream, int* cluster_ctas) {
     using G = Fp8Geom<D, kHi>;
     const int64_t columns = p.num_kv_heads * head_chunks, units = p.batch * columns;
-    const int64_t steps = std::max<int64_t>(1, (std::min(p.seq_kv, p.max_blocks_per_seq * p.block_size) + kSpan - 1) / kSpan);
+    const int64_t longest = std::max<int64_t>(1, std::min(p.seq_kv, p.max_blocks_per_seq * p.block_size));
     const int64_t resident = ResidentCtas<T, D, kHi>();
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(&decode_fp8_cluster_kernel<T, D, kHi>), G::kSmemBytes, "decode_fp8_cluster_kernel")) return rc;
     // as many CTAs per cluster as let all clusters run at the same time
     int cluster = kMaxCluster;
     while (cluster >= 2 && units > ResidentClusters<T, D, kHi>(cluster)) cluster /= 2;
-    if (cluster < 2 || !OneLaunchIsFaster(units, steps, cluster, resident, D, kHi)) cluster = 0;
+    if (cluster < 2 || !OneLaunchIsFaster(units, (longest + 127) / 128, cluster, resident, D, kHi)) cluster = 0;
     *cluster_ctas = cluster;
     if (cluster > 0) {
         LaunchDependent(decode_fp8_cluster_kernel<T, D, kHi>, units * cluster, kThreads, G::kSmemBytes, stream, cluster, p, scales, head_chunks, cluster);
         return CheckLaunch("decode_fp8_cluster_kernel", stream);
     }
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(&decode_fp8_partial_kernel<T, D, kHi>), G::kSmemBytes, "decode_fp8_partial_kernel")) return rc;
-    // one wave: CTAs per column as many as stay resident, never more than the column has steps (or sequences, with one slot)
-    const int64_t useful = p.batch * steps;
-    const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(resident / columns, useful)) : resident;
+    // one wave, almost: CTAs per column as many as stay resident, never more than the column has steps (or sequences, with one slot)
+    const int64_t useful = p.batch * ((longest + G::kSpan - 1) / G::kSpan);
+    const int64_t wave = std::max(columns, resident - kLeftOut);
+    const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(wave / columns, useful)) : resident;
     LaunchDependent(decode_fp8_partial_kernel<T, D, kHi>, blocks, kThreads, G::kSmemBytes, stream, 1, p, scales, head_chunks);
     if (int rc = CheckLaunch("decode_fp8_partial_kernel", stream)) return rc;
     return LaunchFp8Merge<T, D>(p, stream);
@@ -778,7 +806,7 @@ extern "C" int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, 
         return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): block_size=" + std::to_string(p.block_size) +
                                               " (a multiple of 4), and a pool and a table that are not empty nor beyond 2^31 tokens");
     }
-    if (p.num_splits > 0x10000 || p.batch * ((p.max_blocks_per_seq * p.block_size + kSpan - 1) / kSpan) > 0x7fff0000LL || p.batch > 0x7fffff) {
+    if (p.num_splits > 0x10000 || p.batch * (p.max_blocks_per_seq * p.block_size / 64 + 1 + kBorder) > 0x7fff0000LL || p.batch > 0x7fffff) {
         return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): num_splits=" + std::to_string(p.num_splits) + ", batch=" + std::to_string(p.batch) +
                                               ": more work than the schedule counts");
     }

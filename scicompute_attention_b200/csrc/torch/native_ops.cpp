@@ -27,7 +27,7 @@ namespace {
 
 constexpr int64_t kMaxSplits = 64;         // as MAX_SPLITS, DECODE_STEP_TOKENS in ops.py
 constexpr int64_t kDecodeStepTokens = 64;
-constexpr int64_t kFp8StepTokens = 128;    // as FP8_STEP_TOKENS, FP8_MAX_SPLITS
+constexpr int64_t kFp8BorderSteps = 2;     // as FP8_BORDER_STEPS, FP8_MAX_SPLITS
 constexpr int64_t kFp8MaxSplits = 512;
 
 PyObject* g_scratch = nullptr;          // ops._scratch: threading.local with the dict `pool`
@@ -212,10 +212,11 @@ PyObject* Flash(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // Partial slots per row, as slots_for_schedule in ops.py.
-int64_t SlotsForSchedule(int64_t column_steps, int64_t longest_steps, int64_t columns, int64_t sms, int64_t ctas_per_sm = 2, int64_t most = kMaxSplits) {
+int64_t SlotsForSchedule(int64_t column_steps, int64_t longest_steps, int64_t columns, int64_t sms, int64_t ctas_per_sm = 2, int64_t most = kMaxSplits,
+                         bool even = false) {
     if (column_steps <= 0 || longest_steps <= 1) return 1;
     const int64_t sharers = std::max<int64_t>(1, ctas_per_sm * sms / std::max<int64_t>(1, columns));
-    const int64_t per_cta = std::max<int64_t>(1, (column_steps + sharers - 1) / sharers);
+    const int64_t per_cta = std::max<int64_t>(1, even ? column_steps / sharers : (column_steps + sharers - 1) / sharers);
     return std::max<int64_t>(2, std::min((longest_steps + per_cta - 1) / per_cta + 1, most));
 }
 int64_t Steps(int64_t tokens, int64_t step = kDecodeStepTokens) { return (tokens + step - 1) / step; }
@@ -580,11 +581,13 @@ PyObject* PagedFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (p.num_kv_heads < 1 || p.num_heads % p.num_kv_heads != 0 || !Scale(a[8], d, &p.scale)) return NotTaken();
         const int64_t upper = l.shape.num_blocks * block_size;
         p.seq_kv = longest > 0 && lens != nullptr ? std::min(upper, longest) : upper;
-        const int64_t mean = typical > 0 ? typical : std::min(upper, table->size(1) * block_size), steps = Steps(mean, kFp8StepTokens);
-        const int64_t most = longest > 0 ? Steps(longest, kFp8StepTokens) : 2 * steps, group = p.num_heads / p.num_kv_heads;
+        const int64_t mean = typical > 0 ? typical : std::min(upper, table->size(1) * block_size), group = p.num_heads / p.num_kv_heads;
+        const int64_t step = d > 128 ? 64 : 128;  // as fp8_step_tokens
+        int64_t steps = Steps(mean, step), most = longest > 0 ? Steps(longest, step) : 2 * steps;
+        if (most > 1) steps += kFp8BorderSteps, most += kFp8BorderSteps;
         const int64_t sms = at::cuda::getDeviceProperties(q->device().index())->multiProcessorCount;
         const int64_t ctas = d <= 64 ? 4 : group > 8 && d > 96 ? 2 : 3;  // as fp8_ctas_per_sm
-        p.num_splits = mean <= 0 ? 1 : SlotsForSchedule(std::max<int64_t>(1, p.batch) * steps, most, p.num_kv_heads * ((group + 15) / 16), sms, ctas, kFp8MaxSplits);
+        p.num_splits = mean <= 0 ? 1 : SlotsForSchedule(std::max<int64_t>(1, p.batch) * steps, most, p.num_kv_heads * ((group + 15) / 16), sms, ctas, kFp8MaxSplits, true);
         p.q = q->data_ptr(), p.k = l.layer.k_codes, p.v = l.layer.v_codes;
         p.q_stride = ScaDecodeStrides{p.num_heads * d, d, d};
         p.o_stride = p.q_stride;

@@ -187,11 +187,12 @@ def acquire_scratch_fp32(elements: int, device: torch.device, kind: int = 1, *, 
 
 
 DECODE_STEP_TOKENS = 64  # tokens one CTA of the decode kernel consumes per step (4 warps x 16)
-FP8_STEP_TOKENS = 128    # the unit of the schedule over an 8-bit cache
+FP8_BORDER_STEPS = 2     # what the schedule over an 8-bit cache counts for a border between two sequences
 FP8_MAX_SPLITS = 512     # upper bound of its slot count: one sequence on every CTA of the machine
 
 
-def slots_for_schedule(column_steps: int, longest_steps: int, columns: int, sms: int, ctas_per_sm: int = 2, most: int = MAX_SPLITS) -> int:
+def slots_for_schedule(column_steps: int, longest_steps: int, columns: int, sms: int, ctas_per_sm: int = 2, most: int = MAX_SPLITS,
+                       even: bool = False) -> int:
     """Partial slots per row for the decode kernel's schedule: one wave of resident CTAs (2 per SM unless said), the same number
     for every (kv head, head chunk) column; the CTAs of a column split its list of 64-token steps (sequence after
     sequence) into equal contiguous shares, and a sequence cut by share boundaries yields one partial per piece.
@@ -201,7 +202,7 @@ def slots_for_schedule(column_steps: int, longest_steps: int, columns: int, sms:
         return 1
     resident = ctas_per_sm * (sms if sms > 0 else 148)
     sharers = max(1, resident // max(1, columns))
-    per_cta = max(1, -(-column_steps // sharers))
+    per_cta = max(1, column_steps // sharers if even else -(-column_steps // sharers))  # `even`: shares of a step more or less
     return max(2, min(-(-longest_steps // per_cta) + 1, most))
 
 
@@ -214,14 +215,16 @@ def splits_for(seq_kv: int, batch: int, num_kv_heads: int, group: int, sms: int)
 
 
 def paged_splits_for(typical_len: int, num_seqs: int, num_kv_heads: int, group: int, sms: int, longest_len: int = 0,
-                     step_tokens: int = DECODE_STEP_TOKENS, ctas_per_sm: int = 2, most: int = MAX_SPLITS) -> int:
+                     step_tokens: int = DECODE_STEP_TOKENS, ctas_per_sm: int = 2, most: int = MAX_SPLITS, border: int = 0) -> int:
     """Slot count for a ragged batch of mean length `typical_len`; the longest sequence is taken as twice the mean
     unless `longest_len` says otherwise."""
     if typical_len <= 0:
         return 1
     steps = -(-typical_len // step_tokens)
     longest = -(-longest_len // step_tokens) if longest_len > 0 else 2 * steps
-    return slots_for_schedule(max(1, num_seqs) * steps, longest, num_kv_heads * ((group + 15) // 16), sms, ctas_per_sm, most)
+    if longest > 1:  # what a sequence's border counts for
+        steps, longest = steps + border, longest + border
+    return slots_for_schedule(max(1, num_seqs) * steps, longest, num_kv_heads * ((group + 15) // 16), sms, ctas_per_sm, most, border > 0)
 
 
 def _strides(layout: str, seq: int, heads: int, d: int) -> tuple[int, int, int]:
@@ -717,6 +720,11 @@ def fp8_ctas_per_sm(head_dim: int, group: int) -> int:
     return 4 if head_dim <= 64 else 2 if group > 8 and head_dim > 96 else 3
 
 
+def fp8_step_tokens(head_dim: int) -> int:
+    """The unit of its schedule."""
+    return 64 if head_dim > 128 else 128
+
+
 def _require_one_device(first: torch.Tensor, *others: torch.Tensor) -> None:
     for t in others:
         if t.device != first.device:
@@ -859,7 +867,7 @@ def paged_attention_fp8(q, k_pool, v_pool, page_table, seq_lens, *, block_size: 
     max_blocks, upper = page_table.shape[1], nblk * bs
     device, handle = q.device, _stream_ptr(stream)
     splits = paged_splits_for(typical_len if typical_len > 0 else min(upper, max_blocks * bs), s, hkv, hq // hkv, sm_count(device), longest_len,
-                              FP8_STEP_TOKENS, fp8_ctas_per_sm(d, hq // hkv), FP8_MAX_SPLITS)
+                              fp8_step_tokens(d), fp8_ctas_per_sm(d, hq // hkv), FP8_MAX_SPLITS, FP8_BORDER_STEPS)
     base = s * hq * splits
     o_at = -(-2 * base // 4) * 4  # the O of a part starts on 16 bytes
     ws = acquire_scratch_fp32(o_at + base * d, device, stream=stream, handle=handle)
