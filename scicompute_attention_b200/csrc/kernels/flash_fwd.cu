@@ -193,7 +193,7 @@ int CheckSequences(const VarlenWork& vw, bool causal) {
 // block first, and copies both into the workspace (stream-ordered; the host vector may die on return), or into `small` where that is given
 // and they fit it; the lists are null then.
 int UploadVarlenWork(const VarlenWork& vw, int tokens_per_entry, int block_n, bool causal, cudaStream_t stream,
-                     const int4** seqs_out, const int2** entries_out, int* num_entries_out, WorkImage* small = nullptr) {
+                     const int4** seqs_out, const int2** entries_out, WorkImage* small) {
     const size_t seq_bytes = static_cast<size_t>(vw.num_seqs) * sizeof(int4);
     struct Weighted {
         int2 entry;
@@ -221,7 +221,6 @@ int UploadVarlenWork(const VarlenWork& vw, int tokens_per_entry, int block_n, bo
     image.resize((bytes + sizeof(int4) - 1) / sizeof(int4));
     int2* entries = reinterpret_cast<int2*>(reinterpret_cast<unsigned char*>(image.data()) + seq_bytes);
     for (size_t i = 0; i < list.size(); ++i) entries[i] = list[i].entry;
-    *num_entries_out = static_cast<int>(list.size());
     if (small != nullptr && bytes <= sizeof(small->bytes)) {
         std::memcpy(small->bytes, image.data(), bytes);
         small->entries_at = static_cast<int>(seq_bytes);
@@ -349,8 +348,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
     if (varlen != nullptr) {
         most_keys = 0;
         for (int64_t i = 0; i < varlen->num_seqs; ++i) most_keys = std::max<int64_t>(most_keys, static_cast<int64_t>(varlen->cu_kv[i + 1]) - varlen->cu_kv[i]);
-        if (int rc = UploadVarlenWork(*varlen, item_tokens, BN, f.causal != 0, stream, &p.seqs, &p.entries, &p.num_entries,
-                                      paged != nullptr && paged->k_scales != nullptr ? &small : nullptr)) return rc;
+        p.num_entries = static_cast<int>(VarlenEntries(*varlen, item_tokens));
     }
     const int64_t ctas = (varlen != nullptr ? static_cast<int64_t>(p.num_entries) : static_cast<int64_t>(p.m_blocks) * p.batch) *
                          (p.heads >> pack_shift);
@@ -358,6 +356,10 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
         return Fail(SCA_INVALID_ARGUMENT, "flash attention: grid of " + std::to_string(ctas) + " blocks is out of range");
     }
     p.cluster = tiles_per_item == 1 ? SplitCluster<T, DP, QT, BN>(ctas, (most_keys + BN - 1) / BN) : 1;
+    if (varlen != nullptr) {
+        const bool taken = TakesWorkImage(DP, paged != nullptr && paged->k_scales != nullptr, p.cluster > 1);
+        if (int rc = UploadVarlenWork(*varlen, item_tokens, BN, f.causal != 0, stream, &p.seqs, &p.entries, taken ? &small : nullptr)) return rc;
+    }
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, SmCount()));  // one persistent CTA per SM
     constexpr unsigned threads = FlashThreads<T, DP, QT>();
     if (paged != nullptr) {

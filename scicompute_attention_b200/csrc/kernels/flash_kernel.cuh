@@ -123,7 +123,7 @@ struct FlashKernelParams {
     int pack_shift;      // log2 of the query heads that share a tile (see "Packed heads")
     int tiles_per_item;  // query tiles a work item fills (at most QT)
     // packed variable-length batches (null for dense [B, H, S, D] problems): seqs[s] = {first query token,
-    // first key token, S_q, S_kv}; entries[e] = {sequence, query block}, heaviest first. kKv8 kernels: null where the list came as WorkImage
+    // first key token, S_q, S_kv}; entries[e] = {sequence, query block}, heaviest first. Null where the list came as a WorkImage
     const int4* seqs;
     const int2* entries;
     int num_entries;
@@ -144,8 +144,12 @@ struct WorkImage {
     int entries_at;
 };
 struct NoWorkImage {};
-template <bool kKv8>
-using WorkParam = std::conditional_t<kKv8, WorkImage, NoWorkImage>;
+// Not the D=64 kernels in which a CTA has its items to itself: their clocks hang on how the softmax is scheduled around the look-up (9
+// sequences, 4500 tokens against 1000 to 3500 keys, 32 / 8 heads, list in memory / as a parameter: fp16 without a mask 186 / 205 us, bf16
+// 199 / 197; D=128, bf16 235 / 220).
+constexpr bool TakesWorkImage(int padded_dim, bool kv8, bool split) { return kv8 && (padded_dim != 64 || split); }
+template <bool kTaken>
+using WorkParam = std::conditional_t<kTaken, WorkImage, NoWorkImage>;
 
 // 16 elements of an output row: one 32-byte store where every row starts on a 32-byte boundary, else two of 16 bytes. A
 // thread writes a row of its own, so each store of a warp touches 32 separate rows and takes the load/store unit 32 turns
@@ -280,7 +284,7 @@ __device__ __forceinline__ float HalveQueryRow(uint32_t tile, int row) {
 template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kKv8 = false, bool kSplit = false>
 __global__ void __launch_bounds__(FlashThreads<T, DP, QT, kKv8>(), 1)
 flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p, const __grid_constant__ WorkParam<kKv8> image) {
+                       const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p, const __grid_constant__ WorkParam<TakesWorkImage(DP, kKv8, kSplit)> image) {
     using G = FlashGeom<DP, QT, BN, kKv8>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem_base = (SmemAddr(smem_raw) + 1023u) & ~1023u;
@@ -367,7 +371,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if constexpr (kVarlen) {
             const int4* seqs = p.seqs;
             const int2* entries = p.entries;
-            if constexpr (kKv8) {
+            if constexpr (TakesWorkImage(DP, kKv8, kSplit)) {
                 if (seqs == nullptr) {
                     seqs = reinterpret_cast<const int4*>(image.bytes);
                     entries = reinterpret_cast<const int2*>(image.bytes + image.entries_at);
