@@ -1,8 +1,8 @@
 // Paged decode attention (one query token per head) over the 8-bit KV cache of kv_fp8.cuh.
 //
 // Per (sequence, head): s_j = scale * q . k_j, out = sum_j exp(s_j) v_j / sum_j exp(s_j) over the sequence's tokens, with
-// k_j = 2^e_j codes_j and v_j likewise. The schedule, the merge of the parts and the one-launch form on clusters are those of
-// the 16-bit cache (decode_common.cuh); what differs is the pass over a piece of a sequence:
+// k_j = 2^e_j codes_j and v_j likewise. The one-launch form on clusters is that of the 16-bit cache (decode_common.cuh), the schedule
+// and the merge of the parts do the same in less time; what differs is the pass over a piece of a sequence:
 //
 //   * bytes: 2 * (D + 1) per token and kv head, read once for all query heads of the kv head. 4 * D FLOPs per byte pair and
 //     query head: at eight heads 16 FLOPs a byte, so the products run on the tensor cores and HBM stays the bound;
@@ -17,6 +17,11 @@
 //     kv_fp8.cuh). Applied to P instead it would cost less, but P in fp16 has no range for it: 2^21 between two rows of V;
 //   * bf16 queries become fp16 by a power of two per head that puts the largest at 2^14: exact but for numbers below 2^-28 of
 //     it; P is rounded to fp16 (2^-11 of numbers up to 1), V and K not at all. Sums and statistics are fp32.
+//
+// What bounds it: HBM where a call is long - 256 sequences of 512 to 8192 tokens (32 / 8 heads, D=128, 2.31 GB) 368 us = 6.3 TB/s, the
+// slope over the length 6.9 (D=64 6.2; 4.9 with 16 heads to a kv head, where a warp's chain of products and exponentials counts: issue slots 51 % busy). Every
+// other call pays 11 us that no byte moves in: 1.3 until a CTA knows its share, 1.2 until its first loads are out, 2 until they are there,
+// 1 for the CTA's merge, 3 for the merge kernel, and 2 between the median CTA's end and the last one's.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -498,8 +503,8 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
     const int share = grid >= columns ? cta / columns : 0;
     const int first_column = grid >= columns ? cta % columns : cta;
     const int column_stride = grid >= columns ? columns : grid;
-    if (share >= sharers) return;  // a grid that is no multiple of the column count
     WaitForPredecessor();
+    if (share >= sharers) return;  // a grid that is no multiple of the column count
 
     const int batch = static_cast<int>(p.batch), splits = static_cast<int>(p.num_splits);
     const int cap = static_cast<int>(p.max_blocks_per_seq * p.block_size < 0x7fffff00LL ? p.max_blocks_per_seq * p.block_size : 0x7fffff00LL);
@@ -717,11 +722,12 @@ int64_t ResidentClusters(int cluster) {
 }
 
 // Whether the one-launch kernel is the faster one for `units` (sequence, kv head, head chunk) columns of `steps` times 128 tokens (the
-// longest) on clusters of `cluster` CTAs. Both times in us, fitted to 350 graph-timed calls on a B200 (D=64 to 256, 1 to 40 sequences of 60 to
-// 30 thousand tokens): a step of a CTA costs more the wider the head, the more heads share it and the more CTAs share the memory; the schedule
-// works on what a ragged batch holds, a cluster waits for the longest sequence. One launch / schedule: D=128, 32 / 8 heads, B=1, S=800
-// 5.9 / 9.9, S=12000 17.1 / 13.8, B=8, S=2000 12.9 / 16.9; D=256, 16 / 2, B=1, S=5000 16.6 / 11.8; D=64, 32 / 2, B=4, S=12000 17.7 / 14.4.
-// The choices take 1 % longer than the faster of the two on average, 29 % at most (40 sequences of 60 tokens, 32 / 2 heads: 11.1 / 8.6).
+// longest) on clusters of `cluster` CTAs. Both times in us, fitted to 384 graph-timed calls on a B200 (D=64 to 256, 1 to 40 sequences of 60
+// to 30 thousand tokens): a step of a CTA costs more the wider the head, the more heads share it and the more CTAs share the memory; the
+// schedule works on what a ragged batch holds, a cluster waits for the longest sequence. One launch / schedule: D=128, 32 / 8 heads, B=1,
+// S=800 5.6 / 9.1, S=12000 16.8 / 15.5, B=8, S=2000 12.9 / 14.3; D=256, 16 / 2, B=1, S=5000 16.5 / 14.8; D=64, 32 / 2, B=4, S=12000
+// 18.0 / 15.8. The choices take 0.4 % longer than the faster of the two on average, 22 % at most (40 sequences of 60 tokens, 32 / 2 heads,
+// D=128: 11.2 / 9.1).
 bool OneLaunchIsFaster(int64_t units, int64_t steps, int cluster, int64_t resident, int head_dim, bool hi) {
     const double busy = static_cast<double>(units * cluster) / resident;
     const double share = static_cast<double>((steps + cluster - 1) / cluster);
