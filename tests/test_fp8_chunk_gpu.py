@@ -151,11 +151,12 @@ def test_a_query_of_nan_gives_nan(kind, lens, new):
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("seqs", [85, 86, 200])
-def test_work_lists_of_any_length(seqs):
-    """Lists of up to 2 KB (85 sequences of one entry) go with the launch, longer ones ahead of it."""
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("seqs", [3, 85, 86, 200])
+def test_work_lists_of_any_length(seqs, d):
+    """Lists of up to 2 KB (85 sequences of one entry) go with the launch, longer ones - and those of whole D=64 items - ahead of it."""
     from scicompute_attention_b200 import ops
     rng = np.random.default_rng(23)
     new = [1 + i % 7 for i in range(seqs)]
-    q, k, v, table, cu, lens = case(rng, [n + 11 * (i % 5) for i, n in enumerate(new)], new, 16, 4, 2, 64, "fp16")
-    check(run(q, k, v, table, cu, lens), q, k, v, table, cu, lens, 16, True, ops.effective_scale(None, 64), "fp16")
+    q, k, v, table, cu, lens = case(rng, [n + 11 * (i % 5) for i, n in enumerate(new)], new, 16, 4, 2, d, "fp16")
+    check(run(q, k, v, table, cu, lens), q, k, v, table, cu, lens, 16, True, ops.effective_scale(None, d), "fp16")
