@@ -487,6 +487,7 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
 constexpr int kBorder = 2;
 // CTAs of a wave that are left out. The merge kernel of the call before may still hold a place on some SM, and the CTA that finds none runs
 // when all the others have: the 96 sequences 37 us with none left out, 34.3 with 2, 31.4 with 4; D=256, 40 of 100 to 5000 34.5, 31.2, 31.0.
+// Columns of few sharers keep them all: one in sixteen costs as much.
 constexpr int kLeftOut = 4;
 
 // The schedule of decode_common.cuh (WalkSchedule: what it does and why) for lists of less than 2^31 steps, with borders that count, shares
@@ -755,8 +756,9 @@ int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chu
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(&decode_fp8_partial_kernel<T, D, kHi>), G::kSmemBytes, "decode_fp8_partial_kernel")) return rc;
     // one wave, almost: CTAs per column as many as stay resident, never more than the column has steps (or sequences, with one slot)
     const int64_t useful = p.batch * ((longest + G::kSpan - 1) / G::kSpan);
-    const int64_t wave = std::max(columns, resident - kLeftOut);
-    const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(wave / columns, useful)) : resident;
+    int64_t sharers = resident / columns;
+    if (sharers > 16 && sharers * columns > resident - kLeftOut) --sharers;
+    const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(sharers, useful)) : resident;
     LaunchDependent(decode_fp8_partial_kernel<T, D, kHi>, blocks, kThreads, G::kSmemBytes, stream, 1, p, scales, head_chunks);
     if (int rc = CheckLaunch("decode_fp8_partial_kernel", stream)) return rc;
     return LaunchFp8Merge<T, D>(p, stream);
