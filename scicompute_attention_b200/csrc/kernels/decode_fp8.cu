@@ -485,9 +485,9 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
 // Without it the CTAs with a border end 7 us after the others (96 sequences of 200 to 6000 tokens, 32 / 2 heads, D=64 34.3 / 30.5 us; 64 of
 // 300 to 3000, 32 / 8 heads 34.4 / 32.6). One step or three 31.5.
 constexpr int kBorder = 2;
-// CTAs of a wave that are left out. The merge kernel of the call before may still hold a place on some SM, and the CTA that finds none runs
-// when all the others have: the 96 sequences 37 us with none left out, 34.3 with 2, 31.4 with 4; D=256, 40 of 100 to 5000 34.5, 31.2, 31.0.
-// Columns of few sharers keep them all: one in sixteen costs as much.
+// CTAs of a wave that are left out: with every place of the machine taken a call takes 6 us more, as if a CTA found its place still held (the
+// merge kernel of the call before is the one that could) and ran when the others had. The 96 sequences 37 us with none left out, 34.3 with
+// 2, 31.4 with 4; D=256, 40 of 100 to 5000 34.5, 31.2, 31.0. Columns of few sharers keep them all: one in sixteen costs as much.
 constexpr int kLeftOut = 4;
 
 // The schedule of decode_common.cuh (WalkSchedule: what it does and why) for lists of less than 2^31 steps, with borders that count, shares
