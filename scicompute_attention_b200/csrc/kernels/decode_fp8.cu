@@ -392,8 +392,10 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     const float m_new = fmaxf(m_run[t][h], mx);
-                    const float shift = m_new == -CUDART_INF_F ? 0.0f : -m_new * unit[t][h];
-                    alpha[h] = Exp2(fmaf(m_run[t][h], unit[t][h], shift));
+                    const float shift = m_new == -CUDART_INF_F ? 0.0f : -__fmul_rn(m_new, unit[t][h]);
+                    // the difference of the two shifts as they were rounded, so exactly 1 where the maximum stands still: a fused product
+                    // leaves the rounding of the shift, up to 2^-24 of the score, which every tile would multiply l and O by again
+                    alpha[h] = Exp2(__fadd_rn(__fmul_rn(m_run[t][h], unit[t][h]), shift));
                     m_run[t][h] = m_new;
                     float sum = 0.0f;
 #pragma unroll
