@@ -404,7 +404,7 @@ SCA_ABI int sca_launch_kv_gather_fp8(const void* codes, const uint8_t* scales, c
                                      int64_t num_blocks, void* out, const ScaKvCacheShape* shape,
                                      int32_t dtype_id, void* stream);
 /* sca_launch_decode_auto over an 8-bit paged cache: params->k / v are the codes of the pools, the strides of K and V are
- * those of the pool and are not read; q and out are fp16 or bf16, block_size a multiple of 4. seq_kv: tokens of the longest
+ * those of the pool and are not read; q and out are fp16 or bf16, block_size a multiple of 4; scale > 0 and finite. seq_kv: tokens of the longest
  * sequence as far as the caller knows (it sizes the launch), and of every sequence where seq_lens is null. `cluster_ctas` may be null. */
 SCA_ABI int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, const uint8_t* k_scales,
                                            const uint8_t* v_scales, int32_t* cluster_ctas, void* stream);

@@ -809,6 +809,9 @@ extern "C" int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, 
         return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): invalid geometry batch=" + std::to_string(p.batch) + " heads=" +
                                               std::to_string(p.num_heads) + " kv_heads=" + std::to_string(p.num_kv_heads));
     }
+    if (!(p.scale > 0.0f) || !std::isfinite(p.scale)) {  // the kernel's `unit` is positive, and a maximum of scores one of products
+        return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): scale must be > 0 and finite");
+    }
     if (p.num_kv_blocks > 0 && p.block_size > 0 && p.num_kv_heads * p.head_dim / 16 > 0xffffffffLL / std::max<int64_t>(1, p.num_kv_blocks * p.block_size)) {
         return Fail(SCA_INVALID_ARGUMENT, "paged attention (fp8): a pool of more than 64 GiB");
     }
