@@ -28,6 +28,7 @@
 
 #include "common.cuh"
 #include "decode_common.cuh"
+#include "decode_fp8_shares.cuh"
 #include "kv_fp8.cuh"
 
 namespace sca_b200 {
@@ -483,47 +484,33 @@ __device__ __forceinline__ void Fp8Segment(const ScaDecodeFwdParams& p, const Fp
     MergeFp8Warps<D, G::kWarpBytes, kToShared>(p, smem, b, head0, nheads, slot);
 }
 
-// What the border between two sequences of a CTA - the end of one segment, the first loads of the next - counts for in its share, in steps.
-// Without it the CTAs with a border end 7 us after the others (96 sequences of 200 to 6000 tokens, 32 / 2 heads, D=64 34.3 / 30.5 us; 64 of
-// 300 to 3000, 32 / 8 heads 34.4 / 32.6). One step or three 31.5.
-constexpr int kBorder = 2;
-// CTAs of a wave that are left out: with every place of the machine taken a call takes 6 us more, as if a CTA found its place still held (the
-// merge kernel of the call before is the one that could) and ran when the others had. The 96 sequences 37 us with none left out, 34.3 with
-// 2, 31.4 with 4; D=256, 40 of 100 to 5000 34.5, 31.2, 31.0. Columns of few sharers keep them all: one in sixteen costs as much.
-constexpr int kLeftOut = 4;
-
 // The schedule of decode_common.cuh (WalkSchedule: what it does and why) for lists of less than 2^31 steps, with borders that count, shares
 // that differ by a step at most, lengths that are read once, and nothing divided in 64 bits. With the last two it took 3500 clocks until a
-// CTA knew its share; a CTA's K/V is 30000 to 60000.
+// CTA knew its share; a CTA's K/V is 30000 to 60000. Its arithmetic is in decode_fp8_shares.cuh.
 template <int kSpan, typename Segment>
 __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, const int head_chunks, const Segment& segment) {
     __shared__ int s_part[kWarps][2];
     __shared__ int s_found[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int columns = static_cast<int>(p.num_kv_heads) * head_chunks, grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
-    // grids smaller than the number of columns let every CTA walk several columns, each as its only CTA
-    const int sharers = grid >= columns ? grid / columns : 1;
-    const int share = grid >= columns ? cta / columns : 0;
-    const int first_column = grid >= columns ? cta % columns : cta;
-    const int column_stride = grid >= columns ? columns : grid;
+    const int columns = static_cast<int>(p.num_kv_heads) * head_chunks;
+    const SchedulePlace place = PlaceOf(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), columns);
     WaitForPredecessor();
-    if (share >= sharers) return;  // a grid that is no multiple of the column count
+    if (place.share >= place.sharers) return;  // a grid that is no multiple of the column count
 
     const int batch = static_cast<int>(p.batch), splits = static_cast<int>(p.num_splits);
     const int cap = static_cast<int>(p.max_blocks_per_seq * p.block_size < 0x7fffff00LL ? p.max_blocks_per_seq * p.block_size : 0x7fffff00LL);
     const int all = static_cast<int>(min(p.seq_kv, static_cast<int64_t>(cap)));  // without lengths
     auto length = [&](int i) { return max(0, min(p.seq_lens != nullptr ? p.seq_lens[i] : all, cap)); };
-    auto steps_of = [](int len) { return max(1, static_cast<int>((static_cast<uint32_t>(len) + kSpan - 1) / kSpan)); };
     // sequences [mine, end_mine) are this thread's
     const int each = (batch + kThreads - 1) / kThreads;
     const int mine = min(batch, static_cast<int>(threadIdx.x) * each), end_mine = min(batch, mine + each);
     int sum = 0, longest = 0;
     for (int i = mine; i < end_mine; ++i) {
-        const int t = steps_of(length(i));
+        const int t = StepsOf(length(i), kSpan);
         sum += t;
         longest = max(longest, t);
     }
-    const int border = __syncthreads_or(longest > 1) ? kBorder : 0;
+    const int border = BorderOf(__syncthreads_or(longest > 1) ? 2 : 1);
     sum += (end_mine - mine) * border;
     int up = sum;
 #pragma unroll
@@ -542,26 +529,12 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
         total += s_part[w][0];
         longest = max(longest, s_part[w][1]);
     }
-    longest += border;
-    // at least so many that no sequence falls into more than `splits` pieces; with one slot a column goes to its first CTA, unless no sequence
-    // can be cut
-    const int least = splits > 1 ? (longest + splits - 2) / (splits - 1) : longest == 1 ? 1 : total;
-    // `sharing` CTAs take `each_share` steps, the first `more` of them one more
-    const int sharing = max(1, min(sharers, total / least)), each_share = total / sharing, more = total - sharing * each_share;
-    if (share >= sharing) return;
-    const int begin = share * each_share + min(share, more), end = begin + each_share + (share < more ? 1 : 0);
-    auto sharer_of = [&](int step) {
-        const int left = step - more * (each_share + 1);
-        return left < 0 ? step / (each_share + 1) : more + left / each_share;
-    };
+    const Shares shares = ShareSteps(total, longest + border, splits, place.sharers);
+    if (place.share >= shares.sharing) return;
+    const int begin = shares.Begin(place.share);
     if (first <= begin && begin < first + sum) {
         int i = mine, before = first;
-        while (true) {
-            const int t = steps_of(length(i)) + border;
-            if (begin < before + t) break;
-            before += t;
-            ++i;
-        }
+        FindSequence(begin, kSpan, border, length, &i, &before);
         s_found[0] = i;
         s_found[1] = before;
     }
@@ -570,24 +543,15 @@ __device__ __forceinline__ void WalkFp8Schedule(const ScaDecodeFwdParams& p, con
     // the merge kernel that follows on the stream may be set up while this grid streams K/V
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-    for (int column = first_column; column < columns; column += column_stride) {
+    for (int column = place.column; column < columns; column += place.column_stride) {
         const int hk = column / head_chunks, hc = column % head_chunks;
-        int b = b_first, before = before_first, len = length(b), steps = steps_of(len) + border;
-        for (int pos = begin; pos < end;) {
-            const int t0 = pos - before, t1 = min(t0 + (end - pos), steps);
-            const int slot = t0 == 0 ? 0 : share - sharer_of(before);
-            if (t0 == 0) MarkUnusedSlots(p, b, hk, hc, sharer_of(before + steps - 1) - share + 1, splits);
-            const int64_t j_end = min(static_cast<int64_t>(t1 - border) * kSpan, static_cast<int64_t>(len));
-            if (t1 <= border) MarkUnusedSlots(p, b, hk, hc, slot, slot + 1);
-            else segment(b, hk, hc, static_cast<int64_t>(max(t0 - border, 0)) * kSpan, j_end, slot);
-            pos += t1 - t0;
-            if (t1 == steps && pos < end) {
-                before += steps;
-                ++b;
-                len = length(b);
-                steps = steps_of(len) + border;
-            }
-        }
+        WalkShare(
+            shares, place.share, kSpan, border, b_first, before_first, length,
+            [&](int b, int64_t j_begin, int64_t j_end, int slot, bool bare) {
+                if (bare) MarkUnusedSlots(p, b, hk, hc, slot, slot + 1);
+                else segment(b, hk, hc, j_begin, j_end, slot);
+            },
+            [&](int b, int used) { MarkUnusedSlots(p, b, hk, hc, used, splits); });
     }
 }
 
@@ -756,11 +720,7 @@ int LaunchFp8(const ScaDecodeFwdParams& p, const Fp8Scales& scales, int head_chu
         return CheckLaunch("decode_fp8_cluster_kernel", stream);
     }
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(&decode_fp8_partial_kernel<T, D, kHi>), G::kSmemBytes, "decode_fp8_partial_kernel")) return rc;
-    // one wave, almost: CTAs per column as many as stay resident, never more than the column has steps (or sequences, with one slot)
-    const int64_t useful = p.batch * ((longest + G::kSpan - 1) / G::kSpan);
-    int64_t sharers = resident / columns;
-    if (sharers > 16 && sharers * columns > resident - kLeftOut) --sharers;
-    const int64_t blocks = resident >= columns ? columns * std::max<int64_t>(1, std::min(sharers, useful)) : resident;
+    const int64_t blocks = ScheduleGrid(resident, columns, p.batch * ((longest + G::kSpan - 1) / G::kSpan));
     LaunchDependent(decode_fp8_partial_kernel<T, D, kHi>, blocks, kThreads, G::kSmemBytes, stream, 1, p, scales, head_chunks);
     if (int rc = CheckLaunch("decode_fp8_partial_kernel", stream)) return rc;
     return LaunchFp8Merge<T, D>(p, stream);
