@@ -18,16 +18,19 @@ namespace sca_b200 {
 // Without it the CTAs with a border end 7 us after the others (96 sequences of 200 to 6000 tokens, 32 / 2 heads, D=64 34.3 / 30.5 us; 64 of
 // 300 to 3000, 32 / 8 heads 34.4 / 32.6). One step or three 31.5.
 constexpr int kBorder = 2;
-// CTAs of a wave that are left out: with every place of the machine taken a call takes 6 us more, as if a CTA found its place still held (the
-// merge kernel of the call before is the one that could) and ran when the others had. The 96 sequences 37 us with none left out, 34.3 with
-// 2, 31.4 with 4; D=256, 40 of 100 to 5000 34.5, 31.2, 31.0. Columns of few sharers keep them all: one in sixteen costs as much.
+// CTAs of a wave that are left out, at least: with every place of the machine taken a call takes up to 9 us more, as if a CTA found its place
+// still held (the merge kernel of the call before is the one that could) and ran when the others had. With 0, 2, 4, 6, 8 left out, us: 96
+// sequences of 200 to 6001 tokens, D=64, 32 / 2 heads 34.8, 32.2, 30.6, 30.2, 30.2; 32 / 1 33.7, 31.1, 28.9, 28.5, 28.6; 16 / 2 25.4, 23.5, 23.4,
+// 23.4, 23.4; D=256, 40 of 100 to 5000, 16 / 2 32.7, 30.2, 30.1, 30.1, 30.1. By whole columns: 64 of 300 to 3000, D=64, 32 / 8 with 0, 8, 16 left
+// out 37.8, 31.4, 31.6; 32 / 16 with 0, 16, 32 61.4, 52.3, 52.8. Other calls take the same with and without (two CTAs to an SM; 32 / 4 heads
+// 21.1). Columns of few sharers keep them all: one in sixteen costs as much (40 / 40 heads, D=128, 11 sharers or 10: 110, 116).
 constexpr int kLeftOut = 4;
 
 // CTAs to launch: of `resident` that stay on the machine as many for every one of `columns` lists, never more than a list has steps.
 SCA_SHARES_FN int64_t ScheduleGrid(int64_t resident, int64_t columns, int64_t steps) {
     if (resident < columns) return resident;
     int64_t sharers = resident / columns;
-    if (sharers > 16 && sharers * columns > resident - kLeftOut) --sharers;
+    if (sharers > 16 && sharers > (resident - kLeftOut) / columns) sharers = (resident - kLeftOut) / columns;
     if (sharers > steps) sharers = steps;
     return columns * (sharers > 1 ? sharers : 1);
 }

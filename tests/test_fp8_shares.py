@@ -89,3 +89,17 @@ def test_good_hints_leave_no_cta_out(schedule):
         grid, pieces, used = schedule(span, splits, SMS * ctas, 2, len(lens) * -(-max(lens) // span), lens)
         check(lens, splits, 2, pieces, used)
         assert len({share for _, share, *_ in pieces}) >= 0.97 * grid / 2
+
+
+@pytest.mark.parametrize("ctas", [2, 3, 4])
+@pytest.mark.parametrize("columns", [1, 2, 3, 4, 5, 8, 12, 16, 20, 40, 74, 200, 1000])
+def test_size_of_the_wave(schedule, ctas, columns):
+    """Four CTAs of the wave at least are left out where a column has more than sixteen, and no more than whole columns ask for; never a CTA per column too
+    many for the machine, nor more than a list has steps."""
+    resident = ctas * SMS
+    grid, *_ = schedule(128, 8, resident, columns, 10 ** 6, [1000])
+    if resident // columns > 16:
+        assert grid % columns == 0 and resident - 4 - columns < grid <= resident - 4
+    else:
+        assert grid == max(1, resident // columns) * columns if resident >= columns else grid == resident
+    assert schedule(128, 8, resident, columns, 3, [300])[0] == min(grid, 3 * columns)
