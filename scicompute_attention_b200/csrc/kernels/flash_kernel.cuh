@@ -192,6 +192,24 @@ template <int QT, bool kKv8>
 constexpr bool ConvertersApart() {
     return kKv8 && QT == 2;
 }
+// 128 * (kIssueRegs + 2 * kSoftmaxRegs + kConvertRegs) registers of the 512 * 128 that such a CTA is launched with.
+constexpr int kIssueRegs = 96, kSoftmaxRegs = 168, kConvertRegs = 72;
+static_assert(kIssueRegs + 2 * kSoftmaxRegs + kConvertRegs <= 512, "more registers than the CTA has");
+// kKv8: the second warp that issues loads.
+template <int QT>
+constexpr int SecondProducer() {
+    return ConvertersApart<QT, true>() ? 2 : kFirstSoftmax + 4 * QT + 2;
+}
+// kKv8 with bf16 queries: the softmax warps rewrite query tiles as fp16 (HalveQueryRow).
+template <typename T, bool kKv8>
+constexpr bool kHalvesQuery = kKv8 && std::is_same<T, __nv_bfloat16>::value;
+// kKv8: barriers behind the others, from number kFirst on.
+template <int kFirst, int kRawSlots>
+struct RawBarriers {
+    static constexpr int kFull = kFirst;               // [kRawSlots] codes and scales have landed
+    static constexpr int kEmpty = kFull + kRawSlots;   // [kRawSlots] the converters have read them
+    static constexpr int kQHalf = kEmpty + kRawSlots;  // [kTiles] kHalvesQuery: the query tile is fp16
+};
 template <typename T, int DP, int QT, bool kKv8 = false>
 constexpr int FlashThreads() {
     return ConvertersApart<QT, kKv8>() ? 512 : 32 * (kFirstSoftmax + 4 * QT + (ConverterWarps<T, DP, kKv8>() > 2 ? ConverterWarps<T, DP, kKv8>() - 2 : 0) + (kKv8 ? 1 : 0));
@@ -274,6 +292,109 @@ __device__ __forceinline__ float HalveQueryRow(uint32_t tile, int row) {
     return fp8::PowerOfTwo(max(k - 14, -126));
 }
 
+// kKv8, the TMA producers: warp 0 (`producer` 0) and SecondProducer (1). They take the loads in turn (raw slots are even in number: a slot
+// belongs to one of them): one that issues all of them - at 16 tokens to a page 8 boxes of a page each - is what the converters wait for. The
+// lanes fetch the page ids of a warp's next load ahead and copy its scales, four keys each; one lane issues the boxes, whose rows it finds in
+// shared memory. A page that is unmapped is loaded from beyond the pool, i.e. zero-filled, and masked through valid_ring. Returns false where
+// a wait ran out. In a function of its own, and the constants of the 8-bit cache outside the kernel: three constants more in the kernel's
+// body, unused, and the compiler orders the bf16 kernel of D=256 over a 16-bit cache otherwise: 20 chunks 538 us for 531.
+template <int DP, int QT, int BN, bool kSplit, int kQFull, int kQEmpty, int kRawFull, int kRawEmpty, int kValidRing, typename ItemOf, typename Decode, typename Bar>
+__device__ __forceinline__ bool ProduceRaw(const FlashKernelParams& p, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const int producer,
+                                           const int rounds, const ItemOf& item_of_round, const Decode& decode_item, const Bar& bar, const uint32_t q_smem,
+                                           const uint32_t raw_smem, int* page_rows, volatile uint32_t* valid_ring, volatile int* abort_flag) {
+    using G = FlashGeom<DP, QT, BN, true>;
+    const int lane = threadIdx.x & 31;
+    static_assert(G::kRawSlots % 2 == 0, "each producer fills slots of its own");
+    if (lane == 0) {
+        if (producer == 0) PrefetchTensorMap(&map_q);
+        PrefetchTensorMap(&map_k);
+        PrefetchTensorMap(&map_v);
+    }
+    uint32_t q_uses[QT] = {};
+    uint32_t kv_base = 0;       // loads of the items before
+    uint32_t tiles_before = 0;  // KV tiles of them
+    const int pages_per_tile = BN >> p.block_shift, pages_per_v = G::kVKeys >> p.block_shift;
+    bool ok = true;
+    for (int r = 0; r < rounds && ok; ++r) {
+        const int idx = item_of_round(r);
+        if (idx < 0) continue;
+        const auto w = decode_item(idx);
+        if (producer == 0 && lane == 0) {
+            for (int t = 0; t < QT && ok; ++t) {
+                if (w.ntiles[t] == 0) continue;
+                if (q_uses[t] > 0) ok = MbarWait(bar(kQEmpty + t), (q_uses[t] - 1) & 1u, abort_flag);
+                if (!ok) break;
+                MbarExpectTx(bar(kQFull + t), G::kQTileBytes);
+                for (int kb = 0; kb < G::kKBlocks; ++kb) {
+                    TmaLoad4D(q_smem + t * G::kQTileBytes + kb * G::kQBlockBytes, &map_q, bar(kQFull + t), kb * 64,
+                              w.h, w.q_tok0 + w.m0[t], w.b);
+                }
+                ++q_uses[t];
+            }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        const int32_t* row = p.page_table + static_cast<int64_t>(w.seq) * p.max_blocks_per_seq;
+        const int loads = 2 * w.n_max * G::kParts;
+        auto page_ids = [&](int it) {  // of the tile of load `it`, one per lane
+            if (it >= loads) return -1;
+            const int logical = ((kSplit ? w.first_tile : 0) + RingOrder(it / G::kParts, w.n_max, G::kOwnP).tile) * pages_per_tile + lane;
+            const bool in = lane < pages_per_tile && logical < p.max_blocks_per_seq && (static_cast<int64_t>(logical) << p.block_shift) < w.seq_kv;
+            return in ? row[logical] : -1;
+        };
+        int it = (kv_base ^ producer) & 1;
+        int32_t phys, phys_next = page_ids(it);
+        for (; it < loads && ok; it += 2) {
+            phys = phys_next;
+            phys_next = page_ids(it + 2);
+            const RingLoad load = RingOrder(it / G::kParts, w.n_max, G::kOwnP);
+            const bool there = phys >= 0 && phys < p.num_kv_blocks;
+            const uint32_t valid = __ballot_sync(0xffffffffu, there);
+            const uint32_t raw = (kv_base + it) % G::kRawSlots;
+            const uint32_t full = bar(kRawFull + raw);
+            if (lane == 0) {
+                ok = MbarWait(bar(kRawEmpty + raw), (((kv_base + it) / G::kRawSlots) & 1u) ^ 1u, abort_flag);
+                if (ok) {
+                    if (!load.is_v) valid_ring[(tiles_before + load.tile) % kValidRing] = valid;
+                    MbarExpectTx(full, G::kRawCodes);
+                }
+            }
+            page_rows[lane] = there ? phys << p.block_shift : p.num_kv_blocks << p.block_shift;
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (!ok) break;
+            const uint32_t dst = raw_smem + raw * G::kRawCodes;
+            const int part = it % G::kParts;
+            const int first_page = load.is_v ? part * pages_per_v : 0, pages = load.is_v ? pages_per_v : pages_per_tile;
+            __syncwarp();
+            if (ElectOne()) {
+                auto boxes = [&](const CUtensorMap* map, int column, uint32_t to) {
+#pragma unroll 2
+                    for (int pg = first_page; pg < first_page + pages; ++pg, to += G::kBoxWidth << p.block_shift) TmaLoad4D(to, map, full, column, page_rows[pg], w.h_kv, 0);
+                };
+                if (load.is_v) {
+#pragma unroll
+                    for (int box = 0; box < DP / G::kBoxWidth; ++box) boxes(&map_v, box * G::kBoxWidth, dst + box * G::kVKeys * G::kBoxWidth);
+                } else {
+                    boxes(&map_k, part * G::kBoxWidth, dst);
+                }
+            }
+            __syncwarp();
+            {
+                // the scales of four keys of one page per lane; they count as landed when the lane's copies have
+                const int key = 4 * lane, page = (first_page + (key >> p.block_shift)) & 31;
+                const int32_t id = __shfl_sync(0xffffffffu, phys, page);
+                const bool mapped = (valid >> page) & 1u;
+                const uint8_t* from = (load.is_v ? p.v_scales : p.k_scales) +
+                                      (mapped ? (static_cast<int64_t>(id) * p.kv_heads + w.h_kv) * p.scale_row + (key & (p.block_size - 1)) : 0);
+                if (key < (pages << p.block_shift)) CpAsync4(raw_smem + G::kRawSlots * G::kRawCodes + raw * BN + key, from, mapped ? 4 : 0);
+                CpAsyncArrive(full);
+            }
+        }
+        kv_base += static_cast<uint32_t>(loads);
+        tiles_before += static_cast<uint32_t>(w.n_max);
+    }
+    return ok;
+}
+
 // kVarlen: the work list comes from the (sequence, query block) table of a packed ragged batch; otherwise it is
 // computed from the dense [B, H, S, D] geometry and every per-sequence quantity is a launch constant.
 // kPaged (only with kVarlen): K and V of a sequence are scattered over the pages of a KV pool.
@@ -312,11 +433,8 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     constexpr int kPLast = kOFree + kTiles;         // [kTiles]
     constexpr int kVReady = kPLast + kTiles;        // [kSlots] bf16: V tile rewritten as fp16 in place
     constexpr int kSRead = kVReady + G::kSlots;     // [kTiles] kOwnP: scores in registers
-    constexpr int kRawFull = kSRead + kTiles;       // [kRawSlots] kKv8: codes and scales have landed
-    constexpr int kRawEmpty = kRawFull + G::kRawSlots;  // [kRawSlots] kKv8: the converters have read them
-    constexpr int kQHalf = kRawEmpty + G::kRawSlots;    // [kTiles] kKv8, bf16: the query tile is fp16
-    constexpr bool kHalveQ = kKv8 && std::is_same<T, __nv_bfloat16>::value;
-    constexpr int kNumBars = kQHalf + (kHalveQ ? kTiles : 0);
+    using Raw = RawBarriers<kSRead + kTiles, G::kRawSlots>;  // kKv8
+    constexpr int kNumBars = Raw::kQHalf + (kHalvesQuery<T, kKv8> ? kTiles : 0);
     auto full_bar = [&](bool is_v, uint32_t slot) { return bar(kKvFull + RingFullBarrier(is_v, static_cast<int>(slot), G::kSlots)); };
     using PT = typename PvFormat<T>::type;
     constexpr bool kCvtInKernel = kKv8 || PvFormat<T>::kConvertV;
@@ -339,9 +457,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     constexpr int kEndSoftmax = kFirstSoftmax + 4 * QT;
-    constexpr bool kApart = ConvertersApart<QT, kKv8>();
-    constexpr int kProducer1 = kApart ? 2 : kEndSoftmax + 2;  // kKv8: the second warp that issues loads
-    const int converter = kApart ? (warp >= kEndSoftmax ? warp - kEndSoftmax : -1) : warp < kFirstSoftmax ? warp - 2 : warp >= kEndSoftmax ? warp - kEndSoftmax + 2 : -1;
+    const int converter = ConvertersApart<QT, kKv8>() ? (warp >= kEndSoftmax ? warp - kEndSoftmax : -1) : warp < kFirstSoftmax ? warp - 2 : warp >= kEndSoftmax ? warp - kEndSoftmax + 2 : -1;
 
     // ---- Packed heads: P = 1 << pack_shift query heads of one kv head share a query tile (row r = token m0 + r / P, head
     // h + r % P). They read the same K/V tiles, so the rows of a short or ragged chunk fill up with other heads instead
@@ -442,10 +558,10 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         if constexpr (kKv8) {
             for (int i = 0; i < G::kRawSlots; ++i) {
-                MbarInit<1 + 32>(bar(kRawFull + i));  // the codes, and each lane's copy of scales
-                MbarInit<kConverters>(bar(kRawEmpty + i));
+                MbarInit<1 + 32>(bar(Raw::kFull + i));  // the codes, and each lane's copy of scales
+                MbarInit<kConverters>(bar(Raw::kEmpty + i));
             }
-            for (int i = 0; kHalveQ && i < kTiles; ++i) MbarInit<4>(bar(kQHalf + i));
+            for (int i = 0; kHalvesQuery<T, kKv8> && i < kTiles; ++i) MbarInit<4>(bar(Raw::kQHalf + i));
         }
         *abort_flag = 0;
         FenceBarrierInit();
@@ -460,114 +576,20 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     TcFenceAfter();
     const uint32_t tmem_base = *tmem_slot;
     BeginAfterPredecessor();
-    // kApart: 128 * (kIssueRegs + 2 * kSoftmaxRegs + kConvertRegs) registers of the 512 * 128 that the CTA was launched with
-    constexpr int kIssueRegs = 96, kSoftmaxRegs = 168, kConvertRegs = 72;
-    static_assert(kIssueRegs + 2 * kSoftmaxRegs + kConvertRegs <= 512, "more registers than the CTA has");
-    if (kApart && warp < kFirstSoftmax) KeepRegisters<kIssueRegs>();
+    if (ConvertersApart<QT, kKv8>() && warp < kFirstSoftmax) KeepRegisters<kIssueRegs>();
 
     bool failed = false;
     // kSplit: a row of a CTA's part is {O[DP], m, l}, padded so that neighbouring rows lie on different banks
     constexpr int kPartLd = DP + 4;
     static_assert(!kSplit || kBlockM * kPartLd * 4 <= G::kRingBytes, "a part has to fit the ring");
 
-    if (kKv8 && (warp == 0 || warp == kProducer1)) {
+    if (kKv8 && (warp == 0 || warp == SecondProducer<QT>())) {
         // ================================ TMA producers, 8-bit cache =================================
-        // Two warps take the loads in turn (raw slots are even in number: a slot belongs to one of them): one that issues all of
-        // them - at 16 tokens to a page 8 boxes of a page each - is what the converters wait for. The lanes fetch the page
-        // ids of a warp's next load ahead and copy its scales, four keys each; one lane issues the boxes, whose rows it finds in shared memory.
-        // A page that is unmapped is loaded from beyond the pool, i.e. zero-filled, and masked through valid_ring.
-        static_assert(!kKv8 || G::kRawSlots % 2 == 0, "each producer fills slots of its own");
-        const int producer = warp == 0 ? 0 : 1;
-        if (lane == 0) {
-            if (producer == 0) PrefetchTensorMap(&map_q);
-            PrefetchTensorMap(&map_k);
-            PrefetchTensorMap(&map_v);
+        if constexpr (kKv8) {
+            int* page_rows = reinterpret_cast<int*>(smem + (bar_base - smem_base) + G::kBarrierBytes - 256) + (warp == 0 ? 0 : 32);
+            failed = !ProduceRaw<DP, QT, BN, kSplit, kQFull, kQEmpty, Raw::kFull, Raw::kEmpty, kValidRing>(
+                p, map_q, map_k, map_v, warp == 0 ? 0 : 1, rounds, item_of_round, decode_item, bar, q_smem, raw_smem, page_rows, valid_ring, abort_flag);
         }
-        constexpr int kRaw = kKv8 ? G::kRawSlots : 1;
-        int* page_rows = reinterpret_cast<int*>(smem + (bar_base - smem_base) + G::kBarrierBytes - 256) + 32 * producer;
-        uint32_t q_uses[kTiles] = {};
-        uint32_t kv_base = 0;       // loads of the items before
-        uint32_t tiles_before = 0;  // KV tiles of them
-        const int pages_per_tile = BN >> p.block_shift, pages_per_v = G::kVKeys >> p.block_shift;
-        bool ok = true;
-        for (int r = 0; r < rounds && ok; ++r) {
-            const int idx = item_of_round(r);
-            if (idx < 0) continue;
-            const Item w = decode_item(idx);
-            if (producer == 0 && lane == 0) {
-                for (int t = 0; t < QT && ok; ++t) {
-                    if (w.ntiles[t] == 0) continue;
-                    if (q_uses[t] > 0) ok = MbarWait(bar(kQEmpty + t), (q_uses[t] - 1) & 1u, abort_flag);
-                    if (!ok) break;
-                    MbarExpectTx(bar(kQFull + t), G::kQTileBytes);
-                    for (int kb = 0; kb < G::kKBlocks; ++kb) {
-                        TmaLoad4D(q_smem + t * G::kQTileBytes + kb * G::kQBlockBytes, &map_q, bar(kQFull + t), kb * 64,
-                                  w.h, w.q_tok0 + w.m0[t], w.b);
-                    }
-                    ++q_uses[t];
-                }
-            }
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-            const int32_t* row = p.page_table + static_cast<int64_t>(w.seq) * p.max_blocks_per_seq;
-            const int loads = 2 * w.n_max * kParts;
-            auto page_ids = [&](int it) {  // of the tile of load `it`, one per lane
-                if (it >= loads) return -1;
-                const int logical = ((kSplit ? w.first_tile : 0) + RingOrder(it / kParts, w.n_max, kOwnP).tile) * pages_per_tile + lane;
-                const bool in = lane < pages_per_tile && logical < p.max_blocks_per_seq && (static_cast<int64_t>(logical) << p.block_shift) < w.seq_kv;
-                return in ? row[logical] : -1;
-            };
-            int it = (kv_base ^ producer) & 1;
-            int32_t phys, phys_next = page_ids(it);
-            for (; it < loads && ok; it += 2) {
-                phys = phys_next;
-                phys_next = page_ids(it + 2);
-                const RingLoad load = RingOrder(it / kParts, w.n_max, kOwnP);
-                const bool there = phys >= 0 && phys < p.num_kv_blocks;
-                const uint32_t valid = __ballot_sync(0xffffffffu, there);
-                const uint32_t raw = (kv_base + it) % kRaw;
-                const uint32_t full = bar(kRawFull + raw);
-                if (lane == 0) {
-                    ok = MbarWait(bar(kRawEmpty + raw), (((kv_base + it) / kRaw) & 1u) ^ 1u, abort_flag);
-                    if (ok) {
-                        if (!load.is_v) valid_ring[(tiles_before + load.tile) % kValidRing] = valid;
-                        MbarExpectTx(full, G::kRawCodes);
-                    }
-                }
-                page_rows[lane] = there ? phys << p.block_shift : p.num_kv_blocks << p.block_shift;
-                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                if (!ok) break;
-                const uint32_t dst = raw_smem + raw * G::kRawCodes;
-                const int part = it % kParts;
-                const int first_page = load.is_v ? part * pages_per_v : 0, pages = load.is_v ? pages_per_v : pages_per_tile;
-                __syncwarp();
-                if (ElectOne()) {
-                    auto boxes = [&](const CUtensorMap* map, int column, uint32_t to) {
-#pragma unroll 2
-                        for (int pg = first_page; pg < first_page + pages; ++pg, to += G::kBoxWidth << p.block_shift) TmaLoad4D(to, map, full, column, page_rows[pg], w.h_kv, 0);
-                    };
-                    if (load.is_v) {
-#pragma unroll
-                        for (int box = 0; box < DP / G::kBoxWidth; ++box) boxes(&map_v, box * G::kBoxWidth, dst + box * G::kVKeys * G::kBoxWidth);
-                    } else {
-                        boxes(&map_k, part * G::kBoxWidth, dst);
-                    }
-                }
-                __syncwarp();
-                {
-                    // the scales of four keys of one page per lane; they count as landed when the lane's copies have
-                    const int key = 4 * lane, page = (first_page + (key >> p.block_shift)) & 31;
-                    const int32_t id = __shfl_sync(0xffffffffu, phys, page);
-                    const bool mapped = (valid >> page) & 1u;
-                    const uint8_t* from = (load.is_v ? p.v_scales : p.k_scales) +
-                                          (mapped ? (static_cast<int64_t>(id) * p.kv_heads + w.h_kv) * p.scale_row + (key & (p.block_size - 1)) : 0);
-                    if (key < (pages << p.block_shift)) CpAsync4(raw_smem + G::kRawSlots * G::kRawCodes + raw * BN + key, from, mapped ? 4 : 0);
-                    CpAsyncArrive(full);
-                }
-            }
-            kv_base += static_cast<uint32_t>(loads);
-            tiles_before += static_cast<uint32_t>(w.n_max);
-        }
-        failed = !ok;
     } else if (warp == 0 && kPaged) {
         // ================================ TMA producer, paged K/V ===================================
         // The whole warp walks the work list: the lanes fetch the page ids of a tile together (one coalesced read
@@ -774,7 +796,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             uint32_t kv_base = 0;           // ring position of this item's K_0
             RingPhases k_phases, v_phases;  // of the K barriers and of v_ready (no converter: the V barriers)
             bool ok = true;
-            auto q_landed = [&](int t, uint32_t parity) { return MbarWait(bar((kHalveQ ? kQHalf : kQFull) + t), parity, abort_flag); };
+            auto q_landed = [&](int t, uint32_t parity) { return MbarWait(bar((kHalvesQuery<T, kKv8> ? Raw::kQHalf : kQFull) + t), parity, abort_flag); };
             auto k_landed = [&](uint32_t slot) {
                 if constexpr (kKv8) return MbarWait(bar(kVReady + slot), v_phases.Take(slot), abort_flag);  // K and V in turn, one barrier
                 return MbarWait(full_bar(false, slot), k_phases.Take(slot), abort_flag);
@@ -922,7 +944,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         // Walks the ring in the producer's order; every V tile is rewritten in place from bf16 to fp16 once its
         // bytes have landed, then handed to the MMA thread through v_ready. K tiles are not touched. kKv8: the codes
         // of K and V go from their raw slot into a slot of the ring.
-        if constexpr (kApart) KeepRegisters<kConvertRegs>();
+        if constexpr (ConvertersApart<QT, kKv8>()) KeepRegisters<kConvertRegs>();
         uint32_t kv_loads = 0;
         uint32_t tiles_before = 0;  // kKv8: index into valid_ring
         RingPhases v_phases;
@@ -937,7 +959,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 const uint32_t slot = kv_loads % G::kSlots;
                 if constexpr (kKv8) {
                     const uint32_t raw = kv_loads % (kKv8 ? G::kRawSlots : 1);
-                    ok = __all_sync(0xffffffffu, MbarWait(bar(kRawFull + raw), (kv_loads / (kKv8 ? G::kRawSlots : 1)) & 1u, abort_flag) &&
+                    ok = __all_sync(0xffffffffu, MbarWait(bar(Raw::kFull + raw), (kv_loads / (kKv8 ? G::kRawSlots : 1)) & 1u, abort_flag) &&
                                                      MbarWait(bar(kKvEmpty + slot), ((kv_loads / G::kSlots) & 1u) ^ 1u, abort_flag));
                     if (!ok) break;
                     const uint32_t codes = raw_smem + raw * G::kRawCodes, target = ring_smem + slot * G::kSlotBytes;
@@ -960,7 +982,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     __syncwarp();
                     if (lane == 0) {
                         MbarArrive(bar(kVReady + slot));
-                        MbarArrive(bar(kRawEmpty + raw));
+                        MbarArrive(bar(Raw::kEmpty + raw));
                     }
                     continue;
                 }
@@ -987,7 +1009,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         failed = !ok;
     } else if (warp >= kFirstSoftmax && warp < kEndSoftmax) {
         // ================================ softmax groups ============================================
-        if constexpr (kApart) TakeRegisters<kSoftmaxRegs>();
+        if constexpr (ConvertersApart<QT, kKv8>()) TakeRegisters<kSoftmaxRegs>();
         const int t = (warp - kFirstSoftmax) >> 2;
         const int quad = warp & 3;
         const int row_in_tile = quad * 32 + lane;
@@ -996,7 +1018,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const uint32_t p_addr = tmem_base + lane_bits + G::kPCol + t * G::kPStride;
         const uint32_t o_addr = tmem_base + lane_bits + G::kOCol + t * DP;
         uint32_t steps = 0;  // KV tiles this group has processed (phase of s_full / p_full / o_done)
-        uint32_t items = 0;  // kHalveQ: query tiles it has rewritten (phase of q_full)
+        uint32_t items = 0;  // kHalvesQuery<T, kKv8>: query tiles it has rewritten (phase of q_full)
         uint32_t tiles_before = 0;  // paged K/V: KV tiles of the items this CTA has finished (index into valid_ring)
         float* part_row = reinterpret_cast<float*>(smem + (ring_smem - smem_base)) + row_in_tile * kPartLd;  // kSplit
         const uint32_t all_pages = kPaged ? ((BN >> p.block_shift) >= 32 ? 0xffffffffu : (1u << (BN >> p.block_shift)) - 1u) : 0u;
@@ -1020,7 +1042,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const int row = m_t + (row_in_tile >> p.pack_shift);                 // token of the sequence
             const int head = w.h + (row_in_tile & ((1 << p.pack_shift) - 1));
             float scale_log2 = p.scale_log2;
-            if constexpr (kHalveQ) {
+            if constexpr (kHalvesQuery<T, kKv8>) {
                 ok = __all_sync(0xffffffffu, MbarWait(bar(kQFull + t), items & 1u, abort_flag));
                 if (!ok) break;
                 ++items;
@@ -1028,7 +1050,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 scale_log2 = fmaxf(scale_log2 * HalveQueryRow<DP>(q_smem + t * G::kQTileBytes, row_in_tile), fp8::PowerOfTwo(-126));
                 FenceProxyAsync();
                 __syncwarp();
-                if (lane == 0) MbarArrive(bar(kQHalf + t));
+                if (lane == 0) MbarArrive(bar(Raw::kQHalf + t));
             }
             float m_ref = -CUDART_INF_F;  // reference point of the exponentials (log2 domain)
             float l_sum = 0.0f;
