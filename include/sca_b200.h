@@ -380,6 +380,8 @@ SCA_ABI int sca_launch_kv_append_batched(void* layer_k, void* layer_v, const voi
 /* 448 in size (NaN stays NaN); value = code * 2^e, exact in fp16 and bf16.                       */
 /* codes  [num_blocks, block_size, kv_heads, D], 16-byte aligned, D a multiple of 16 up to 256     */
 /* scales [num_blocks, kv_heads, block_size rounded up to 16], one byte e + 15                     */
+/* That is what append and read-back take; attention takes D = 32, 64, 96, 128, 160, 192 and 256,   */
+/* with pages as its entries say. Other pools are for storage alone.                              */
 /* ------------------------------------------------------------------------------------------ */
 typedef struct ScaFp8Layer {
     void* k_codes;
@@ -409,7 +411,7 @@ SCA_ABI int sca_launch_kv_gather_fp8(const void* codes, const uint8_t* scales, c
 SCA_ABI int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, const uint8_t* k_scales,
                                            const uint8_t* v_scales, int32_t* cluster_ctas, void* stream);
 /* sca_launch_flash_paged over an 8-bit paged cache: params->k_pool / v_pool are the codes, scales 16-byte aligned, q and out are fp16 or
- * bf16. What lies behind a sequence's last token counts for nothing, whatever it is. */
+ * bf16, block_size 8, 16, 32 or 64. What lies behind a sequence's last token counts for nothing, whatever it is. */
 SCA_ABI int sca_launch_flash_paged_fp8(const ScaFlashPagedParams* params, const uint8_t* k_scales,
                                        const uint8_t* v_scales, void* stream);
 

@@ -699,7 +699,9 @@ class Fp8Pool(NamedTuple):
     codes   float8_e4m3fn (or uint8) [num_blocks, block_size, H_kv, D], D a multiple of 16 up to 256
     scales  uint8 [num_blocks, H_kv, block_size rounded up to 16]: e + 15
 
-    The operators take any pair of such tensors. Blocks are freed by kv_reset on the codes: a code of 0 is 0 under every scale."""
+    Append and read-back take any such pair. Attention takes D = 32, 64, 96, 128, 160, 192 and 256: a token per sequence (paged_attention_fp8) a
+    block_size that is a multiple of 4, chunks (flash_attention_paged_fp8) one of 8, 16, 32 or 64. Other pools are for storage alone.
+    Blocks are freed by kv_reset on the codes: a code of 0 is 0 under every scale."""
     codes: torch.Tensor
     scales: torch.Tensor
 
