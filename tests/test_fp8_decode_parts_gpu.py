@@ -87,3 +87,17 @@ def test_many_rows(hq, hkv, d):
                                          return_stats=True, **hints)
     assert stats["cluster"] == 0
     check(out[few], q[few], k, v, table[few], [lens[i] for i in few], bs, scale, "bf16")
+
+
+@pytest.mark.parametrize("hq,hkv,d,n", [(16, 1, 64, 140_000), (8, 1, 128, 100_003), (16, 1, 256, 60_001)])
+def test_one_long_sequence(hq, hkv, d, n):
+    """One sequence on every CTA of the machine: with and without hints, through the native and the general form."""
+    from scicompute_attention_b200 import ops
+    bs = 32
+    q, k, v, table = case(n, [n], hq, hkv, d, bs, "fp16", -(-n // bs))
+    args = q, to_device(k), to_device(v), torch.from_numpy(table).cuda(), torch.tensor([n], dtype=torch.int32).cuda()
+    want, bound = expected(q, k, v, table, [n], bs, ops.effective_scale(None, d), "fp16")
+    for hints in ({}, dict(typical_len=n, longest_len=n)):
+        out, stats = ops.paged_attention_fp8(*args, block_size=bs, return_stats=True, **hints)
+        assert stats["cluster"] == 0 and (np.abs(out[:, :, 0].double().cpu().numpy() - want) <= bound).all()
+        assert torch.equal(ops.paged_attention_fp8(*args, block_size=bs, **hints), out)
