@@ -16,7 +16,7 @@
 //   * the scale of K multiplies the scores in fp32; the scale of V multiplies V's codes in fp16, which is exact too (see
 //     kv_fp8.cuh). Applied to P instead it would cost less, but P in fp16 has no range for it: 2^21 between two rows of V;
 //   * bf16 queries become fp16 by a power of two per head that puts the largest at 2^14: exact but for numbers below 2^-28 of
-//     it; P is rounded to fp16 (2^-11 of numbers up to 1), V and K not at all. Sums and statistics are fp32.
+//     it; P is rounded to fp16 (2^-11 of a weight; below 2^-14 of the largest one 2^-25 of that), V and K not at all. Sums and statistics are fp32.
 //
 // What bounds it: HBM where a call is long - 256 sequences of 512 to 8192 tokens (32 / 8 heads, D=128, 2.31 GB) 368 us = 6.3 TB/s, the
 // slope over the length 6.9 (D=64 6.2; 4.9 with 16 heads to a kv head, where a warp's chain of products and exponentials counts: issue slots 51 % busy). Every

@@ -2,7 +2,8 @@
 // flash_kernel.cuh), so that the scores and the products run on the tensor cores as they do over a 16-bit cache, from half the bytes.
 //
 // What bounds it, D=128: the chain of scores, softmax and products of a tile, as over a 16-bit cache (20 chunks of 5140 tokens, 32 / 8 heads:
-// tensor pipe 47 % of the time, special-function unit 47 %, issue slots 46 %), and in a lasting load the power cap. The converters take
+// tensor pipe 47 % of the time, special-function unit 47 %, issue slots 45 %): 770 to 910 TFLOP/s, where products alone sustain 1390 under the
+// same power cap, so that the cap is the smaller part of a lasting load's 440 us against 375 in a burst. The converters take
 // issue slots from the softmax: 5 instructions for 4 codes, K as well as V, where the 16-bit kernel rewrites V only. 373 us against 332
 // over the 16-bit cache; D=64 3 % to 10 % more; D=256, where the bytes in shared memory are what counts, 404 us, a sixth less. Shared
 // memory sees as much as with 16 bits: codes in and out, numbers in, against numbers in, out and in for V.

@@ -138,15 +138,22 @@ struct FlashKernelParams {
 };
 
 // kKv8: the work list of a small batch as a parameter of the kernel. A copy ahead of the launch costs 4 us, and lets the launch wait for the
-// kernel before it (32 / 8 heads, D=128, 37 tokens against 733 keys 18.2 / 13.3 us).
+// kernel before it (32 / 8 heads, D=128, 37 tokens against 733 keys 18.2 / 13.3 us). Longer lists go ahead (4 tokens each against 500 keys, 85
+// sequences and 86: 32 / 8 heads 63.4, 67.6 us, 8 / 2 heads 27.2, 30.8).
 struct WorkImage {
     alignas(16) unsigned char bytes[2048];  // the sequences, then the entries
     int entries_at;
 };
 struct NoWorkImage {};
-// Not the D=64 kernels in which a CTA has its items to itself: their clocks hang on how the softmax is scheduled around the look-up (9
-// sequences, 4500 tokens against 1000 to 3500 keys, 32 / 8 heads, list in memory / as a parameter: fp16 without a mask 186 / 205 us, bf16
-// 199 / 197; D=128, bf16 235 / 220).
+// Not the D=64 kernels in which a CTA has its items to itself: their clocks hang on how the compiler orders the softmax around the look-up.
+// List in memory / as a parameter, us, 32 / 8 heads, causal and without a mask:
+//   9 sequences, 4500 tokens against 1000 to 3500 keys   fp16 171 / 194, 183 / 209   bf16 182 / 187, 198 / 196
+//   20, 5150 tokens against 512 to 6000                  fp16 323 / 374, 331 / 377   bf16 347 / 358, 356 / 360
+//   4 of 2000 against 6000                               fp16 555 / 650, 647 / 712   bf16 627 / 613, 716 / 676
+//   2 of 1000 against 2000                               fp16  59 /  63,  74 /  76   bf16  60 /  60,  77 /  72
+//   5 of 300 against 900                                 fp16  39 /  37,  43 /  42   bf16  39 /  37,  45 /  40
+//   8 of 120 against 700                                 fp16 22.5 / 18.6, 22.4 / 18.6   bf16 22.5 / 18.5, 22.5 / 18.5
+// fp16 loses up to 17 % on long calls, short calls lose the copy ahead of the launch; bf16 goes either way. D=128, bf16, the 9: 235 / 220.
 constexpr bool TakesWorkImage(int padded_dim, bool kv8, bool split) { return kv8 && (padded_dim != 64 || split); }
 template <bool kTaken>
 using WorkParam = std::conditional_t<kTaken, WorkImage, NoWorkImage>;
