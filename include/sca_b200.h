@@ -415,6 +415,60 @@ SCA_ABI int sca_launch_paged_attention_fp8(const ScaDecodeFwdParams* params, con
 SCA_ABI int sca_launch_flash_paged_fp8(const ScaFlashPagedParams* params, const uint8_t* k_scales,
                                        const uint8_t* v_scales, void* stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* A paged 16-bit cache that stays small (no counterpart in the reference): decode that adds up   */
+/* what each cached token weighs and reads pages that sequences share once, weights of a chunk,    */
+/* and the eviction of tokens that weigh least.                                                    */
+/*   weights  fp32 [sequences][kv_heads][weights_row], weights[s][g][j] += the sum over the new    */
+/*            tokens of sequence s and the query heads of kv head g of softmax(scale q.k)[j]       */
+/* ------------------------------------------------------------------------------------------ */
+typedef struct ScaPagedStep {
+    /* Groups of sequences that share pages: HOST arrays. Group i is the sequences cu_groups[i] .. cu_groups[i + 1] - 1; the entries of
+     * the whole pages of their first prefix_lens[i] tokens are the same in all their page-table rows, and each of them has those tokens.
+     * num_groups = 0: nothing is shared. At most 128 groups of two or more sequences that share a page; pages of 8, 16, 32 or 64 tokens. */
+    const int32_t* cu_groups;   /* num_groups + 1 */
+    const int32_t* prefix_lens; /* num_groups */
+    int64_t num_groups;
+    /* NULL: no weights. Rows of at least max_blocks_per_seq * block_size. Tokens of shared pages are left out, as are those behind a
+     * sequence's last one. */
+    float* weights;
+    int64_t weights_row;
+    int64_t typical_len; /* mean length, 0: unknown; sizes the launch */
+    int64_t longest_len; /* no sequence is longer, 0: unknown; what lies behind it counts for nothing */
+    float* scratch;      /* device, 32-byte aligned, untouched until the launches have finished */
+    int64_t scratch_floats;
+} ScaPagedStep;
+
+/* Floats of scratch that sca_launch_paged_step wants for the same arguments (pointers to tensors are not looked at, `weights` but for
+ * whether it is there); negative: they are refused. */
+SCA_ABI long long sca_paged_step_scratch_floats(const ScaDecodeFwdParams* params, const ScaPagedStep* step);
+/* sca_launch_decode_auto over a paged fp16 / bf16 cache, with weights, shared prefixes, or both. params: q, k, v, out, page_table, seq_lens
+ * and the sizes as there; the partial arrays, num_splits, seq_kv and the strides of K and V are not looked at. scale > 0 and finite. */
+SCA_ABI int sca_launch_paged_step(const ScaDecodeFwdParams* params, const ScaPagedStep* step, void* stream);
+
+/* Eviction, in place, of each kv head of each sequence on its own. Of n = seq_lens[s] tokens, where n > m = max(keep, first + recent), the first
+ * `first` are kept, the last `recent`, and of those in between the m - first - recent of the largest weights (equal ones: the lower place;
+ * NaN counts as the largest). Afterwards [0, first) and [m - recent, m) hold the first and the last ones in order; in [first, m - recent) those
+ * kept stay where they are, and the i-th place that comes free takes the i-th of those kept behind m - recent, both counted upwards.
+ * The weights go along; those of places [m, n) become 0. Sequences of up to m tokens are left alone. new_lens[s] = min(n, m): the caller may
+ * free the pages behind it. Pages of tokens in [first, n) belong to one sequence only; rows on unmapped pages are not copied. */
+typedef struct ScaKvEvict {
+    void* layer_k; /* [num_blocks, block_size, kv_heads, D] */
+    void* layer_v;
+    float* weights; /* [num_seqs][kv_heads][weights_row], rows of at least max_blocks_per_seq * block_size */
+    int64_t weights_row;
+    const int32_t* page_table; /* device [num_seqs, max_blocks_per_seq] */
+    const int32_t* seq_lens;   /* device [num_seqs] */
+    const int32_t* first_lens; /* device [num_seqs]: `first` of every sequence; NULL: `first` below */
+    int32_t* new_lens;         /* device [num_seqs], not seq_lens */
+    int64_t num_seqs, max_blocks_per_seq;
+    int64_t first, keep, recent;
+    int32_t* scratch; /* device, sca_kv_evict_scratch_ints of it, untouched until the launch has finished */
+    int64_t scratch_ints;
+} ScaKvEvict;
+SCA_ABI long long sca_kv_evict_scratch_ints(int64_t num_seqs, int64_t num_kv_heads, int64_t keep, int64_t max_tokens);
+SCA_ABI int sca_launch_kv_evict(const ScaKvEvict* params, const ScaKvCacheShape* shape, int64_t elem_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,8 +41,9 @@ __device__ __forceinline__ float* CtaPartial(unsigned char* smem) {
 }
 // The end of a segment: the warps' results, each in its ring as {m[16], l[16], O[16][D]}, become the CTA's: in `slot` of the
 // partial arrays, or (kToShared) m and l at CtaPartial<D>(smem) and O in the place of warp 0's, each number written by the thread
-// that alone has read it.
-template <int D, int kWarpBytes, bool kToShared>
+// that alone has read it. In the arrays m stands in natural units like in the reference's workspace, or (kLog2) as it is; then a part
+// counts for nothing only where its sum is 0 too: a row of NaN has no maximum either, and stays NaN.
+template <int D, int kWarpBytes, bool kToShared, bool kLog2 = false>
 __device__ __forceinline__ void MergeWarps(const ScaDecodeFwdParams& p, unsigned char* smem, const int64_t b, const int head0,
                                            const int nheads, const int slot) {
     for (int item = threadIdx.x; item < nheads * D; item += kThreads) {
@@ -58,7 +59,7 @@ __device__ __forceinline__ void MergeWarps(const ScaDecodeFwdParams& p, unsigned
         for (int w = 0; w < kWarps; ++w) {
             const float* wm = reinterpret_cast<const float*>(smem + w * kWarpBytes);
             const float mw = wm[row];
-            if (mw == -CUDART_INF_F) continue;
+            if (mw == -CUDART_INF_F && (!kLog2 || wm[16 + row] == 0.0f)) continue;
             const float wgt = Exp2(mw - m_all);
             acc += wm[32 + row * D + d] * wgt;
             l_all += wm[16 + row] * wgt;
@@ -75,7 +76,7 @@ __device__ __forceinline__ void MergeWarps(const ScaDecodeFwdParams& p, unsigned
         const int64_t flat = (b * p.num_heads + head0 + row) * p.num_splits + slot;
         p.partial_o[flat * D + d] = acc;
         if (d == 0) {
-            p.partial_m[flat] = m_all * kLn2;  // stored in natural units like the reference workspace
+            p.partial_m[flat] = kLog2 ? m_all : m_all * kLn2;
             p.partial_l[flat] = l_all;
         }
     }
@@ -83,7 +84,8 @@ __device__ __forceinline__ void MergeWarps(const ScaDecodeFwdParams& p, unsigned
 }
 
 // Marks slots [first, end) of every head of one (sequence, kv head, head chunk) as empty (m = -inf; the merge
-// skips such entries without reading l or O).
+// skips such entries without reading l or O; kLog2: m = -inf and l = 0).
+template <bool kLog2 = false>
 __device__ __forceinline__ void MarkUnusedSlots(const ScaDecodeFwdParams& p, int64_t b, int hk, int hc, int first, int end) {
     const int group = static_cast<int>(p.num_heads / p.num_kv_heads);
     const int head0 = hk * group + hc * 16;
@@ -93,6 +95,7 @@ __device__ __forceinline__ void MarkUnusedSlots(const ScaDecodeFwdParams& p, int
         const int row = item / unused;
         const int slot = first + item % unused;
         p.partial_m[(b * p.num_heads + head0 + row) * p.num_splits + slot] = -CUDART_INF_F;
+        if (kLog2) p.partial_l[(b * p.num_heads + head0 + row) * p.num_splits + slot] = 0.0f;
     }
 }
 
@@ -110,11 +113,18 @@ __device__ __forceinline__ void MarkUnusedSlots(const ScaDecodeFwdParams& p, int
 // any sequence by num_splits (with num_splits == 1 shares are made of whole sequences); slots that stay unused are
 // marked empty by the CTA that holds the sequence's first step.
 // Sequence lengths are read on the device (seq_lens), so the schedule needs no host knowledge of a ragged batch.
-template <bool kPaged, int kSpan, typename Segment>
-__device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const int head_chunks, const Segment& segment) {
+// `lens` says how many tokens of a sequence are walked (lens(b)) and whether that is the same number for all (lens.Regular()); kLog2 as
+// in MergeWarps.
+template <bool kPaged>
+struct WholeSequences {
+    const ScaDecodeFwdParams& p;
+    __device__ __forceinline__ int64_t operator()(int64_t b) const { return SeqLen<kPaged>(p, b); }
+    __device__ __forceinline__ bool Regular() const { return p.seq_lens == nullptr; }
+};
+template <bool kPaged, int kSpan, bool kLog2, typename Lens, typename Segment>
+__device__ __forceinline__ void WalkSteps(const ScaDecodeFwdParams& p, const int head_chunks, const Lens& lens, const Segment& segment) {
     __shared__ int64_t s_part[kWarps][2];
     __shared__ int64_t s_found[2];
-    WaitForPredecessor();
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
     const int columns = static_cast<int>(p.num_kv_heads) * head_chunks;
@@ -128,9 +138,9 @@ __device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const 
 
     // ---- this CTA's share [begin, end) of a column's step list, and the sequence that holds `begin` ----------
     int64_t b, before, len, steps, per_cta, begin, end;
-    if (p.seq_lens == nullptr) {
+    if (lens.Regular()) {
         // every sequence has the same length: the list is regular and needs no look at device memory
-        len = SeqLen<kPaged>(p, 0);
+        len = lens(0);
         steps = StepsFor<kSpan>(len);
         const int64_t total = p.batch * steps;
         per_cta = (total + sharers - 1) / sharers;
@@ -146,7 +156,7 @@ __device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const 
         // pass 1: total steps and the longest sequence
         int64_t sum = 0, longest = 0;
         for (int64_t i = threadIdx.x; i < p.batch; i += kThreads) {
-            const int64_t t = StepsFor<kSpan>(SeqLen<kPaged>(p, i));
+            const int64_t t = StepsFor<kSpan>(lens(i));
             sum += t;
             longest = t > longest ? t : longest;
         }
@@ -182,7 +192,7 @@ __device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const 
         __syncthreads();
         for (int64_t base = 0; base < p.batch && running <= begin; base += kThreads) {
             const int64_t i = base + threadIdx.x;
-            const int64_t t = i < p.batch ? StepsFor<kSpan>(SeqLen<kPaged>(p, i)) : 0;
+            const int64_t t = i < p.batch ? StepsFor<kSpan>(lens(i)) : 0;
             int64_t incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -207,7 +217,7 @@ __device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const 
         }
         b = s_found[0];
         before = s_found[1];  // steps of this column before sequence b
-        len = SeqLen<kPaged>(p, b);
+        len = lens(b);
         steps = StepsFor<kSpan>(len);
     }
     // the merge kernel that follows on the stream may be set up while this grid streams K/V
@@ -229,7 +239,7 @@ __device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const 
             const int slot = static_cast<int>(share - before / per_cta);
             if (t0 == 0) {
                 const int used = static_cast<int>((before + steps - 1) / per_cta - before / per_cta) + 1;
-                MarkUnusedSlots(p, b, hk, hc, used, static_cast<int>(p.num_splits));
+                MarkUnusedSlots<kLog2>(p, b, hk, hc, used, static_cast<int>(p.num_splits));
             }
             const int64_t j_end = t1 * kSpan < len ? t1 * kSpan : len;
             segment(b, hk, hc, t0 * kSpan, j_end, slot);
@@ -237,11 +247,17 @@ __device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const 
             if (t1 == steps && pos < end) {
                 before += steps;
                 ++b;
-                len = SeqLen<kPaged>(p, b);
+                len = lens(b);
                 steps = StepsFor<kSpan>(len);
             }
         }
     }
+}
+
+template <bool kPaged, int kSpan, typename Segment>
+__device__ __forceinline__ void WalkSchedule(const ScaDecodeFwdParams& p, const int head_chunks, const Segment& segment) {
+    WaitForPredecessor();
+    WalkSteps<kPaged, kSpan, false>(p, head_chunks, WholeSequences<kPaged>{p}, segment);
 }
 
 // Decode of a problem that does not fill the machine, in one launch: the CTAs of a cluster split one (sequence, kv head,

@@ -447,6 +447,17 @@ int LaunchFlashTyped(const ScaFlashFwdParams& f, cudaStream_t stream, const Varl
 }
 
 }  // namespace
+
+namespace flash {
+
+int MakeRowsMap(CUtensorMap* map, const void* base, int dtype_id, int64_t d, int64_t heads, int64_t rows, int64_t head_stride, int64_t row_stride, int box_heads,
+                int box_rows, const char* what) {
+    return MakeMap(map, base, dtype_id, d, heads, rows, 1, head_stride, row_stride, rows * row_stride, box_heads, what, box_rows);
+}
+int* ErrorWord() { return ErrorWordForCurrentDevice(); }
+int CheckFlashLaunch(cudaStream_t stream) { return CheckFlash(stream); }
+
+}  // namespace flash
 }  // namespace sca_b200
 
 using namespace sca_b200;

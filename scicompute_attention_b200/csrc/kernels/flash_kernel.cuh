@@ -40,6 +40,7 @@
 #include "common.cuh"
 #include "kv_fp8.cuh"
 #include "kv_ring.cuh"
+#include "shared_prefix.cuh"
 #include "sm100.cuh"
 
 namespace sca_b200 {
@@ -155,8 +156,14 @@ struct NoWorkImage {};
 //   8 of 120 against 700                                 fp16 22.5 / 18.6, 22.4 / 18.6   bf16 22.5 / 18.5, 22.5 / 18.5
 // fp16 loses up to 17 % on long calls, short calls lose the copy ahead of the launch; bf16 goes either way. D=128, bf16, the 9: 235 / 220.
 constexpr bool TakesWorkImage(int padded_dim, bool kv8, bool split) { return kv8 && (padded_dim != 64 || split); }
-template <bool kTaken>
-using WorkParam = std::conditional_t<kTaken, WorkImage, NoWorkImage>;
+// kShared: what the launch is about (flash_shared.cu).
+struct SharedImage {
+    PrefixGroups groups;
+    PrefixParts parts;
+    const int32_t* seq_lens;  // of the sequences, one query token each; null: none is shorter than its prefix
+};
+template <bool kTaken, bool kShared>
+using WorkParam = std::conditional_t<kShared, SharedImage, std::conditional_t<kTaken, WorkImage, NoWorkImage>>;
 
 // 16 elements of an output row: one 32-byte store where every row starts on a 32-byte boundary, else two of 16 bytes. A
 // thread writes a row of its own, so each store of a warp touches 32 separate rows and takes the load/store unit 32 turns
@@ -409,10 +416,12 @@ __device__ __forceinline__ bool ProduceRaw(const FlashKernelParams& p, const CUt
 // through distributed shared memory at the end (SplitCluster says when).
 // kKv8 (only with kPaged): the pages hold codes, which the converters rewrite as fp16; the products of the scores run in fp16 too, for bf16
 // queries after HalveQueryRow.
-template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kKv8 = false, bool kSplit = false>
+// kShared (only with kPaged): decode of groups of sequences over the pages they have in common. The query tokens of a group are a "sequence" of
+// the list, an item takes a part of its keys, and what it leaves is that part of every row, not an output (flash_shared.cu).
+template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kKv8 = false, bool kSplit = false, bool kShared = false>
 __global__ void __launch_bounds__(FlashThreads<T, DP, QT, kKv8>(), 1)
 flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p, const __grid_constant__ WorkParam<TakesWorkImage(DP, kKv8, kSplit)> image) {
+                       const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p, const __grid_constant__ WorkParam<TakesWorkImage(DP, kKv8, kSplit), kShared> image) {
     using G = FlashGeom<DP, QT, BN, kKv8>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem_base = (SmemAddr(smem_raw) + 1023u) & ~1023u;
@@ -450,6 +459,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     constexpr int kPEarly = DP == 256 ? 64 : 96;
     static_assert(!kPaged || kVarlen, "paged K/V runs on the packed work list");
     static_assert(!kKv8 || kPaged, "the 8-bit cache is paged");
+    static_assert(!kShared || (kPaged && !kKv8 && !kSplit), "shared pages");
     static_assert(kNumBars * 8 + 16 <= G::kBarrierBytes, "barrier area too small");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_base - smem_base) + kNumBars * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -486,12 +496,34 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         int m0[kTiles];               // first token of each tile, relative to the sequence
         int ntiles[kTiles];
         int n_max;
-        int first_tile;               // kSplit: this CTA's first KV tile; 0 otherwise
+        int first_tile;               // kSplit: this CTA's first KV tile; kShared: the part's; 0 otherwise
+        int part;                     // kShared
     };
     auto decode_item = [&](int idx) {
         Item w;
         int mb;
-        if constexpr (kVarlen) {
+        if constexpr (kShared) {
+            const PrefixGroups& groups = image.groups;
+            const int entry = idx / packed_heads;
+            int lo = 0, hi = groups.count - 1;  // the last group that begins at this entry or before
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (groups.group[mid].first_entry <= entry) lo = mid;
+                else hi = mid - 1;
+            }
+            const PrefixGroup group = groups.group[lo];
+            const int tiles = (group.tokens + BN - 1) / BN, parts = (tiles + groups.part_tiles - 1) / groups.part_tiles;
+            mb = (entry - group.first_entry) / parts;
+            w.part = (entry - group.first_entry) % parts;
+            w.seq = group.first;
+            w.b = 0;
+            w.h = (idx % packed_heads) << p.pack_shift;
+            w.q_tok0 = group.first;
+            w.kv_tok0 = 0;
+            w.seq_q = group.end - group.first;
+            w.seq_kv = group.tokens;
+            w.diagonal = 0;
+        } else if constexpr (kVarlen) {
             const int4* seqs = p.seqs;
             const int2* entries = p.entries;
             if constexpr (TakesWorkImage(DP, kKv8, kSplit)) {
@@ -536,6 +568,12 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const int share = (w.n_max + p.cluster - 1) / p.cluster;
             w.first_tile = min(static_cast<int>(ClusterRank()) * share, w.n_max);
             w.n_max = w.ntiles[0] = min(share, w.n_max - w.first_tile);
+        }
+        if constexpr (kShared) {
+            w.first_tile = w.part * image.groups.part_tiles;
+            w.n_max = min(image.groups.part_tiles, w.n_max - w.first_tile);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) w.ntiles[t] = min(w.ntiles[t], w.n_max);
         }
         return w;
     };
@@ -641,7 +679,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // chunks against 512 to 6000 keys, lasting load, ahead / per load: D=128 429 / 400 us, D=64 299 / 324, D=256 1032 / 1125).
             constexpr bool kLookAhead = kOwnP;
             auto page_ids = [&](int tile) {
-                const int logical = ((kSplit ? w.first_tile : 0) + tile) * pages_per_tile + lane;
+                const int logical = ((kSplit || kShared ? w.first_tile : 0) + tile) * pages_per_tile + lane;
                 const bool in = lane < pages_per_tile && logical < p.max_blocks_per_seq && (static_cast<int64_t>(logical) << p.block_shift) < w.seq_kv;
                 return in ? row[logical] : -1;
             };
@@ -1059,6 +1097,10 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 __syncwarp();
                 if (lane == 0) MbarArrive(bar(Raw::kQHalf + t));
             }
+            int row_keys = 0x7fffffff;  // kShared: keys that the row sees at most
+            if constexpr (kShared) {
+                if (image.seq_lens != nullptr && row < w.seq_q) row_keys = image.seq_lens[w.q_tok0 + row];
+            }
             float m_ref = -CUDART_INF_F;  // reference point of the exponentials (log2 domain)
             float l_sum = 0.0f;
 
@@ -1071,9 +1113,10 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // (always in the first step of an item), the reference moves and O and the row sum are rescaled.
                 // P (16-bit pairs) goes to columns of its own or to the first BN / 2 columns of S_t, which has been read by
                 // then; its first kPEarly keys are handed over early, so that P V starts under the last exponentials.
-                const int col0 = ((kSplit ? w.first_tile : 0) + j) * BN;
+                const int col0 = ((kSplit || kShared ? w.first_tile : 0) + j) * BN;
                 const int kv_limit = w.seq_kv - col0;                                   // columns >= kv_limit do not exist
-                const int causal_limit = p.causal ? (row + w.diagonal - col0 + 1) : BN;  // columns >= limit are masked
+                // columns >= limit are masked
+                const int causal_limit = kShared ? row_keys - col0 : p.causal ? (row + w.diagonal - col0 + 1) : BN;
                 const int limit = min(kv_limit, causal_limit);
                 const uint32_t pages = kPaged ? valid_ring[(tiles_base + j) % kValidRing] : 0u;
                 const bool holes = kPaged && pages != all_pages;   // some page of this tile is unmapped
@@ -1225,6 +1268,33 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 *reinterpret_cast<float2*>(part_row + DP) = make_float2(m_ref, l_sum);
                 continue;
             }
+            if constexpr (kShared) {
+                const int64_t part = (static_cast<int64_t>(w.q_tok0 + row) * p.heads + head) * image.groups.parts + w.part;
+                float* o_part = image.parts.o + part * p.head_dim;
+#pragma unroll
+                for (int cblk = 0; cblk < DP / 32; ++cblk) {
+                    uint32_t r[32];
+                    TmemLd32(o_addr + cblk * 32, r);
+                    TmemWaitLd();
+                    if (cblk == DP / 32 - 1) {
+                        TcFenceBefore();
+                        __syncwarp();
+                        if (lane == 0) MbarArrive(bar(kOFree + t));
+                    }
+                    if (row < w.seq_q && cblk * 32 < p.head_dim) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            const uint32_t v[8] = {r[i], r[i + 1], r[i + 2], r[i + 3], r[i + 4], r[i + 5], r[i + 6], r[i + 7]};
+                            StoreRow16(o_part + cblk * 32 + i, v, true);
+                        }
+                    }
+                }
+                if (row < w.seq_q) {
+                    image.parts.m[part] = m_ref;
+                    image.parts.l[part] = l_sum;
+                }
+                continue;
+            }
             const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;
             T* o_row = reinterpret_cast<T*>(p.out) + w.b * p.o_sb + head * p.o_sh + static_cast<int64_t>(w.q_tok0 + row) * p.o_ss;
 #pragma unroll
@@ -1332,6 +1402,13 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         ClusterBarrier();  // nobody leaves while its shared memory is being read
     }
 }
+
+// Host pieces of flash_fwd.cu that the launches of flash_shared.cu need too: a map of [seq][heads][D] rows through element strides, with boxes of
+// 64 numbers x box_heads x box_rows (see MakeMap), the current device's error word, and the check behind a launch.
+int MakeRowsMap(CUtensorMap* map, const void* base, int dtype_id, int64_t d, int64_t heads, int64_t rows, int64_t head_stride, int64_t row_stride, int box_heads,
+                int box_rows, const char* what);
+int* ErrorWord();
+int CheckFlashLaunch(cudaStream_t stream);
 
 // The kSplit kernels are compiled in flash_split.cu.
 template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged>

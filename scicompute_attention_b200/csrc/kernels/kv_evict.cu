@@ -1,0 +1,354 @@
+// Eviction from a paged cache by accumulated weight: every kv head of a sequence that is longer than its limit m keeps its first tokens, its
+// last ones, and of those in between the heaviest, in place.
+//
+// What is kept stays where it is if it can. With n tokens, `first` and `recent` protected and stay = m - first - recent, the places are
+//   [0, first)               the first tokens, untouched
+//   [first, m - recent)      `stay` of those in between: the kept ones that are here already, and in the places that come free, lowest
+//                            first, the kept ones from behind m - recent, lowest first
+//   [m - recent, m)          the last `recent` tokens in their order
+// so that a row moves once at most, and of the places in between only those whose token goes. Attention does not depend on the order of the
+// keys; what does, the last tokens and a causal mask over new ones, keeps its order.
+//
+// A cluster of CTAs takes one (sequence, kv head). The `stay`-th largest weight is found digit by digit (11, 11 and 10 bits of a key that
+// orders like the numbers) from histograms in shared memory, which the CTAs read from one another; ties go to the lower place by counting.
+// Free places and rows that move are listed by rank in scratch, then all CTAs copy. No free place is the source of a move, so that these
+// copies need no order. The last tokens move down behind them, all rows of a wave read before the first one of it is written: the
+// destination of a row is never behind its source, so that later waves read what no earlier one has written.
+// Algorithmic traffic: 8 bytes a token and kv head of weights, and 4 * row bytes a moved row (K and V, read and written).
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace sca_b200 {
+namespace {
+
+constexpr int kEvictThreads = 512;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kDigits = 3;
+constexpr int kBins = 2048;
+constexpr int kEvictCluster = 8;   // CTAs to a (sequence, kv head) at most
+constexpr int kHeld = 8;           // pieces of the last rows that a thread holds at once
+constexpr int kMoves = 4;          // pieces of other rows
+
+struct EvictParams {
+    void *k, *v;
+    float* weights;            // [num_seqs][kv_heads][weights_row]
+    const int32_t* page_table; // [num_seqs][max_blocks]
+    const int32_t* seq_lens;
+    const int32_t* first;      // [num_seqs]; null: first_of_all
+    int32_t* new_lens;
+    int32_t* lists;            // [num_seqs * kv_heads][2][list]: free places, sources
+    int64_t weights_row, list;
+    int32_t max_blocks, block_size, num_blocks, kv_heads;
+    int32_t first_of_all, keep, recent;
+    int32_t cached;            // keys that a CTA keeps in shared memory
+    int32_t cluster;
+    int32_t row_pieces;        // of K: pieces of sizeof(V) bytes to a token of one kv head
+};
+
+// Orders like the numbers: NaN above all, both zeros alike.
+__device__ __forceinline__ uint32_t KeyOf(float w) {
+    if (w != w) return 0xffffffffu;
+    const uint32_t bits = __float_as_uint(w == 0.0f ? 0.0f : w);
+    return (bits >> 31) ? ~bits : bits | 0x80000000u;
+}
+
+template <typename V>
+__global__ void __launch_bounds__(kEvictThreads)
+kv_evict_kernel(const EvictParams p) {
+    extern __shared__ __align__(16) uint32_t smem[];
+    uint32_t(*hist)[kBins] = reinterpret_cast<uint32_t(*)[kBins]>(smem);
+    uint32_t* cache = smem + kDigits * kBins;
+    __shared__ int s_ties[kEvictWarps], s_free[kEvictWarps], s_late[kEvictWarps];
+    __shared__ int s_counts[2];            // free places and late rows of this CTA's slice
+    __shared__ uint32_t s_warp[kEvictWarps];
+    __shared__ uint32_t s_bin, s_above;
+    BeginAfterPredecessor();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(ClusterRank()), cluster = p.cluster;
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) / cluster;
+    const int64_t seq = unit / p.kv_heads;
+    const int head = static_cast<int>(unit % p.kv_heads);
+    const int64_t capacity = static_cast<int64_t>(p.max_blocks) * p.block_size;
+    const int n = static_cast<int>(min(max(static_cast<int64_t>(p.seq_lens[seq]), int64_t{0}), capacity));
+    const int64_t first64 = max(p.first != nullptr ? p.first[seq] : p.first_of_all, 0);
+    const int64_t m64 = max(static_cast<int64_t>(p.keep), first64 + p.recent);
+    if (head == 0 && rank == 0 && threadIdx.x == 0) p.new_lens[seq] = static_cast<int32_t>(min(static_cast<int64_t>(n), m64));
+    if (n <= m64) return;  // all CTAs of the cluster
+    const int first = static_cast<int>(first64), m = static_cast<int>(m64), recent = p.recent;
+    const int stay = m - first - recent, between = n - recent - first, keep_end = m - recent;
+    float* w = p.weights + unit * p.weights_row;
+    int32_t* free_places = p.lists + unit * 2 * p.list;
+    int32_t* sources = free_places + p.list;
+    const int32_t* table = p.page_table + seq * p.max_blocks;
+    int moves = 0;
+
+    if (stay > 0) {
+        // ---- the stay-th largest key -------------------------------------------------------------------------
+        const int slice = (between + cluster - 1) / cluster;
+        const int begin = first + min(rank * slice, between), count = first + min((rank + 1) * slice, between) - begin;
+        for (int i = threadIdx.x; i < kDigits * kBins; i += kEvictThreads) smem[i] = 0;
+        __syncthreads();
+        auto key_at = [&](int i) { return i < p.cached ? cache[i] : KeyOf(w[begin + i]); };
+        uint32_t prefix = 0, need = static_cast<uint32_t>(stay);
+#pragma unroll
+        for (int digit = 0; digit < kDigits; ++digit) {
+            constexpr int kShift[kDigits] = {21, 10, 0};
+            const int shift = kShift[digit];
+            const uint32_t mask = digit == 2 ? 1023u : 2047u;
+            for (int i = threadIdx.x; i < count; i += kEvictThreads) {
+                uint32_t key;
+                if (digit == 0) {
+                    key = KeyOf(w[begin + i]);
+                    if (i < p.cached) cache[i] = key;
+                } else {
+                    key = key_at(i);
+                    if ((key >> kShift[digit - 1]) != prefix) continue;
+                }
+                atomicAdd(&hist[digit][(key >> shift) & mask], 1u);
+            }
+            ClusterBarrier();
+            // four bins a thread, the highest first, of all CTAs
+            const int bin0 = kBins - 4 - 4 * threadIdx.x;
+            uint32_t bins[4] = {0, 0, 0, 0};
+            for (int r = 0; r < cluster; ++r) {
+                const float4 x = LoadFromRank4(SmemAddr(&hist[digit][bin0]), r);
+                bins[0] += __float_as_uint(x.w), bins[1] += __float_as_uint(x.z), bins[2] += __float_as_uint(x.y), bins[3] += __float_as_uint(x.x);
+            }
+            const uint32_t mine = bins[0] + bins[1] + bins[2] + bins[3];
+            uint32_t incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            if (lane == 31) s_warp[warp] = incl;
+            __syncthreads();
+            uint32_t above = incl - mine;
+            for (int i = 0; i < warp; ++i) above += s_warp[i];
+            if (above < need && need <= above + mine) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (need > above && need <= above + bins[i]) {
+                        s_bin = static_cast<uint32_t>(bin0 + 3 - i);
+                        s_above = above;
+                    }
+                    above += bins[i];
+                }
+            }
+            __syncthreads();
+            prefix = digit == 0 ? s_bin : digit == 1 ? (prefix << 11) | s_bin : (prefix << 10) | s_bin;
+            need -= s_above;
+            __syncthreads();  // s_warp, s_bin and s_above are written again
+        }
+        const uint32_t border = prefix;  // keys above it stay, and `need` of those equal to it, the lowest places first
+        int ties_before = 0;
+        for (int r = 0; r < rank; ++r) ties_before += __float_as_int(LoadFromRank(SmemAddr(&hist[kDigits - 1][border & 1023u]), r));
+
+        // ---- ranks: every warp walks a piece of the slice --------------------------------------------------------
+        const int piece = ((count + kEvictWarps - 1) / kEvictWarps + 31) / 32 * 32;
+        const int piece_begin = min(warp * piece, count), piece_end = min(piece_begin + piece, count);
+        int ties = 0;
+        for (int i = piece_begin; i < piece_end; i += 32) {
+            const bool tie = i + lane < piece_end && key_at(i + lane) == border;
+            ties += __popc(__ballot_sync(0xffffffffu, tie));
+        }
+        if (lane == 0) s_ties[warp] = ties;
+        __syncthreads();
+        for (int i = 0; i < warp; ++i) ties_before += s_ties[i];
+        const uint32_t below = (1u << lane) - 1u;
+        // f(place, is free, is late, ballots of both)
+        auto walk = [&](auto f) {
+            int tie_rank = ties_before;
+            for (int i = piece_begin; i < piece_end; i += 32) {
+                const bool in = i + lane < piece_end;
+                const uint32_t key = in ? key_at(i + lane) : 0u;
+                const uint32_t tie = __ballot_sync(0xffffffffu, in && key == border);
+                const bool kept = in && (key > border || (key == border && tie_rank + __popc(tie & below) < static_cast<int>(need)));
+                tie_rank += __popc(tie);
+                const int place = begin + i + lane;
+                const bool is_free = in && !kept && place < keep_end, is_late = kept && place >= keep_end;
+                f(place, is_free, is_late, __ballot_sync(0xffffffffu, is_free), __ballot_sync(0xffffffffu, is_late));
+            }
+        };
+        int free_count = 0, late_count = 0;
+        walk([&](int, bool, bool, uint32_t free_lanes, uint32_t late_lanes) {
+            free_count += __popc(free_lanes);
+            late_count += __popc(late_lanes);
+        });
+        if (lane == 0) {
+            s_free[warp] = free_count;
+            s_late[warp] = late_count;
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            const int* counts = threadIdx.x == 0 ? s_free : s_late;
+            int sum = 0;
+            for (int i = 0; i < kEvictWarps; ++i) sum += counts[i];
+            s_counts[threadIdx.x] = sum;
+        }
+        ClusterBarrier();
+        int free_rank = 0, late_rank = 0;
+        for (int r = 0; r < cluster; ++r) {
+            const float2 x = make_float2(LoadFromRank(SmemAddr(&s_counts[0]), r), LoadFromRank(SmemAddr(&s_counts[1]), r));
+            moves += __float_as_int(x.x);
+            if (r < rank) {
+                free_rank += __float_as_int(x.x);
+                late_rank += __float_as_int(x.y);
+            }
+        }
+        for (int i = 0; i < warp; ++i) {
+            free_rank += s_free[i];
+            late_rank += s_late[i];
+        }
+        walk([&](int place, bool is_free, bool is_late, uint32_t free_lanes, uint32_t late_lanes) {
+            if (is_free) free_places[free_rank + __popc(free_lanes & below)] = place;
+            if (is_late) sources[late_rank + __popc(late_lanes & below)] = place;
+            free_rank += __popc(free_lanes);
+            late_rank += __popc(late_lanes);
+        });
+        ClusterBarrier();
+    }
+
+    // ---- copies --------------------------------------------------------------------------------------------------
+    const int row_pieces = p.row_pieces, move_pieces = 2 * row_pieces;
+    const int64_t token_pieces = static_cast<int64_t>(p.kv_heads) * row_pieces;
+    auto row_of = [&](int place) -> int64_t {  // first piece of this head's row; negative: its page is not mapped
+        const int32_t id = table[place / p.block_size];
+        return id >= 0 && id < p.num_blocks ? (static_cast<int64_t>(id) * p.block_size + place % p.block_size) * token_pieces + static_cast<int64_t>(head) * row_pieces : -1;
+    };
+    V* const pools[2] = {static_cast<V*>(p.k), static_cast<V*>(p.v)};
+    const int64_t threads = static_cast<int64_t>(cluster) * kEvictThreads, me = static_cast<int64_t>(rank) * kEvictThreads + threadIdx.x;
+    const int64_t total = static_cast<int64_t>(moves) * move_pieces;
+    for (int64_t at = me; at < total; at += kMoves * threads) {
+        V held[kMoves];
+        int64_t to[kMoves];
+        bool is_v[kMoves];
+#pragma unroll
+        for (int i = 0; i < kMoves; ++i) {
+            const int64_t item = at + i * threads;
+            to[i] = -1;
+            if (item >= total) continue;
+            const int move = static_cast<int>(item / move_pieces), part = static_cast<int>(item % move_pieces);
+            const int src = sources[move], dst = free_places[move];
+            const int64_t from = row_of(src), into = row_of(dst);
+            is_v[i] = part >= row_pieces;
+            const int offset = is_v[i] ? part - row_pieces : part;
+            if (part == 0) w[dst] = w[src];
+            if (from < 0 || into < 0) continue;
+            held[i] = (is_v[i] ? pools[1] : pools[0])[from + offset];
+            to[i] = into + offset;
+        }
+#pragma unroll
+        for (int i = 0; i < kMoves; ++i) {
+            if (to[i] >= 0) (is_v[i] ? pools[1] : pools[0])[to[i]] = held[i];
+        }
+    }
+    const int64_t last = static_cast<int64_t>(recent) * move_pieces;
+    int64_t wave = 0;
+    do {
+        V held[kHeld];
+        float weight[kHeld];
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int64_t item = wave + me + i * threads;
+            if (item >= last) continue;
+            const int row = static_cast<int>(item / move_pieces), part = static_cast<int>(item % move_pieces);
+            const int64_t from = row_of(n - recent + row);
+            if (part == 0) weight[i] = w[n - recent + row];
+            if (from >= 0) held[i] = part >= row_pieces ? pools[1][from + part - row_pieces] : pools[0][from + part];
+        }
+        ClusterBarrier();
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int64_t item = wave + me + i * threads;
+            if (item >= last) continue;
+            const int row = static_cast<int>(item / move_pieces), part = static_cast<int>(item % move_pieces);
+            const int64_t from = row_of(n - recent + row), into = row_of(keep_end + row);
+            if (part == 0) w[keep_end + row] = weight[i];
+            if (from < 0 || into < 0) continue;
+            if (part >= row_pieces) pools[1][into + part - row_pieces] = held[i];
+            else pools[0][into + part] = held[i];
+        }
+        wave += kHeld * threads;
+    } while (wave < last);
+    for (int64_t j = m + me; j < n; j += threads) w[j] = 0.0f;  // every weight has been read by now
+}
+
+// Keys that stay in shared memory between the digits; what a CTA has beyond them is read again.
+constexpr int kCachedKeys = 8192;
+
+template <typename V>
+int LaunchEvict(const EvictParams& p, int64_t units, cudaStream_t stream) {
+    constexpr size_t kHistograms = kDigits * kBins * sizeof(uint32_t);
+    const size_t smem = kHistograms + static_cast<size_t>(p.cached) * sizeof(uint32_t);
+    auto kernel = kv_evict_kernel<V>;
+    if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kHistograms + kCachedKeys * sizeof(uint32_t), "kv_evict_kernel")) return rc;
+    LaunchDependent(kernel, units * p.cluster, kEvictThreads, smem, stream, p.cluster, p);
+    return CheckLaunch("kv_evict_kernel", stream);
+}
+
+int64_t ListLength(int64_t keep, int64_t capacity) { return std::max<int64_t>(1, std::min(keep, capacity)); }
+
+}  // namespace
+}  // namespace sca_b200
+
+using namespace sca_b200;
+
+extern "C" long long sca_kv_evict_scratch_ints(int64_t num_seqs, int64_t num_kv_heads, int64_t keep, int64_t max_tokens) {
+    if (num_seqs < 1 || num_kv_heads < 1 || keep < 0 || max_tokens < 1) return -1;
+    return num_seqs * num_kv_heads * 2 * ListLength(keep, max_tokens);
+}
+
+extern "C" int sca_launch_kv_evict(const ScaKvEvict* params, const ScaKvCacheShape* shape, int64_t elem_bytes, void* stream) {
+    ClearError();
+    auto invalid = [](const std::string& why) { return Fail(SCA_INVALID_ARGUMENT, "kv evict: " + why); };
+    if (params == nullptr || shape == nullptr) return invalid("null parameter block");
+    const ScaKvEvict& x = *params;
+    if (x.layer_k == nullptr || x.layer_v == nullptr || x.weights == nullptr || x.page_table == nullptr || x.seq_lens == nullptr || x.new_lens == nullptr ||
+        x.scratch == nullptr) {
+        return invalid("null pointer");
+    }
+    if (x.new_lens == x.seq_lens) return invalid("the new lengths go to memory of their own");
+    if (shape->num_blocks < 1 || shape->block_size < 1 || shape->num_kv_heads < 1 || shape->head_dim < 1 || elem_bytes < 1 || x.num_seqs < 1 || x.max_blocks_per_seq < 1) {
+        return invalid("sizes must be positive");
+    }
+    const int64_t capacity = x.max_blocks_per_seq * shape->block_size, units = x.num_seqs * shape->num_kv_heads;
+    const int64_t row_bytes = shape->head_dim * elem_bytes;
+    if (capacity > 0x7fffff00LL || shape->num_blocks > 0x7fffffffLL || row_bytes > (1 << 20) || units > 0x7fffffffLL / kEvictCluster) return invalid("sizes are out of range");
+    if (x.keep < 0 || x.recent < 0 || x.first < 0) return invalid("keep, recent and first must not be negative");
+    if (x.weights_row < capacity) {
+        return invalid("rows of " + std::to_string(x.weights_row) + " weights for page-table rows of " + std::to_string(capacity) + " tokens");
+    }
+    const int64_t need = sca_kv_evict_scratch_ints(x.num_seqs, shape->num_kv_heads, x.keep, capacity);
+    if (x.scratch_ints < need) return invalid("scratch of " + std::to_string(x.scratch_ints) + " int32 is too small (" + std::to_string(need) + " needed)");
+    EvictParams p{};
+    p.k = x.layer_k;
+    p.v = x.layer_v;
+    p.weights = x.weights;
+    p.page_table = x.page_table;
+    p.seq_lens = x.seq_lens;
+    p.first = x.first_lens;
+    p.new_lens = x.new_lens;
+    p.lists = x.scratch;
+    p.weights_row = x.weights_row;
+    p.list = ListLength(x.keep, capacity);
+    p.max_blocks = static_cast<int32_t>(x.max_blocks_per_seq);
+    p.block_size = static_cast<int32_t>(shape->block_size);
+    p.num_blocks = static_cast<int32_t>(shape->num_blocks);
+    p.kv_heads = static_cast<int32_t>(shape->num_kv_heads);
+    // no sequence is longer than `capacity`: protected tokens beyond it are as good as that
+    p.first_of_all = static_cast<int32_t>(std::min(x.first, capacity));
+    p.keep = static_cast<int32_t>(std::min(x.keep, capacity));
+    p.recent = static_cast<int32_t>(std::min(x.recent, capacity));
+    p.cluster = 1;
+    p.cached = static_cast<int32_t>(std::min<int64_t>((capacity + p.cluster - 1) / p.cluster, kCachedKeys));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (row_bytes % 16 == 0 && Aligned16(x.layer_k) && Aligned16(x.layer_v)) {
+        p.row_pieces = static_cast<int32_t>(row_bytes / 16);
+        return LaunchEvict<uint4>(p, units, s);
+    }
+    p.row_pieces = static_cast<int32_t>(row_bytes);
+    return LaunchEvict<unsigned char>(p, units, s);
+}

@@ -1,0 +1,41 @@
+// What the kernels of a decode over shared prefixes know about the groups: a parameter of the launch, so that nothing is copied ahead of it
+// and a captured graph keeps it.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace sca_b200 {
+
+constexpr int kMaxGroups = 128;
+
+// Sequences [first, end) whose first `tokens` tokens (whole pages) are read through the page-table row of the first of them.
+struct PrefixGroup {
+    int first, end, tokens;
+    int first_entry;  // in the work list of the prefix kernel
+};
+struct PrefixGroups {
+    int count;       // groups that share something, in the order of their sequences
+    int part_tiles;  // tiles of 128 keys to a part of a prefix
+    int parts;       // parts of the longest prefix: a row's parts in the arrays below
+    PrefixGroup group[kMaxGroups];
+};
+
+// The group of sequence b; null where it shares nothing.
+__device__ __forceinline__ const PrefixGroup* GroupOf(const PrefixGroups& groups, int64_t b) {
+    int lo = 0, hi = groups.count;  // the last one that begins at b or before is below hi
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (groups.group[mid].first <= b) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo > 0 && b < groups.group[lo - 1].end ? &groups.group[lo - 1] : nullptr;
+}
+
+// Where the parts of the prefixes are left, fp32: m (log2 domain) and l [rows][parts], O [rows][parts][D]; a row is sequence * heads + head.
+struct PrefixParts {
+    float *m, *l, *o;
+};
+
+}  // namespace sca_b200

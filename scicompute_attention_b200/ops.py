@@ -939,3 +939,164 @@ def flash_attention_paged_fp8(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_l
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().sca_launch_flash_paged_fp8(C.byref(p), k_pool[1].data_ptr(), v_pool[1].data_ptr(), _stream_ptr(stream)))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# a paged cache that stays small: what each cached token weighs, shared prefixes, eviction
+# ------------------------------------------------------------------------------------------------
+def _require_weights(weights, rows: int, kv_heads: int, tokens: int) -> None:
+    _require_cuda(weights)
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[0] < rows or weights.shape[1] != kv_heads or weights.shape[2] < tokens or \
+            not weights.is_contiguous():
+        raise _lib.ScaError(4, f"weights must be contiguous float32 [{rows}, {kv_heads}, {tokens}] or more rows and columns; got {weights.dtype}{list(weights.shape)}")
+
+
+def _host_ints(what: str, values):
+    """A host list as a contiguous int32 array of one dimension."""
+    import numpy as np
+    given = np.asarray(values)
+    if given.ndim != 1 or given.dtype.kind not in "iu":
+        raise _lib.ScaError(4, f"{what} must be a list of whole numbers on the host; got {given.dtype}{list(given.shape)}")
+    out = np.ascontiguousarray(given, dtype=np.int32)
+    if not np.array_equal(out, given):
+        raise _lib.ScaError(4, f"{what} must fit 32 bits")
+    return out
+
+
+def _paged_step(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens, weights, block_size, scale, typical_len, longest_len, stream):
+    _require_cuda(q, k_pool, v_pool, page_table, seq_lens)
+    if q.dim() != 4:
+        raise _lib.ScaError(4, f"paged_attention expects q=[num_seqs, H_q, seq_q, D]; got ndims={q.dim()}")
+    s, hq, sq, d = q.shape
+    if sq != 1:
+        raise _lib.ScaError(5, f"paged attention implements the decode form only (seq_q=1); got seq_q={sq}")
+    if k_pool.dim() != 4:
+        raise _lib.ScaError(4, "pool geometry mismatch")
+    nblk, bs, hkv, dk = k_pool.shape
+    if bs != block_size or dk != d or tuple(v_pool.shape) != tuple(k_pool.shape):
+        raise _lib.ScaError(4, "pool geometry mismatch")
+    _require_like(q, k_pool, v_pool)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise _lib.ScaError(4, f"weights and shared prefixes are for float16 or bfloat16; got {q.dtype}")
+    if hkv < 1 or hq < 1 or hq % hkv != 0:
+        raise _lib.ScaError(4, f"num_heads={hq} % num_kv_heads={hkv} != 0")
+    _require_packed("q or pool", q, k_pool, v_pool)
+    _require_table(page_table, s)
+    if seq_lens is not None:
+        _require_ints("seq_lens", seq_lens, s)
+    max_blocks = page_table.shape[1]
+    tensors = [k_pool, v_pool, page_table] + ([seq_lens] if seq_lens is not None else [])
+    if weights is not None:
+        _require_weights(weights, s, hkv, max_blocks * bs)
+        tensors.append(weights)
+    _require_one_device(q, *tensors)
+    if _elsewhere(q, stream):
+        with torch.cuda.device(q.device):
+            return _paged_step(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens, weights, block_size, scale, typical_len, longest_len, None)
+    handle = _stream_ptr(stream)
+    out = _empty((s, hq, 1, d), q.dtype, q.device, stream)
+    if s == 0:
+        return out
+    p = DecodeFwdParams()
+    p.q, p.k, p.v, p.out = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
+    p.batch, p.num_heads, p.num_kv_heads, p.head_dim = s, hq, hkv, d
+    p.q_stride = DecodeStrides(hq * d, d, d)
+    p.o_stride = DecodeStrides(hq * d, d, d)
+    p.scale = effective_scale(scale, d)
+    p.dtype = dtype_id(q.dtype)
+    p.page_table = page_table.data_ptr()
+    p.seq_lens = seq_lens.data_ptr() if seq_lens is not None else None
+    p.block_size, p.max_blocks_per_seq, p.num_kv_blocks = bs, max_blocks, nblk
+    x = _lib.PagedStep()
+    if prefix_lens is not None:
+        x.cu_groups, x.prefix_lens, x.num_groups = cu_groups.ctypes.data, prefix_lens.ctypes.data, prefix_lens.shape[0]
+    if weights is not None:
+        x.weights, x.weights_row = weights.data_ptr(), weights.shape[2]
+    x.typical_len, x.longest_len = max(0, int(typical_len)), max(0, int(longest_len))
+    need = lib().sca_paged_step_scratch_floats(C.byref(p), C.byref(x))
+    if need < 0:
+        check(4)
+    ws = acquire_scratch_fp32(need, q.device, stream=stream, handle=handle)
+    x.scratch, x.scratch_floats = ws.data_ptr(), ws.numel()
+    check(lib().sca_launch_paged_step(C.byref(p), C.byref(x), handle))
+    return out
+
+
+def paged_attention_weights(q, k_pool, v_pool, page_table, seq_lens, weights, *, block_size: int, scale=None, typical_len: int = 0, longest_len: int = 0,
+                            stream=None):
+    """paged_attention that adds up what each cached token weighs: weights[s, g, j] += the sum over the query heads h of kv head g of
+    softmax_j(scale q[s, h] . k[j]), in float32, for every token j of sequence s; what lies behind its last token is left as it is. The order of
+    the sum is fixed: the same call gives the same bits.
+
+    q, pools, table, lengths as paged_attention takes them, of float16 or bfloat16; weights float32 [num_seqs, H_kv, max_blocks_per_seq *
+    block_size] or more rows and columns, on the device. A query of NaN makes the weights of its kv head NaN. `typical_len` sizes the launch;
+    `longest_len` does too and bounds the lengths: no sequence is longer, and a token behind it would count for nothing."""
+    return _paged_step(q, k_pool, v_pool, page_table, seq_lens, None, None, weights, block_size, scale, typical_len, longest_len, stream)
+
+
+def paged_attention_shared(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens, *, block_size: int, weights=None, scale=None, typical_len: int = 0,
+                           longest_len: int = 0, stream=None):
+    """paged_attention over sequences that have the pages of a prefix in common, which are read once for all of them.
+
+    Group i is the sequences cu_groups[i] .. cu_groups[i + 1] - 1 (neighbours; cu_groups has num_groups + 1 entries from 0 to num_seqs), and all of
+    them begin with the same prefix_lens[i] tokens: the table's entries of the whole pages of those tokens are the same in all rows of the group
+    and are taken from its first row; tokens of a page that the prefix does not fill are each sequence's own, as are the ones behind. Both lists
+    are on the HOST. At most 128 groups of two or more sequences that share a page; pages of 8, 16, 32 or 64 tokens. Values of bfloat16
+    beyond +-65504 in shared pages count as +-65504, as in the prefill.
+    With `weights` (see paged_attention_weights) the weights of each sequence's own tokens are added up; those of shared pages are left alone.
+    The rest is as paged_attention_weights has it."""
+    cu, lens = _host_ints("cu_groups", cu_groups), _host_ints("prefix_lens", prefix_lens)
+    if cu.shape[0] != lens.shape[0] + 1:
+        raise _lib.ScaError(4, "cu_groups needs num_groups + 1 entries, prefix_lens num_groups")
+    return _paged_step(q, k_pool, v_pool, page_table, seq_lens, cu, lens, weights, block_size, scale, typical_len, longest_len, stream)
+
+
+def kv_evict(layer_k, layer_v, weights, page_table, seq_lens, *, keep: int, recent: int = 0, first=0, stream=None) -> torch.Tensor:
+    """Brings every sequence down to m = max(keep, first + recent) tokens, each kv head on its own: of n > m tokens the first `first` are kept, the
+    last `recent`, and of those in between the m - first - recent of the largest weights (equal ones: the lower place; NaN counts as the
+    largest). Returns the new lengths, int32 [num_seqs]: min(n, m). The pages behind them may be freed.
+
+    In place, and a row moves once at most: afterwards [0, first) and [m - recent, m) hold the first and the last tokens in order; in
+    [first, m - recent) those kept stay where they are, and the i-th place that comes free takes the i-th of those kept behind m - recent, both
+    counted upwards. weights (float32, as paged_attention_weights takes them) go along and become 0 in places [m, n). Sequences of up to m tokens
+    are left alone.
+    `first`: a number, or int32 [num_seqs] on the device - the tokens of a shared prefix, say, whose pages belong to others too: a page that
+    holds any other token belongs to one sequence only. Pools as kv_append takes them, of any type; rows on unmapped pages are not copied."""
+    _require_cuda(layer_k, layer_v, weights, page_table, seq_lens)
+    if layer_k.dim() != 4 or layer_v.dim() != 4:
+        raise _lib.ScaError(4, "pool geometry mismatch")
+    _require_pools(layer_k, layer_v)
+    if page_table.dim() != 2:
+        raise _lib.ScaError(4, "page_table must be int32 [num_seqs, max_blocks_per_seq], contiguous")
+    n = seq_lens.numel()
+    _require_ints("seq_lens", seq_lens, 0)
+    _require_table(page_table, n)
+    shape, max_blocks = _kv_shape(layer_k), page_table.shape[1]
+    _require_weights(weights, n, shape.num_kv_heads, max_blocks * shape.block_size)
+    tensors = [layer_v, weights, page_table, seq_lens]
+    by_sequence = isinstance(first, torch.Tensor)
+    if by_sequence:
+        _require_ints("first", first, n)
+        tensors.append(first)
+    if keep < 0 or recent < 0 or (not by_sequence and first < 0):
+        raise _lib.ScaError(4, f"keep={keep}, recent={recent} and first must not be negative")
+    _require_one_device(layer_k, *tensors)
+    if _elsewhere(layer_k, stream):
+        with torch.cuda.device(layer_k.device):
+            return kv_evict(layer_k, layer_v, weights, page_table, seq_lens, keep=keep, recent=recent, first=first)
+    new_lens = _empty((n,), torch.int32, layer_k.device, stream)
+    if n == 0:
+        return new_lens
+    x = _lib.KvEvict()
+    x.layer_k, x.layer_v, x.weights, x.weights_row = layer_k.data_ptr(), layer_v.data_ptr(), weights.data_ptr(), weights.shape[2]
+    x.page_table, x.seq_lens, x.new_lens = page_table.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr()
+    x.first_lens, x.first = (first.data_ptr(), 0) if by_sequence else (None, first)
+    x.num_seqs, x.max_blocks_per_seq, x.keep, x.recent = n, max_blocks, keep, recent
+    need = lib().sca_kv_evict_scratch_ints(n, shape.num_kv_heads, keep, max_blocks * shape.block_size)
+    if need < 0:
+        raise _lib.ScaError(4, "kv evict: sizes must be positive")
+    handle = _stream_ptr(stream)
+    ws = acquire_scratch_fp32(need, layer_k.device, stream=stream, handle=handle)
+    x.scratch, x.scratch_ints = ws.data_ptr(), ws.numel()
+    check(lib().sca_launch_kv_evict(C.byref(x), C.byref(shape), layer_k.element_size(), handle))
+    return new_lens
