@@ -446,6 +446,16 @@ SCA_ABI long long sca_paged_step_scratch_floats(const ScaDecodeFwdParams* params
  * and the sizes as there; the partial arrays, num_splits, seq_kv and the strides of K and V are not looked at. scale > 0 and finite. */
 SCA_ABI int sca_launch_paged_step(const ScaDecodeFwdParams* params, const ScaPagedStep* step, void* stream);
 
+/* sca_launch_flash_paged over a 16-bit cache, and the weights of every cached token in it. `lse` is scratch: fp32 [num_heads][total_q], the
+ * natural logarithm of each row's sum afterwards. `last`: the weights of the last so many new tokens of each sequence count, 0: all of them. */
+typedef struct ScaChunkWeights {
+    float* lse;
+    float* weights; /* [num_seqs][kv_heads][weights_row], rows of at least max_blocks_per_seq * block_size */
+    int64_t weights_row;
+    int64_t last;
+} ScaChunkWeights;
+SCA_ABI int sca_launch_flash_paged_weights(const ScaFlashPagedParams* params, const ScaChunkWeights* weights, void* stream);
+
 /* Eviction, in place, of each kv head of each sequence on its own. Of n = seq_lens[s] tokens, where n > m = max(keep, first + recent), the first
  * `first` are kept, the last `recent`, and of those in between the m - first - recent of the largest weights (equal ones: the lower place;
  * NaN counts as the largest). Afterwards [0, first) and [m - recent, m) hold the first and the last ones in order; in [first, m - recent) those

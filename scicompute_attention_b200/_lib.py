@@ -27,7 +27,8 @@ EXPORTED_SYMBOLS = [
     "sca_peer_buffer_destroy", "sca_peer_exchange_status", "sca_peer_exchange_clear", "sca_launch_seqsplit_exchange",
     "sca_flash_varlen_workspace_bytes", "sca_launch_flash_varlen", "sca_launch_flash_paged",
     "sca_launch_kv_append_fp8", "sca_launch_kv_append_batched_fp8", "sca_launch_kv_gather_fp8", "sca_launch_paged_attention_fp8",
-    "sca_launch_flash_paged_fp8", "sca_paged_step_scratch_floats", "sca_launch_paged_step", "sca_kv_evict_scratch_ints", "sca_launch_kv_evict",
+    "sca_launch_flash_paged_fp8", "sca_paged_step_scratch_floats", "sca_launch_paged_step", "sca_launch_flash_paged_weights",
+    "sca_kv_evict_scratch_ints", "sca_launch_kv_evict",
     "sca_mgpu_unique_id", "sca_mgpu_init", "sca_mgpu_allgather_triples", "sca_mgpu_abort", "sca_mgpu_destroy",
 ]
 
@@ -119,6 +120,10 @@ class PagedStep(C.Structure):
                 ("typical_len", C.c_int64), ("longest_len", C.c_int64), ("scratch", C.c_void_p), ("scratch_floats", C.c_int64)]
 
 
+class ChunkWeights(C.Structure):
+    _fields_ = [("lse", C.c_void_p), ("weights", C.c_void_p), ("weights_row", C.c_int64), ("last", C.c_int64)]
+
+
 class KvEvict(C.Structure):
     _fields_ = [("layer_k", C.c_void_p), ("layer_v", C.c_void_p), ("weights", C.c_void_p), ("weights_row", C.c_int64), ("page_table", C.c_void_p),
                 ("seq_lens", C.c_void_p), ("first_lens", C.c_void_p), ("new_lens", C.c_void_p)] + [
@@ -188,6 +193,7 @@ def lib() -> C.CDLL:
     l.sca_paged_step_scratch_floats.argtypes = [C.POINTER(DecodeFwdParams), C.POINTER(PagedStep)]
     l.sca_paged_step_scratch_floats.restype = C.c_longlong
     l.sca_launch_paged_step.argtypes = [C.POINTER(DecodeFwdParams), C.POINTER(PagedStep), C.c_void_p]
+    l.sca_launch_flash_paged_weights.argtypes = [C.POINTER(FlashPagedParams), C.POINTER(ChunkWeights), C.c_void_p]
     l.sca_kv_evict_scratch_ints.argtypes = [C.c_int64] * 4
     l.sca_kv_evict_scratch_ints.restype = C.c_longlong
     l.sca_launch_kv_evict.argtypes = [C.POINTER(KvEvict), C.POINTER(KvCacheShape), C.c_int64, C.c_void_p]

@@ -1,6 +1,7 @@
 // Host side of the prefill: tensor maps, work lists of ragged batches, the choice of the launch. The kernel is in
 // flash_kernel.cuh.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -546,8 +547,8 @@ extern "C" int sca_launch_flash_varlen(const ScaFlashVarlenParams* params, void*
 
 namespace {
 
-// Chunks over a paged cache; `k_scales` null: of f.dtype_id, else of 8 bits.
-int LaunchPaged(const ScaFlashPagedParams* params, const uint8_t* k_scales, const uint8_t* v_scales, void* stream) {
+// Chunks over a paged cache; `k_scales` null: of f.dtype_id, else of 8 bits. `lse`: null, or [heads][total_q].
+int LaunchPaged(const ScaFlashPagedParams* params, const uint8_t* k_scales, const uint8_t* v_scales, void* stream, float* lse = nullptr) {
     if (params == nullptr || params->cu_seqlens_q == nullptr || params->seq_lens_kv == nullptr) {
         return Fail(SCA_INVALID_ARGUMENT, "flash paged: null parameter block or host lengths");
     }
@@ -598,6 +599,8 @@ int LaunchPaged(const ScaFlashPagedParams* params, const uint8_t* k_scales, cons
     f.o_sb = f.q_sb;
     f.scale = x.scale;
     f.causal = x.causal;
+    f.lse = lse;
+    f.return_lse = lse != nullptr;
     f.dtype_id = x.dtype_id;
     if (int rc = ValidateFlash(&f)) return rc;
     VarlenWork vw{x.cu_seqlens_q, cu_kv.data(), x.num_seqs, x.workspace, x.workspace_bytes};
@@ -619,6 +622,35 @@ extern "C" int sca_launch_flash_paged(const ScaFlashPagedParams* params, void* s
     return LaunchPaged(params, nullptr, nullptr, stream);
 } catch (const std::exception& e) {  // host memory for the work list
     return Fail(SCA_CUDA_ERROR, std::string("flash paged: on the host: ") + e.what());
+}
+
+namespace sca_b200 {
+namespace flash {
+int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, const int4* seqs, cudaStream_t stream);  // flash_weights.cu
+}
+}  // namespace sca_b200
+
+extern "C" int sca_launch_flash_paged_weights(const ScaFlashPagedParams* params, const ScaChunkWeights* weights, void* stream) try {
+    ClearError();
+    if (params == nullptr || weights == nullptr || weights->lse == nullptr || weights->weights == nullptr) {
+        return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): null pointer");
+    }
+    const ScaFlashPagedParams& x = *params;
+    if (weights->last < 0) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): last must not be negative");
+    if (weights->weights_row < x.max_blocks_per_seq * x.block_size) {
+        return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): rows of " + std::to_string(weights->weights_row) + " weights for page-table rows of " +
+                                              std::to_string(x.max_blocks_per_seq * x.block_size) + " tokens");
+    }
+    if (x.num_seqs > 0 && x.num_kv_heads > 0 && x.num_seqs > 0x7fffffffLL / x.num_kv_heads) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): too many sequences");
+    if (x.max_blocks_per_seq * x.block_size > 65535LL * 128) {
+        return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): page-table rows of more than 8388480 tokens");
+    }
+    if (!std::isfinite(x.scale)) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): scale must be a positive number");
+    if (int rc = LaunchPaged(params, nullptr, nullptr, stream, weights->lse)) return rc;
+    // the work list of the prefill begins with the sequences (UploadVarlenWork)
+    return flash::LaunchChunkWeights(x, *weights, static_cast<const int4*>(x.workspace), static_cast<cudaStream_t>(stream));
+} catch (const std::exception& e) {  // host memory for the work list
+    return Fail(SCA_CUDA_ERROR, std::string("flash paged (weights): on the host: ") + e.what());
 }
 
 extern "C" int sca_launch_flash_paged_fp8(const ScaFlashPagedParams* params, const uint8_t* k_scales, const uint8_t* v_scales, void* stream) try {

@@ -1321,7 +1321,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
             }
             if (p.lse != nullptr && row < w.seq_q) {
-                p.lse[(static_cast<int64_t>(w.b) * p.heads + head) * p.seq_q + row] =
+                p.lse[(static_cast<int64_t>(w.b) * p.heads + head) * p.seq_q + w.q_tok0 + row] =
                     l_sum > 0.0f ? (m_ref + log2f(l_sum)) * kLn2 : -CUDART_INF_F;
             }
         }
@@ -1378,7 +1378,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             }
             int token, head;
             if (p.lse != nullptr && out_row(row0 + i, &token, &head)) {
-                p.lse[(static_cast<int64_t>(w.b) * p.heads + head) * p.seq_q + token] = l_all > 0.0f ? (m_all + log2f(l_all)) * kLn2 : -CUDART_INF_F;
+                p.lse[(static_cast<int64_t>(w.b) * p.heads + head) * p.seq_q + w.q_tok0 + token] = l_all > 0.0f ? (m_all + log2f(l_all)) * kLn2 : -CUDART_INF_F;
             }
         }
         __syncthreads();

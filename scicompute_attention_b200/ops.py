@@ -1051,6 +1051,57 @@ def paged_attention_shared(q, k_pool, v_pool, page_table, seq_lens, cu_groups, p
     return _paged_step(q, k_pool, v_pool, page_table, seq_lens, cu, lens, weights, block_size, scale, typical_len, longest_len, stream)
 
 
+def flash_attention_paged_weights(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_kv, weights, *, causal=True, scale=None, last: int = 0, stream=None):
+    """flash_attention_paged that adds up what each cached token weighs: weights[s, g, j] += the sum over the new tokens i of sequence s and the query
+    heads h of kv head g of softmax_j(scale q[i, h] . k[j]), in float32; what lies behind a sequence's last token is left as it is. The order of
+    the sum is fixed: the same call gives the same bits. With `last` > 0 the last so many new tokens of each sequence count, with 0 all of them.
+
+    q, pools, table and the lists on the host as flash_attention_paged takes them, of float16 or bfloat16; weights float32 [num_seqs, H_kv,
+    max_blocks_per_seq * block_size] or more rows and columns, on the device. A query of NaN makes the weights it counts for NaN."""
+    import numpy as np
+    _require_cuda(q, k_pool, v_pool, page_table)
+    if q.dim() != 3 or k_pool.dim() != 4 or tuple(k_pool.shape) != tuple(v_pool.shape):
+        raise _lib.ScaError(4, "paged prefill expects packed q [T, H, D] and contiguous pools [blocks, block_size, H_kv, D]")
+    _require_packed("q or pool", q, k_pool, v_pool)
+    _require_like(q, k_pool, v_pool)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise _lib.ScaError(4, f"weights and shared prefixes are for float16 or bfloat16; got {q.dtype}")
+    cu_q, lens = _host_ints("cu_seqlens_q", cu_seqlens_q), _host_ints("seq_lens_kv", seq_lens_kv)
+    n = lens.shape[0]
+    if cu_q.shape[0] != n + 1:
+        raise _lib.ScaError(4, "cu_seqlens_q needs num_seqs + 1 entries, seq_lens_kv and the page table num_seqs")
+    _require_table(page_table, n)
+    tq, hq, d = q.shape
+    nblk, bs, hkv, dk = k_pool.shape
+    if dk != d:
+        raise _lib.ScaError(4, "pool head_dim differs from q")
+    if hkv < 1 or hq < 1 or hq % hkv != 0:
+        raise _lib.ScaError(4, f"num_heads={hq} % num_kv_heads={hkv} != 0")
+    if last < 0:
+        raise _lib.ScaError(4, f"last={last} must not be negative")
+    _require_weights(weights, n, hkv, page_table.shape[1] * bs)
+    _require_one_device(q, k_pool, v_pool, page_table, weights)
+    if _elsewhere(q, stream):
+        with torch.cuda.device(q.device):
+            return flash_attention_paged_weights(q, k_pool, v_pool, page_table, cu_q, lens, weights, causal=causal, scale=scale, last=last)
+    out = _empty(q.shape, q.dtype, q.device, stream)
+    ws_bytes = max(int(lib().sca_flash_varlen_workspace_bytes(n, tq)), 16)
+    ws = _empty(ws_bytes, torch.uint8, q.device, stream)
+    lse = _empty((hq, tq), torch.float32, q.device, stream)
+    p = _lib.FlashPagedParams()
+    p.q, p.out, p.k_pool, p.v_pool, p.page_table = q.data_ptr(), out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr()
+    p.total_q, p.num_heads, p.num_kv_heads, p.head_dim, p.num_seqs = tq, hq, hkv, d, n
+    p.num_blocks, p.block_size, p.max_blocks_per_seq = nblk, bs, page_table.shape[1]
+    p.cu_seqlens_q, p.seq_lens_kv = cu_q.ctypes.data, lens.ctypes.data
+    p.scale = effective_scale(scale, d)
+    p.causal = 1 if causal else 0
+    p.dtype_id = dtype_id(q.dtype)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+    w = _lib.ChunkWeights(lse.data_ptr(), weights.data_ptr(), weights.shape[2], last)
+    check(lib().sca_launch_flash_paged_weights(C.byref(p), C.byref(w), _stream_ptr(stream)))
+    return out
+
+
 def kv_evict(layer_k, layer_v, weights, page_table, seq_lens, *, keep: int, recent: int = 0, first=0, stream=None) -> torch.Tensor:
     """Brings every sequence down to m = max(keep, first + recent) tokens, each kv head on its own: of n > m tokens the first `first` are kept, the
     last `recent`, and of those in between the m - first - recent of the largest weights (equal ones: the lower place; NaN counts as the
