@@ -9,8 +9,8 @@
 // so that a row moves once at most, and of the places in between only those whose token goes. Attention does not depend on the order of the
 // keys; what does, the last tokens and a causal mask over new ones, keeps its order.
 //
-// A cluster of CTAs takes one (sequence, kv head). The `stay`-th largest weight is found digit by digit (11, 11 and 10 bits of a key that
-// orders like the numbers) from histograms in shared memory, which the CTAs read from one another; ties go to the lower place by counting.
+// A cluster of CTAs takes one (sequence, kv head). The `stay`-th largest weight is found digit by digit (8 bits of a key that orders
+// like the numbers at a time) from histograms in shared memory, which the CTAs read from one another; ties go to the lower place by counting.
 // Free places and rows that move are listed by rank in scratch, then all CTAs copy. No free place is the source of a move, so that these
 // copies need no order. The last tokens move down behind them, all rows of a wave read before the first one of it is written: the
 // destination of a row is never behind its source, so that later waves read what no earlier one has written.
@@ -23,13 +23,15 @@
 namespace sca_b200 {
 namespace {
 
-constexpr int kEvictThreads = 512;
+constexpr int kEvictThreads = 256;
 constexpr int kEvictWarps = kEvictThreads / 32;
-constexpr int kDigits = 3;
-constexpr int kBins = 2048;
-constexpr int kEvictCluster = 8;   // CTAs to a (sequence, kv head) at most
-constexpr int kHeld = 8;           // pieces of the last rows that a thread holds at once
-constexpr int kMoves = 4;          // pieces of other rows
+constexpr int kDigits = 4;
+constexpr int kBins = 256;
+static_assert(kBins == kEvictThreads, "a bin to a thread");
+constexpr int kEvictCluster = 16;  // CTAs to a (sequence, kv head) at most
+constexpr int kEvictCtas = 4;      // CTAs to an SM at least
+constexpr int kLoads = 8;          // weights that a thread has on their way at once
+constexpr int kHeld = 8;           // pieces that a thread has on their way at once
 
 struct EvictParams {
     void *k, *v;
@@ -55,15 +57,14 @@ __device__ __forceinline__ uint32_t KeyOf(float w) {
 }
 
 template <typename V>
-__global__ void __launch_bounds__(kEvictThreads)
+__global__ void __launch_bounds__(kEvictThreads, kEvictCtas)
 kv_evict_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t smem[];
     uint32_t(*hist)[kBins] = reinterpret_cast<uint32_t(*)[kBins]>(smem);
     uint32_t* cache = smem + kDigits * kBins;
     __shared__ int s_ties[kEvictWarps], s_free[kEvictWarps], s_late[kEvictWarps];
     __shared__ int s_counts[2];            // free places and late rows of this CTA's slice
-    __shared__ uint32_t s_warp[kEvictWarps];
-    __shared__ uint32_t s_bin, s_above;
+    __shared__ uint32_t s_warp[2][kEvictWarps], s_found[2][3];
     BeginAfterPredecessor();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(ClusterRank()), cluster = p.cluster;
@@ -91,75 +92,99 @@ kv_evict_kernel(const EvictParams p) {
         for (int i = threadIdx.x; i < kDigits * kBins; i += kEvictThreads) smem[i] = 0;
         __syncthreads();
         auto key_at = [&](int i) { return i < p.cached ? cache[i] : KeyOf(w[begin + i]); };
-        uint32_t prefix = 0, need = static_cast<uint32_t>(stay);
+        uint32_t prefix = 0, need = static_cast<uint32_t>(stay), equal = 0;
 #pragma unroll
         for (int digit = 0; digit < kDigits; ++digit) {
-            constexpr int kShift[kDigits] = {21, 10, 0};
-            const int shift = kShift[digit];
-            const uint32_t mask = digit == 2 ? 1023u : 2047u;
-            for (int i = threadIdx.x; i < count; i += kEvictThreads) {
-                uint32_t key;
-                if (digit == 0) {
-                    key = KeyOf(w[begin + i]);
-                    if (i < p.cached) cache[i] = key;
-                } else {
-                    key = key_at(i);
-                    if ((key >> kShift[digit - 1]) != prefix) continue;
+            const int shift = 24 - 8 * digit;
+            if (digit == 0) {
+                // Few values are possible here, a sign and seven bits of exponent, but a warp that adds up equal ones by itself (__match_any_sync)
+                // is slower: 100 thousand tokens, one CTA, 814 us for 779.
+                for (int i0 = 0; i0 < count; i0 += kLoads * kEvictThreads) {
+                    float x[kLoads];
+#pragma unroll
+                    for (int e = 0; e < kLoads; ++e) {
+                        const int i = i0 + e * kEvictThreads + threadIdx.x;
+                        if (i < count) x[e] = w[begin + i];
+                    }
+#pragma unroll
+                    for (int e = 0; e < kLoads; ++e) {
+                        const int i = i0 + e * kEvictThreads + threadIdx.x;
+                        if (i >= count) continue;
+                        const uint32_t key = KeyOf(x[e]);
+                        if (i < p.cached) cache[i] = key;
+                        atomicAdd(&hist[0][key >> shift], 1u);
+                    }
                 }
-                atomicAdd(&hist[digit][(key >> shift) & mask], 1u);
+            } else {
+#pragma unroll 4
+                for (int i = threadIdx.x; i < count; i += kEvictThreads) {
+                    const uint32_t key = key_at(i);
+                    if ((key >> (shift + 8)) == prefix) atomicAdd(&hist[digit][(key >> shift) & 255u], 1u);
+                }
             }
             ClusterBarrier();
-            // four bins a thread, the highest first, of all CTAs
-            const int bin0 = kBins - 4 - 4 * threadIdx.x;
-            uint32_t bins[4] = {0, 0, 0, 0};
-            for (int r = 0; r < cluster; ++r) {
-                const float4 x = LoadFromRank4(SmemAddr(&hist[digit][bin0]), r);
-                bins[0] += __float_as_uint(x.w), bins[1] += __float_as_uint(x.z), bins[2] += __float_as_uint(x.y), bins[3] += __float_as_uint(x.x);
+            // a bin a thread, the highest first, of all CTAs; each begins with its own, so that they do not all read from one
+            const int bin = kBins - 1 - static_cast<int>(threadIdx.x);
+            uint32_t mine = 0;
+            for (int i0 = 0; i0 < cluster; i0 += kLoads) {
+                uint32_t x[kLoads];
+#pragma unroll
+                for (int e = 0; e < kLoads; ++e) {
+                    const int i = rank + i0 + e;
+                    x[e] = i0 + e < cluster ? __float_as_uint(LoadFromRank(SmemAddr(&hist[digit][bin]), i < cluster ? i : i - cluster)) : 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < kLoads; ++e) mine += x[e];
             }
-            const uint32_t mine = bins[0] + bins[1] + bins[2] + bins[3];
             uint32_t incl = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += up;
             }
-            if (lane == 31) s_warp[warp] = incl;
+            if (lane == 31) s_warp[digit & 1][warp] = incl;
             __syncthreads();
             uint32_t above = incl - mine;
-            for (int i = 0; i < warp; ++i) above += s_warp[i];
+            for (int i = 0; i < warp; ++i) above += s_warp[digit & 1][i];
             if (above < need && need <= above + mine) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (need > above && need <= above + bins[i]) {
-                        s_bin = static_cast<uint32_t>(bin0 + 3 - i);
-                        s_above = above;
-                    }
-                    above += bins[i];
-                }
+                s_found[digit & 1][0] = static_cast<uint32_t>(bin);
+                s_found[digit & 1][1] = above;
+                s_found[digit & 1][2] = mine;
             }
             __syncthreads();
-            prefix = digit == 0 ? s_bin : digit == 1 ? (prefix << 11) | s_bin : (prefix << 10) | s_bin;
-            need -= s_above;
-            __syncthreads();  // s_warp, s_bin and s_above are written again
+            prefix = (prefix << 8) | s_found[digit & 1][0];
+            need -= s_found[digit & 1][1];
+            equal = s_found[digit & 1][2];
         }
         const uint32_t border = prefix;  // keys above it stay, and `need` of those equal to it, the lowest places first
-        int ties_before = 0;
-        for (int r = 0; r < rank; ++r) ties_before += __float_as_int(LoadFromRank(SmemAddr(&hist[kDigits - 1][border & 1023u]), r));
-
         // ---- ranks: every warp walks a piece of the slice --------------------------------------------------------
         const int piece = ((count + kEvictWarps - 1) / kEvictWarps + 31) / 32 * 32;
         const int piece_begin = min(warp * piece, count), piece_end = min(piece_begin + piece, count);
-        int ties = 0;
-        for (int i = piece_begin; i < piece_end; i += 32) {
-            const bool tie = i + lane < piece_end && key_at(i + lane) == border;
-            ties += __popc(__ballot_sync(0xffffffffu, tie));
+        int ties_before = 0;
+        if (equal != need) {  // some of the equal ones go
+            for (int r = 0; r < rank; ++r) ties_before += __float_as_int(LoadFromRank(SmemAddr(&hist[kDigits - 1][border & 255u]), r));
+            int ties = 0;
+            for (int i = piece_begin; i < piece_end; i += 32) {
+                const bool tie = i + lane < piece_end && key_at(i + lane) == border;
+                ties += __popc(__ballot_sync(0xffffffffu, tie));
+            }
+            if (lane == 0) s_ties[warp] = ties;
+            __syncthreads();
+            for (int i = 0; i < warp; ++i) ties_before += s_ties[i];
         }
-        if (lane == 0) s_ties[warp] = ties;
-        __syncthreads();
-        for (int i = 0; i < warp; ++i) ties_before += s_ties[i];
         const uint32_t below = (1u << lane) - 1u;
         // f(place, is free, is late, ballots of both)
         auto walk = [&](auto f) {
+            if (equal == need) {
+#pragma unroll 4
+                for (int i = piece_begin; i < piece_end; i += 32) {
+                    const bool in = i + lane < piece_end, kept = in && key_at(i + lane) >= border;
+                    const int place = begin + i + lane;
+                    const bool is_free = in && !kept && place < keep_end, is_late = kept && place >= keep_end;
+                    f(place, is_free, is_late, __ballot_sync(0xffffffffu, is_free), __ballot_sync(0xffffffffu, is_late));
+                }
+                return;
+            }
             int tie_rank = ties_before;
             for (int i = piece_begin; i < piece_end; i += 32) {
                 const bool in = i + lane < piece_end;
@@ -211,73 +236,96 @@ kv_evict_kernel(const EvictParams p) {
         ClusterBarrier();
     }
 
-    // ---- copies --------------------------------------------------------------------------------------------------
-    const int row_pieces = p.row_pieces, move_pieces = 2 * row_pieces;
+    // ---- copies: a warp looks up as many moves as it has lanes, one each, and copies their rows together ---------------
+    // A step copies `moves_a_step` of them, or one in several steps where its pieces are more than a warp's lanes.
+    const int row_pieces = p.row_pieces, move_pieces = 2 * row_pieces;  // K, then V
+    const int moves_a_step = max(1, 32 / move_pieces), steps_a_move = (move_pieces + 31) / 32;
+    const int lane_move = steps_a_move > 1 ? 0 : lane / move_pieces, lane_part = lane - lane_move * move_pieces;
+    const bool lane_works = lane_move < moves_a_step;
     const int64_t token_pieces = static_cast<int64_t>(p.kv_heads) * row_pieces;
-    auto row_of = [&](int place) -> int64_t {  // first piece of this head's row; negative: its page is not mapped
-        const int32_t id = table[place / p.block_size];
-        return id >= 0 && id < p.num_blocks ? (static_cast<int64_t>(id) * p.block_size + place % p.block_size) * token_pieces + static_cast<int64_t>(head) * row_pieces : -1;
+    auto row_of = [&](int place) {  // of the pool; negative: its page is not mapped
+        const int page = place / p.block_size;
+        const int32_t id = table[page];
+        return id >= 0 && id < p.num_blocks ? id * p.block_size + (place - page * p.block_size) : -1;
     };
-    V* const pools[2] = {static_cast<V*>(p.k), static_cast<V*>(p.v)};
-    const int64_t threads = static_cast<int64_t>(cluster) * kEvictThreads, me = static_cast<int64_t>(rank) * kEvictThreads + threadIdx.x;
-    const int64_t total = static_cast<int64_t>(moves) * move_pieces;
-    for (int64_t at = me; at < total; at += kMoves * threads) {
-        V held[kMoves];
-        int64_t to[kMoves];
-        bool is_v[kMoves];
-#pragma unroll
-        for (int i = 0; i < kMoves; ++i) {
-            const int64_t item = at + i * threads;
-            to[i] = -1;
-            if (item >= total) continue;
-            const int move = static_cast<int>(item / move_pieces), part = static_cast<int>(item % move_pieces);
-            const int src = sources[move], dst = free_places[move];
-            const int64_t from = row_of(src), into = row_of(dst);
-            is_v[i] = part >= row_pieces;
-            const int offset = is_v[i] ? part - row_pieces : part;
-            if (part == 0) w[dst] = w[src];
-            if (from < 0 || into < 0) continue;
-            held[i] = (is_v[i] ? pools[1] : pools[0])[from + offset];
-            to[i] = into + offset;
+    // where piece `part` of this head's row 0 of the pool is
+    auto piece_of = [&](int part) {
+        return (part < row_pieces ? static_cast<V*>(p.k) + part : static_cast<V*>(p.v) + (part - row_pieces)) + static_cast<int64_t>(head) * row_pieces;
+    };
+    V* const lane_base = piece_of(lane_part);
+    // step `s` of the moves whose rows the lanes hold in `row`: this lane's piece; null: none
+    auto piece_at = [&](int s, int row, int count) -> V* {
+        const int first = steps_a_move == 1 ? s * moves_a_step : s / steps_a_move;
+        const int at = __shfl_sync(0xffffffffu, row, (first + lane_move) & 31);
+        if (first + lane_move >= count || at < 0 || !lane_works) return nullptr;
+        if (steps_a_move == 1) return lane_base + at * token_pieces;
+        const int part = (s - first * steps_a_move) * 32 + lane;
+        return part < move_pieces ? piece_of(part) + at * token_pieces : nullptr;
+    };
+    const int warps = cluster * kEvictWarps, my_warp = rank * kEvictWarps + warp;
+    // few moves are spread over all warps
+    const int batch = min(32, max(4, (moves + warps - 1) / warps));
+    for (int move0 = batch * my_warp; move0 < moves; move0 += batch * warps) {
+        const int count = min(batch, moves - move0);
+        int from = -1, into = -1;
+        if (lane < count) {
+            const int src = sources[move0 + lane], dst = free_places[move0 + lane];
+            const float weight = w[src];
+            from = row_of(src);
+            into = row_of(dst);
+            if (from < 0 || into < 0) from = into = -1;
+            w[dst] = weight;
         }
+        const int steps = (count + moves_a_step - 1) / moves_a_step * steps_a_move;
+        for (int s0 = 0; s0 < steps; s0 += kHeld) {
+            V held[kHeld];
 #pragma unroll
-        for (int i = 0; i < kMoves; ++i) {
-            if (to[i] >= 0) (is_v[i] ? pools[1] : pools[0])[to[i]] = held[i];
+            for (int i = 0; i < kHeld; ++i) {
+                const V* at = piece_at(s0 + i, from, count);
+                if (at != nullptr) held[i] = *at;
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                V* at = piece_at(s0 + i, into, count);
+                if (at != nullptr) *at = held[i];
+            }
         }
     }
-    const int64_t last = static_cast<int64_t>(recent) * move_pieces;
-    int64_t wave = 0;
-    do {
-        V held[kHeld];
-        float weight[kHeld];
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const int64_t item = wave + me + i * threads;
-            if (item >= last) continue;
-            const int row = static_cast<int>(item / move_pieces), part = static_cast<int>(item % move_pieces);
-            const int64_t from = row_of(n - recent + row);
-            if (part == 0) weight[i] = w[n - recent + row];
-            if (from >= 0) held[i] = part >= row_pieces ? pools[1][from + part - row_pieces] : pools[0][from + part];
+    // The last tokens: a warp has kHeld steps at a time. A row of more steps takes several turns, of other columns each.
+    const int wave_rows = steps_a_move == 1 ? min(32, kHeld * moves_a_step) : max(1, kHeld / steps_a_move);  // of a warp
+    const int turns = (steps_a_move + kHeld - 1) / kHeld;
+    for (int row0 = 0; row0 < recent || row0 == 0; row0 += wave_rows * warps) {
+        const int mine = row0 + my_warp * wave_rows, count = min(max(recent - mine, 0), wave_rows);
+        int from = -1, into = -1;
+        float weight = 0.0f;
+        if (lane < count) {
+            weight = w[n - recent + mine + lane];
+            from = row_of(n - recent + mine + lane);
+            into = row_of(keep_end + mine + lane);
+            if (from < 0 || into < 0) from = into = -1;
         }
-        ClusterBarrier();
+        for (int turn = 0; turn < turns; ++turn) {
+            V held[kHeld];
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const int64_t item = wave + me + i * threads;
-            if (item >= last) continue;
-            const int row = static_cast<int>(item / move_pieces), part = static_cast<int>(item % move_pieces);
-            const int64_t from = row_of(n - recent + row), into = row_of(keep_end + row);
-            if (part == 0) w[keep_end + row] = weight[i];
-            if (from < 0 || into < 0) continue;
-            if (part >= row_pieces) pools[1][into + part - row_pieces] = held[i];
-            else pools[0][into + part] = held[i];
+            for (int i = 0; i < kHeld; ++i) {
+                const V* at = piece_at(turn * kHeld + i, from, count);
+                if (at != nullptr) held[i] = *at;
+            }
+            ClusterBarrier();
+            if (turn == 0 && lane < count) w[keep_end + mine + lane] = weight;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                V* at = piece_at(turn * kHeld + i, into, count);
+                if (at != nullptr) *at = held[i];
+            }
         }
-        wave += kHeld * threads;
-    } while (wave < last);
-    for (int64_t j = m + me; j < n; j += threads) w[j] = 0.0f;  // every weight has been read by now
+    }
+    const int threads = cluster * kEvictThreads, me = rank * kEvictThreads + threadIdx.x;
+    for (int j = m + me; j < n; j += threads) w[j] = 0.0f;  // every weight has been read by now
 }
 
 // Keys that stay in shared memory between the digits; what a CTA has beyond them is read again.
-constexpr int kCachedKeys = 8192;
+constexpr int kCachedKeys = 16384;
 
 template <typename V>
 int LaunchEvict(const EvictParams& p, int64_t units, cudaStream_t stream) {
@@ -285,8 +333,26 @@ int LaunchEvict(const EvictParams& p, int64_t units, cudaStream_t stream) {
     const size_t smem = kHistograms + static_cast<size_t>(p.cached) * sizeof(uint32_t);
     auto kernel = kv_evict_kernel<V>;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kHistograms + kCachedKeys * sizeof(uint32_t), "kv_evict_kernel")) return rc;
+    static PerDevice allowed;  // per instantiation: clusters of more than 8 CTAs have to be asked for
+    if (p.cluster > 8 && allowed.Get([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess ? 1 : -1; }) < 1) {
+        return FailCuda(cudaGetLastError(), "kv_evict_kernel: clusters of more than 8 CTAs");
+    }
     LaunchDependent(kernel, units * p.cluster, kEvictThreads, smem, stream, p.cluster, p);
     return CheckLaunch("kv_evict_kernel", stream);
+}
+
+// CTAs to a (sequence, kv head). More of them shorten the chain of phases of a long one and cost barriers in a short one; up to 8 as long as
+// all CTAs are resident (4 to an SM), 16 where that leaves one to an SM. us for 8 kv heads, D=128, 16 bits, 1 / 2 / 4 / 8 / 16 CTAs:
+//   one sequence of 1100 tokens down to 1024   14.4 / 15.8 / 15.2 / 15.4 / 21.9     4 of 8192 to 4096    107 / 62 / 38 / 32 / 56
+//   of 2200 to 1024                            34.7 / 28.1 / 18.9 / 17.3 / 21.7     8 of 16000 to 4000   167 / 94 / 65 / 66 / 108
+//   of 8192 to 4096                            90.7 / 52.7 / 32.4 / 23.6 / 25.1     16 of 4096 to 2048    67 / 50 / 47 / 63 / 135
+//   of 16000 to 8000                            178 / 95 / 53 / 34.5 / 30.8         32 of 8192 to 4096   147 / 145 / 141 / 169 / 287
+//   of 33000 to 4000                            265 / 103 / 60 / 38.3 / 32.4        64 of 2200 to 1024    83 / 96 / 112 / 186 / 442
+int ClusterFor(int64_t units, int64_t capacity) {
+    if (units * 16 <= SmCount() && capacity >= 12000) return 16;
+    int cluster = 8;
+    while (cluster > 1 && (units * cluster > kEvictCtas * SmCount() || capacity / cluster < 256)) cluster /= 2;
+    return cluster;
 }
 
 int64_t ListLength(int64_t keep, int64_t capacity) { return std::max<int64_t>(1, std::min(keep, capacity)); }
@@ -316,7 +382,7 @@ extern "C" int sca_launch_kv_evict(const ScaKvEvict* params, const ScaKvCacheSha
     }
     const int64_t capacity = x.max_blocks_per_seq * shape->block_size, units = x.num_seqs * shape->num_kv_heads;
     const int64_t row_bytes = shape->head_dim * elem_bytes;
-    if (capacity > 0x7fffff00LL || shape->num_blocks > 0x7fffffffLL || row_bytes > (1 << 20) || units > 0x7fffffffLL / kEvictCluster) return invalid("sizes are out of range");
+    if (capacity > 0x7fffff00LL || shape->num_blocks > 0x7fffff00LL / shape->block_size || row_bytes > (1 << 20) || units > 0x7fffffffLL / kEvictCluster) return invalid("sizes are out of range");
     if (x.keep < 0 || x.recent < 0 || x.first < 0) return invalid("keep, recent and first must not be negative");
     if (x.weights_row < capacity) {
         return invalid("rows of " + std::to_string(x.weights_row) + " weights for page-table rows of " + std::to_string(capacity) + " tokens");
@@ -342,7 +408,7 @@ extern "C" int sca_launch_kv_evict(const ScaKvEvict* params, const ScaKvCacheSha
     p.first_of_all = static_cast<int32_t>(std::min(x.first, capacity));
     p.keep = static_cast<int32_t>(std::min(x.keep, capacity));
     p.recent = static_cast<int32_t>(std::min(x.recent, capacity));
-    p.cluster = 1;
+    p.cluster = ClusterFor(units, capacity);
     p.cached = static_cast<int32_t>(std::min<int64_t>((capacity + p.cluster - 1) / p.cluster, kCachedKeys));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (row_bytes % 16 == 0 && Aligned16(x.layer_k) && Aligned16(x.layer_v)) {
