@@ -137,6 +137,15 @@ __device__ __forceinline__ void CpAsync16(uint32_t smem_dst, const void* gmem_sr
                  "r"(src_bytes)
                  : "memory");
 }
+// The same for bytes that nobody reads again soon: the L2 cache gives them up first.
+__device__ __forceinline__ uint64_t EvictFirstPolicy() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void CpAsync16(uint32_t smem_dst, const void* gmem_src, int src_bytes, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;\n" ::"r"(smem_dst), "l"(gmem_src), "r"(src_bytes), "l"(policy) : "memory");
+}
 __device__ __forceinline__ void CpAsync4(uint32_t smem_dst, const void* gmem_src, int src_bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_dst), "l"(gmem_src), "r"(src_bytes) : "memory");
 }

@@ -51,17 +51,18 @@ struct NoTap {
     static constexpr bool kTaken = false;
 };
 // The scores themselves, in the log2 domain and -inf where a token does not exist: [(sequence * heads + head) * row + token], rows of a
-// multiple of kTile floats. scores null: nothing either.
+// multiple of kTile floats.
 struct ScoreTap {
     static constexpr bool kTaken = true;
     float* scores;
     int64_t row;
 };
 
+// kLog2: ends with MergeWarpsLog2.
 // One segment = tokens [j_begin, j_end) of one (sequence, kv head, head chunk): streams K/V once, keeps the running
 // softmax state of up to 16 query heads, and leaves one (m, l, O) partial per head: in `slot` of the partial arrays, or
 // (kToShared) in this CTA's shared memory (see MergeWarps): m[16] in the log2 domain, l[16], O[16][D].
-template <typename T, int D, bool kPaged, bool kHi, bool kToShared = false, typename Tap = NoTap>
+template <typename T, int D, bool kPaged, bool kHi, bool kToShared = false, typename Tap = NoTap, bool kLog2 = false>
 __device__ __forceinline__ void DecodeSegment(const ScaDecodeFwdParams& p, unsigned char* smem, const int64_t b,
                                               const int hk, const int hc, const int64_t j_begin, const int64_t j_end,
                                               const int slot, const Tap& tap = Tap{}) {
@@ -130,6 +131,8 @@ __device__ __forceinline__ void DecodeSegment(const ScaDecodeFwdParams& p, unsig
         fetch_entry(jt);
     }
 
+    uint64_t policy = 0;  // Tap: K and V leave the cache to the scores, which are read again
+    if constexpr (Tap::kTaken) policy = EvictFirstPolicy();
     // Issues the copies of this warp's `tl`-th tile into `stage`, tile after tile; returns the 16-bit token validity.
     auto issue = [&](int tl, int stage) -> uint32_t {
         const int64_t jt = j_begin + static_cast<int64_t>(warp + tl * kWarps) * kTile + (lane & (kTile - 1));
@@ -157,10 +160,15 @@ __device__ __forceinline__ void DecodeSegment(const ScaDecodeFwdParams& p, unsig
             const int pr = __shfl_sync(0xffffffffu, prow, row);
             const int bytes = pr >= 0 ? 16 : 0;
             const int64_t r = pr >= 0 ? pr : 0;
-            CpAsync16(k_stage + row * G::kRowBytes + SwizzleK<G::kSwizzle>(row, ch) * 16,
-                      k_base + r * k_row_bytes + ch * 16, bytes);
-            CpAsync16(v_stage + row * G::kRowBytes + SwizzleV<G::kSwizzle>(row, ch) * 16,
-                      v_base + r * v_row_bytes + ch * 16, bytes);
+            const uint32_t k_dst = k_stage + row * G::kRowBytes + SwizzleK<G::kSwizzle>(row, ch) * 16;
+            const uint32_t v_dst = v_stage + row * G::kRowBytes + SwizzleV<G::kSwizzle>(row, ch) * 16;
+            if constexpr (Tap::kTaken) {
+                CpAsync16(k_dst, k_base + r * k_row_bytes + ch * 16, bytes, policy);
+                CpAsync16(v_dst, v_base + r * v_row_bytes + ch * 16, bytes, policy);
+            } else {
+                CpAsync16(k_dst, k_base + r * k_row_bytes + ch * 16, bytes);
+                CpAsync16(v_dst, v_base + r * v_row_bytes + ch * 16, bytes);
+            }
         }
         CpAsyncCommit();
         return mask;
@@ -177,6 +185,13 @@ __device__ __forceinline__ void DecodeSegment(const ScaDecodeFwdParams& p, unsig
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[r][j][e] = 0.0f;
     const float scale_log2 = p.scale * kLog2e;
+
+    float* scores_to = nullptr;  // Tap: where this lane's scores of its next tile go, and how far up those of row g + 8 are
+    int64_t scores_up = 0;
+    if constexpr (Tap::kTaken) {
+        scores_to = tap.scores + (b * p.num_heads + head0 + g) * tap.row + j_begin + warp * kTile + 2 * c;
+        scores_up = 8 * tap.row;
+    }
 
     uint32_t mask_queue = 0;
 #pragma unroll
@@ -203,15 +218,15 @@ __device__ __forceinline__ void DecodeSegment(const ScaDecodeFwdParams& p, unsig
             // rows g and g + 8 of the 16 scores: a lane has tokens 2c, 2c + 1 and 8 + 2c, 9 + 2c
             auto store_scores = [&](const float (&s)[2][4]) {
                 if constexpr (Tap::kTaken) {
-                    if (tap.scores == nullptr) return;
-                    const int64_t j0 = j_begin + static_cast<int64_t>(warp + tl * kWarps) * kTile + 2 * c;
-#pragma unroll
-                    for (int h = 0; h < (kHi ? 2 : 1); ++h) {
-                        if (g + 8 * h >= nheads) continue;
-                        float* to = tap.scores + (b * p.num_heads + head0 + g + 8 * h) * tap.row + j0;
-                        *reinterpret_cast<float2*>(to) = make_float2(s[0][2 * h], s[0][2 * h + 1]);
-                        *reinterpret_cast<float2*>(to + 8) = make_float2(s[1][2 * h], s[1][2 * h + 1]);
+                    if (g < nheads) {
+                        *reinterpret_cast<float2*>(scores_to) = make_float2(s[0][0], s[0][1]);
+                        *reinterpret_cast<float2*>(scores_to + 8) = make_float2(s[1][0], s[1][1]);
                     }
+                    if (kHi && g + 8 < nheads) {
+                        *reinterpret_cast<float2*>(scores_to + scores_up) = make_float2(s[0][2], s[0][3]);
+                        *reinterpret_cast<float2*>(scores_to + scores_up + 8) = make_float2(s[1][2], s[1][3]);
+                    }
+                    scores_to += kSpan;
                 }
             };
             if constexpr (Tap::kTaken) {
@@ -353,7 +368,35 @@ __device__ __forceinline__ void DecodeSegment(const ScaDecodeFwdParams& p, unsig
     }
     __syncthreads();
 
-    MergeWarps<D, G::kWarpBytes, kToShared, Tap::kTaken>(p, smem, b, head0, nheads, slot);
+    if constexpr (kLog2) MergeWarpsLog2<D, G::kWarpBytes, kToShared>(p, smem, b, head0, nheads, slot);
+    else MergeWarps<D, G::kWarpBytes, kToShared>(p, smem, b, head0, nheads, slot);
+}
+
+// Whether the one-launch kernel is the faster one for `units` (sequence, kv head, head chunk) columns of `steps` steps
+// (the longest) on clusters of `cluster` CTAs. Both times in us, fitted to graph-timed calls of D=128 on a B200 (one-wave
+// schedule with its merge / one launch): B=1, S=1000 10.9 / 6.2, S=4000 18.5 / 11.1, S=16000 27.5 / 28.5, S=60000 57 /
+// 90; B=4, S=4000 21.0 / 16.5; B=16, S=2000 29.9 / 27.5, paged with lengths from 250 to 2000 25.6 / 27.7; paged B=4, 500
+// to 4000 22.6 / 16.9, B=8 26.9 / 27.2. A step costs more the more CTAs share the memory; the schedule works on what a
+// ragged batch holds (0.55 of the bound is assumed), a cluster waits for the longest sequence.
+// Other head dims, from 1056 calls of D=32 to 256 (batch 1 to 32, 60 to 16000 tokens):
+//   * above 128 one CTA fills an SM and a step is up to twice the bytes, so that clusters which leave SMs idle lose to the
+//     wave: D=256, 8 kv heads, B=2, S=4000 24.2 / 20.5 (one launch / schedule), B=1, S=8000 23.1 / 21.9. Two times fitted
+//     at 192 and 256, with 0.15 us per slot for the merge and 0.7 or 0.8 of the bound for a ragged batch. Groups of more than 8
+//     heads pay for both row halves in the exchange; clusters of less than 8 do not make up for it in short streams,
+//     unless long sequences are ragged (D=256, 16 / 1 heads, B=16, S=4000 32.8 / 24.5; B=32, S=4000 34.4 / 38.5);
+//   * below 128 the memory is the limit once the stream takes 35 us, and the wave uses it better: D=64, B=32, S=8000 90 / 83.
+inline bool ClusterIsFaster(int64_t units, int64_t steps, int cluster, int64_t resident, bool ragged, int head_dim, bool hi, int64_t splits) {
+    const double busy = static_cast<double>(units * cluster) / resident;
+    const double share = static_cast<double>((steps + cluster - 1) / cluster);
+    const double waves = static_cast<double>(units * steps) / resident;
+    const double stream_us = static_cast<double>(units * steps) * kSpan * head_dim * 4 / 6.5e6;
+    if (head_dim > 128) {
+        if (hi && cluster < kMaxCluster && steps > 1 && (!ragged || steps < 8) && stream_us < 12.0) return false;
+        const double one_launch = (hi ? 3.5 + 0.027 * head_dim : 5.4) + share * (0.95 + 0.3 * busy);
+        return one_launch < (hi ? 11.0 : 7.5) + 1.5 * std::max(1.0, waves * (!ragged ? 1.0 : hi ? 0.8 : 0.7)) + 0.15 * static_cast<double>(splits);
+    }
+    if (head_dim < 128 && stream_us > 35.0) return false;
+    return 4.8 + share * (0.55 + 1.1 * busy) < 11.5 + 1.55 * std::max(1.0, waves * (ragged ? 0.55 : 1.0));
 }
 
 }  // namespace

@@ -10,6 +10,7 @@
 // kv head against 32 written and read), and nobody knows M and L before the last key.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "decode_segment.cuh"
 #include "shared_prefix.cuh"
@@ -41,7 +42,17 @@ struct OwnTokens {
     __device__ __forceinline__ bool Regular() const { return p.seq_lens == nullptr && groups.count == 0; }
 };
 
-template <typename T, int D, bool kHi>
+// kWeights: the scores go to scratch. Without, 96 sequences of 200 to 6000 tokens, 32 / 2 heads, D=64, take 44 us; with a look in every tile
+// whether they are wanted 49.
+template <bool kWeights>
+using TapFor = std::conditional_t<kWeights, ScoreTap, NoTap>;
+template <bool kWeights>
+__device__ __forceinline__ TapFor<kWeights> MakeTap(const WeightsParams& x) {
+    if constexpr (kWeights) return {x.scores, x.score_row};
+    else return {};
+}
+
+template <typename T, int D, bool kHi, bool kWeights>
 __global__ void __launch_bounds__(kThreads)
 decode_own_kernel(const ScaDecodeFwdParams p, const int head_chunks, const WeightsParams x, const __grid_constant__ PrefixGroups groups) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -49,60 +60,130 @@ decode_own_kernel(const ScaDecodeFwdParams p, const int head_chunks, const Weigh
     // here reads what it writes. The wait at the end makes the end of this kernel that of both.
     if (!x.behind_prefix) WaitForPredecessor();
     const OwnTokens own{p, groups, x.bound};
-    const ScoreTap tap{x.scores, x.score_row};
+    const auto tap = MakeTap<kWeights>(x);
     WalkSteps<true, kSpan, true>(p, head_chunks, own, [&](int64_t b, int hk, int hc, int64_t j_begin, int64_t j_end, int slot) {
         const int64_t first = own.First(b);
-        DecodeSegment<T, D, true, kHi, false, ScoreTap>(p, smem, b, hk, hc, first + j_begin, first + j_end, slot, tap);
+        DecodeSegment<T, D, true, kHi, false, TapFor<kWeights>, true>(p, smem, b, hk, hc, first + j_begin, first + j_end, slot, tap);
     });
     if (x.behind_prefix) WaitForPredecessor();
 }
 
+// A call that does not fill the machine, in one launch (see ClusterDecode): the CTAs of a cluster share one (sequence, kv head), all of its
+// tokens, those of common pages too, and weigh the tokens they have read once the row's maximum and sum are known. Up to 16 heads to a kv head.
+template <typename T, int D, bool kHi, bool kWeights>
+__global__ void __launch_bounds__(kThreads)
+decode_step_cluster_kernel(const ScaDecodeFwdParams p, const int cluster, const WeightsParams x, const __grid_constant__ PrefixGroups groups) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float s_m[16], s_inv[16];
+    BeginAfterPredecessor();
+    const OwnTokens own{p, groups, x.bound};
+    const int rank = static_cast<int>(ClusterRank()), unit = static_cast<int>(blockIdx.x) / cluster;
+    const int64_t b = unit / p.num_kv_heads;
+    const int hk = static_cast<int>(unit % p.num_kv_heads), heads = static_cast<int>(p.num_heads / p.num_kv_heads), head0 = hk * heads;
+    const int64_t len = own.Length(b), steps = StepsFor<kSpan>(len), share = (steps + cluster - 1) / cluster;
+    const int64_t t0 = min(rank * share, steps), t1 = min(t0 + share, steps);
+    const int64_t begin = t0 * kSpan, end = min(t1 * kSpan, len);
+    DecodeSegment<T, D, true, kHi, true, TapFor<kWeights>, true>(p, smem, b, hk, 0, begin, end, 0, MakeTap<kWeights>(x));
+    ClusterBarrier();
+    const uint32_t partial = SmemAddr(CtaPartial<D>(smem)), partial_o = SmemAddr(smem) + 32 * 4;
+    if (threadIdx.x < heads) {  // a thread per head; s_m: the maximum, s_inv: 1 / sum
+        float m[kMaxCluster], l[kMaxCluster], m_all = -CUDART_INF_F, l_all = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            m[r] = r < cluster ? LoadFromRank(partial + 4 * threadIdx.x, r) : -CUDART_INF_F;
+            l[r] = r < cluster ? LoadFromRank(partial + 4 * (16 + threadIdx.x), r) : 0.0f;
+            m_all = fmaxf(m_all, m[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            if (m[r] != -CUDART_INF_F || l[r] != 0.0f) l_all += l[r] * Exp2(m[r] - m_all);
+        }
+        s_m[threadIdx.x] = m_all;
+        s_inv[threadIdx.x] = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+    }
+    __syncthreads();
+    T* out = reinterpret_cast<T*>(p.out) + b * p.o_stride.s_b;
+    for (int item = rank * kThreads + threadIdx.x; item < heads * D; item += cluster * kThreads) {
+        const int row = item / D, d = item % D;
+        float m[kMaxCluster], o[kMaxCluster], acc = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            m[r] = r < cluster ? LoadFromRank(partial + 4 * row, r) : -CUDART_INF_F;
+            o[r] = r < cluster ? LoadFromRank(partial_o + 4 * (row * D + d), r) : 0.0f;
+        }
+        // a part without a key has O = 0 beside its maximum of -inf, a part of NaN keeps it
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            if (m[r] != -CUDART_INF_F || o[r] != 0.0f) acc += o[r] * Exp2(m[r] - s_m[row]);
+        }
+        out[(head0 + row) * p.o_stride.s_h + d] = FromFloat<T>(acc * s_inv[row]);
+    }
+    if constexpr (kWeights) {
+        float* w = x.weights + unit * x.row;
+        const float* scores = x.scores + (b * p.num_heads + head0) * x.score_row;
+        for (int64_t j = max(begin, own.First(b)) + threadIdx.x; j < end; j += kThreads) {
+            float sum = 0.0f;
+            for (int h = 0; h < heads; ++h) sum += Exp2(scores[h * x.score_row + j] - (s_m[h] == -CUDART_INF_F ? 0.0f : s_m[h])) * s_inv[h];
+            w[j] += sum;
+        }
+    }
+    ClusterBarrier();  // nobody leaves while its shared memory is being read
+}
+
 constexpr int kFinishThreads = 256;
-constexpr int kChunk = 4 * kFinishThreads;  // tokens a CTA weighs at once
+constexpr int kTokens = 4 * kFinishThreads; // tokens a CTA weighs at once
 constexpr int kHeadSlab = 32;               // query heads whose M and 1 / L stand in shared memory
+constexpr int kTogether = 4;                // query heads whose scores a thread has on their way
+constexpr int64_t kMostSplits = 64;         // parts of a sequence's own tokens
+constexpr int kMostParts = 32;              // and of its prefix (PlanPrefixParts)
 
 // Maximum and sum over the parts of a row, by a whole warp.
 struct RowStats {
     float m, l;
 };
 __device__ __forceinline__ RowStats StatsOf(const ScaDecodeFwdParams& p, const PrefixParts& prefix, int parts, int prefix_parts, int64_t row) {
-    const int lane = threadIdx.x & 31;
-    const int own = static_cast<int>(p.num_splits);
-    auto each = [&](auto f) {
-        for (int i = lane; i < own; i += 32) f(p.partial_m[row * own + i], p.partial_l[row * own + i]);
-        for (int i = lane; i < prefix_parts; i += 32) f(prefix.m[row * parts + i], prefix.l[row * parts + i]);
-    };
-    float m = -CUDART_INF_F, l = 0.0f;
-    each([&](float mi, float) { m = fmaxf(m, mi); });
+    constexpr int kOwn = kMostSplits / 32, kAll = kOwn + kMostParts / 32;
+    const int lane = threadIdx.x & 31, own = static_cast<int>(p.num_splits);
+    float mi[kAll], li[kAll], m = -CUDART_INF_F, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAll; ++i) {
+        const int at = i < kOwn ? 32 * i + lane : 32 * (i - kOwn) + lane;
+        const bool in = at < (i < kOwn ? own : prefix_parts);
+        mi[i] = !in ? -CUDART_INF_F : i < kOwn ? p.partial_m[row * own + at] : prefix.m[row * parts + at];
+        li[i] = !in ? 0.0f : i < kOwn ? p.partial_l[row * own + at] : prefix.l[row * parts + at];
+    }
+#pragma unroll
+    for (int i = 0; i < kAll; ++i) m = fmaxf(m, mi[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    each([&](float mi, float li) {
-        if (mi != -CUDART_INF_F || li != 0.0f) l += li * Exp2(mi - m);
-    });
+#pragma unroll
+    for (int i = 0; i < kAll; ++i) {
+        if (mi[i] != -CUDART_INF_F || li[i] != 0.0f) l += li[i] * Exp2(mi[i] - m);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     return {m, l};
 }
 
-// Blocks [0, merge_blocks) merge output rows, the others weigh tokens: block (s * kv_heads + g) * chunks + c of those has chunk c.
+// Blocks [0, merge_blocks) merge output rows, the others weigh tokens: block (s * kv_heads + g) * chunks + c of those has the c-th `chunk` tokens.
 template <typename T>
-__global__ void __launch_bounds__(kFinishThreads)
+__global__ void __launch_bounds__(kFinishThreads, 4)
 decode_finish_kernel(const ScaDecodeFwdParams p, const WeightsParams x, const int merge_blocks, const int chunks,
-                     const __grid_constant__ PrefixGroups groups) {
+                     const int64_t chunk, const __grid_constant__ PrefixGroups groups) {
     __shared__ float s_m[kHeadSlab], s_inv[kHeadSlab];
     BeginAfterPredecessor();
     const int own = static_cast<int>(p.num_splits), parts = groups.parts;
     auto prefix_parts_of = [&](int64_t b) {
         const PrefixGroup* g = GroupOf(groups, b);
-        const int tiles = g != nullptr ? (g->tokens + 127) / 128 : 0;
-        return groups.part_tiles > 0 ? (tiles + groups.part_tiles - 1) / groups.part_tiles : 0;
+        return g != nullptr ? ((g->tokens + 127) / 128 + groups.part_tiles - 1) / groups.part_tiles : 0;
     };
     if (static_cast<int>(blockIdx.x) < merge_blocks) {
-        const int lanes = static_cast<int>(p.head_dim) / 4;  // threads to a row, four numbers each
-        const int64_t total = p.batch * p.num_heads * lanes;
-        for (int64_t item = static_cast<int64_t>(blockIdx.x) * kFinishThreads + threadIdx.x; item < total; item += static_cast<int64_t>(merge_blocks) * kFinishThreads) {
-            const int64_t row = item / lanes, b = row / p.num_heads;
-            const int d = static_cast<int>(item % lanes) * 4;
+        // a thread has four numbers of a row; 32-bit divisions, 64-bit ones are what this kernel would spend its time on
+        const uint32_t lanes = static_cast<uint32_t>(p.head_dim) / 4, block_rows = kFinishThreads / lanes, of_block = threadIdx.x / lanes;
+        const int d = static_cast<int>(threadIdx.x - of_block * lanes) * 4;
+        const uint32_t rows = static_cast<uint32_t>(p.batch * p.num_heads), heads = static_cast<uint32_t>(p.num_heads);
+        for (uint32_t row32 = blockIdx.x * block_rows + of_block; of_block < block_rows && row32 < rows; row32 += merge_blocks * block_rows) {
+            const int64_t row = row32, b = row32 / heads;
             const int prefix_parts = prefix_parts_of(b);
             float m = -CUDART_INF_F, l = 0.0f;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -118,56 +199,82 @@ decode_finish_kernel(const ScaDecodeFwdParams p, const WeightsParams x, const in
             for (int i = 0; i < own; ++i) add(p.partial_m[row * own + i], p.partial_l[row * own + i], p.partial_o + (row * own + i) * p.head_dim + d);
             for (int i = 0; i < prefix_parts; ++i) add(x.prefix.m[row * parts + i], x.prefix.l[row * parts + i], x.prefix.o + (row * parts + i) * p.head_dim + d);
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            T* out = reinterpret_cast<T*>(p.out) + b * p.o_stride.s_b + (row % p.num_heads) * p.o_stride.s_h + d;
+            T* out = reinterpret_cast<T*>(p.out) + b * p.o_stride.s_b + (row - b * heads) * p.o_stride.s_h + d;
             *reinterpret_cast<uint2*>(out) = make_uint2(Pack2<T>(acc.x * inv, acc.y * inv), Pack2<T>(acc.z * inv, acc.w * inv));
         }
         return;
     }
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) - merge_blocks) / chunks;
-    const int chunk = static_cast<int>((static_cast<int64_t>(blockIdx.x) - merge_blocks) % chunks);
-    const int64_t b = unit / p.num_kv_heads, g = unit % p.num_kv_heads;
+    const uint32_t block = blockIdx.x - merge_blocks, unit32 = block / static_cast<uint32_t>(chunks), seq32 = unit32 / static_cast<uint32_t>(p.num_kv_heads);
+    const int64_t unit = unit32, b = seq32, g = unit32 - seq32 * static_cast<uint32_t>(p.num_kv_heads);
     const OwnTokens tokens{p, groups, x.bound};
-    const int64_t first = tokens.First(b), end = tokens.Length(b);
-    if (end <= static_cast<int64_t>(chunk) * kChunk || first >= static_cast<int64_t>(chunk + 1) * kChunk) return;
-    const int64_t j = static_cast<int64_t>(chunk) * kChunk + 4 * threadIdx.x;  // the first of four tokens that this thread weighs
-    const int group = static_cast<int>(p.num_heads / p.num_kv_heads);
+    const int64_t chunk_begin = (block - unit32 * static_cast<uint32_t>(chunks)) * chunk;
+    const int64_t first = tokens.First(b), end = min(tokens.Length(b), chunk_begin + chunk);
+    if (end <= chunk_begin || first >= end) return;
+    const int group = static_cast<int>(static_cast<uint32_t>(p.num_heads) / static_cast<uint32_t>(p.num_kv_heads));
     const int prefix_parts = prefix_parts_of(b);
     const int64_t row0 = b * p.num_heads + g * group;
-    const bool mine = j + 3 >= first && j < end;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int h0 = 0; h0 < group; h0 += kHeadSlab) {
-        const int heads = min(kHeadSlab, group - h0);
+    const float* scores = x.scores + row0 * x.score_row;
+    float* weights = x.weights + unit * x.row;
+    const bool aligned = (reinterpret_cast<uintptr_t>(weights) & 15u) == 0;
+    // a thread has four tokens: all of them own ones of the sequence, or some, or none
+    float4 s[kTogether], old;
+    auto load = [&](int64_t j, int h0) {
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+            if (h0 + i < group) s[i] = *reinterpret_cast<const float4*>(scores + (h0 + i) * x.score_row + j);
+        }
+    };
+    auto some = [&](int64_t j) { return j + 3 >= first && j < end; };
+    auto whole = [&](int64_t j) { return aligned && j >= first && j + 3 < end; };  // one load and one store for all four
+    auto load_tokens = [&](int64_t j) {
+        if (some(j)) load(j, 0);
+        if (whole(j)) old = *reinterpret_cast<const float4*>(weights + j);
+    };
+    const int64_t j = max(chunk_begin, first & ~static_cast<int64_t>(kTokens - 1)) + 4 * threadIdx.x;
+    load_tokens(j);  // on their way while the rows' maxima and sums are made
+    for (int slab = 0; slab < group; slab += kHeadSlab) {
+        const int heads = min(kHeadSlab, group - slab);
+        __syncthreads();  // the last slab has been read
         for (int h = threadIdx.x >> 5; h < heads; h += kFinishThreads / 32) {
-            const RowStats r = StatsOf(p, x.prefix, parts, prefix_parts, row0 + h0 + h);
+            const RowStats r = StatsOf(p, x.prefix, parts, prefix_parts, row0 + slab + h);
             if ((threadIdx.x & 31) == 0) {
                 s_m[h] = r.m == -CUDART_INF_F ? 0.0f : r.m;
                 s_inv[h] = r.l == 0.0f ? 0.0f : 1.0f / r.l;
             }
         }
         __syncthreads();
-        if (mine) {
-            const float* scores = x.scores + (row0 + h0) * x.score_row + j;
-            for (int h = 0; h < heads; ++h) {
-                const float4 s = *reinterpret_cast<const float4*>(scores + h * x.score_row);
-                const float m = s_m[h], inv = s_inv[h];
-                sum.x += Exp2(s.x - m) * inv;
-                sum.y += Exp2(s.y - m) * inv;
-                sum.z += Exp2(s.z - m) * inv;
-                sum.w += Exp2(s.w - m) * inv;
+        for (int64_t at = j; at - 4 * threadIdx.x < end; at += kTokens) {
+            if (!some(at)) continue;
+            if (at != j || slab > 0) {
+                load(at, slab);
+                if (whole(at)) old = *reinterpret_cast<const float4*>(weights + at);
+            }
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int h0 = 0; h0 < heads; h0 += kTogether) {
+                if (h0 > 0) load(at, slab + h0);
+#pragma unroll
+                for (int i = 0; i < kTogether; ++i) {
+                    if (h0 + i >= heads) continue;
+                    const float m = s_m[h0 + i], inv = s_inv[h0 + i];
+                    sum.x += Exp2(s[i].x - m) * inv;
+                    sum.y += Exp2(s[i].y - m) * inv;
+                    sum.z += Exp2(s[i].z - m) * inv;
+                    sum.w += Exp2(s[i].w - m) * inv;
+                }
+            }
+            float* w = weights + at;
+            if (whole(at)) {
+                *reinterpret_cast<float4*>(w) = make_float4(old.x + sum.x, old.y + sum.y, old.z + sum.z, old.w + sum.w);
+            } else {
+                const float add[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (at + i >= first && at + i < end) w[i] += add[i];
+                }
             }
         }
-        __syncthreads();
-    }
-    if (!mine) return;
-    float* w = x.weights + unit * x.row + j;
-    const float add[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (j + i >= first && j + i < end) w[i] += add[i];
     }
 }
-
-constexpr int64_t kMostSplits = 64;
 
 // What a call is made of: sizes of its launches, and where its arrays lie in the scratch.
 struct Plan {
@@ -265,15 +372,61 @@ Plan MakePlan(const ScaDecodeFwdParams& p, const ScaPagedStep& x) {
     plan.prefix_l = plan.prefix_m + rows * groups.parts;
     plan.prefix_o = RoundUp(plan.prefix_l + rows * groups.parts, 8);  // 32
     plan.scores = RoundUp(plan.prefix_o + rows * groups.parts * p.head_dim, 8);
-    plan.score_row = x.weights != nullptr ? RoundUp(plan.bound, kTile) : 0;
+    // a tile of 16 scores may begin at any page of a prefix, 8 tokens say, and is stored whole
+    plan.score_row = x.weights != nullptr ? RoundUp(plan.bound, kTile) + kTile : 0;
     plan.floats = plan.scores + rows * plan.score_row;
     return plan;
 }
 
-template <typename T, int D, bool kHi>
+// Where sequences share pages, the one launch reads them once for each; that pays as long as a CTA has few steps. us, one launch / with the
+// prefix kernel, and the steps of a CTA: 32 / 8 heads, D=128: 5 sequences of 600 tokens 9.0 / 13.5 (2), 3 of 4100 15.1 / 17.0 (8), 12 of 1300 16.6
+// / 19.8 (10), 2 of 8100 21.8 / 19.8 (16), 5 of 4200 22.9 / 21.7 (16). 32 / 2 heads, D=64: 3 of 8100 15.5 / 16.7 (16), 2 of 16100 24.7 / 19.0 (32).
+// 16 / 2 heads, D=256: 16 of 400 12.5 / 17.8 (1), 8 of 1100 17.1 / 16.4 (3), 8 of 2100 23.4 / 17.4 (5).
+// Launches decode_step_cluster_kernel if it is the kernel for this call; *taken = its CTAs per cluster, 0 if it is not.
+template <typename T, int D, bool kHi, bool kWeights>
+int LaunchStepCluster(const ScaDecodeFwdParams& p, const WeightsParams& x, const PrefixGroups& groups, cudaStream_t stream, int* taken) {
+    auto kernel = decode_step_cluster_kernel<T, D, kHi, kWeights>;
+    constexpr int kSmem = DecodeGeom<D>::kSmemBytes;
+    if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kSmem, "decode_step_cluster_kernel")) return rc;
+    static PerDevice resident[kMaxCluster + 1], per_sm;  // per instantiation
+    auto clusters = [&](int cluster) -> int64_t {
+        return std::max(0, resident[cluster].Get([&] {
+            cudaLaunchAttribute attr{};
+            cudaLaunchConfig_t cfg = ClusterConfig(static_cast<unsigned>(cluster), cluster, kSmem, nullptr, &attr);
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                return -1;
+            }
+            return n;
+        }));
+    };
+    const int ctas = per_sm.Get([&] {
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, kSmem) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            return -1;
+        }
+        return n;
+    });
+    const int64_t units = p.batch * p.num_kv_heads, steps = std::max<int64_t>(1, (x.bound + kSpan - 1) / kSpan);
+    int cluster = kMaxCluster;
+    while (cluster >= 2 && units > clusters(cluster)) cluster /= 2;
+    *taken = 0;
+    const int64_t share = (steps + cluster - 1) / cluster;
+    if (D > 128 && share > 6) return SCA_OK;  // one sequence of 4000 tokens, D=256, 16 / 2 heads: 8 steps a CTA 23.6 us, three kernels 18.9
+    const bool pays = groups.count > 0 ? share <= (D <= 64 ? 20 : D <= 128 ? 12 : 2)
+                                       : ClusterIsFaster(units, steps, cluster, static_cast<int64_t>(SmCount()) * std::max(1, ctas), p.seq_lens != nullptr, D, kHi, p.num_splits);
+    if (cluster < 2 || !pays) return SCA_OK;
+    *taken = cluster;
+    LaunchDependent(kernel, units * cluster, kThreads, kSmem, stream, cluster, p, cluster, x, groups);
+    return CheckLaunch("decode_step_cluster_kernel", stream);
+}
+
+template <typename T, int D, bool kHi, bool kWeights>
 int LaunchOwn(const ScaDecodeFwdParams& p, const WeightsParams& x, const PrefixGroups& groups, cudaStream_t stream) {
     using G = DecodeGeom<D>;
-    auto kernel = decode_own_kernel<T, D, kHi>;
+    auto kernel = decode_own_kernel<T, D, kHi, kWeights>;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), G::kSmemBytes, "decode_own_kernel")) return rc;
     static PerDevice per_sm;  // per instantiation
     const int resident = per_sm.Get([&] {
@@ -294,26 +447,46 @@ int LaunchOwn(const ScaDecodeFwdParams& p, const WeightsParams& x, const PrefixG
     return CheckLaunch("decode_own_kernel", stream);
 }
 
-template <typename T>
-int LaunchStep(const ScaDecodeFwdParams& p, const WeightsParams& x, const PrefixGroups& groups, cudaStream_t stream) {
+// f(head dim, more than 8 heads to a kv head, weights wanted), as types
+template <typename F>
+int ForGeometry(const ScaDecodeFwdParams& p, bool weights, const F& f) {
     const bool hi = p.num_heads / p.num_kv_heads > 8;
-    int rc = SCA_OK;
+    auto with = [&](auto d) {
+        if (weights) return hi ? f(d, std::true_type{}, std::true_type{}) : f(d, std::false_type{}, std::true_type{});
+        return hi ? f(d, std::true_type{}, std::false_type{}) : f(d, std::false_type{}, std::false_type{});
+    };
     switch (p.head_dim) {
-        case 32: rc = hi ? LaunchOwn<T, 32, true>(p, x, groups, stream) : LaunchOwn<T, 32, false>(p, x, groups, stream); break;
-        case 64: rc = hi ? LaunchOwn<T, 64, true>(p, x, groups, stream) : LaunchOwn<T, 64, false>(p, x, groups, stream); break;
-        case 96: rc = hi ? LaunchOwn<T, 96, true>(p, x, groups, stream) : LaunchOwn<T, 96, false>(p, x, groups, stream); break;
-        case 128: rc = hi ? LaunchOwn<T, 128, true>(p, x, groups, stream) : LaunchOwn<T, 128, false>(p, x, groups, stream); break;
-        case 160: rc = hi ? LaunchOwn<T, 160, true>(p, x, groups, stream) : LaunchOwn<T, 160, false>(p, x, groups, stream); break;
-        case 192: rc = hi ? LaunchOwn<T, 192, true>(p, x, groups, stream) : LaunchOwn<T, 192, false>(p, x, groups, stream); break;
-        default: rc = hi ? LaunchOwn<T, 256, true>(p, x, groups, stream) : LaunchOwn<T, 256, false>(p, x, groups, stream); break;
+        case 32: return with(std::integral_constant<int, 32>{});
+        case 64: return with(std::integral_constant<int, 64>{});
+        case 96: return with(std::integral_constant<int, 96>{});
+        case 128: return with(std::integral_constant<int, 128>{});
+        case 160: return with(std::integral_constant<int, 160>{});
+        case 192: return with(std::integral_constant<int, 192>{});
+        default: return with(std::integral_constant<int, 256>{});
     }
-    if (rc != SCA_OK) return rc;
-    const int64_t merge_items = p.batch * p.num_heads * (p.head_dim / 4);
-    const int64_t merge_blocks = std::min<int64_t>((merge_items + kFinishThreads - 1) / kFinishThreads, 1 << 16);
-    const int64_t chunks = x.weights != nullptr ? (x.bound + kChunk - 1) / kChunk : 0;
+}
+
+template <typename T>
+int LaunchStep(const ScaDecodeFwdParams& p, WeightsParams x, const PrefixGroups& groups, cudaStream_t stream) {
+    const int64_t heads = p.num_heads / p.num_kv_heads;
+    if (heads <= 16) {
+        int taken = 0;
+        if (int rc = ForGeometry(p, x.weights != nullptr, [&](auto d, auto hi, auto weights) { return LaunchStepCluster<T, decltype(d)::value, decltype(hi)::value, decltype(weights)::value>(p, x, groups, stream, &taken); })) return rc;
+        if (taken > 0) return SCA_OK;
+    }
+    if (groups.count > 0) {
+        if (int rc = LaunchPrefixParts(p, groups, x.prefix, stream)) return rc;
+    }
+    if (int rc = ForGeometry(p, x.weights != nullptr, [&](auto d, auto hi, auto weights) { return LaunchOwn<T, decltype(d)::value, decltype(hi)::value, decltype(weights)::value>(p, x, groups, stream); })) return rc;
+    const int64_t block_rows = kFinishThreads / (p.head_dim / 4);
+    const int64_t merge_blocks = std::min<int64_t>((p.batch * p.num_heads + block_rows - 1) / block_rows, 1 << 16);
+    // tokens to a CTA: few enough that all SMs have some, as many as let a CTA make the maxima and sums once
+    const int64_t units = p.batch * p.num_kv_heads;
+    const int64_t chunk = std::min<int64_t>(8 * kTokens, std::max<int64_t>(1, units * x.bound / (8 * SmCount() * kTokens)) * kTokens);
+    const int64_t chunks = x.weights != nullptr ? (x.bound + chunk - 1) / chunk : 0;
     const int64_t blocks = merge_blocks + p.batch * p.num_kv_heads * chunks;
     if (blocks > 0x7fffffffLL) return Fail(SCA_INVALID_ARGUMENT, "paged attention (weights): grid of " + std::to_string(blocks) + " blocks is out of range");
-    LaunchDependent(decode_finish_kernel<T>, blocks, kFinishThreads, 0, stream, 1, p, x, static_cast<int>(merge_blocks), static_cast<int>(std::max<int64_t>(chunks, 1)), groups);
+    LaunchDependent(decode_finish_kernel<T>, blocks, kFinishThreads, 0, stream, 1, p, x, static_cast<int>(merge_blocks), static_cast<int>(std::max<int64_t>(chunks, 1)), chunk, groups);
     return CheckLaunch("decode_finish_kernel", stream);
 }
 
@@ -360,8 +533,5 @@ extern "C" int sca_launch_paged_step(const ScaDecodeFwdParams* params, const Sca
     w.prefix = PrefixParts{scratch + plan.prefix_m, scratch + plan.prefix_l, scratch + plan.prefix_o};
     w.behind_prefix = plan.groups.count > 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (plan.groups.count > 0) {
-        if (int rc = LaunchPrefixParts(p, plan.groups, w.prefix, s)) return rc;
-    }
     return p.dtype == SCA_DTYPE_F16 ? LaunchStep<__half>(p, w, plan.groups, s) : LaunchStep<__nv_bfloat16>(p, w, plan.groups, s);
 }

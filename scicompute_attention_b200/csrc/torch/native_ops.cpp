@@ -628,6 +628,131 @@ PyObject* ChunkFp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- a paged cache that stays small ------------------------------------------------------------------------------------------
+#pragma weak sca_paged_step_scratch_floats
+#pragma weak sca_launch_paged_step
+#pragma weak sca_launch_flash_paged_weights
+#pragma weak sca_kv_evict_scratch_ints
+#pragma weak sca_launch_kv_evict
+
+// As _require_weights in ops.py.
+bool Weights(const at::Tensor& w, int64_t rows, int64_t kv_heads, int64_t tokens) {
+    return w.scalar_type() == at::kFloat && w.dim() == 3 && w.is_contiguous() && w.size(0) >= rows && w.size(1) == kv_heads && w.size(2) >= tokens &&
+           Fp8Layer::Here(w);
+}
+
+// paged_step(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens, weights, block_size, scale, typical_len, longest_len)
+PyObject* PagedStep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        int64_t block_size;
+        ScaDecodeFwdParams p{};
+        ScaPagedStep x{};
+        if (sca_launch_paged_step == nullptr || n != 12 || !Int(a[8], &block_size) || !Int(a[10], &x.typical_len) || !Int(a[11], &x.longest_len)) return NotTaken();
+        const at::Tensor *q = Plain(a[0]), *k = Plain(a[1]), *v = Plain(a[2]), *table = Plain(a[3]), *lens = nullptr, *weights = nullptr;
+        if ((a[4] != Py_None && (lens = Plain(a[4])) == nullptr) || (a[7] != Py_None && (weights = Plain(a[7])) == nullptr)) return NotTaken();
+        HostInts cu, prefix;
+        if (a[5] != Py_None) {
+            if (!cu.Take(a[5]) || !prefix.Take(a[6]) || cu.size() != prefix.size() + 1) return NotTaken();
+            x.cu_groups = cu.data(), x.prefix_lens = prefix.data(), x.num_groups = prefix.size();
+        }
+        if (!q || !k || !v || !table || q->dim() != 4 || q->size(0) < 1 || q->size(2) != 1 || k->dim() != 4 || k->size(1) != block_size || k->size(3) != q->size(3) ||
+            k->sizes() != v->sizes() || !SameType(*q, *k, *v) || !DtypeId(*q, &p.dtype) || p.dtype == SCA_DTYPE_F32 || !q->is_contiguous() || !k->is_contiguous() ||
+            !v->is_contiguous() || !Table(*table, q->size(0)) || (lens != nullptr && (!Ints(*lens, q->size(0)) || !Fp8Layer::Here(*lens))) ||
+            (weights != nullptr && !Weights(*weights, q->size(0), k->size(2), table->size(1) * block_size)) || !Fp8Layer::Here(*q) || !Fp8Layer::Here(*k) ||
+            !Fp8Layer::Here(*v) || !Fp8Layer::Here(*table) || !Scale(a[9], q->size(3), &p.scale)) {
+            return NotTaken();
+        }
+        const int64_t d = q->size(3);
+        p.batch = q->size(0), p.num_heads = q->size(1), p.num_kv_heads = k->size(2), p.head_dim = d;
+        p.q = q->data_ptr(), p.k = k->data_ptr(), p.v = v->data_ptr();
+        p.q_stride = ScaDecodeStrides{p.num_heads * d, d, d};
+        p.o_stride = p.q_stride;
+        p.seq_lens = lens != nullptr ? static_cast<const int32_t*>(lens->data_ptr()) : nullptr;
+        p.page_table = static_cast<const int32_t*>(table->data_ptr());
+        p.block_size = block_size, p.max_blocks_per_seq = table->size(1), p.num_kv_blocks = k->size(0);
+        if (weights != nullptr) x.weights = static_cast<float*>(weights->data_ptr()), x.weights_row = weights->size(2);
+        x.scratch_floats = sca_paged_step_scratch_floats(&p, &x);
+        if (x.scratch_floats < 0) return NotTaken();
+        void* stream = CurrentStream();
+        PyObject* device = PyObject_GetAttrString(a[0], "device");
+        if (device == nullptr) throw std::runtime_error("device");
+        x.scratch = Scratch(x.scratch_floats, *q, stream, device);
+        Py_DECREF(device);
+        if (x.scratch == nullptr) return NotTaken();
+        at::Tensor out = Empty(q->sizes(), *q, q->scalar_type());
+        p.out = out.data_ptr();
+        if (const int rc = Launch([&] { return sca_launch_paged_step(&p, &x, stream); })) return NotLaunched(rc);
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// chunk_weights(q, k_pool, v_pool, page_table, cu_q, seq_lens, weights, causal, scale, last)
+PyObject* ChunkWeights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        if (sca_launch_flash_paged_weights == nullptr || n != 10) return NotTaken();
+        const at::Tensor *q = Plain(a[0]), *k = Plain(a[1]), *v = Plain(a[2]), *table = Plain(a[3]), *weights = Plain(a[6]);
+        HostInts cu_q, lens;
+        bool causal;
+        ScaFlashPagedParams p{};
+        ScaChunkWeights w{};
+        if (!q || !k || !v || !table || !weights || !cu_q.Take(a[4]) || !lens.Take(a[5]) || !Flag(a[7], &causal) || !Int(a[9], &w.last) || !DtypeId(*q, &p.dtype_id)) return NotTaken();
+        if (p.dtype_id == SCA_DTYPE_F32 || q->dim() != 3 || k->dim() != 4 || k->sizes() != v->sizes() || !SameType(*q, *k, *v) || !q->is_contiguous() || !k->is_contiguous() ||
+            !v->is_contiguous() || !Table(*table, lens.size()) || cu_q.size() != lens.size() + 1 || k->size(3) != q->size(2) || k->size(2) < 1 || q->size(1) % k->size(2) != 0 ||
+            !Weights(*weights, lens.size(), k->size(2), table->size(1) * k->size(1)) || !Fp8Layer::Here(*q) || !Fp8Layer::Here(*k) || !Fp8Layer::Here(*v) ||
+            !Fp8Layer::Here(*table) || !Scale(a[8], q->size(2), &p.scale)) {
+            return NotTaken();
+        }
+        p.total_q = q->size(0), p.num_heads = q->size(1), p.head_dim = q->size(2), p.num_seqs = lens.size();
+        p.num_blocks = k->size(0), p.block_size = k->size(1), p.num_kv_heads = k->size(2), p.max_blocks_per_seq = table->size(1);
+        at::Tensor out = Empty(q->sizes(), *q, q->scalar_type()), ws = VarlenWorkspace(p.num_seqs, p.total_q, *q);
+        at::Tensor lse = Empty({p.num_heads, p.total_q}, *q, at::kFloat);
+        p.q = q->data_ptr(), p.out = out.data_ptr(), p.k_pool = k->data_ptr(), p.v_pool = v->data_ptr();
+        p.page_table = static_cast<const int32_t*>(table->data_ptr());
+        p.cu_seqlens_q = cu_q.data(), p.seq_lens_kv = lens.data(), p.causal = causal;
+        p.workspace = ws.data_ptr(), p.workspace_bytes = ws.numel();
+        w.lse = static_cast<float*>(lse.data_ptr()), w.weights = static_cast<float*>(weights->data_ptr()), w.weights_row = weights->size(2);
+        void* stream = CurrentStream();
+        if (const int rc = Launch([&] { return sca_launch_flash_paged_weights(&p, &w, stream); })) return NotLaunched(rc);
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// evict(k_pool, v_pool, weights, page_table, seq_lens, keep, recent, first)
+PyObject* Evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return Guarded([&]() -> PyObject* {
+        ScaKvEvict x{};
+        ScaKvCacheShape shape;
+        if (sca_launch_kv_evict == nullptr || n != 8 || !Int(a[5], &x.keep) || !Int(a[6], &x.recent)) return NotTaken();
+        const at::Tensor *k = Plain(a[0]), *v = Plain(a[1]), *weights = Plain(a[2]), *table = Plain(a[3]), *lens = Plain(a[4]), *first = nullptr;
+        if (!k || !v || !weights || !table || !lens || !Pools(*k, *v, &shape) || !Ints(*lens, 1) || !Table(*table, lens->numel())) return NotTaken();
+        x.num_seqs = lens->numel(), x.max_blocks_per_seq = table->size(1);
+        if (!Int(a[7], &x.first)) {
+            first = Plain(a[7]);
+            if (first == nullptr || !Ints(*first, x.num_seqs) || !Fp8Layer::Here(*first)) return NotTaken();
+            x.first_lens = static_cast<const int32_t*>(first->data_ptr());
+        }
+        if (x.keep < 0 || x.recent < 0 || x.first < 0 || !Weights(*weights, x.num_seqs, shape.num_kv_heads, x.max_blocks_per_seq * shape.block_size) ||
+            !Fp8Layer::Here(*k) || !Fp8Layer::Here(*v) || !Fp8Layer::Here(*table) || !Fp8Layer::Here(*lens)) {
+            return NotTaken();
+        }
+        x.scratch_ints = sca_kv_evict_scratch_ints(x.num_seqs, shape.num_kv_heads, x.keep, x.max_blocks_per_seq * shape.block_size);
+        if (x.scratch_ints < 0) return NotTaken();
+        void* stream = CurrentStream();
+        PyObject* device = PyObject_GetAttrString(a[0], "device");
+        if (device == nullptr) throw std::runtime_error("device");
+        x.scratch = reinterpret_cast<int32_t*>(Scratch(x.scratch_ints, *k, stream, device));
+        Py_DECREF(device);
+        if (x.scratch == nullptr) return NotTaken();
+        at::Tensor new_lens = Empty({x.num_seqs}, *k, at::kInt);
+        x.layer_k = k->data_ptr(), x.layer_v = v->data_ptr();
+        x.weights = static_cast<float*>(weights->data_ptr()), x.weights_row = weights->size(2);
+        x.page_table = static_cast<const int32_t*>(table->data_ptr()), x.seq_lens = static_cast<const int32_t*>(lens->data_ptr());
+        x.new_lens = static_cast<int32_t*>(new_lens.data_ptr());
+        if (const int rc = Launch([&] { return sca_launch_kv_evict(&x, &shape, k->element_size(), stream); })) return NotLaunched(rc);
+        return THPVariable_Wrap(std::move(new_lens));
+    });
+}
+
 // init(scratch_local, acquire_scratch, check)
 PyObject* Init(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 3) {
@@ -658,6 +783,7 @@ PyMethodDef g_methods[] = {SCA_METHOD("init", Init), SCA_METHOD("flash", Flash),
                            SCA_METHOD("append_batched", AppendBatched), SCA_METHOD("reset", Reset), SCA_METHOD("gather", Gather),
                            SCA_METHOD("append_fp8", AppendFp8), SCA_METHOD("append_batched_fp8", AppendBatchedFp8),
                            SCA_METHOD("gather_fp8", GatherFp8), SCA_METHOD("paged_fp8", PagedFp8), SCA_METHOD("chunk_fp8", ChunkFp8),
+                           SCA_METHOD("paged_step", PagedStep), SCA_METHOD("chunk_weights", ChunkWeights), SCA_METHOD("evict", Evict),
                            SCA_METHOD("slots", Slots), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Plain operator calls without the Python in between.", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -964,6 +964,10 @@ def _host_ints(what: str, values):
 
 
 def _paged_step(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens, weights, block_size, scale, typical_len, longest_len, stream):
+    if stream is None:
+        out = _native().paged_step(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens, weights, block_size, scale, typical_len, longest_len)
+        if out is not None:
+            return out
     _require_cuda(q, k_pool, v_pool, page_table, seq_lens)
     if q.dim() != 4:
         raise _lib.ScaError(4, f"paged_attention expects q=[num_seqs, H_q, seq_q, D]; got ndims={q.dim()}")
@@ -1031,6 +1035,8 @@ def paged_attention_weights(q, k_pool, v_pool, page_table, seq_lens, weights, *,
     q, pools, table, lengths as paged_attention takes them, of float16 or bfloat16; weights float32 [num_seqs, H_kv, max_blocks_per_seq *
     block_size] or more rows and columns, on the device. A query of NaN makes the weights of its kv head NaN. `typical_len` sizes the launch;
     `longest_len` does too and bounds the lengths: no sequence is longer, and a token behind it would count for nothing."""
+    if weights is None:
+        raise _lib.ScaError(4, "weights must be a tensor")
     return _paged_step(q, k_pool, v_pool, page_table, seq_lens, None, None, weights, block_size, scale, typical_len, longest_len, stream)
 
 
@@ -1045,6 +1051,10 @@ def paged_attention_shared(q, k_pool, v_pool, page_table, seq_lens, cu_groups, p
     beyond +-65504 in shared pages count as +-65504, as in the prefill.
     With `weights` (see paged_attention_weights) the weights of each sequence's own tokens are added up; those of shared pages are left alone.
     The rest is as paged_attention_weights has it."""
+    if stream is None and cu_groups is not None:
+        out = _native().paged_step(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens, weights, block_size, scale, typical_len, longest_len)
+        if out is not None:
+            return out
     cu, lens = _host_ints("cu_groups", cu_groups), _host_ints("prefix_lens", prefix_lens)
     if cu.shape[0] != lens.shape[0] + 1:
         raise _lib.ScaError(4, "cu_groups needs num_groups + 1 entries, prefix_lens num_groups")
@@ -1058,7 +1068,10 @@ def flash_attention_paged_weights(q, k_pool, v_pool, page_table, cu_seqlens_q, s
 
     q, pools, table and the lists on the host as flash_attention_paged takes them, of float16 or bfloat16; weights float32 [num_seqs, H_kv,
     max_blocks_per_seq * block_size] or more rows and columns, on the device. A query of NaN makes the weights it counts for NaN."""
-    import numpy as np
+    if stream is None:
+        out = _native().chunk_weights(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_kv, weights, causal, scale, last)
+        if out is not None:
+            return out
     _require_cuda(q, k_pool, v_pool, page_table)
     if q.dim() != 3 or k_pool.dim() != 4 or tuple(k_pool.shape) != tuple(v_pool.shape):
         raise _lib.ScaError(4, "paged prefill expects packed q [T, H, D] and contiguous pools [blocks, block_size, H_kv, D]")
@@ -1113,6 +1126,10 @@ def kv_evict(layer_k, layer_v, weights, page_table, seq_lens, *, keep: int, rece
     are left alone.
     `first`: a number, or int32 [num_seqs] on the device - the tokens of a shared prefix, say, whose pages belong to others too: a page that
     holds any other token belongs to one sequence only. Pools as kv_append takes them, of any type; rows on unmapped pages are not copied."""
+    if stream is None:
+        new_lens = _native().evict(layer_k, layer_v, weights, page_table, seq_lens, keep, recent, first)
+        if new_lens is not None:
+            return new_lens
     _require_cuda(layer_k, layer_v, weights, page_table, seq_lens)
     if layer_k.dim() != 4 or layer_v.dim() != 4:
         raise _lib.ScaError(4, "pool geometry mismatch")
