@@ -2,37 +2,48 @@
 // query heads h of kv head g of exp(scale q[i, h] . k[j] - lse[i, h]). It follows the prefill kernel, which leaves lse, the logarithm of each
 // row's sum.
 //
-// A CTA has one tile of 128 keys of one (sequence, kv head) and walks the query tiles that see it; nobody else adds to its weights, so there are
-// no atomics and the same call gives the same bits. The scores are computed with the keys as rows, S = K Q^T (tcgen05, M = 128 keys, N = 128
-// queries, into one of two buffers of tensor memory): a thread then has one key, and its sum over the queries needs no other thread. lse of
-// the 128 queries lies in shared memory, where all threads read the same number at the same time.
-//   warps 0 - 3  a key each thread: 2^(score * scale - lse), summed up
-//   warp 4       TMA: the tile of keys once, page by page, then query tiles into a ring, and their lse
-//   warp 5       issues the products
+// An item is one tile of 128 keys of one (sequence, kv head): a CTA takes it and walks the query tiles that see it. Nobody else adds to its
+// weights, so there are no atomics and the same call gives the same bits. The scores are computed with the keys as rows, S = K Q^T (tcgen05,
+// M = 128 keys, N = 128 queries, into one of four buffers of tensor memory): a thread then has one key, and its sum over the queries needs no
+// other thread until the end of the item. lse of the 128 queries lies in shared memory, where all threads read the same number at a time.
+//   warps 0 - 15   two groups, which take the query tiles in turn; in a group two warps to 32 keys, with half of the columns each:
+//                  2^(score * scale - lse), summed up
+//   warp 16        TMA: tiles of keys, page by page, then their query tiles into a ring, and the queries' lse
+//   warp 17        issues the products
+// One CTA to an SM walks the list of items, those that most queries see first, and loads the next tile of keys under the current one: with a
+// CTA to an item its start - barriers, tensor memory, the look-up of sequence and pages, the first loads - took 6 us (4 prompts of 2000, 32 / 8
+// heads, D=128: 512 items 126 us; 9 sequences of which the last 64 tokens count, D=64: 2016 items 40 us).
 // A query tile is 128 / P tokens of P query heads, as in the prefill, and starts with the first token that sees the tile's first key, so
 // that a causal mask cuts 128 / P tokens' rows at most.
-// Bound by the special-function unit: 16384 exponentials a tile take 1024 clocks of an SM, the products 540.
+// Bound by the special-function unit, of which it uses 71 % while an SM has work (16384 exponentials a tile take 1024 clocks of an SM, the
+// products 540), and by items that do not come out even: 87 % of the SMs' time. 4 prompts of 1900 to 2048 tokens, 32 / 8 heads, D=128: 115 us
+// alone, 260 us with the prefill. A quarter of the exponentials by a polynomial of degree 5 on the multipliers instead: 256 us, half 266.
+#include <algorithm>
+
 #include "flash_kernel.cuh"
 
 namespace sca_b200 {
 namespace flash {
 namespace {
 
-constexpr int kKeys = 128;     // keys of a CTA
+constexpr int kKeys = 128;     // keys of an item
 constexpr int kColumns = 128;  // (token, head) rows of a query tile
-constexpr int kSumWarps = 4;
+constexpr int kGroups = 2, kGroupWarps = 8, kSumWarps = kGroups * kGroupWarps;
+constexpr int kLoadWarp = kSumWarps, kMmaWarp = kSumWarps + 1;
 constexpr int kWeightThreads = 32 * (kSumWarps + 2);
-constexpr int kBuffers = 2;    // of scores in tensor memory
+constexpr int kBuffers = 4;    // of scores in tensor memory
 
 template <int DP>
 struct WeightsGeom {
     static constexpr int kBlocks = DP / 64;              // 128-byte column blocks
     static constexpr int kTileBytes = kBlocks * kKeys * 128;
-    static constexpr int kSlots = DP == 64 ? 4 : 2;      // query tiles in flight; two CTAs to an SM up to D=128
-    static constexpr int kLse = (1 + kSlots) * kTileBytes;
-    static constexpr int kBars = kLse + kSlots * kColumns * 4;
+    static constexpr int kKeySlots = DP == 256 ? 1 : 2;  // tiles of keys
+    static constexpr int kSlots = DP == 64 ? 8 : DP == 128 ? 4 : 2;  // query tiles
+    static constexpr int kLse = (kKeySlots + kSlots) * kTileBytes;
+    static constexpr int kSums = kLse + kSlots * kColumns * 4;        // [2][2 * kGroups][kKeys], items in turn
+    static constexpr int kBars = kSums + 2 * 2 * kGroups * kKeys * 4;
     static constexpr int kSmemBytes = 1024 + kBars + 256;
-    static constexpr int kCtas = DP == 256 ? 1 : 2;
+    static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB per-CTA limit");
 };
 
 struct ChunkParams {
@@ -44,52 +55,60 @@ struct ChunkParams {
     int* error_word;
     int max_blocks, num_blocks, block_size, block_shift;
     int heads, kv_heads, pack_shift, last, causal;
+    int units, items;  // sequences * kv heads, and that times the tiles of the longest sequence
     float scale_log2;
 };
 
+// A barrier of the warps that add up; whether all of them say so.
+__device__ __forceinline__ bool AllSumWarps(bool mine) {
+    uint32_t all;
+    asm volatile(
+        "{\n"
+        ".reg .pred in, out;\n"
+        "setp.ne.u32 in, %1, 0;\n"
+        "barrier.cta.red.and.pred out, 1, %2, in;\n"
+        "selp.u32 %0, 1, 0, out;\n"
+        "}\n"
+        : "=r"(all)
+        : "r"(mine ? 1u : 0u), "n"(32 * kSumWarps)
+        : "memory");
+    return all != 0;
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWeightThreads, WeightsGeom<DP>::kCtas)
+__global__ void __launch_bounds__(kWeightThreads, 1)
 chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const ChunkParams p) {
     using G = WeightsGeom<DP>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t base = (SmemAddr(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (base - SmemAddr(smem_raw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    BeginAfterPredecessor();
-    const int seq = static_cast<int>(blockIdx.x) / p.kv_heads, head_kv = static_cast<int>(blockIdx.x) % p.kv_heads;
-    const int4 s = p.seqs[seq];
-    const int new_tokens = s.z, keys = s.w, key0 = static_cast<int>(blockIdx.y) * kKeys;
-    if (key0 >= keys) return;
-    // token t of the chunk sees keys up to t + diagonal; counted are tokens from `counted` on
-    const int diagonal = p.causal ? keys - new_tokens : keys;
-    const int counted = p.last > 0 ? max(0, new_tokens - p.last) : 0;
-    const int first_token = max(counted, key0 - diagonal);
-    const int heads_tile = 1 << p.pack_shift, tile_tokens = kColumns >> p.pack_shift;
-    const int group = p.heads / p.kv_heads, packs = group >> p.pack_shift;
-    const int tiles = (new_tokens - first_token + tile_tokens - 1) / tile_tokens * packs;  // one at least: the last token sees every key
-
-    const uint32_t k_smem = base, q_smem = base + G::kTileBytes;
+    const uint32_t k_smem = base, q_smem = base + G::kKeySlots * G::kTileBytes;
     float* lse_ring = reinterpret_cast<float*>(smem + G::kLse);
     auto bar = [&](int i) { return base + G::kBars + 8u * i; };
-    constexpr int kKFull = 0, kQFull = 1, kQEmpty = kQFull + G::kSlots, kSFull = kQEmpty + G::kSlots, kSEmpty = kSFull + kBuffers,
-                  kNumBars = kSEmpty + kBuffers;
+    constexpr int kKFull = 0, kKEmpty = kKFull + G::kKeySlots, kQFull = kKEmpty + G::kKeySlots, kQEmpty = kQFull + G::kSlots, kSFull = kQEmpty + G::kSlots,
+                  kSEmpty = kSFull + kBuffers, kNumBars = kSEmpty + kBuffers;
     static_assert(kNumBars * 8 + 8 <= 256, "barrier area too small");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + G::kBars + kNumBars * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     if (threadIdx.x == 0) {
-        MbarInit<1>(bar(kKFull));
+        for (int i = 0; i < G::kKeySlots; ++i) {
+            MbarInit<1>(bar(kKFull + i));
+            MbarInit<1>(bar(kKEmpty + i));
+        }
         for (int i = 0; i < G::kSlots; ++i) {
-            MbarInit<1 + 32>(bar(kQFull + i));         // the tile, and each lane's part of lse
-            MbarInit<1 + kSumWarps>(bar(kQEmpty + i)); // the products and the sums are done with it
+            MbarInit<1 + 32>(bar(kQFull + i));            // the tile, and each lane's part of lse
+            MbarInit<1 + kGroupWarps>(bar(kQEmpty + i));  // the products and the sums are done with it
         }
         for (int i = 0; i < kBuffers; ++i) {
             MbarInit<1>(bar(kSFull + i));
-            MbarInit<kSumWarps>(bar(kSEmpty + i));
+            MbarInit<kGroupWarps>(bar(kSEmpty + i));
         }
         *abort_flag = 0;
         FenceBarrierInit();
     }
-    if (warp == 5) {
+    BeginAfterPredecessor();
+    if (warp == kMmaWarp) {
         TmemAlloc(SmemAddr(tmem_slot), kBuffers * kColumns);
         TmemRelinquish();
     }
@@ -97,124 +116,196 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     __syncthreads();
     TcFenceAfter();
     const uint32_t tmem = *tmem_slot;
-    const int32_t* table = p.page_table + static_cast<int64_t>(seq) * p.max_blocks;
-    auto token_of = [&](int tile) { return first_token + tile / packs * tile_tokens; };
+
+    // ---- items: tile after tile of all sequences and kv heads, dealt in rounds of gridDim.x, every other one in reverse order ----
+    const int heads_tile = 1 << p.pack_shift, tile_tokens = kColumns >> p.pack_shift;
+    const int group = p.heads / p.kv_heads, packs = group >> p.pack_shift;
+    const int rounds = (p.items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    struct Item {
+        int seq, head_kv, key0, keys, new_tokens, q0;
+        int first_token;  // that sees the first key and counts
+        int tiles;        // 0: the sequence has no such keys
+        int diagonal;     // token t sees keys up to t + diagonal
+    };
+    // what an item is, in two steps, so that the look-up in memory is made an item ahead
+    struct Look {
+        int seq, head_kv, key0;
+        int4 s;
+    };
+    auto look = [&](int round) {
+        Look l;
+        const int64_t index = static_cast<int64_t>(round) * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        l.s = make_int4(0, 0, 0, 0);
+        l.seq = l.head_kv = l.key0 = 0;
+        if (round < rounds && index < p.items) {
+            const uint32_t tile = static_cast<uint32_t>(index) / static_cast<uint32_t>(p.units), unit = static_cast<uint32_t>(index) - tile * static_cast<uint32_t>(p.units);
+            l.seq = static_cast<int>(unit / static_cast<uint32_t>(p.kv_heads));
+            l.head_kv = static_cast<int>(unit) - l.seq * p.kv_heads;
+            l.key0 = static_cast<int>(tile) * kKeys;
+            l.s = p.seqs[l.seq];
+        }
+        return l;
+    };
+    auto item_of = [&](const Look& l) {
+        Item w;
+        w.seq = l.seq, w.head_kv = l.head_kv, w.key0 = l.key0;
+        w.q0 = l.s.x, w.new_tokens = l.s.z, w.keys = l.s.w;
+        w.diagonal = p.causal ? w.keys - w.new_tokens : w.keys;
+        w.first_token = max(p.last > 0 ? max(0, w.new_tokens - p.last) : 0, w.key0 - w.diagonal);
+        w.tiles = w.key0 < w.keys ? (w.new_tokens - w.first_token + tile_tokens - 1) / tile_tokens * packs : 0;  // the last token sees every key
+        return w;
+    };
+    auto token_of = [&](const Item& w, int tile) { return w.first_token + tile / packs * tile_tokens; };
+    auto head_of = [&](const Item& w, int tile) { return w.head_kv * group + (tile % packs << p.pack_shift); };
     bool ok = true;
 
-    if (warp == 4) {
+    if (warp == kLoadWarp) {
         // ---- loads ----
-        const int pages = kKeys >> p.block_shift, page = (key0 >> p.block_shift) + lane;
-        const bool in = lane < pages && page < p.max_blocks && (static_cast<int64_t>(page) << p.block_shift) < keys;
-        const int32_t id = in ? table[page] : -1;
-        const int first_row = id >= 0 && id < p.num_blocks ? id << p.block_shift : p.num_blocks << p.block_shift;  // behind the pool: zeros
         if (lane == 0) {
             PrefetchTensorMap(&map_q);
             PrefetchTensorMap(&map_k);
-            MbarExpectTx(bar(kKFull), G::kTileBytes);
         }
-        __syncwarp();
-        for (int i = 0; i < pages; ++i) {
-            const int row = __shfl_sync(0xffffffffu, first_row, i);
-            if (ElectOne()) {
-#pragma unroll
-                for (int kb = 0; kb < G::kBlocks; ++kb) {
-                    TmaLoad4D(k_smem + kb * (kKeys * 128) + i * p.block_size * 128, &map_k, bar(kKFull), kb * 64, row, head_kv, 0);
-                }
-            }
-        }
-        auto lse_of = [&](int tile, float (&v)[4]) {
-            const int token0 = token_of(tile), head0 = head_kv * group + (tile % packs << p.pack_shift);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = lane + 32 * i, token = token0 + (c >> p.pack_shift), head = head0 + (c & (heads_tile - 1));
-                v[i] = tile < tiles && token < new_tokens ? p.lse[static_cast<int64_t>(head) * p.total_q + s.x + token] : -CUDART_INF_F;
-            }
+        const int pages = kKeys >> p.block_shift;
+        uint32_t items = 0, loads = 0;
+        auto page_of = [&](const Look& l) {  // of this lane, in the pool
+            const int page = (l.key0 >> p.block_shift) + lane;
+            const bool in = lane < pages && page < p.max_blocks && (static_cast<int64_t>(page) << p.block_shift) < l.s.w;
+            return in ? p.page_table[static_cast<int64_t>(l.seq) * p.max_blocks + page] : -1;
         };
-        float next[4];
-        lse_of(0, next);
-        for (int tile = 0; tile < tiles && ok; ++tile) {
-            const int slot = tile % G::kSlots;
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = next[i];
-            lse_of(tile + 1, next);
-            ok = __all_sync(0xffffffffu, MbarWait(bar(kQEmpty + slot), ((tile / G::kSlots) & 1u) ^ 1u, abort_flag));
+        Look next = look(0);
+        int32_t next_id = page_of(next);
+        for (int r = 0; r < rounds && ok; ++r) {
+            const Item w = item_of(next);
+            const int32_t id = next_id;
+            next = look(r + 1);
+            next_id = page_of(next);
+            if (w.tiles == 0) continue;
+            const int first_row = id >= 0 && id < p.num_blocks ? id << p.block_shift : p.num_blocks << p.block_shift;  // behind the pool: zeros
+            const uint32_t k_slot = items % G::kKeySlots;
+            ok = __all_sync(0xffffffffu, MbarWait(bar(kKEmpty + k_slot), ((items / G::kKeySlots) & 1u) ^ 1u, abort_flag));
             if (!ok) break;
-            if (ElectOne()) {
-                MbarExpectTx(bar(kQFull + slot), G::kTileBytes);
+            ++items;
+            if (lane == 0) MbarExpectTx(bar(kKFull + k_slot), G::kTileBytes);
+            __syncwarp();
+            for (int i = 0; i < pages; ++i) {
+                const int row = __shfl_sync(0xffffffffu, first_row, i);
+                if (ElectOne()) {
 #pragma unroll
-                for (int kb = 0; kb < G::kBlocks; ++kb) {
-                    TmaLoad4D(q_smem + slot * G::kTileBytes + kb * (kColumns * 128), &map_q, bar(kQFull + slot), kb * 64,
-                              head_kv * group + (tile % packs << p.pack_shift), s.x + token_of(tile), 0);
+                    for (int kb = 0; kb < G::kBlocks; ++kb) {
+                        TmaLoad4D(k_smem + k_slot * G::kTileBytes + kb * (kKeys * 128) + i * p.block_size * 128, &map_k, bar(kKFull + k_slot), kb * 64, row, w.head_kv, 0);
+                    }
                 }
             }
-            __syncwarp();
-            // a row that sees nothing has no sum: 2^-inf
+            auto lse_of = [&](int tile, float (&v)[4]) {
+                const int token0 = token_of(w, tile), head0 = head_of(w, tile);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lse_ring[slot * kColumns + lane + 32 * i] = v[i] == -CUDART_INF_F ? v[i] : -v[i] * kLog2e;
-            MbarArrive(bar(kQFull + slot));
+                for (int i = 0; i < 4; ++i) {
+                    const int c = lane + 32 * i, token = token0 + (c >> p.pack_shift), head = head0 + (c & (heads_tile - 1));
+                    v[i] = tile < w.tiles && token < w.new_tokens ? p.lse[static_cast<int64_t>(head) * p.total_q + w.q0 + token] : -CUDART_INF_F;
+                }
+            };
+            float ahead[4];
+            lse_of(0, ahead);
+            for (int tile = 0; tile < w.tiles && ok; ++tile, ++loads) {
+                const uint32_t slot = loads % G::kSlots;
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = ahead[i];
+                lse_of(tile + 1, ahead);
+                ok = __all_sync(0xffffffffu, MbarWait(bar(kQEmpty + slot), ((loads / G::kSlots) & 1u) ^ 1u, abort_flag));
+                if (!ok) break;
+                if (ElectOne()) {
+                    MbarExpectTx(bar(kQFull + slot), G::kTileBytes);
+#pragma unroll
+                    for (int kb = 0; kb < G::kBlocks; ++kb) {
+                        TmaLoad4D(q_smem + slot * G::kTileBytes + kb * (kColumns * 128), &map_q, bar(kQFull + slot), kb * 64, head_of(w, tile), w.q0 + token_of(w, tile), 0);
+                    }
+                }
+                __syncwarp();
+                // a row that sees nothing has no sum: 2^-inf
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lse_ring[slot * kColumns + lane + 32 * i] = v[i] == -CUDART_INF_F ? v[i] : -v[i] * kLog2e;
+                MbarArrive(bar(kQFull + slot));
+            }
         }
-    } else if (warp == 5) {
+    } else if (warp == kMmaWarp) {
         // ---- products ----
         if (ElectOne()) {
             constexpr uint32_t fmt = std::is_same<T, __half>::value ? kFmtF16 : kFmtBf16;
             constexpr uint32_t idesc = MakeInstrDesc(fmt, fmt, 0, 0, kKeys, kColumns);
             const uint64_t major = MakeSmemDesc(0, 16, 1024);  // both K-major
-            const uint64_t a0 = major | ((k_smem & 0x3FFFFu) >> 4);
-            ok = MbarWait(bar(kKFull), 0, abort_flag);
-            for (int tile = 0; tile < tiles && ok; ++tile) {
-                const int slot = tile % G::kSlots, buffer = tile % kBuffers;
-                ok = MbarWait(bar(kQFull + slot), (tile / G::kSlots) & 1u, abort_flag) &&
-                     MbarWait(bar(kSEmpty + buffer), ((tile / kBuffers) & 1u) ^ 1u, abort_flag);
-                if (!ok) break;
-                TcFenceAfter();
-                const uint64_t b0 = major | (((q_smem + slot * G::kTileBytes) & 0x3FFFFu) >> 4);
+            uint32_t items = 0, count = 0;
+            Look next = look(0);
+            for (int r = 0; r < rounds && ok; ++r) {
+                const Item w = item_of(next);
+                next = look(r + 1);
+                if (w.tiles == 0) continue;
+                const uint32_t k_slot = items % G::kKeySlots;
+                const uint64_t a0 = major | (((k_smem + k_slot * G::kTileBytes) & 0x3FFFFu) >> 4);
+                ok = MbarWait(bar(kKFull + k_slot), (items / G::kKeySlots) & 1u, abort_flag);
+                ++items;
+                for (int tile = 0; tile < w.tiles && ok; ++tile, ++count) {
+                    const uint32_t slot = count % G::kSlots, buffer = count % kBuffers;
+                    ok = MbarWait(bar(kQFull + slot), (count / G::kSlots) & 1u, abort_flag) && MbarWait(bar(kSEmpty + buffer), ((count / kBuffers) & 1u) ^ 1u, abort_flag);
+                    if (!ok) break;
+                    TcFenceAfter();
+                    const uint64_t b0 = major | (((q_smem + slot * G::kTileBytes) & 0x3FFFFu) >> 4);
 #pragma unroll
-                for (int ks = 0; ks < DP / 16; ++ks) {
-                    const uint32_t at = ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32) >> 4;
-                    if (ks == 0) MmaSS<false>(tmem + buffer * kColumns, a0 + at, b0 + at, idesc);
-                    else MmaSS<true>(tmem + buffer * kColumns, a0 + at, b0 + at, idesc);
+                    for (int ks = 0; ks < DP / 16; ++ks) {
+                        const uint32_t at = ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32) >> 4;
+                        if (ks == 0) MmaSS<false>(tmem + buffer * kColumns, a0 + at, b0 + at, idesc);
+                        else MmaSS<true>(tmem + buffer * kColumns, a0 + at, b0 + at, idesc);
+                    }
+                    MmaCommit(bar(kQEmpty + slot));
+                    MmaCommit(bar(kSFull + buffer));
                 }
-                MmaCommit(bar(kQEmpty + slot));
-                MmaCommit(bar(kSFull + buffer));
+                if (ok) MmaCommit(bar(kKEmpty + k_slot));
             }
         }
     } else {
         // ---- sums ----
-        const int key = key0 + 32 * warp + lane;
-        const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
-        // a column that the key is visible to and that counts: [first, end) below; the same in every tile but the first and last tokens'
-        const int sees_from = p.causal ? key - diagonal : 0;  // first token that sees the key
-        float sum = 0.0f;
-        for (int tile = 0; tile < tiles && ok; ++tile) {
-            const int slot = tile % G::kSlots, buffer = tile % kBuffers;
-            ok = __all_sync(0xffffffffu, MbarWait(bar(kSFull + buffer), (tile / kBuffers) & 1u, abort_flag) &&
-                                             MbarWait(bar(kQFull + slot), (tile / G::kSlots) & 1u, abort_flag));
-            if (!ok) break;
-            TcFenceAfter();
-            const int token0 = token_of(tile);
-            const int first = max(sees_from - token0, 0) << p.pack_shift, end = min(new_tokens - token0, tile_tokens) << p.pack_shift;
-            const bool ragged = first > 0 || end < kColumns;
-            const float4* lse = reinterpret_cast<const float4*>(lse_ring + slot * kColumns);
-            const float2 scale = make_float2(p.scale_log2, p.scale_log2);
-            float2 acc[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t sc[2][32];
-                TmemLd32(tmem + lanes + buffer * kColumns + half * 64, sc[0]);
-                TmemLd32(tmem + lanes + buffer * kColumns + half * 64 + 32, sc[1]);
-                TmemWaitLd();
-                if (half == 1) {
-                    TcFenceBefore();
-                    __syncwarp();
-                    if (lane == 0) MbarArrive(bar(kSEmpty + buffer));
+        const int mine = warp / kGroupWarps, half = warp / 4 % 2, row = 32 * (warp & 3) + lane;
+        const uint32_t scores = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + half * 64;
+        float* sums = reinterpret_cast<float*>(smem + G::kSums);
+        const float2 scale = make_float2(p.scale_log2, p.scale_log2);
+        uint32_t count = 0, items = 0;  // tiles before this item
+        Look next = look(0);
+        for (int r = 0; r < rounds && ok; ++r) {
+            const Item w = item_of(next);
+            next = look(r + 1);
+            if (w.tiles == 0) continue;
+            const int key = w.key0 + row;
+            float* weight = nullptr;  // the threads of the first four warps add up and store
+            float before = 0.0f;
+            if (warp < 4 && key < w.keys) {
+                const int32_t id = p.page_table[static_cast<int64_t>(w.seq) * p.max_blocks + (key >> p.block_shift)];
+                if (id >= 0 && id < p.num_blocks) {
+                    weight = p.weights + (static_cast<int64_t>(w.seq) * p.kv_heads + w.head_kv) * p.weights_row + key;
+                    before = *weight;
                 }
-                if (ragged) {
+            }
+            const int sees_from = p.causal ? key - w.diagonal : 0;  // first token that sees the key
+            float sum = 0.0f;
+            for (int tile = static_cast<int>((count ^ mine) & 1u); tile < w.tiles && ok; tile += kGroups) {
+                const uint32_t n = count + tile, slot = n % G::kSlots, buffer = n % kBuffers;
+                ok = __all_sync(0xffffffffu, MbarWait(bar(kSFull + buffer), (n / kBuffers) & 1u, abort_flag) && MbarWait(bar(kQFull + slot), (n / G::kSlots) & 1u, abort_flag));
+                if (!ok) break;
+                TcFenceAfter();
+                // columns [first, end) of this half count and see the key
+                const int token0 = token_of(w, tile);
+                const int first = (max(sees_from - token0, 0) << p.pack_shift) - half * 64, end = (min(w.new_tokens - token0, tile_tokens) << p.pack_shift) - half * 64;
+                const float4* lse = reinterpret_cast<const float4*>(lse_ring + slot * kColumns + half * 64);
+                uint32_t sc[2][32];
+                TmemLd32(scores + buffer * kColumns, sc[0]);
+                TmemLd32(scores + buffer * kColumns + 32, sc[1]);
+                TmemWaitLd();
+                TcFenceBefore();
+                __syncwarp();
+                if (lane == 0) MbarArrive(bar(kSEmpty + buffer));
+                if (first > 0 || end < 64) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        const int c0 = half * 64 + b * 32;
+                        const int c0 = b * 32;
                         const uint32_t below_end = end - c0 >= 32 ? 0xffffffffu : end <= c0 ? 0u : (1u << (end - c0)) - 1u;
                         const uint32_t below_first = first - c0 >= 32 ? 0xffffffffu : first <= c0 ? 0u : (1u << (first - c0)) - 1u;
                         const uint32_t visible = below_end & ~below_first;
@@ -224,32 +315,37 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
                         }
                     }
                 }
+                float2 acc[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        const float4 l = lse[half * 16 + b * 8 + i / 4];
+                        const float4 l = lse[b * 8 + i / 4];
                         const float2 x = Fma2(make_float2(__uint_as_float(sc[b][i]), __uint_as_float(sc[b][i + 1])), scale, make_float2(l.x, l.y));
                         const float2 y = Fma2(make_float2(__uint_as_float(sc[b][i + 2]), __uint_as_float(sc[b][i + 3])), scale, make_float2(l.z, l.w));
                         acc[(i / 4) % 2 * 2] = Add2(acc[(i / 4) % 2 * 2], make_float2(Exp2(x.x), Exp2(x.y)));
                         acc[(i / 4) % 2 * 2 + 1] = Add2(acc[(i / 4) % 2 * 2 + 1], make_float2(Exp2(y.x), Exp2(y.y)));
                     }
                 }
+                __syncwarp();
+                if (lane == 0) MbarArrive(bar(kQEmpty + slot));
+                sum += ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) + ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
             }
-            __syncwarp();
-            if (lane == 0) MbarArrive(bar(kQEmpty + slot));
-            sum += ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) + ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
-        }
-        if (ok && key < keys) {
-            const int32_t id = table[key >> p.block_shift];
-            if (id >= 0 && id < p.num_blocks) p.weights[(static_cast<int64_t>(seq) * p.kv_heads + head_kv) * p.weights_row + key] += sum;
+            count += w.tiles;
+            // Items take turns with two sets of sums: the next barrier is behind the reads of this set.
+            float* set = sums + (items++ & 1u) * (2 * kGroups * kKeys) + row;
+            set[(2 * mine + half) * kKeys] = sum;
+            ok = AllSumWarps(ok);  // one that gave up takes all along: none may wait here for one that has left
+            if (weight != nullptr && ok) *weight = before + ((set[0] + set[kKeys]) + (set[2 * kKeys] + set[3 * kKeys]));
         }
     }
     if (!ok && p.error_word != nullptr) *p.error_word = 1 + warp;
     __syncwarp();
     TcFenceBefore();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == kMmaWarp) {
         __syncwarp();
         TcFenceAfter();
         TmemDealloc(tmem, kBuffers * kColumns);
@@ -257,7 +353,7 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 }
 
 template <typename T, int DP>
-int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, int64_t most_keys, cudaStream_t stream) {
+int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, cudaStream_t stream) {
     using G = WeightsGeom<DP>;
     CUtensorMap map_q, map_k;
     const int64_t rows = x.num_blocks * x.block_size, row = x.num_kv_heads * x.head_dim;
@@ -266,27 +362,15 @@ int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, int64_t most_keys
     if (int rc = MakeRowsMap(&map_k, x.k_pool, x.dtype_id, x.head_dim, rows, x.num_kv_heads, row, x.head_dim, static_cast<int>(x.block_size), 1, "k pool")) return rc;
     auto kernel = chunk_weights_kernel<T, DP>;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), G::kSmemBytes, "chunk_weights_kernel")) return rc;
-    // the tiles of the first keys, which most tokens see, go first
-    const dim3 grid(static_cast<unsigned>(x.num_seqs * x.num_kv_heads), static_cast<unsigned>((most_keys + kKeys - 1) / kKeys));
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(kWeightThreads);
-    cfg.dynamicSmemBytes = G::kSmemBytes;
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, map_q, map_k, p);
+    LaunchDependent(kernel, std::min(p.items, SmCount()), kWeightThreads, G::kSmemBytes, stream, 1, map_q, map_k, p);
     return CheckFlashLaunch(stream);
 }
 
 template <typename T>
-int LaunchTyped(const ScaFlashPagedParams& x, const ChunkParams& p, int64_t most_keys, cudaStream_t stream) {
-    if (x.head_dim <= 64) return Launch<T, 64>(x, p, most_keys, stream);
-    if (x.head_dim <= 128) return Launch<T, 128>(x, p, most_keys, stream);
-    return Launch<T, 256>(x, p, most_keys, stream);
+int LaunchTyped(const ScaFlashPagedParams& x, const ChunkParams& p, cudaStream_t stream) {
+    if (x.head_dim <= 64) return Launch<T, 64>(x, p, stream);
+    if (x.head_dim <= 128) return Launch<T, 128>(x, p, stream);
+    return Launch<T, 256>(x, p, stream);
 }
 
 }  // namespace
@@ -314,7 +398,11 @@ int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, c
     p.scale_log2 = x.scale * kLog2e;
     int64_t most_keys = 0;
     for (int64_t i = 0; i < x.num_seqs; ++i) most_keys = most_keys < x.seq_lens_kv[i] ? x.seq_lens_kv[i] : most_keys;
-    return x.dtype_id == SCA_DTYPE_F16 ? LaunchTyped<__half>(x, p, most_keys, stream) : LaunchTyped<__nv_bfloat16>(x, p, most_keys, stream);
+    const int64_t units = x.num_seqs * x.num_kv_heads, items = units * ((most_keys + kKeys - 1) / kKeys);
+    if (items > 0x7fffffffLL) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): " + std::to_string(items) + " tiles of keys are out of range");
+    p.units = static_cast<int>(units);
+    p.items = static_cast<int>(items);
+    return x.dtype_id == SCA_DTYPE_F16 ? LaunchTyped<__half>(x, p, stream) : LaunchTyped<__nv_bfloat16>(x, p, stream);
 }
 
 }  // namespace flash
