@@ -14,6 +14,8 @@
 // Free places and rows that move are listed by rank in scratch, then all CTAs copy. No free place is the source of a move, so that these
 // copies need no order. The last tokens move down behind them, all rows of a wave read before the first one of it is written: the
 // destination of a row is never behind its source, so that later waves read what no earlier one has written.
+// Bound by memory where there are many sequences: 192 of 500 to 6000 tokens, 8 kv heads, D=128, down to 2000: 246 us, 5.2 TB/s. One sequence is
+// a chain of phases: of 100 thousand tokens 49 us, of which 19 are the copies, 16 the digits, 9 the lists; of 1100 13 us.
 // Algorithmic traffic: 8 bytes a token and kv head of weights, and 4 * row bytes a moved row (K and V, read and written).
 #include <algorithm>
 #include <type_traits>
@@ -30,8 +32,9 @@ constexpr int kBins = 256;
 static_assert(kBins == kEvictThreads, "a bin to a thread");
 constexpr int kEvictCluster = 16;  // CTAs to a (sequence, kv head) at most
 constexpr int kEvictCtas = 4;      // CTAs to an SM at least
+// Pieces that a thread has on their way at once; 16, with registers for one CTA to an SM, take 53.7 us for 49.2 (100 thousand tokens).
+constexpr int kHeld = 8;
 constexpr int kLoads = 8;          // weights that a thread has on their way at once
-constexpr int kHeld = 8;           // pieces that a thread has on their way at once
 
 struct EvictParams {
     void *k, *v;
@@ -85,20 +88,21 @@ kv_evict_kernel(const EvictParams p) {
     const int32_t* table = p.page_table + seq * p.max_blocks;
     int moves = 0;
 
-    if (stay > 0) {
+    const int slice = (between + cluster - 1) / cluster;
+    const int begin = first + min(rank * slice, between), count = first + min((rank + 1) * slice, between) - begin;
+    auto select = [&](auto all_cached) {
+        constexpr bool kAllCached = decltype(all_cached)::value;  // a look at every key costs half of the phases' time otherwise
         // ---- the stay-th largest key -------------------------------------------------------------------------
-        const int slice = (between + cluster - 1) / cluster;
-        const int begin = first + min(rank * slice, between), count = first + min((rank + 1) * slice, between) - begin;
         for (int i = threadIdx.x; i < kDigits * kBins; i += kEvictThreads) smem[i] = 0;
         __syncthreads();
-        auto key_at = [&](int i) { return i < p.cached ? cache[i] : KeyOf(w[begin + i]); };
-        uint32_t prefix = 0, need = static_cast<uint32_t>(stay), equal = 0;
+        auto key_at = [&](int i) { return kAllCached || i < p.cached ? cache[i] : KeyOf(w[begin + i]); };
+        uint32_t prefix = 0, border = 0, need = static_cast<uint32_t>(stay), equal = 0;
 #pragma unroll
         for (int digit = 0; digit < kDigits; ++digit) {
             const int shift = 24 - 8 * digit;
             if (digit == 0) {
                 // Few values are possible here, a sign and seven bits of exponent, but a warp that adds up equal ones by itself (__match_any_sync)
-                // is slower: 100 thousand tokens, one CTA, 814 us for 779.
+                // is slower: 100 thousand tokens, one CTA, 817 us for 780.
                 for (int i0 = 0; i0 < count; i0 += kLoads * kEvictThreads) {
                     float x[kLoads];
 #pragma unroll
@@ -155,8 +159,10 @@ kv_evict_kernel(const EvictParams p) {
             prefix = (prefix << 8) | s_found[digit & 1][0];
             need -= s_found[digit & 1][1];
             equal = s_found[digit & 1][2];
+            border = prefix << shift;
+            if (equal == need) break;  // all keys that begin like this stay
         }
-        const uint32_t border = prefix;  // keys above it stay, and `need` of those equal to it, the lowest places first
+        // keys above the border stay, and `need` of those equal to it, the lowest places first
         // ---- ranks: every warp walks a piece of the slice --------------------------------------------------------
         const int piece = ((count + kEvictWarps - 1) / kEvictWarps + 31) / 32 * 32;
         const int piece_begin = min(warp * piece, count), piece_end = min(piece_begin + piece, count);
@@ -234,6 +240,10 @@ kv_evict_kernel(const EvictParams p) {
             late_rank += __popc(late_lanes);
         });
         ClusterBarrier();
+    };
+    if (stay > 0) {
+        if (count <= p.cached) select(std::true_type{});
+        else select(std::false_type{});
     }
 
     // ---- copies: a warp looks up as many moves as it has lanes, one each, and copies their rows together ---------------
@@ -343,11 +353,11 @@ int LaunchEvict(const EvictParams& p, int64_t units, cudaStream_t stream) {
 
 // CTAs to a (sequence, kv head). More of them shorten the chain of phases of a long one and cost barriers in a short one; up to 8 as long as
 // all CTAs are resident (4 to an SM), 16 where that leaves one to an SM. us for 8 kv heads, D=128, 16 bits, 1 / 2 / 4 / 8 / 16 CTAs:
-//   one sequence of 1100 tokens down to 1024   14.4 / 15.8 / 15.2 / 15.4 / 21.9     4 of 8192 to 4096    107 / 62 / 38 / 32 / 56
-//   of 2200 to 1024                            34.7 / 28.1 / 18.9 / 17.3 / 21.7     8 of 16000 to 4000   167 / 94 / 65 / 66 / 108
-//   of 8192 to 4096                            90.7 / 52.7 / 32.4 / 23.6 / 25.1     16 of 4096 to 2048    67 / 50 / 47 / 63 / 135
-//   of 16000 to 8000                            178 / 95 / 53 / 34.5 / 30.8         32 of 8192 to 4096   147 / 145 / 141 / 169 / 287
-//   of 33000 to 4000                            265 / 103 / 60 / 38.3 / 32.4        64 of 2200 to 1024    83 / 96 / 112 / 186 / 442
+//   one sequence of 1100 tokens down to 1024   12.5 / 13.6 / 13.4 / 13.7 / 17.7     4 of 8192 to 4096    101 / 58 / 35 / 30 / 49
+//   of 2200 to 1024                            32.4 / 26.1 / 16.8 / 15.4 / 18.1     8 of 16000 to 4000   160 / 89 / 60 / 61 / 95
+//   of 8192 to 4096                            85.6 / 48.8 / 30.0 / 21.8 / 22.2     16 of 4096 to 2048    62 / 46 / 44 / 56 / 115
+//   of 16000 to 8000                            168 / 90 / 50 / 31.6 / 26.9         32 of 8192 to 4096   142 / 138 / 133 / 154 / 254
+//   of 33000 to 4000                            248 / 91 / 53 / 33.8 / 28.2         64 of 2200 to 1024    80 / 90 / 101 / 161 / 367
 int ClusterFor(int64_t units, int64_t capacity) {
     if (units * 16 <= SmCount() && capacity >= 12000) return 16;
     int cluster = 8;
