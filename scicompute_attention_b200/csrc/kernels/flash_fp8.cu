@@ -16,7 +16,7 @@ namespace {
 template <typename T, int DP, int QT, int BN, bool kSplit>
 int Launch(int64_t ctas, int cluster, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
            const FlashKernelParams& p, const WorkImage& image) {
-    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, true, true, true, kSplit>;
+    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, true, true, true, false, kSplit>;
     constexpr int kSmem = FlashGeom<DP, QT, BN, true>::kSmemBytes;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kSmem, "flash_fwd_sm100_kernel")) return rc;
     constexpr int kThreads = FlashThreads<T, DP, QT, true>();

@@ -418,7 +418,7 @@ __device__ __forceinline__ bool ProduceRaw(const FlashKernelParams& p, const CUt
 // queries after HalveQueryRow.
 // kShared (only with kPaged): decode of groups of sequences over the pages they have in common. The query tokens of a group are a "sequence" of
 // the list, an item takes a part of its keys, and what it leaves is that part of every row, not an output (flash_shared.cu).
-template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kKv8 = false, bool kSplit = false, bool kShared = false>
+template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kKv8 = false, bool kShared = false, bool kSplit = false>
 __global__ void __launch_bounds__(FlashThreads<T, DP, QT, kKv8>(), 1)
 flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p, const __grid_constant__ WorkParam<TakesWorkImage(DP, kKv8, kSplit), kShared> image) {

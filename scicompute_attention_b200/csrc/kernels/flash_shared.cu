@@ -58,7 +58,7 @@ int Launch(const ScaDecodeFwdParams& d, const PrefixGroups& groups, const Prefix
     const int64_t items = static_cast<int64_t>(p.num_entries) * (p.heads >> pack_shift);
     if (items > 0x7fffffffLL) return Fail(SCA_INVALID_ARGUMENT, "shared prefix: grid of " + std::to_string(items) + " blocks is out of range");
     SharedImage image{groups, parts, d.seq_lens};
-    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, kTileKeys, true, true, false, false, true>;
+    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, kTileKeys, true, true, false, true>;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), G::kSmemBytes, "flash_fwd_sm100_kernel")) return rc;
     LaunchDependent(kernel, std::min<int64_t>(items, SmCount()), FlashThreads<T, DP, QT>(), G::kSmemBytes, stream, 1, map_q, map_k, map_v, p, image);
     return CheckFlashLaunch(stream);
@@ -79,7 +79,11 @@ int LaunchPrefixParts(const ScaDecodeFwdParams& p, const PrefixGroups& groups, c
 }
 
 // Parts that fill the SMs: with more of them an SM has fewer tiles to walk, but each costs its start, 4 bytes a number and row for its O, and
-// its share of the merge. The cost of an item is its tiles and three more.
+// its share of the merge. The cost of an item is its tiles and three more, that of a part in the merge half a tile. us of a call by the tiles of a
+// part (32 / 8 heads, D=128; taken: 5, 8, 21):
+//   32 sequences, prefix of 4000    2: 26.5  3: 27.3  4: 23.7  5: 24.0  6: 25.2  8: 28.4  16: 42
+//   128, 8100, 20 to 1500 of their own   4: 121  6: 119  7: 110.5  8: 109.2  9: 109.1  12: 111  16: 117  32: 145
+//   300, 8000                       4: 143  6: 126  8: 126.5  9: 116.2  10: 120  16: 129  21: 116.8  32: 138
 void PlanPrefixParts(const ScaDecodeFwdParams& p, PrefixGroups* groups) {
     const int pack_shift = flash::PackShift(p.num_heads / p.num_kv_heads);
     const int64_t packed_heads = p.num_heads >> pack_shift;
@@ -91,7 +95,7 @@ void PlanPrefixParts(const ScaDecodeFwdParams& p, PrefixGroups* groups) {
         const int tiles = (x.tokens + flash::kTileKeys - 1) / flash::kTileKeys;
         return static_cast<int64_t>((x.end - x.first + item_tokens - 1) / item_tokens) * ((tiles + part_tiles - 1) / part_tiles);
     };
-    int64_t best = 0;
+    double best = 0.0;
     int last = 0;
     for (int parts = 1; parts <= 32 && parts <= longest; ++parts) {
         const int part_tiles = (longest + parts - 1) / parts;
@@ -99,12 +103,11 @@ void PlanPrefixParts(const ScaDecodeFwdParams& p, PrefixGroups* groups) {
         last = part_tiles;
         int64_t items = 0;
         for (int g = 0; g < groups->count; ++g) items += items_of(groups->group[g], part_tiles);
-        const int64_t rounds = (items * packed_heads + sms - 1) / sms, cost = rounds * (part_tiles + 3);
+        const double rounds = static_cast<double>((items * packed_heads + sms - 1) / sms), cost = rounds * (part_tiles + 3) + 0.5 * parts;
         if (groups->part_tiles == 0 || cost < best) {
             best = cost;
             groups->part_tiles = part_tiles;
         }
-        if (rounds > 1 && parts > 4) break;
     }
     groups->parts = (longest + groups->part_tiles - 1) / groups->part_tiles;
     int64_t entries = 0;

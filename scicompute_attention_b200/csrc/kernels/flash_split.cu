@@ -9,7 +9,7 @@ template <typename T, int DP, int QT, int BN>
 int ResidentClusters(int cluster) {
     static PerDevice resident[kMaxSplit + 1];  // per instantiation
     const int n = resident[cluster].Get([cluster] {
-        auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, false, false, false, true>;
+        auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, false, false, false, false, true>;
         // the query answers for the shared memory the kernel is allowed at that point
         if (EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), FlashGeom<DP, QT, BN>::kSmemBytes, "flash_fwd_sm100_kernel") != SCA_OK) return -1;
         cudaLaunchAttribute attr{};
@@ -36,7 +36,7 @@ int ResidentClusters(int cluster) {
 template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged>
 int LaunchSplit(int64_t items, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
                 const FlashKernelParams& p) {
-    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, kVarlen, kPaged, false, true>;
+    auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, kVarlen, kPaged, false, false, true>;
     constexpr int kSmem = FlashGeom<DP, QT, BN>::kSmemBytes;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kSmem, "flash_fwd_sm100_kernel")) return rc;
     LaunchDependent(kernel, items * p.cluster, FlashThreads<T, DP, QT>(), kSmem, stream, p.cluster, map_q, map_k, map_v, p, NoWorkImage{});

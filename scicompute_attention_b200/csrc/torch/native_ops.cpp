@@ -652,7 +652,7 @@ PyObject* PagedStep(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if ((a[4] != Py_None && (lens = Plain(a[4])) == nullptr) || (a[7] != Py_None && (weights = Plain(a[7])) == nullptr)) return NotTaken();
         HostInts cu, prefix;
         if (a[5] != Py_None) {
-            if (!cu.Take(a[5]) || !prefix.Take(a[6]) || cu.size() != prefix.size() + 1) return NotTaken();
+            if (!cu.Take(a[5]) || !prefix.Take(a[6]) || cu.size() < 2 || cu.size() != prefix.size() + 1) return NotTaken();
             x.cu_groups = cu.data(), x.prefix_lens = prefix.data(), x.num_groups = prefix.size();
         }
         if (!q || !k || !v || !table || q->dim() != 4 || q->size(0) < 1 || q->size(2) != 1 || k->dim() != 4 || k->size(1) != block_size || k->size(3) != q->size(3) ||

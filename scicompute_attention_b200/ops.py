@@ -988,6 +988,8 @@ def _paged_step(q, k_pool, v_pool, page_table, seq_lens, cu_groups, prefix_lens,
     _require_table(page_table, s)
     if seq_lens is not None:
         _require_ints("seq_lens", seq_lens, s)
+    if cu_groups is not None and (cu_groups[0] != 0 or cu_groups[-1] != s):
+        raise _lib.ScaError(4, f"cu_groups must go from 0 to num_seqs={s}")
     max_blocks = page_table.shape[1]
     tensors = [k_pool, v_pool, page_table] + ([seq_lens] if seq_lens is not None else [])
     if weights is not None:
@@ -1056,7 +1058,7 @@ def paged_attention_shared(q, k_pool, v_pool, page_table, seq_lens, cu_groups, p
         if out is not None:
             return out
     cu, lens = _host_ints("cu_groups", cu_groups), _host_ints("prefix_lens", prefix_lens)
-    if cu.shape[0] != lens.shape[0] + 1:
+    if cu.shape[0] < 1 or cu.shape[0] != lens.shape[0] + 1:
         raise _lib.ScaError(4, "cu_groups needs num_groups + 1 entries, prefix_lens num_groups")
     return _paged_step(q, k_pool, v_pool, page_table, seq_lens, cu, lens, weights, block_size, scale, typical_len, longest_len, stream)
 
@@ -1067,7 +1069,8 @@ def flash_attention_paged_weights(q, k_pool, v_pool, page_table, cu_seqlens_q, s
     the sum is fixed: the same call gives the same bits. With `last` > 0 the last so many new tokens of each sequence count, with 0 all of them.
 
     q, pools, table and the lists on the host as flash_attention_paged takes them, of float16 or bfloat16; weights float32 [num_seqs, H_kv,
-    max_blocks_per_seq * block_size] or more rows and columns, on the device. A query of NaN makes the weights it counts for NaN."""
+    max_blocks_per_seq * block_size] or more rows and columns, on the device. A query of NaN makes the weights it counts for NaN. As there, a sequence's last page is
+    read whole: what it holds behind the last token counts for nothing, but must be finite in V."""
     if stream is None:
         out = _native().chunk_weights(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_kv, weights, causal, scale, last)
         if out is not None:
@@ -1110,7 +1113,7 @@ def flash_attention_paged_weights(q, k_pool, v_pool, page_table, cu_seqlens_q, s
     p.causal = 1 if causal else 0
     p.dtype_id = dtype_id(q.dtype)
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-    w = _lib.ChunkWeights(lse.data_ptr(), weights.data_ptr(), weights.shape[2], last)
+    w = _lib.ChunkWeights(lse.data_ptr(), weights.data_ptr(), weights.shape[2], int(last))
     check(lib().sca_launch_flash_paged_weights(C.byref(p), C.byref(w), _stream_ptr(stream)))
     return out
 
@@ -1146,6 +1149,7 @@ def kv_evict(layer_k, layer_v, weights, page_table, seq_lens, *, keep: int, rece
     if by_sequence:
         _require_ints("first", first, n)
         tensors.append(first)
+    keep, recent, first = int(keep), int(recent), first if by_sequence else int(first)
     if keep < 0 or recent < 0 or (not by_sequence and first < 0):
         raise _lib.ScaError(4, f"keep={keep}, recent={recent} and first must not be negative")
     _require_one_device(layer_k, *tensors)

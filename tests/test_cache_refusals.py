@@ -36,7 +36,8 @@ def _calls(dev):
              ("weights of 16 bits", step(w=weights.half())), ("weights too narrow", step(w=narrow)), ("few rows of weights", step(w=weights[:1])),
              ("weights of other heads", step(w=t(B, HQ, W * BS, dtype=torch.float32))), ("weights turned", step(w=t(B, W * BS, HKV, dtype=torch.float32).transpose(1, 2))),
              ("shared, few offsets", shared(c=cu[:1])), ("shared, offsets of two dims", shared(c=cu[None])), ("shared, offsets of floats", shared(c=np.array([0.0, 2.0]))),
-             ("shared, beyond 32 bits", shared(p=np.array([1 << 40]))), ("shared, weights too narrow", shared(w=narrow)), ("shared, head dims", shared(k=other)),
+             ("shared, offsets that end early", shared(c=np.array([0, 1], np.int32))), ("shared, no groups for two sequences", shared(c=np.array([0]), p=np.array([], np.int32))),
+             ("shared, offsets of a tensor that begin late", shared(c=torch.tensor([1, 2]))), ("shared, beyond 32 bits", shared(p=np.array([1 << 40]))), ("shared, weights too narrow", shared(w=narrow)), ("shared, head dims", shared(k=other)),
              ("chunk, fp32", chunk(q_=q.float(), k=pool.float(), v=pool.float())), ("chunk, q of four dims", chunk(q_=q1)), ("chunk, q strided", chunk(q_=t(9, 2 * HQ, D)[:, ::2])),
              ("chunk, head dims", chunk(k=other, v=other)), ("chunk, pools differ", chunk(v=other)), ("chunk, few offsets", chunk(c=new[:2])),
              ("chunk, table sliced", chunk(tab=ints(B, 9)[:, :W])), ("chunk, few table rows", chunk(tab=table[:1])), ("chunk, weights too narrow", chunk(w=narrow)),

@@ -59,6 +59,11 @@ def test_groups_and_pages(groups, own, bs):
     _run(b, cu, prefix, True, typical_len=int(b.lens_host.mean()), longest_len=int(b.lens_host.max()))
 
 
+def test_as_many_groups_as_a_call_takes():
+    b, cu, prefix = _batch([(2, 16 + i % 5) for i in range(128)] + [(1, 40)] * 7 + [(3, 5)], [3, 1])  # the last ones share no page
+    _run(b, cu, prefix, True)
+
+
 def test_sequences_that_end_with_the_prefix():
     b, cu, prefix = _batch([(6, 256)], [0])
     _run(b, cu, prefix, True)
@@ -118,6 +123,16 @@ def test_captured_and_on_another_stream():
         w2.copy_(w0)
         graph.replay()
         assert torch.equal(got, want) and torch.equal(w2, b.weights)
+
+
+def test_numbers_of_other_types():
+    from scicompute_attention_b200 import ops
+    b, cu, prefix = _batch([(3, 100)], [20])
+    run = lambda t, n: ops.paged_attention_shared(b.q, b.k, b.v, b.table, b.lens, cu, prefix, block_size=b.bs, typical_len=t, longest_len=n)
+    assert torch.equal(run(110, 200), run(np.int64(110), np.int32(200)))
+    w = [b.weights.clone() for _ in range(2)]
+    evict = lambda w, f: ops.kv_evict(b.k.clone(), b.v.clone(), w, b.table, b.lens, keep=f(110), recent=f(3), first=f(96))
+    assert torch.equal(evict(w[0], int), evict(w[1], np.int64)) and torch.equal(*w)
 
 
 def test_back_to_back_calls_on_one_stream():
