@@ -8,6 +8,13 @@
 //                   in the order of the heads: no atomics, the same bits every time.
 // The scores are stored and not computed again: K once more would be half of the traffic (D=128, 4 heads to a kv head: 256 bytes a token and
 // kv head against 32 written and read), and nobody knows M and L before the last key.
+// A call that does not fill the machine runs in one launch, decode_step_cluster_kernel.
+// Bound by memory. 192 sequences of 500 to 6000 tokens, 32 / 8 heads, D=128, bf16: 439 us for 2.6 GB, 389 without weights. Of the 50 us the stores of
+// 80 MB of scores in the stream of loads cost 33, reading them back and adding 19. 96 of 200 to 6001, 32 / 2 heads, D=64, fp16: 53 us, 41.5
+// without. One of 701 tokens 7.6 us in one launch, 11.1 in two.
+// K and V go through the cache as what is given up first, so that the scores stay: the 96 sequences 56.0 / 52.6 us without / with it; with more scores
+// than the cache holds it makes no difference. Adding the weights of whole sequences in the partial kernel, from a scratch of 128 KB a CTA, saved
+// 2 % of the 192 sequences and cost the 96 a fifth: registers.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

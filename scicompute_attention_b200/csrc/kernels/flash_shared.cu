@@ -4,6 +4,9 @@
 // An item is 256 rows (one token of up to 16 query heads of a kv head, as many sequences as fill it up) against `part_tiles` tiles of 128
 // keys of the prefix. It leaves {m, l, O} of each of its rows in fp32; the finish kernel of decode_weights.cu merges them with the parts of
 // the sequence's own tokens.
+// Bound by the chain of a tile's scores, softmax and products where a prefix is long and many share it, 128 sequences behind 8100 tokens (32 / 8 heads,
+// D=128): 32 us, 550 TFLOP/s, of which 4 are the O of 9 parts in fp32. 14 groups of 4 to 12 behind 300 to 4000 tokens, 123 MB: 39 us; a quarter of
+// the rows are filled, and a step of one tile takes 1.8 us whatever it holds.
 #include <algorithm>
 
 #include "flash_kernel.cuh"
