@@ -20,7 +20,7 @@ int Launch(int64_t ctas, int cluster, cudaStream_t stream, const CUtensorMap& ma
     constexpr int kSmem = FlashGeom<DP, QT, BN, true>::kSmemBytes;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kSmem, "flash_fwd_sm100_kernel")) return rc;
     constexpr int kThreads = FlashThreads<T, DP, QT, true>();
-    if constexpr (TakesWorkImage(DP, true, kSplit)) LaunchDependent(kernel, ctas, kThreads, kSmem, stream, cluster, map_q, map_k, map_v, p, image);
+    if constexpr (TakesWorkImage(DP, true, kSplit, true)) LaunchDependent(kernel, ctas, kThreads, kSmem, stream, cluster, map_q, map_k, map_v, p, image);
     else LaunchDependent(kernel, ctas, kThreads, kSmem, stream, cluster, map_q, map_k, map_v, p, NoWorkImage{});
     return SCA_OK;
 }

@@ -358,7 +358,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
     }
     p.cluster = tiles_per_item == 1 ? SplitCluster<T, DP, QT, BN>(ctas, (most_keys + BN - 1) / BN) : 1;
     if (varlen != nullptr) {
-        const bool taken = TakesWorkImage(DP, paged != nullptr && paged->k_scales != nullptr, p.cluster > 1);
+        const bool taken = TakesWorkImage(DP, paged != nullptr && paged->k_scales != nullptr, p.cluster > 1, paged != nullptr);
         if (int rc = UploadVarlenWork(*varlen, item_tokens, BN, f.causal != 0, stream, &p.seqs, &p.entries, taken ? &small : nullptr)) return rc;
     }
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, SmCount()));  // one persistent CTA per SM
@@ -378,7 +378,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
             return CheckFlash(stream);
         }
         if (p.cluster > 1) {
-            if (int rc = LaunchSplit<T, DP, QT, BN, true, true>(ctas, stream, map_q, map_k, map_v, p)) return rc;
+            if (int rc = LaunchSplit<T, DP, QT, BN, true, true>(ctas, stream, map_q, map_k, map_v, p, small)) return rc;
             return CheckFlash(stream);
         }
         const void* fn = reinterpret_cast<const void*>(&flash_fwd_sm100_kernel<T, DP, QT, BN, true, true>);
@@ -386,7 +386,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
         LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, true, true>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p, NoWorkImage{});
     } else if (varlen != nullptr) {
         if (p.cluster > 1) {
-            if (int rc = LaunchSplit<T, DP, QT, BN, true, false>(ctas, stream, map_q, map_k, map_v, p)) return rc;
+            if (int rc = LaunchSplit<T, DP, QT, BN, true, false>(ctas, stream, map_q, map_k, map_v, p, small)) return rc;
             return CheckFlash(stream);
         }
         const void* fn = reinterpret_cast<const void*>(&flash_fwd_sm100_kernel<T, DP, QT, BN, true>);
@@ -394,7 +394,7 @@ int LaunchFlash(const ScaFlashFwdParams& f, cudaStream_t stream, const VarlenWor
         LaunchDependent(flash_fwd_sm100_kernel<T, DP, QT, BN, true>, grid, threads, G::kSmemBytes, stream, 1, map_q, map_k, map_v, p, NoWorkImage{});
     } else {
         if (p.cluster > 1) {
-            if (int rc = LaunchSplit<T, DP, QT, BN, false, false>(ctas, stream, map_q, map_k, map_v, p)) return rc;
+            if (int rc = LaunchSplit<T, DP, QT, BN, false, false>(ctas, stream, map_q, map_k, map_v, p, small)) return rc;
             return CheckFlash(stream);
         }
         const void* fn = reinterpret_cast<const void*>(&flash_fwd_sm100_kernel<T, DP, QT, BN, false>);
@@ -647,7 +647,7 @@ extern "C" int sca_launch_flash_paged_weights(const ScaFlashPagedParams* params,
     }
     if (!std::isfinite(x.scale)) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): scale must be a positive number");
     if (int rc = LaunchPaged(params, nullptr, nullptr, stream, weights->lse)) return rc;
-    // the work list of the prefill begins with the sequences (UploadVarlenWork)
+    // where the prefill has sent its work list ahead, it begins with the sequences (UploadVarlenWork)
     return flash::LaunchChunkWeights(x, *weights, static_cast<const int4*>(x.workspace), static_cast<cudaStream_t>(stream));
 } catch (const std::exception& e) {  // host memory for the work list
     return Fail(SCA_CUDA_ERROR, std::string("flash paged (weights): on the host: ") + e.what());

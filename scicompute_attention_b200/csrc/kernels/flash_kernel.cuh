@@ -155,7 +155,8 @@ struct NoWorkImage {};
 //   5 of 300 against 900                                 fp16  39 /  37,  43 /  42   bf16  39 /  37,  45 /  40
 //   8 of 120 against 700                                 fp16 22.5 / 18.6, 22.4 / 18.6   bf16 22.5 / 18.5, 22.5 / 18.5
 // fp16 loses up to 17 % on long calls, short calls lose the copy ahead of the launch; bf16 goes either way. D=128, bf16, the 9: 235 / 220.
-constexpr bool TakesWorkImage(int padded_dim, bool kv8, bool split) { return kv8 && (padded_dim != 64 || split); }
+// Over a 16-bit cache only the paged kernels of calls that do not fill the machine: 37 tokens against 733 keys with their weights 24.6 / 20.1 us.
+constexpr bool TakesWorkImage(int padded_dim, bool kv8, bool split, bool paged) { return kv8 ? padded_dim != 64 || split : paged && split; }
 // kShared: what the launch is about (flash_shared.cu).
 struct SharedImage {
     PrefixGroups groups;
@@ -421,7 +422,7 @@ __device__ __forceinline__ bool ProduceRaw(const FlashKernelParams& p, const CUt
 template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged = false, bool kKv8 = false, bool kShared = false, bool kSplit = false>
 __global__ void __launch_bounds__(FlashThreads<T, DP, QT, kKv8>(), 1)
 flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p, const __grid_constant__ WorkParam<TakesWorkImage(DP, kKv8, kSplit), kShared> image) {
+                       const __grid_constant__ CUtensorMap map_v, const FlashKernelParams p, const __grid_constant__ WorkParam<TakesWorkImage(DP, kKv8, kSplit, kPaged), kShared> image) {
     using G = FlashGeom<DP, QT, BN, kKv8>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem_base = (SmemAddr(smem_raw) + 1023u) & ~1023u;
@@ -526,7 +527,7 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         } else if constexpr (kVarlen) {
             const int4* seqs = p.seqs;
             const int2* entries = p.entries;
-            if constexpr (TakesWorkImage(DP, kKv8, kSplit)) {
+            if constexpr (TakesWorkImage(DP, kKv8, kSplit, kPaged)) {
                 if (seqs == nullptr) {
                     seqs = reinterpret_cast<const int4*>(image.bytes);
                     entries = reinterpret_cast<const int2*>(image.bytes + image.entries_at);
@@ -1413,7 +1414,7 @@ int CheckFlashLaunch(cudaStream_t stream);
 // The kSplit kernels are compiled in flash_split.cu.
 template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged>
 int LaunchSplit(int64_t items, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
-                const FlashKernelParams& p);
+                const FlashKernelParams& p, const WorkImage& image);
 // The kernels over an 8-bit cache are compiled in flash_fp8.cu; p.cluster > 1: the CTAs of a cluster share an item.
 template <typename T, int DP, int QT, int BN>
 int LaunchKv8(int64_t items, unsigned grid, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,

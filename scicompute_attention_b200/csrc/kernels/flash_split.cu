@@ -35,22 +35,24 @@ int ResidentClusters(int cluster) {
 
 template <typename T, int DP, int QT, int BN, bool kVarlen, bool kPaged>
 int LaunchSplit(int64_t items, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
-                const FlashKernelParams& p) {
+                const FlashKernelParams& p, const WorkImage& image) {
     auto kernel = flash_fwd_sm100_kernel<T, DP, QT, BN, kVarlen, kPaged, false, false, true>;
     constexpr int kSmem = FlashGeom<DP, QT, BN>::kSmemBytes;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), kSmem, "flash_fwd_sm100_kernel")) return rc;
-    LaunchDependent(kernel, items * p.cluster, FlashThreads<T, DP, QT>(), kSmem, stream, p.cluster, map_q, map_k, map_v, p, NoWorkImage{});
+    constexpr int kThreads = FlashThreads<T, DP, QT>();
+    if constexpr (TakesWorkImage(DP, false, true, kPaged)) LaunchDependent(kernel, items * p.cluster, kThreads, kSmem, stream, p.cluster, map_q, map_k, map_v, p, image);
+    else LaunchDependent(kernel, items * p.cluster, kThreads, kSmem, stream, p.cluster, map_q, map_k, map_v, p, NoWorkImage{});
     return SCA_OK;
 }
 
 #define SCA_SPLIT(T, DP, QT)                                                                                                       \
     template int ResidentClusters<T, DP, QT, 128>(int);                                                                            \
     template int LaunchSplit<T, DP, QT, 128, false, false>(int64_t, cudaStream_t, const CUtensorMap&, const CUtensorMap&,          \
-                                                           const CUtensorMap&, const FlashKernelParams&);                          \
+                                                           const CUtensorMap&, const FlashKernelParams&, const WorkImage&);                          \
     template int LaunchSplit<T, DP, QT, 128, true, false>(int64_t, cudaStream_t, const CUtensorMap&, const CUtensorMap&,           \
-                                                          const CUtensorMap&, const FlashKernelParams&);                           \
+                                                          const CUtensorMap&, const FlashKernelParams&, const WorkImage&);                           \
     template int LaunchSplit<T, DP, QT, 128, true, true>(int64_t, cudaStream_t, const CUtensorMap&, const CUtensorMap&,            \
-                                                         const CUtensorMap&, const FlashKernelParams&);
+                                                         const CUtensorMap&, const FlashKernelParams&, const WorkImage&);
 SCA_SPLIT(__half, 64, 2)
 SCA_SPLIT(__half, 128, 2)
 SCA_SPLIT(__half, 256, 1)

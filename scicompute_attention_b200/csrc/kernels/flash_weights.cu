@@ -46,8 +46,14 @@ struct WeightsGeom {
     static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB per-CTA limit");
 };
 
+// The sequences of a call of up to so many, as a parameter of the kernel: the prefill sends no list ahead where it is small.
+constexpr int kImageSeqs = static_cast<int>(sizeof(WorkImage::bytes) / sizeof(int4));
+struct SeqImage {
+    int4 seqs[kImageSeqs];
+};
+
 struct ChunkParams {
-    const int4* seqs;  // {first query token, -, S_q, S_kv}
+    const int4* seqs;  // {first query token, -, S_q, S_kv}; null: in the image
     const float* lse;  // [heads][total_q], natural logarithm; -inf: the row sees nothing
     float* weights;
     int64_t weights_row, total_q;
@@ -77,7 +83,8 @@ __device__ __forceinline__ bool AllSumWarps(bool mine) {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kWeightThreads, 1)
-chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const ChunkParams p) {
+chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const ChunkParams p,
+                     const __grid_constant__ SeqImage image) {
     using G = WeightsGeom<DP>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t base = (SmemAddr(smem_raw) + 1023u) & ~1023u;
@@ -142,7 +149,7 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             l.seq = static_cast<int>(unit / static_cast<uint32_t>(p.kv_heads));
             l.head_kv = static_cast<int>(unit) - l.seq * p.kv_heads;
             l.key0 = static_cast<int>(tile) * kKeys;
-            l.s = p.seqs[l.seq];
+            l.s = p.seqs != nullptr ? p.seqs[l.seq] : image.seqs[l.seq];
         }
         return l;
     };
@@ -353,7 +360,7 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 }
 
 template <typename T, int DP>
-int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, cudaStream_t stream) {
+int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, const SeqImage& image, cudaStream_t stream) {
     using G = WeightsGeom<DP>;
     CUtensorMap map_q, map_k;
     const int64_t rows = x.num_blocks * x.block_size, row = x.num_kv_heads * x.head_dim;
@@ -362,20 +369,20 @@ int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, cudaStream_t stre
     if (int rc = MakeRowsMap(&map_k, x.k_pool, x.dtype_id, x.head_dim, rows, x.num_kv_heads, row, x.head_dim, static_cast<int>(x.block_size), 1, "k pool")) return rc;
     auto kernel = chunk_weights_kernel<T, DP>;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), G::kSmemBytes, "chunk_weights_kernel")) return rc;
-    LaunchDependent(kernel, std::min(p.items, SmCount()), kWeightThreads, G::kSmemBytes, stream, 1, map_q, map_k, p);
+    LaunchDependent(kernel, std::min(p.items, SmCount()), kWeightThreads, G::kSmemBytes, stream, 1, map_q, map_k, p, image);
     return CheckFlashLaunch(stream);
 }
 
 template <typename T>
-int LaunchTyped(const ScaFlashPagedParams& x, const ChunkParams& p, cudaStream_t stream) {
-    if (x.head_dim <= 64) return Launch<T, 64>(x, p, stream);
-    if (x.head_dim <= 128) return Launch<T, 128>(x, p, stream);
-    return Launch<T, 256>(x, p, stream);
+int LaunchTyped(const ScaFlashPagedParams& x, const ChunkParams& p, const SeqImage& image, cudaStream_t stream) {
+    if (x.head_dim <= 64) return Launch<T, 64>(x, p, image, stream);
+    if (x.head_dim <= 128) return Launch<T, 128>(x, p, image, stream);
+    return Launch<T, 256>(x, p, image, stream);
 }
 
 }  // namespace
 
-// Behind the prefill of the same validated call, which has left `seqs` and `lse`.
+// Behind the prefill of the same validated call, which has left `lse`, and `seqs` where there are more than kImageSeqs.
 int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, const int4* seqs, cudaStream_t stream) {
     ChunkParams p{};
     p.seqs = seqs;
@@ -402,7 +409,14 @@ int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, c
     if (items > 0x7fffffffLL) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): " + std::to_string(items) + " tiles of keys are out of range");
     p.units = static_cast<int>(units);
     p.items = static_cast<int>(items);
-    return x.dtype_id == SCA_DTYPE_F16 ? LaunchTyped<__half>(x, p, stream) : LaunchTyped<__nv_bfloat16>(x, p, stream);
+    SeqImage image;
+    if (x.num_seqs <= kImageSeqs) {
+        p.seqs = nullptr;
+        for (int64_t i = 0; i < x.num_seqs; ++i) {
+            image.seqs[i] = make_int4(x.cu_seqlens_q[i], 0, x.cu_seqlens_q[i + 1] - x.cu_seqlens_q[i], x.seq_lens_kv[i]);
+        }
+    }
+    return x.dtype_id == SCA_DTYPE_F16 ? LaunchTyped<__half>(x, p, image, stream) : LaunchTyped<__nv_bfloat16>(x, p, image, stream);
 }
 
 }  // namespace flash

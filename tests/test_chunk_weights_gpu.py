@@ -60,7 +60,7 @@ def test_last_tokens(last):
 
 
 @pytest.mark.parametrize("lens,new,bs", [([1], [1], 16), ([733], [37], 16), ([2000], [2000], 32), ([128, 129, 127], [128, 129, 127], 8), ([3000], [1], 64),
-                                         ([40] * 30, [40] * 30, 16), ([1500, 20], [700, 3], 64)])
+                                         ([40] * 30, [40] * 30, 16), ([1500, 20], [700, 3], 64), ([9] * 128, [2] * 128, 8), ([9] * 129, [2] * 129, 8)])
 def test_lengths_and_pages(lens, new, bs):
     _run(_batch(lens, bs=bs), new)
 
