@@ -42,7 +42,7 @@ def test_heads_and_types(hq, hkv, d, dtype):
     _run(ref.Batch([1, 15, 16, 17, 63, 64, 65, 500, 1100], hq=hq, hkv=hkv, d=d, dtype=dtype))
 
 
-@pytest.mark.parametrize("lens,bs", [([1], 16), ([0], 16), ([701], 16), ([7, 0, 900, 3], 1), ([130, 4000], 24), ([2500] * 3, 64), ([33] * 70, 8), ([12000], 32)])
+@pytest.mark.parametrize("lens,bs", [([1], 16), ([0], 16), ([701], 16), ([7, 0, 900, 3], 1), ([130, 4000], 24), ([2500] * 3, 64), ([33] * 70, 8), ([12000], 32), ([1 + i % 60 for i in range(200)], 16)])
 def test_lengths_and_pages(lens, bs):
     b = ref.Batch(lens, bs=bs)
     _run(b)
