@@ -49,8 +49,8 @@ struct OwnTokens {
     __device__ __forceinline__ bool Regular() const { return p.seq_lens == nullptr && groups.count == 0; }
 };
 
-// kWeights: the scores go to scratch. Without, 96 sequences of 200 to 6000 tokens, 32 / 2 heads, D=64, take 44 us; with a look in every tile
-// whether they are wanted 49.
+// kWeights: the scores go to scratch. A kernel that looks in every tile whether they are wanted takes 5 us more where they are not (96 sequences of
+// 200 to 6001 tokens, 32 / 2 heads, D=64: 44 / 49).
 template <bool kWeights>
 using TapFor = std::conditional_t<kWeights, ScoreTap, NoTap>;
 template <bool kWeights>
