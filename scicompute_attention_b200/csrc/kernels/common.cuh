@@ -34,8 +34,9 @@ int SmCount();
 int SendToDevice(void* device, const void* host, size_t bytes, cudaStream_t stream, const char* what);
 
 // Launches `kernel` as a programmatic dependent of the kernel ahead of it on the stream (cluster > 1: on clusters of that many
-// CTAs): its CTAs may be set up while that one still runs. So the kernel calls one of the two functions below ahead of its first
+// CTAs): its CTAs may be set up while that one still runs. So the kernel calls WaitForPredecessor or BeginAfterPredecessor ahead of its first
 // access to global memory, reads and writes alike, in every CTA - its end then says that all kernels before it have ended.
+// (decode_own_kernel may wait at its end instead: HasBegun in shared_prefix.cuh has told it by then that what it touches is there.)
 // It also reads global memory with ordinary loads only: the kernel ahead may write while this one is already there, and the
 // loads of __ldg and of const __restrict__ pointers are for memory that nobody writes while the kernel lives; neither the
 // wait nor its memory clobber holds such a load back.
@@ -90,10 +91,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Kernels launched by LaunchDependent: waits until the kernel ahead on the stream has ended and its writes are visible (at
 // once where there is none).
 __device__ __forceinline__ void WaitForPredecessor() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
-// The same, and lets the next kernel on the stream be set up from here on.
+// Lets the next kernel on the stream be set up from here on.
+__device__ __forceinline__ void LetSuccessorBegin() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 __device__ __forceinline__ void BeginAfterPredecessor() {
     WaitForPredecessor();
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    LetSuccessorBegin();
 }
 
 __device__ __forceinline__ uint32_t ClusterRank() {

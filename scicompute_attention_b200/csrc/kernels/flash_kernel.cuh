@@ -621,7 +621,16 @@ flash_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     __syncthreads();
     TcFenceAfter();
     const uint32_t tmem_base = *tmem_slot;
-    BeginAfterPredecessor();
+    if constexpr (kShared) {
+        WaitForPredecessor();
+        if (blockIdx.x == 0) {  // ahead of the launch that it is for
+            if (threadIdx.x == 0) SayBegun(image.parts.begun);
+            __syncthreads();
+        }
+        LetSuccessorBegin();
+    } else {
+        BeginAfterPredecessor();
+    }
     if (ConvertersApart<QT, kKv8>() && warp < kFirstSoftmax) KeepRegisters<kIssueRegs>();
 
     bool failed = false;

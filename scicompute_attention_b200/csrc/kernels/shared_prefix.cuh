@@ -36,6 +36,20 @@ __device__ __forceinline__ const PrefixGroup* GroupOf(const PrefixGroups& groups
 // Where the parts of the prefixes are left, fp32: m (log2 domain) and l [rows][parts], O [rows][parts][D]; a row is sequence * heads + head.
 struct PrefixParts {
     float *m, *l, *o;
+    unsigned long long* begun;  // see SayBegun; 0 between two calls
 };
+
+// The kernel that takes the sequences' own tokens may run beside the prefix kernel ahead of it, but the order of a launch says nothing about what that
+// one has waited for. So the prefix kernel, which has, releases this mark (the pattern of two signalling NaN: no kernel leaves these numbers in
+// scratch), and who acquires it stands behind all kernels ahead of the call, as the prefix kernel does. The finish kernel takes the mark away.
+constexpr unsigned long long kBegun = 0xff8b4d277f9a3c51ull;
+// One thread, behind its wait for the kernel ahead.
+__device__ __forceinline__ void SayBegun(unsigned long long* begun) { asm volatile("st.release.gpu.global.u64 [%0], %1;\n" ::"l"(begun), "l"(kBegun) : "memory"); }
+// All threads of a CTA; the barrier passes on what the first thread has acquired.
+__device__ __forceinline__ bool HasBegun(const unsigned long long* begun) {
+    unsigned long long seen = 0;
+    if (threadIdx.x == 0) asm volatile("ld.acquire.gpu.global.u64 %0, [%1];\n" : "=l"(seen) : "l"(begun) : "memory");
+    return __syncthreads_or(seen == kBegun) != 0;
+}
 
 }  // namespace sca_b200
