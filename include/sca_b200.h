@@ -440,7 +440,9 @@ typedef struct ScaPagedStep {
 } ScaPagedStep;
 
 /* Floats of scratch that sca_launch_paged_step wants for the same arguments (pointers to tensors are not looked at, `weights` but for
- * whether it is there); negative: they are refused. */
+ * whether it is there); negative: they are refused. With weights most of it is a score for every query head and token that a sequence may have:
+ * `longest_len` where it is given, all of the table's row otherwise. 2 GB of scores at most, or those of one sequence: a larger call runs in slices of
+ * sequences that use the same scratch. */
 SCA_ABI long long sca_paged_step_scratch_floats(const ScaDecodeFwdParams* params, const ScaPagedStep* step);
 /* sca_launch_decode_auto over a paged fp16 / bf16 cache, with weights, shared prefixes, or both. params: q, k, v, out, page_table, seq_lens
  * and the sizes as there; the partial arrays, num_splits, seq_kv and the strides of K and V are not looked at. scale > 0 and finite. */

@@ -285,7 +285,7 @@ decode_finish_kernel(const ScaDecodeFwdParams p, const WeightsParams x, const in
     }
 }
 
-// What a call is made of: sizes of its launches, and where its arrays lie in the scratch.
+// What a slice of a call is made of (see SliceOf): sizes of its launches, and where its arrays lie in the scratch.
 struct Plan {
     PrefixGroups groups;
     int64_t splits;
@@ -348,38 +348,62 @@ int Validate(const ScaDecodeFwdParams* params, const ScaPagedStep* step, const c
     return SCA_OK;
 }
 
-// A validated call.
-Plan MakePlan(const ScaDecodeFwdParams& p, const ScaPagedStep& x) {
+// Tokens of a sequence at most, as far as the host knows.
+int64_t BoundOf(const ScaDecodeFwdParams& p, const ScaPagedStep& x) {
+    const int64_t capacity = p.max_blocks_per_seq * p.block_size;
+    return x.longest_len > 0 ? std::min(x.longest_len, capacity) : capacity;
+}
+// Scores of a query head. A tile of 16 may begin at any page of a prefix, 8 tokens say, and is stored whole.
+int64_t ScoreRow(const ScaDecodeFwdParams& p, const ScaPagedStep& x) { return x.weights != nullptr ? RoundUp(BoundOf(p, x), kTile) + kTile : 0; }
+
+// Sequences that go through the kernels together. The scratch has a score for every token that a sequence may have, whatever it has, so a call
+// with weights whose table is wide, or one of whose sequences is long, is taken in slices of sequences whose scores fit kMostScores, 2 GB, or of one.
+// us and MB of scratch without slices / of 2 GB / of 1 GB (D=128, 32 / 8 heads unless said):
+//   192 sequences of 500 to 6000 tokens, table of 131 072         456, 3848 / 473, 1924 / 487, 962
+//   one of 100 000 among 191 of 200 to 1500, exact hints          235, 2987 / 241, 1518 / 245, 1030
+//   2 groups, 128 sequences behind 3000 tokens, table of 131 072  110, 2580 / 117, 1291 / 139, 867
+//   96 of 200 to 6001, 32 / 2 heads, D=64, table of 131 072        64, 1925 /  64, 1925 /  78, 963
+constexpr int64_t kMostScores = int64_t{1} << 29;
+int64_t SliceOf(const ScaDecodeFwdParams& p, const ScaPagedStep& x) {
+    if (x.weights == nullptr) return p.batch;
+    const int64_t most = std::max<int64_t>(1, kMostScores / (p.num_heads * ScoreRow(p, x))), slices = (p.batch + most - 1) / most;
+    return (p.batch + slices - 1) / slices;
+}
+
+// Sequences [begin, end) of a validated call.
+Plan MakePlan(const ScaDecodeFwdParams& p, const ScaPagedStep& x, int64_t begin, int64_t end) {
     Plan plan{};
     PrefixGroups& groups = plan.groups;
-    const int64_t capacity = p.max_blocks_per_seq * p.block_size;
-    plan.bound = x.longest_len > 0 ? std::min(x.longest_len, capacity) : capacity;
+    const int64_t batch = end - begin;
+    plan.bound = BoundOf(p, x);
     int64_t prefix_of_all = 0;                                  // tokens that are read for others
     int64_t least_prefix = x.num_groups > 0 ? plan.bound : 0;  // of a sequence
     for (int64_t g = 0; g < x.num_groups; ++g) {
         const int64_t tokens = std::min<int64_t>(x.prefix_lens[g], plan.bound) / p.block_size * p.block_size;
-        const int64_t sequences = x.cu_groups[g + 1] - x.cu_groups[g];
-        if (sequences > 0) least_prefix = std::min(least_prefix, sequences > 1 ? tokens : 0);
-        if (sequences < 2 || tokens == 0) continue;
-        groups.group[groups.count++] = {x.cu_groups[g], x.cu_groups[g + 1], static_cast<int>(tokens), 0};
-        prefix_of_all += sequences * tokens;
+        const bool shared = x.cu_groups[g + 1] - x.cu_groups[g] > 1 && tokens > 0;  // one that a slice cuts stays a group, of one sequence too
+        const int64_t from = std::max<int64_t>(x.cu_groups[g], begin), to = std::min<int64_t>(x.cu_groups[g + 1], end);
+        if (from >= to) continue;
+        least_prefix = std::min(least_prefix, shared ? tokens : 0);
+        if (!shared) continue;
+        groups.group[groups.count++] = {static_cast<int>(from - begin), static_cast<int>(to - begin), static_cast<int>(tokens), 0};
+        prefix_of_all += (to - from) * tokens;
     }
     if (groups.count > 0) PlanPrefixParts(p, &groups);
 
     // Slots for the parts of a sequence's own tokens: enough for an even schedule (see slots_for_schedule in ops.py). The kernel takes
     // larger shares where these hold fewer.
-    const int64_t typical = std::max<int64_t>(1, (x.typical_len > 0 ? std::min(x.typical_len, plan.bound) : plan.bound) - prefix_of_all / p.batch);
+    const int64_t typical = std::max<int64_t>(1, (x.typical_len > 0 ? std::min(x.typical_len, plan.bound) : plan.bound) - prefix_of_all / batch);
     const int64_t group_heads = p.num_heads / p.num_kv_heads;
     const int64_t columns = p.num_kv_heads * ((group_heads + 15) / 16);
     const int64_t steps = (typical + kSpan - 1) / kSpan;
     const int64_t longest = x.longest_len > 0 ? std::max<int64_t>(1, (plan.bound - least_prefix + kSpan - 1) / kSpan) : 2 * steps;
     const int64_t sharers = std::max<int64_t>(1, 2 * SmCount() / columns);
-    const int64_t share = std::max<int64_t>(1, (p.batch * steps + sharers - 1) / sharers);
+    const int64_t share = std::max<int64_t>(1, (batch * steps + sharers - 1) / sharers);
     // two at least, for sequences of one step too: with one the first CTA of a column would have all of them (256 sequences of 1 to 60 tokens, 32 / 8
     // heads, D=128: 806 us, 40.6 with two)
     plan.splits = std::max<int64_t>(2, std::min((longest + share - 1) / share + 1, kMostSplits));
 
-    const int64_t rows = p.batch * p.num_heads;
+    const int64_t rows = batch * p.num_heads;
     plan.own_m = 8;
     plan.own_l = plan.own_m + rows * plan.splits;
     plan.own_o = RoundUp(plan.own_l + rows * plan.splits, 4);  // an O starts on 16 bytes
@@ -387,10 +411,26 @@ Plan MakePlan(const ScaDecodeFwdParams& p, const ScaPagedStep& x) {
     plan.prefix_l = plan.prefix_m + rows * groups.parts;
     plan.prefix_o = RoundUp(plan.prefix_l + rows * groups.parts, 8);  // 32
     plan.scores = RoundUp(plan.prefix_o + rows * groups.parts * p.head_dim, 8);
-    // a tile of 16 scores may begin at any page of a prefix, 8 tokens say, and is stored whole
-    plan.score_row = x.weights != nullptr ? RoundUp(plan.bound, kTile) + kTile : 0;
+    plan.score_row = ScoreRow(p, x);
     plan.floats = plan.scores + rows * plan.score_row;
     return plan;
+}
+
+// f(begin, end, plan) for every slice of a validated call; a number other than 0 ends it.
+template <typename F>
+int ForSlices(const ScaDecodeFwdParams& p, const ScaPagedStep& x, const F& f) {
+    const int64_t slice = SliceOf(p, x);
+    for (int64_t begin = 0; begin < p.batch; begin += slice) {
+        const int64_t end = std::min(begin + slice, p.batch);
+        if (int rc = f(begin, end, MakePlan(p, x, begin, end))) return rc;
+    }
+    return 0;
+}
+// The slices follow one another on the stream and use the same scratch.
+int64_t ScratchFloats(const ScaDecodeFwdParams& p, const ScaPagedStep& x) {
+    int64_t most = 0;
+    ForSlices(p, x, [&](int64_t, int64_t, const Plan& plan) { return most = std::max(most, plan.floats), 0; });
+    return most;
 }
 
 // Where sequences share pages, the one launch reads them once for each; that pays as long as a CTA has few steps. us, one launch / with the
@@ -513,7 +553,7 @@ using namespace sca_b200;
 extern "C" long long sca_paged_step_scratch_floats(const ScaDecodeFwdParams* params, const ScaPagedStep* step) {
     ClearError();
     if (Validate(params, step, "paged step") != SCA_OK) return -1;
-    return MakePlan(*params, *step).floats;
+    return ScratchFloats(*params, *step);
 }
 
 extern "C" int sca_launch_paged_step(const ScaDecodeFwdParams* params, const ScaPagedStep* step, void* stream) {
@@ -528,25 +568,37 @@ extern "C" int sca_launch_paged_step(const ScaDecodeFwdParams* params, const Sca
         p.o_stride.s_b % 8 != 0 || p.o_stride.s_h % 8 != 0 || (reinterpret_cast<uintptr_t>(x.scratch) & 31u) != 0) {
         return Fail(SCA_INVALID_ARGUMENT, "paged step: q/k/v/out must be 16-byte aligned with strides that are multiples of 8 elements, the scratch 32-byte aligned");
     }
-    const Plan plan = MakePlan(p, x);
-    if (x.scratch_floats < plan.floats) {
-        return Fail(SCA_INVALID_ARGUMENT, "paged step: scratch of " + std::to_string(x.scratch_floats) + " floats is too small (" + std::to_string(plan.floats) + " needed)");
+    auto scratch_holds = [&](int64_t need) {
+        if (x.scratch_floats >= need) return static_cast<int>(SCA_OK);
+        return Fail(SCA_INVALID_ARGUMENT, "paged step: scratch of " + std::to_string(x.scratch_floats) + " floats is too small (" + std::to_string(need) + " needed)");
+    };
+    if (SliceOf(p, x) < p.batch) {  // ahead of the first slice's launches
+        if (int rc = scratch_holds(ScratchFloats(p, x))) return rc;
     }
     float* scratch = x.scratch;
-    p.num_splits = plan.splits;
-    p.partial_m = scratch + plan.own_m;
-    p.partial_l = scratch + plan.own_l;
-    p.partial_o = scratch + plan.own_o;
     p.seq_kv = p.num_kv_blocks * p.block_size;  // of a sequence without a length: all of its row
     p.k_stride = p.v_stride = ScaDecodeStrides{0, p.head_dim, p.num_kv_heads * p.head_dim};
-    WeightsParams w{};
-    w.weights = x.weights;
-    w.row = x.weights_row;
-    w.scores = x.weights != nullptr ? scratch + plan.scores : nullptr;
-    w.score_row = plan.score_row;
-    w.bound = plan.bound;
-    w.prefix = PrefixParts{scratch + plan.prefix_m, scratch + plan.prefix_l, scratch + plan.prefix_o, reinterpret_cast<unsigned long long*>(scratch)};
-    w.behind_prefix = plan.groups.count > 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return p.dtype == SCA_DTYPE_F16 ? LaunchStep<__half>(p, w, plan.groups, s) : LaunchStep<__nv_bfloat16>(p, w, plan.groups, s);
+    return ForSlices(p, x, [&](int64_t begin, int64_t end, const Plan& plan) {
+        if (int rc = scratch_holds(plan.floats)) return rc;
+        ScaDecodeFwdParams part = p;
+        part.batch = end - begin;
+        part.q = static_cast<const char*>(p.q) + begin * p.q_stride.s_b * 2;
+        part.out = static_cast<char*>(p.out) + begin * p.o_stride.s_b * 2;
+        part.page_table = p.page_table + begin * p.max_blocks_per_seq;
+        if (p.seq_lens != nullptr) part.seq_lens = p.seq_lens + begin;
+        part.num_splits = plan.splits;
+        part.partial_m = scratch + plan.own_m;
+        part.partial_l = scratch + plan.own_l;
+        part.partial_o = scratch + plan.own_o;
+        WeightsParams w{};
+        w.weights = x.weights != nullptr ? x.weights + begin * p.num_kv_heads * x.weights_row : nullptr;
+        w.row = x.weights_row;
+        w.scores = x.weights != nullptr ? scratch + plan.scores : nullptr;
+        w.score_row = plan.score_row;
+        w.bound = plan.bound;
+        w.prefix = PrefixParts{scratch + plan.prefix_m, scratch + plan.prefix_l, scratch + plan.prefix_o, reinterpret_cast<unsigned long long*>(scratch)};
+        w.behind_prefix = plan.groups.count > 0;
+        return p.dtype == SCA_DTYPE_F16 ? LaunchStep<__half>(part, w, plan.groups, s) : LaunchStep<__nv_bfloat16>(part, w, plan.groups, s);
+    });
 }

@@ -1036,7 +1036,9 @@ def paged_attention_weights(q, k_pool, v_pool, page_table, seq_lens, weights, *,
 
     q, pools, table, lengths as paged_attention takes them, of float16 or bfloat16; weights float32 [num_seqs, H_kv, max_blocks_per_seq *
     block_size] or more rows and columns, on the device. A query of NaN makes the weights of its kv head NaN. `typical_len` sizes the launch;
-    `longest_len` does too and bounds the lengths: no sequence is longer, and a token behind it would count for nothing."""
+    `longest_len` does too and bounds the lengths: no sequence is longer, and a token behind it would count for nothing. The scratch of a call with weights has a
+    score for every query head and token up to `longest_len`, or up to the end of the table's rows without it (2 GB at most, or one sequence's: what needs more
+    runs in slices of sequences); it is kept as paged_attention's is. Give it where the table is wide."""
     if weights is None:
         raise _lib.ScaError(4, "weights must be a tensor")
     return _paged_step(q, k_pool, v_pool, page_table, seq_lens, None, None, weights, block_size, scale, typical_len, longest_len, stream)
