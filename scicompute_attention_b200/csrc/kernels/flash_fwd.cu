@@ -637,14 +637,13 @@ extern "C" int sca_launch_flash_paged_weights(const ScaFlashPagedParams* params,
     }
     const ScaFlashPagedParams& x = *params;
     if (weights->last < 0) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): last must not be negative");
+    // a key's place is a 32-bit number, the tile of 128 that it is in too
+    if (x.block_size > 0 && x.max_blocks_per_seq > 0x7fffff00LL / x.block_size) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): page-table rows of more than 2^31 tokens");
     if (weights->weights_row < x.max_blocks_per_seq * x.block_size) {
         return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): rows of " + std::to_string(weights->weights_row) + " weights for page-table rows of " +
                                               std::to_string(x.max_blocks_per_seq * x.block_size) + " tokens");
     }
     if (x.num_seqs > 0 && x.num_kv_heads > 0 && x.num_seqs > 0x7fffffffLL / x.num_kv_heads) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): too many sequences");
-    if (x.max_blocks_per_seq * x.block_size > 65535LL * 128) {
-        return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): page-table rows of more than 8388480 tokens");
-    }
     if (!std::isfinite(x.scale)) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): scale must be a positive number");
     if (int rc = LaunchPaged(params, nullptr, nullptr, stream, weights->lse)) return rc;
     // where the prefill has sent its work list ahead, it begins with the sequences (UploadVarlenWork)
