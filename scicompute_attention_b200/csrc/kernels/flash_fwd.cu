@@ -626,7 +626,9 @@ extern "C" int sca_launch_flash_paged(const ScaFlashPagedParams* params, void* s
 
 namespace sca_b200 {
 namespace flash {
-int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, const int4* seqs, cudaStream_t stream);  // flash_weights.cu
+// flash_weights.cu
+int CheckChunkTiles(const ScaFlashPagedParams& x);
+int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, const int4* seqs, cudaStream_t stream);
 }
 }  // namespace sca_b200
 
@@ -645,6 +647,7 @@ extern "C" int sca_launch_flash_paged_weights(const ScaFlashPagedParams* params,
     }
     if (x.num_seqs > 0 && x.num_kv_heads > 0 && x.num_seqs > 0x7fffffffLL / x.num_kv_heads) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): too many sequences");
     if (!std::isfinite(x.scale)) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): scale must be a positive number");
+    if (int rc = flash::CheckChunkTiles(x)) return rc;  // ahead of the prefill, which writes the output
     if (int rc = LaunchPaged(params, nullptr, nullptr, stream, weights->lse)) return rc;
     // where the prefill has sent its work list ahead, it begins with the sequences (UploadVarlenWork)
     return flash::LaunchChunkWeights(x, *weights, static_cast<const int4*>(x.workspace), static_cast<cudaStream_t>(stream));

@@ -127,7 +127,7 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     // ---- items: tile after tile of all sequences and kv heads, dealt in rounds of gridDim.x, every other one in reverse order ----
     const int heads_tile = 1 << p.pack_shift, tile_tokens = kColumns >> p.pack_shift;
     const int group = p.heads / p.kv_heads, packs = group >> p.pack_shift;
-    const int rounds = (p.items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    const int rounds = (p.items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);  // at most kMostTiles items
     struct Item {
         int seq, head_kv, key0, keys, new_tokens, q0;
         int first_token;  // that sees the first key and counts
@@ -380,7 +380,22 @@ int LaunchTyped(const ScaFlashPagedParams& x, const ChunkParams& p, const SeqIma
     return Launch<T, 256>(x, p, image, stream);
 }
 
+// Tiles of keys of a call: what is dealt to the CTAs, those that a shorter sequence does not have among them. 2^30 of them stand for 512 GB of weights.
+constexpr int64_t kMostTiles = int64_t{1} << 30;
+int64_t ChunkTiles(const ScaFlashPagedParams& x) {
+    int64_t most_keys = 0;
+    for (int64_t i = 0; i < x.num_seqs; ++i) most_keys = std::max<int64_t>(most_keys, x.seq_lens_kv[i]);
+    return x.num_seqs * x.num_kv_heads * ((most_keys + kKeys - 1) / kKeys);
+}
+
 }  // namespace
+
+int CheckChunkTiles(const ScaFlashPagedParams& x) {
+    if (x.seq_lens_kv == nullptr) return SCA_OK;  // the prefill refuses it
+    const int64_t tiles = ChunkTiles(x);
+    if (tiles <= kMostTiles) return SCA_OK;
+    return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): " + std::to_string(tiles) + " tiles of keys are out of range");
+}
 
 // Behind the prefill of the same validated call, which has left `lse`, and `seqs` where there are more than kImageSeqs.
 int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, const int4* seqs, cudaStream_t stream) {
@@ -403,12 +418,8 @@ int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, c
     p.last = static_cast<int>(w.last < x.total_q ? w.last : 0);
     p.causal = x.causal ? 1 : 0;
     p.scale_log2 = x.scale * kLog2e;
-    int64_t most_keys = 0;
-    for (int64_t i = 0; i < x.num_seqs; ++i) most_keys = most_keys < x.seq_lens_kv[i] ? x.seq_lens_kv[i] : most_keys;
-    const int64_t units = x.num_seqs * x.num_kv_heads, items = units * ((most_keys + kKeys - 1) / kKeys);
-    if (items > 0x7fffffffLL) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): " + std::to_string(items) + " tiles of keys are out of range");
-    p.units = static_cast<int>(units);
-    p.items = static_cast<int>(items);
+    p.units = static_cast<int>(x.num_seqs * x.num_kv_heads);
+    p.items = static_cast<int>(ChunkTiles(x));
     SeqImage image;
     if (x.num_seqs <= kImageSeqs) {
         p.seqs = nullptr;

@@ -28,6 +28,13 @@ def test_rows_of_more_tokens_than_32_bits_hold_are_refused(blocks):
     assert rc == 4 and "2^31 tokens" in message, message
 
 
+# 2^30 + 128 tiles; and 2^31 - 128, to which the number of CTAs cannot be added in 32 bits
+@pytest.mark.parametrize("kv_heads,tokens", [(128, (1 << 30) + 128), (384, 5592405 * 128)])
+def test_more_tiles_than_a_launch_has_are_refused_ahead_of_it(kv_heads, tokens):
+    rc, message = _entry(num_heads=kv_heads, num_kv_heads=kv_heads, max_blocks_per_seq=(1 << 27) - 16, tokens=tokens)
+    assert rc == 4 and "tiles of keys" in message, message
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("pages", [524281, 600_000])  # of 16 tokens: the first is the least that is wider than 65535 tiles of 128
 def test_wide_tables(pages):
