@@ -628,7 +628,7 @@ namespace sca_b200 {
 namespace flash {
 // flash_weights.cu
 int CheckChunkTiles(const ScaFlashPagedParams& x);
-int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, const int4* seqs, cudaStream_t stream);
+int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, cudaStream_t stream);
 }
 }  // namespace sca_b200
 
@@ -649,8 +649,7 @@ extern "C" int sca_launch_flash_paged_weights(const ScaFlashPagedParams* params,
     if (!std::isfinite(x.scale)) return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): scale must be a positive number");
     if (int rc = flash::CheckChunkTiles(x)) return rc;  // ahead of the prefill, which writes the output
     if (int rc = LaunchPaged(params, nullptr, nullptr, stream, weights->lse)) return rc;
-    // where the prefill has sent its work list ahead, it begins with the sequences (UploadVarlenWork)
-    return flash::LaunchChunkWeights(x, *weights, static_cast<const int4*>(x.workspace), static_cast<cudaStream_t>(stream));
+    return flash::LaunchChunkWeights(x, *weights, static_cast<cudaStream_t>(stream));
 } catch (const std::exception& e) {  // host memory for the work list
     return Fail(SCA_CUDA_ERROR, std::string("flash paged (weights): on the host: ") + e.what());
 }

@@ -10,15 +10,20 @@
 //                  2^(score * scale - lse), summed up
 //   warp 16        TMA: tiles of keys, page by page, then their query tiles into a ring, and the queries' lse
 //   warp 17        issues the products
+// Items are dealt tile after tile, to the sequences that have it: with a place for every sequence up to the longest one's last tile a CTA walks what is not
+// there (one sequence of 100 000 tokens among 255 of 500, 16 new ones each: 4.4 ms of 6.2).
 // One CTA to an SM walks the list of items, those that most queries see first, and loads the next tile of keys under the current one: with a
 // CTA to an item its start - barriers, tensor memory, the look-up of sequence and pages, the first loads - took 6 us (4 prompts of 2000, 32 / 8
 // heads, D=128: 512 items 126 us; 9 sequences of which the last 64 tokens count, D=64: 2016 items 40 us).
 // A query tile is 128 / P tokens of P query heads, as in the prefill, and starts with the first token that sees the tile's first key, so
 // that a causal mask cuts 128 / P tokens' rows at most.
-// Bound by the special-function unit, of which it uses 71 % while an SM has work (16384 exponentials a tile take 1024 clocks of an SM, the
-// products 540), and by items that do not come out even: 87 % of the SMs' time. 4 prompts of 1900 to 2048 tokens, 32 / 8 heads, D=128: 115 us
-// alone, 260 us with the prefill. A quarter of the exponentials by a polynomial of degree 5 on the multipliers instead: 256 us, half 266.
+// No unit is at its limit: while an SM has work its special-function unit is busy 71 % of the time (16384 exponentials a tile take 1024 clocks, the
+// products 540), and a quarter of the exponentials by a polynomial of degree 5 on the multipliers instead gained next to nothing (260 -> 256 us, half
+// of them 266). A warp waits on the chain of its own tile and on shared memory, from which every thread reads 64 numbers of lse beside its 64 exponentials (stalls per issue:
+// wait 2.4, long scoreboard 2.3, MIO throttle 2.1), and items do not come out even: the SMs have work 87 % of the time. 4 prompts of 1900 to 2048
+// tokens, 32 / 8 heads, D=128: 115 us alone, 257 us with the prefill.
 #include <algorithm>
+#include <vector>
 
 #include "flash_kernel.cuh"
 
@@ -46,14 +51,17 @@ struct WeightsGeom {
     static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB per-CTA limit");
 };
 
-// The sequences of a call of up to so many, as a parameter of the kernel: the prefill sends no list ahead where it is small.
-constexpr int kImageSeqs = static_cast<int>(sizeof(WorkImage::bytes) / sizeof(int4));
+// The sequences of a launch, as a parameter of the kernel, so that nothing is sent ahead: {first query token, place in the batch, S_q, S_kv}, those of
+// the most tiles of keys first, and how many items there are up to the last tile of each; behind the last one a sequence of no tiles. A call of more of
+// them takes several launches.
+constexpr int kImageSeqs = 160;
 struct SeqImage {
-    int4 seqs[kImageSeqs];
+    int4 seqs[kImageSeqs + 1];
+    int ends[kImageSeqs + 1];
 };
+__host__ __device__ inline int TilesOf(const int4& seq) { return (seq.w + kKeys - 1) / kKeys; }
 
 struct ChunkParams {
-    const int4* seqs;  // {first query token, -, S_q, S_kv}; null: in the image
     const float* lse;  // [heads][total_q], natural logarithm; -inf: the row sees nothing
     float* weights;
     int64_t weights_row, total_q;
@@ -61,7 +69,7 @@ struct ChunkParams {
     int* error_word;
     int max_blocks, num_blocks, block_size, block_shift;
     int heads, kv_heads, pack_shift, last, causal;
-    int units, items;  // sequences * kv heads, and that times the tiles of the longest sequence
+    int seqs, items;   // in the image, and the tiles of keys that they have, times the kv heads
     float scale_log2;
 };
 
@@ -124,10 +132,10 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     TcFenceAfter();
     const uint32_t tmem = *tmem_slot;
 
-    // ---- items: tile after tile of all sequences and kv heads, dealt in rounds of gridDim.x, every other one in reverse order ----
+    // ---- items: tile after tile of all sequences that have it and their kv heads, dealt in rounds of gridDim.x, every other one in reverse order ----
     const int heads_tile = 1 << p.pack_shift, tile_tokens = kColumns >> p.pack_shift;
     const int group = p.heads / p.kv_heads, packs = group >> p.pack_shift;
-    const int rounds = (p.items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);  // at most kMostTiles items
+    const int rounds = (p.items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);  // at most 2^30 items
     struct Item {
         int seq, head_kv, key0, keys, new_tokens, q0;
         int first_token;  // that sees the first key and counts
@@ -139,17 +147,21 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         int seq, head_kv, key0;
         int4 s;
     };
+    int active = p.seqs;  // those that have the tile: the first so many. Rounds go upwards, so this goes down
     auto look = [&](int round) {
         Look l;
-        const int64_t index = static_cast<int64_t>(round) * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const int ctas = static_cast<int>(gridDim.x), me = static_cast<int>(blockIdx.x), index = round * ctas + ((round & 1) ? ctas - 1 - me : me);
         l.s = make_int4(0, 0, 0, 0);
         l.seq = l.head_kv = l.key0 = 0;
         if (round < rounds && index < p.items) {
-            const uint32_t tile = static_cast<uint32_t>(index) / static_cast<uint32_t>(p.units), unit = static_cast<uint32_t>(index) - tile * static_cast<uint32_t>(p.units);
-            l.seq = static_cast<int>(unit / static_cast<uint32_t>(p.kv_heads));
-            l.head_kv = static_cast<int>(unit) - l.seq * p.kv_heads;
-            l.key0 = static_cast<int>(tile) * kKeys;
-            l.s = p.seqs != nullptr ? p.seqs[l.seq] : image.seqs[l.seq];
+            while (index >= image.ends[active - 1]) --active;
+            // from the tile on at which the next shorter sequence ends
+            const uint32_t units = static_cast<uint32_t>(active * p.kv_heads), at = static_cast<uint32_t>(index - image.ends[active]);
+            const uint32_t tile = at / units, unit = at - tile * units, place = unit / static_cast<uint32_t>(p.kv_heads);
+            l.s = image.seqs[place];
+            l.seq = l.s.y;
+            l.head_kv = static_cast<int>(unit - place * static_cast<uint32_t>(p.kv_heads));
+            l.key0 = (TilesOf(image.seqs[active]) + static_cast<int>(tile)) * kKeys;
         }
         return l;
     };
@@ -360,7 +372,7 @@ chunk_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 }
 
 template <typename T, int DP>
-int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, const SeqImage& image, cudaStream_t stream) {
+int Launch(const ScaFlashPagedParams& x, ChunkParams p, const std::vector<int4>& seqs, cudaStream_t stream) {
     using G = WeightsGeom<DP>;
     CUtensorMap map_q, map_k;
     const int64_t rows = x.num_blocks * x.block_size, row = x.num_kv_heads * x.head_dim;
@@ -369,38 +381,44 @@ int Launch(const ScaFlashPagedParams& x, const ChunkParams& p, const SeqImage& i
     if (int rc = MakeRowsMap(&map_k, x.k_pool, x.dtype_id, x.head_dim, rows, x.num_kv_heads, row, x.head_dim, static_cast<int>(x.block_size), 1, "k pool")) return rc;
     auto kernel = chunk_weights_kernel<T, DP>;
     if (int rc = EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), G::kSmemBytes, "chunk_weights_kernel")) return rc;
-    LaunchDependent(kernel, std::min(p.items, SmCount()), kWeightThreads, G::kSmemBytes, stream, 1, map_q, map_k, p, image);
-    return CheckFlashLaunch(stream);
+    const size_t launches = (seqs.size() + kImageSeqs - 1) / kImageSeqs, share = (seqs.size() + launches - 1) / launches;
+    for (size_t first = 0; first < seqs.size(); first += share) {
+        SeqImage image;
+        p.seqs = static_cast<int>(std::min(share, seqs.size() - first));
+        image.seqs[p.seqs] = make_int4(0, 0, 0, 0);
+        image.ends[p.seqs] = 0;
+        for (int i = p.seqs - 1; i >= 0; --i) {  // from the tile on at which i + 1 ends, i + 1 sequences go on to where i does
+            image.seqs[i] = seqs[first + i];
+            image.ends[i] = image.ends[i + 1] + (TilesOf(image.seqs[i]) - TilesOf(image.seqs[i + 1])) * (i + 1) * p.kv_heads;
+        }
+        p.items = image.ends[0];
+        LaunchDependent(kernel, std::min(p.items, SmCount()), kWeightThreads, G::kSmemBytes, stream, 1, map_q, map_k, p, image);
+        if (int rc = CheckFlashLaunch(stream)) return rc;
+    }
+    return SCA_OK;
 }
 
 template <typename T>
-int LaunchTyped(const ScaFlashPagedParams& x, const ChunkParams& p, const SeqImage& image, cudaStream_t stream) {
-    if (x.head_dim <= 64) return Launch<T, 64>(x, p, image, stream);
-    if (x.head_dim <= 128) return Launch<T, 128>(x, p, image, stream);
-    return Launch<T, 256>(x, p, image, stream);
-}
-
-// Tiles of keys of a call: what is dealt to the CTAs, those that a shorter sequence does not have among them. 2^30 of them stand for 512 GB of weights.
-constexpr int64_t kMostTiles = int64_t{1} << 30;
-int64_t ChunkTiles(const ScaFlashPagedParams& x) {
-    int64_t most_keys = 0;
-    for (int64_t i = 0; i < x.num_seqs; ++i) most_keys = std::max<int64_t>(most_keys, x.seq_lens_kv[i]);
-    return x.num_seqs * x.num_kv_heads * ((most_keys + kKeys - 1) / kKeys);
+int LaunchTyped(const ScaFlashPagedParams& x, const ChunkParams& p, const std::vector<int4>& seqs, cudaStream_t stream) {
+    if (x.head_dim <= 64) return Launch<T, 64>(x, p, seqs, stream);
+    if (x.head_dim <= 128) return Launch<T, 128>(x, p, seqs, stream);
+    return Launch<T, 256>(x, p, seqs, stream);
 }
 
 }  // namespace
 
+// Tiles of keys of a call, as many as 32-bit arithmetic on them holds. 2^30 of them have 512 GB of weights.
 int CheckChunkTiles(const ScaFlashPagedParams& x) {
     if (x.seq_lens_kv == nullptr) return SCA_OK;  // the prefill refuses it
-    const int64_t tiles = ChunkTiles(x);
-    if (tiles <= kMostTiles) return SCA_OK;
+    int64_t tiles = 0;
+    for (int64_t i = 0; i < x.num_seqs; ++i) tiles += (std::max<int64_t>(x.seq_lens_kv[i], 0) + kKeys - 1) / kKeys * std::max<int64_t>(x.num_kv_heads, 0);
+    if (tiles <= int64_t{1} << 30) return SCA_OK;
     return Fail(SCA_INVALID_ARGUMENT, "flash paged (weights): " + std::to_string(tiles) + " tiles of keys are out of range");
 }
 
-// Behind the prefill of the same validated call, which has left `lse`, and `seqs` where there are more than kImageSeqs.
-int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, const int4* seqs, cudaStream_t stream) {
+// Behind the prefill of the same validated call, which has left `lse`.
+int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, cudaStream_t stream) {
     ChunkParams p{};
-    p.seqs = seqs;
     p.lse = w.lse;
     p.weights = w.weights;
     p.weights_row = w.weights_row;
@@ -418,16 +436,10 @@ int LaunchChunkWeights(const ScaFlashPagedParams& x, const ScaChunkWeights& w, c
     p.last = static_cast<int>(w.last < x.total_q ? w.last : 0);
     p.causal = x.causal ? 1 : 0;
     p.scale_log2 = x.scale * kLog2e;
-    p.units = static_cast<int>(x.num_seqs * x.num_kv_heads);
-    p.items = static_cast<int>(ChunkTiles(x));
-    SeqImage image;
-    if (x.num_seqs <= kImageSeqs) {
-        p.seqs = nullptr;
-        for (int64_t i = 0; i < x.num_seqs; ++i) {
-            image.seqs[i] = make_int4(x.cu_seqlens_q[i], 0, x.cu_seqlens_q[i + 1] - x.cu_seqlens_q[i], x.seq_lens_kv[i]);
-        }
-    }
-    return x.dtype_id == SCA_DTYPE_F16 ? LaunchTyped<__half>(x, p, image, stream) : LaunchTyped<__nv_bfloat16>(x, p, image, stream);
+    std::vector<int4> seqs(static_cast<size_t>(x.num_seqs));
+    for (int i = 0; i < x.num_seqs; ++i) seqs[static_cast<size_t>(i)] = make_int4(x.cu_seqlens_q[i], i, x.cu_seqlens_q[i + 1] - x.cu_seqlens_q[i], x.seq_lens_kv[i]);
+    std::stable_sort(seqs.begin(), seqs.end(), [](const int4& a, const int4& b) { return TilesOf(a) > TilesOf(b); });
+    return x.dtype_id == SCA_DTYPE_F16 ? LaunchTyped<__half>(x, p, seqs, stream) : LaunchTyped<__nv_bfloat16>(x, p, seqs, stream);
 }
 
 }  // namespace flash

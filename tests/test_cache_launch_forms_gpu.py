@@ -163,7 +163,7 @@ def test_weights_in_two_kernels(d, group, tmp_path):
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("d,hq", [(64, 8), (128, 4), (128, 12), (192, 8), (256, 16)])
 def test_several_tiles_of_keys_to_a_cta(d, hq, dtype, causal, tmp_path):
-    """640 tiles for 148 CTAs, a third of them of sequences that are shorter: every CTA comes back to its first slot of keys."""
+    """332 tiles for 148 CTAs: every CTA takes a second one - at D above 128 into the slot of the first - and some a third."""
     from scicompute_attention_b200 import ops
     b = chunks._batch([3000, 2500, 700, 4000, 100], hq=hq, hkv=4, d=d, dtype=dtype)
     new = [40, 600, 700, 1, 13]

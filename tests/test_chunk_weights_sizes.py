@@ -51,3 +51,22 @@ def test_wide_tables(pages):
     wide[:, :, :b.width * 16] = b.weights
     assert torch.equal(ops.flash_attention_paged_weights(q, b.k, b.v, table, cu, b.lens_host, wide), want)
     assert torch.equal(wide[:, :, :b.width * 16], narrow) and not wide[:, :, b.width * 16:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,longest,hkv,launched", [(3, 30_000, 2, 1), (160, 5000, 1, 1), (161, 5000, 2, 2), (400, 700, 1, 3)])
+def test_ragged_batches(n, longest, hkv, launched, tmp_path):
+    """One sequence far longer than the others, anywhere in the batch, equal ones, every number of tiles below that: only tiles that exist are dealt, those of
+    up to 160 sequences to a launch."""
+    import test_chunk_weights_gpu as chunks
+    from launches import CHUNK, launches
+    from scicompute_attention_b200 import ops
+    lens = [1 + (113 * i) % 640 for i in range(n)]
+    lens[n // 3] = longest
+    new = [min(k, 1 + i % 5) for i, k in enumerate(lens)]
+    b = chunks._batch(lens, hq=2 * hkv, hkv=hkv)
+    q, cu = chunks._chunk(b, new)
+    call = lambda: ops.flash_attention_paged_weights(q, b.k, b.v, b.table, cu, b.lens_host, b.weights.clone())
+    assert launches(call, tmp_path)[-launched - 1:].count(CHUNK) == launched
+    chunks._run(b, new)
+    chunks._run(b, new, causal=False, last=2)
