@@ -32,7 +32,7 @@ def _turn(b, cu, prefix, tokens, queries, wait):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("d,groups", [(128, [(30, 700), (2, 16), (18, 300)]), (64, [(90, 500), (20, 40)]), (256, [(20, 200)])])
-def test_appends_and_steps_back_to_back(d, groups, dtype, tmp_path):
+def test_appends_and_steps_back_to_back(d, groups, dtype):
     hkv, prefixes, cu = (8 if d == 128 else 4), [], [0]
     for n, tokens in groups:
         prefixes.append((cu[-1], cu[-1] + n, tokens))
@@ -47,7 +47,7 @@ def test_appends_and_steps_back_to_back(d, groups, dtype, tmp_path):
     outs, *left = _turn(b, cu, prefix, tokens, queries, True)
     from scicompute_attention_b200 import ops
     step = lambda: ops.paged_attention_shared(b.q, b.k, b.v, b.table, b.lens, cu, prefix, block_size=b.bs, weights=b.weights.clone())
-    assert launches(step, tmp_path) == THREE
+    assert launches(step) == THREE
     for _ in range(3):
         torch.cuda.synchronize()
         got, *again = _turn(b, cu, prefix, tokens, queries, False)
@@ -62,12 +62,12 @@ def test_appends_and_steps_back_to_back(d, groups, dtype, tmp_path):
         ref.check_output(outs[-1][s, :, 0], want[0], p[0], b.keys(s)[2], ref.weights_bound(d, len(at), 1, size), 2.0 ** -11)
 
 
-def test_a_mark_that_is_not_there_or_left_over(tmp_path):
+def test_a_mark_that_is_not_there_or_left_over():
     """Scratch that begins with anything: the mark of an earlier call too."""
     from scicompute_attention_b200 import ops
     b = ref.Batch([600 + i for i in range(40)], hq=16, hkv=8, d=128, prefixes=[(0, 40, 512)])
     run = lambda: ops.paged_attention_shared(b.q, b.k, b.v, b.table, b.lens, np.array([0, 40], np.int32), np.array([512], np.int32), block_size=16)
-    assert launches(run, tmp_path) == THREE
+    assert launches(run) == THREE
     want = run()
     scratch = ops.acquire_scratch_fp32(1, b.q.device, handle=ops._stream_ptr(None))
     assert (scratch[:2].view(torch.int64) == 0).all()  # taken away by the end of a call

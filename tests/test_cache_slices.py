@@ -43,14 +43,14 @@ def test_what_fits_has_a_score_for_every_token():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("hq,hkv,d,dtype,n,slices", [(128, 1, 64, torch.bfloat16, 70, 3), (32, 8, 128, torch.float16, 130, 2), (40, 2, 96, torch.bfloat16, 110, 2)])
-def test_weights_in_slices(hq, hkv, d, dtype, n, slices, tmp_path):
+def test_weights_in_slices(hq, hkv, d, dtype, n, slices):
     import cache_reference as ref
     from launches import TWO, launches
     from scicompute_attention_b200 import ops
     from test_cache_weights_gpu import _check
     b = ref.Batch([(37 * i) % 300 + i % 2 for i in range(n)], hq=hq, hkv=hkv, d=d, dtype=dtype, extra_pages=8192 - 19)
     run = lambda w: ops.paged_attention_weights(b.q, b.k, b.v, b.table, b.lens, w, block_size=b.bs)
-    assert launches(lambda: run(b.weights.clone()), tmp_path) == TWO * slices
+    assert launches(lambda: run(b.weights.clone())) == TWO * slices
     before, again = b.weights.clone(), b.weights.clone()
     out = run(b.weights)
     _check(b, out, b.weights, before)
@@ -65,12 +65,12 @@ def test_weights_in_slices(hq, hkv, d, dtype, n, slices, tmp_path):
 
 
 @pytest.mark.gpu
-def test_groups_that_slices_cut(tmp_path):
+def test_groups_that_slices_cut():
     """Slices end behind sequences 24 and 48: the first group leaves one sequence to the second slice, the fourth goes over into the last one."""
     import test_cache_shared_gpu as shared
     from launches import THREE, launches
     from scicompute_attention_b200 import ops
     b, cu, prefix = shared._batch([(25, 300), (1, 40), (10, 70), (30, 529), (4, 16)], [1, 30, 0, 200], hq=128, hkv=1, d=64, extra_pages=8192 - 46)
     run = lambda w: ops.paged_attention_shared(b.q, b.k, b.v, b.table, b.lens, cu, prefix, block_size=b.bs, weights=w)
-    assert launches(lambda: run(b.weights.clone()), tmp_path) == THREE * 3
+    assert launches(lambda: run(b.weights.clone())) == THREE * 3
     shared._run(b, cu, prefix, True)

@@ -55,7 +55,7 @@ def test_wide_tables(pages):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,longest,hkv,launched", [(3, 30_000, 2, 1), (160, 5000, 1, 1), (161, 5000, 2, 2), (400, 700, 1, 3)])
-def test_ragged_batches(n, longest, hkv, launched, tmp_path):
+def test_ragged_batches(n, longest, hkv, launched):
     """One sequence far longer than the others, anywhere in the batch, equal ones, every number of tiles below that: only tiles that exist are dealt, those of
     up to 160 sequences to a launch."""
     import test_chunk_weights_gpu as chunks
@@ -67,6 +67,6 @@ def test_ragged_batches(n, longest, hkv, launched, tmp_path):
     b = chunks._batch(lens, hq=2 * hkv, hkv=hkv)
     q, cu = chunks._chunk(b, new)
     call = lambda: ops.flash_attention_paged_weights(q, b.k, b.v, b.table, cu, b.lens_host, b.weights.clone())
-    assert launches(call, tmp_path)[-launched - 1:].count(CHUNK) == launched
+    assert launches(call)[-launched - 1:].count(CHUNK) == launched
     chunks._run(b, new)
     chunks._run(b, new, causal=False, last=2)
