@@ -425,7 +425,8 @@ SCA_ABI int sca_launch_flash_paged_fp8(const ScaFlashPagedParams* params, const 
 typedef struct ScaPagedStep {
     /* Groups of sequences that share pages: HOST arrays. Group i is the sequences cu_groups[i] .. cu_groups[i + 1] - 1; the entries of
      * the whole pages of their first prefix_lens[i] tokens are the same in all their page-table rows, and each of them has those tokens.
-     * num_groups = 0: nothing is shared. At most 128 groups of two or more sequences that share a page; pages of 8, 16, 32 or 64 tokens. */
+     * num_groups = 0: nothing is shared. At most 128 groups of two or more sequences that share a page; pages of 8, 16, 32 or 64 tokens.
+     * bf16 V in shared pages may be taken as fp16, as the prefill takes it: +-65504 at most, multiples of 2^-24 below 2^-14. */
     const int32_t* cu_groups;   /* num_groups + 1 */
     const int32_t* prefix_lens; /* num_groups */
     int64_t num_groups;

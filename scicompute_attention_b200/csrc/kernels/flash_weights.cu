@@ -20,8 +20,8 @@
 // No unit is at its limit: while an SM has work its special-function unit is busy 71 % of the time (16384 exponentials a tile take 1024 clocks, the
 // products 540), and a quarter of the exponentials by a polynomial of degree 5 on the multipliers instead gained next to nothing (260 -> 256 us, half
 // of them 266). A warp waits on the chain of its own tile and on shared memory, from which every thread reads 64 numbers of lse beside its 64 exponentials (stalls per issue:
-// wait 2.4, long scoreboard 2.3, MIO throttle 2.1), and items do not come out even: the SMs have work 87 % of the time. 4 prompts of 1900 to 2048
-// tokens, 32 / 8 heads, D=128: 115 us alone, 257 us with the prefill.
+// MIO throttle 2.4, wait 2.3, long scoreboard 2.2), and items do not come out even: the SMs have work 87 % of the time. 4 prompts of 1900 to 2048
+// tokens, 32 / 8 heads, D=128: 112 us alone, 257 us with the prefill.
 #include <algorithm>
 #include <vector>
 

@@ -31,7 +31,7 @@ constexpr int kDigits = 4;
 constexpr int kBins = 256;
 static_assert(kBins == kEvictThreads, "a bin to a thread");
 constexpr int kEvictCluster = 16;  // CTAs to a (sequence, kv head) at most
-constexpr int kEvictCtas = 4;      // CTAs to an SM at least
+constexpr int kEvictCtas = 4;      // CTAs to an SM that there are registers for; shared memory for, where a CTA keeps up to 13 thousand keys
 // Pieces that a thread has on their way at once; 16, with registers for one CTA to an SM, take 53.7 us for 49.2 (100 thousand tokens).
 constexpr int kHeld = 8;
 constexpr int kLoads = 8;          // weights that a thread has on their way at once
@@ -334,7 +334,8 @@ kv_evict_kernel(const EvictParams p) {
     for (int j = m + me; j < n; j += threads) w[j] = 0.0f;  // every weight has been read by now
 }
 
-// Keys that stay in shared memory between the digits; what a CTA has beyond them is read again.
+// Keys that stay in shared memory between the digits; what a CTA has beyond them is read again. So many leave three CTAs to an SM; with 12 800, which leave
+// four, 192 sequences of up to 6000 tokens in a table of 131 072 take 263 us for 277, but 100 of 15 000 tokens 664 for 485 and 20 of 30 000 306 for 223.
 constexpr int kCachedKeys = 16384;
 
 template <typename V>
@@ -352,7 +353,9 @@ int LaunchEvict(const EvictParams& p, int64_t units, cudaStream_t stream) {
 }
 
 // CTAs to a (sequence, kv head). More of them shorten the chain of phases of a long one and cost barriers in a short one; up to 8 as long as
-// all CTAs are resident (4 to an SM), 16 where that leaves one to an SM. us for 8 kv heads, D=128, 16 bits, 1 / 2 / 4 / 8 / 16 CTAs:
+// all CTAs are resident (counted as 4 to an SM), 16 where that leaves one to an SM. The lengths are on the device: the width of the table stands for
+// them here and for the keys that a CTA keeps, and one that is much wider than its sequences costs (one of 1100 tokens in a table of 1104 / 131 072: 11.8 /
+// 15.7 us, 192 of 500 to 6000 in one of 6016 / 131 072: 220 / 276). us for 8 kv heads, D=128, 16 bits, 1 / 2 / 4 / 8 / 16 CTAs:
 //   one sequence of 1100 tokens down to 1024   12.5 / 13.6 / 13.4 / 13.7 / 17.7     4 of 8192 to 4096    101 / 58 / 35 / 30 / 49
 //   of 2200 to 1024                            32.4 / 26.1 / 16.8 / 15.4 / 18.1     8 of 16000 to 4000   160 / 89 / 60 / 61 / 95
 //   of 8192 to 4096                            85.6 / 48.8 / 30.0 / 21.8 / 22.2     16 of 4096 to 2048    62 / 46 / 44 / 56 / 115

@@ -1051,8 +1051,10 @@ def paged_attention_shared(q, k_pool, v_pool, page_table, seq_lens, cu_groups, p
     Group i is the sequences cu_groups[i] .. cu_groups[i + 1] - 1 (neighbours; cu_groups has num_groups + 1 entries from 0 to num_seqs), and all of
     them begin with the same prefix_lens[i] tokens: the table's entries of the whole pages of those tokens are the same in all rows of the group
     and are taken from its first row; tokens of a page that the prefix does not fill are each sequence's own, as are the ones behind. Both lists
-    are on the HOST. At most 128 groups of two or more sequences that share a page; pages of 8, 16, 32 or 64 tokens. Values of bfloat16
-    beyond +-65504 in shared pages count as +-65504, as in the prefill.
+    are on the HOST. At most 128 groups of two or more sequences that share a page; pages of 8, 16, 32 or 64 tokens.
+    Where the shared pages are read once, their V of bfloat16 and the softmax weights become float16 numbers, as in the prefill: values beyond +-65504
+    count as +-65504, those below 2^-14 as multiples of 2^-24, and a weight has 11 bits. A call that does not fill the machine may read shared pages once
+    per sequence, without either: outputs of the two differ by roundings.
     With `weights` (see paged_attention_weights) the weights of each sequence's own tokens are added up; those of shared pages are left alone.
     The rest is as paged_attention_weights has it."""
     if stream is None and cu_groups is not None:
@@ -1130,7 +1132,9 @@ def kv_evict(layer_k, layer_v, weights, page_table, seq_lens, *, keep: int, rece
     counted upwards. weights (float32, as paged_attention_weights takes them) go along and become 0 in places [m, n). Sequences of up to m tokens
     are left alone.
     `first`: a number, or int32 [num_seqs] on the device - the tokens of a shared prefix, say, whose pages belong to others too: a page that
-    holds any other token belongs to one sequence only. Pools as kv_append takes them, of any type; rows on unmapped pages are not copied."""
+    holds any other token belongs to one sequence only. Pools as kv_append takes them, of any type, but not the codes of an 8-bit layer, whose
+    scales would stay where they are; rows on unmapped pages are not copied. The launch is sized by the width of the table: one that fits its sequences is
+    the faster one."""
     if stream is None:
         new_lens = _native().evict(layer_k, layer_v, weights, page_table, seq_lens, keep, recent, first)
         if new_lens is not None:
